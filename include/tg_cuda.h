@@ -342,6 +342,98 @@ typedef struct {
 int tg_cuda_ssm_profile(tg_cuda_ssm *g, int enable);
 int tg_cuda_ssm_get_stats(const tg_cuda_ssm *g, tg_cuda_ssm_stats *out);
 
+/* ---- paged key/value caches -------------------------------------------------------
+ * A decoder's cache in pages, for servers: attention of several drafted tokens at once
+ * (speculative decoding; one token is the plain decode step), the attention weight each
+ * cached position receives, the commit of accepted tokens, and eviction by that weight.
+ * No reference counterpart: the reference recomputes every position's keys and values
+ * (examples/qwen3/import.py:90-132).
+ *
+ * Position p of sequence b lies in row p % page of pool page table[b][p / page]; row
+ * elements are contiguous, and the element (page g, head h, row r) of either pool starts
+ * at g * page_stride + h * head_stride + r * pos_stride elements. All pointers are DEVICE
+ * pointers on the current device; calls are asynchronous on `stream` (NULL = the legacy
+ * default stream), allocate no device memory and keep nothing between calls. Every row
+ * (cache, q, drafted k and v, out) starts on a 16-byte boundary and has a multiple of 16
+ * bytes; head_dim is at most 256.
+ *
+ * len and table are read by the kernels. A len outside [0, max_len] is taken as the
+ * nearest of the two, rows of a page number outside [0, pages) read as zeros and are
+ * never written; a later call on the device then returns TG_CUDA_EDEVICE, like CUDA's
+ * own asynchronous errors. The first call on a device allocates a pinned status word, so
+ * it must not come inside a stream capture. */
+enum { TG_CUDA_F32, TG_CUDA_F16, TG_CUDA_BF16 };
+
+typedef struct {
+	int type;                /* TG_CUDA_F32 / F16 / BF16: the pools, q, out, drafted k and v */
+	int seqs, nkv, head_dim;
+	int page, pages;         /* positions per page (any number >= 1), pages in each pool */
+	int table_cols;          /* row stride of table */
+	int max_len;             /* upper bound of len, at most page * table_cols: it sizes the launches */
+	void *k, *v;             /* pools */
+	long long page_stride, head_stride, pos_stride; /* elements, of both pools */
+	const int *table;        /* [seqs][table_cols]; entries past a sequence's pages are not read */
+	const int *len;          /* [seqs] positions in the cache */
+} tg_cuda_kv;
+
+typedef struct {
+	int tokens;              /* drafted tokens per sequence: at most 64 for attention */
+	int nq;                  /* query heads, a multiple of nkv: head j attends with kv head j / (nq / nkv) */
+	float scale;             /* of the scores */
+	const void *q;           /* [seqs][tokens][nq][head_dim], strides in elements */
+	long long q_seq, q_tok, q_head;
+	const void *k, *v;       /* the drafted tokens' own rows [seqs][tokens][nkv][head_dim], one set of strides */
+	long long kv_seq, kv_tok, kv_head;
+	const unsigned long long *mask; /* [seqs][tokens]: bit u set = the token attends to drafted token u
+	                                   of its sequence; NULL = a chain, bits 0..t */
+	const int *count;        /* [seqs] tokens actually drafted, clamped to [0, tokens]; NULL = all */
+} tg_cuda_drafts;
+
+/* Attention of every drafted token over its sequence's whole cache and the drafted tokens
+ * its mask names (rows past count are named by nobody): out [seqs][tokens][nq][head_dim]
+ * = softmax(scale q.k) v in the cache's type, lse [seqs][tokens][nq] = the natural log of
+ * the sum of exp(scale q.k). A token that sees nothing, or only scores of -infinity, has
+ * out 0 and lse -infinity, and so have tokens past count. What a masked row holds
+ * (infinities and NaN too) does not matter. Scores, softmax and sums are f32; 16-bit
+ * caches round each probability to the cache's type for its product with v. work: scratch
+ * of at least tg_cuda_tree_attn_workspace bytes, 16-byte aligned, not shared with a call
+ * that may run at the same time (NULL where that is 0). */
+long long tg_cuda_tree_attn_workspace(const tg_cuda_kv *c, const tg_cuda_drafts *d);
+int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, void *out, long long out_seq, long long out_tok,
+		      long long out_head, float *lse, void *work, long long work_bytes, void *stream);
+
+/* The attention weight that positions receive: for cached position x,
+ *   acc_out[b][h][x] = acc[b][h][x] + sum of exp(scale q.k_x - lse) over the tokens t < count
+ *   whose bit in select[b] is set and the query heads of h,
+ * and for drafted position u, fresh[b][h][u] the same sum over the tokens whose mask names
+ * it. lse as tg_cuda_tree_attn wrote it; rows with lse -infinity add nothing. select NULL =
+ * every token, acc NULL = zeros; acc is [seqs][nkv][>= len] with the given strides and may
+ * be acc_out if these are acc_out's own, nkv * max_len and max_len. acc_out is
+ * [seqs][nkv][max_len], zero from len on; fresh [seqs][nkv][tokens]. d->v is not read. */
+int tg_cuda_attn_weights(const tg_cuda_kv *c, const tg_cuda_drafts *d, const float *lse, const unsigned long long *select,
+			 const float *acc, long long acc_seq, long long acc_head, float *acc_out, float *fresh, void *stream);
+
+/* Accepted tokens into the cache: for i < count[b], cache row len[b] + i receives drafted
+ * row path[b][i] (path [seqs][tokens]; NULL = row i), keys and values, and len_out[b] =
+ * len[b] + count[b] (len_out may not be len). fresh and acc, both or neither: acc[b][h][len + i]
+ * = fresh[b][h][path[b][i]], acc [seqs][nkv][acc_cols] with the given strides. tokens may be
+ * any number here, d->q is not read, and max_len bounds len before the call. A row past the
+ * table, a path entry outside [0, tokens) or a column past acc_cols is not written and is
+ * reported like a bad page. No two rows written may share a page row. */
+int tg_cuda_kv_commit(const tg_cuda_kv *c, const tg_cuda_drafts *d, const int *path, int *len_out, const float *fresh,
+		      float *acc, long long acc_seq, long long acc_head, int acc_cols, void *stream);
+
+/* Eviction: for every sequence and kv head, at most `budget` positions of src go to dst in
+ * ascending order. A sequence of at most budget positions keeps all; a longer one keeps its
+ * first `sink` and last `recent` and, of those between, the budget - sink - recent with the
+ * largest acc (ties: the lower position; NaN counts below every number). keep [seqs][nkv]
+ * [budget] = the kept positions, -1 past the last; acc_out, alike, their acc, 0 past the
+ * last; len_out[b] = min(len, budget). dst's pages (of src's pools or others) may not be
+ * among the pages src's sequences hold; dst->len and dst->max_len are not read. A kept row
+ * past dst's table is not written and is reported like a bad page. */
+int tg_cuda_kv_evict(const tg_cuda_kv *src, const tg_cuda_kv *dst, const float *acc, long long acc_seq, long long acc_head,
+		     int budget, int recent, int sink, int *keep, float *acc_out, int *len_out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

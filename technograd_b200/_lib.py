@@ -30,7 +30,9 @@ SYMBOLS = ["tg_cuda_error", "tg_cuda_init", "tg_cuda_ngpus", "tg_cuda_selftest_w
            "tg_cuda_batcher_stats", "tg_cuda_batcher_free",
            "tg_cuda_lm_load", "tg_cuda_lm_forward", "tg_cuda_lm_generate", "tg_cuda_lm_free", "tg_cuda_lm_profile",
            "tg_cuda_lm_get_stats", "tg_cuda_ssm_load", "tg_cuda_ssm_forward", "tg_cuda_ssm_forward_device",
-           "tg_cuda_ssm_free", "tg_cuda_ssm_profile", "tg_cuda_ssm_get_stats"]
+           "tg_cuda_ssm_free", "tg_cuda_ssm_profile", "tg_cuda_ssm_get_stats",
+           "tg_cuda_tree_attn_workspace", "tg_cuda_tree_attn", "tg_cuda_attn_weights", "tg_cuda_kv_commit",
+           "tg_cuda_kv_evict"]
 
 
 class TgCudaError(RuntimeError):
@@ -102,6 +104,24 @@ class LmStats(C.Structure):
                 ("decode_gemm_ms", C.c_double), ("decode_gemm_weight_bytes", C.c_double)]
 
 
+# element types of a paged cache (tg_cuda_kv.type)
+F32, F16, BF16 = 0, 1, 2
+
+
+class Kv(C.Structure):
+    _fields_ = [("type", C.c_int), ("seqs", C.c_int), ("nkv", C.c_int), ("head_dim", C.c_int), ("page", C.c_int),
+                ("pages", C.c_int), ("table_cols", C.c_int), ("max_len", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("page_stride", C.c_longlong), ("head_stride", C.c_longlong), ("pos_stride", C.c_longlong),
+                ("table", C.c_void_p), ("len", C.c_void_p)]
+
+
+class Drafts(C.Structure):
+    _fields_ = [("tokens", C.c_int), ("nq", C.c_int), ("scale", C.c_float), ("q", C.c_void_p),
+                ("q_seq", C.c_longlong), ("q_tok", C.c_longlong), ("q_head", C.c_longlong), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("kv_seq", C.c_longlong), ("kv_tok", C.c_longlong), ("kv_head", C.c_longlong),
+                ("mask", C.c_void_p), ("count", C.c_void_p)]
+
+
 _lib = None
 
 
@@ -112,7 +132,7 @@ def lib() -> C.CDLL:
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(f"libtgcuda is not built ({LIB_PATH}); run __graft_entry__.build()")
         L = C.CDLL(LIB_PATH)
-        vp, i, l = C.c_void_p, C.c_int, C.c_long
+        vp, i, l, ll = C.c_void_p, C.c_int, C.c_long, C.c_longlong
         sigs = {
             "tg_cuda_error": ([], C.c_char_p),
             "tg_cuda_init": ([i, C.POINTER(i)], i),
@@ -151,6 +171,11 @@ def lib() -> C.CDLL:
             "tg_cuda_ssm_free": ([vp], None),
             "tg_cuda_ssm_profile": ([vp, i], i),
             "tg_cuda_ssm_get_stats": ([vp, C.POINTER(SsmStats)], i),
+            "tg_cuda_tree_attn_workspace": ([vp, vp], ll),
+            "tg_cuda_tree_attn": ([vp, vp, vp, ll, ll, ll, vp, vp, ll, vp], i),
+            "tg_cuda_attn_weights": ([vp, vp, vp, vp, vp, ll, ll, vp, vp, vp], i),
+            "tg_cuda_kv_commit": ([vp, vp, vp, vp, vp, vp, ll, ll, i, vp], i),
+            "tg_cuda_kv_evict": ([vp, vp, vp, ll, ll, i, i, i, vp, vp, vp, vp], i),
         }
         for name, (args, res) in sigs.items():
             f = getattr(L, name)

@@ -1,0 +1,87 @@
+// paged.cuh -- what the kernels over a paged key/value cache share: its device view, the
+// address of a row, the status word, element types and the host's checks of a description.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace tgc {
+
+// What a paged-cache kernel can meet in device data: each has a word of its own in mapped host
+// memory, set by a plain store (no read-modify-write over the bus) and cleared by the next call.
+enum : int { PG_LEN, PG_PAGE, PG_PATH, PG_ROOM, PG_WORDS };
+
+// A pool in bytes: positions are table lookups, so every offset is 64-bit.
+struct PgCache {
+	char *k, *v;
+	const int *table, *len;
+	long long page_b, head_b, pos_b; // strides in bytes
+	int page, pages, cols, max_len, nkv, dim;
+	int *status;                     // PG_WORDS words, written only on an error
+
+	__device__ __forceinline__ void report(int what) const { *(volatile int *)(status + what) = 1; }
+	__device__ __forceinline__ int length(int b) const
+	{
+		const int n = len[b];
+		if (n < 0 || n > max_len) report(PG_LEN);
+		return n < 0 ? 0 : n > max_len ? max_len : n;
+	}
+	// byte offset of a sequence's row (head 0) at position p, -1 where the page number is not one
+	__device__ __forceinline__ long long row(const int *tab, int p) const
+	{
+		const int c = p / page, g = tab[c];
+		if ((unsigned)g >= (unsigned)pages) {
+			report(PG_PAGE);
+			return -1;
+		}
+		return (long long)g * page_b + (long long)(p - c * page) * pos_b;
+	}
+};
+
+struct PgDrafts {
+	const char *q, *k, *v;
+	long long q_seq, q_tok, q_head, kv_seq, kv_tok, kv_head; // bytes
+	const unsigned long long *mask;
+	const int *count;
+	int tokens, nq, group;
+	float scale;
+
+	__device__ __forceinline__ int drafted(int b) const
+	{
+		const int n = count ? count[b] : tokens;
+		return n < 0 ? 0 : n > tokens ? tokens : n;
+	}
+	// the drafted tokens that token t attends to, those past the count taken out
+	__device__ __forceinline__ unsigned long long sees(int b, int t, int n) const
+	{
+		const unsigned long long live = n >= 64 ? ~0ull : (1ull << n) - 1;
+		return (mask ? mask[(long long)b * tokens + t] : (2ull << t) - 1) & live;
+	}
+};
+
+template <class T> struct PgElem;
+template <> struct PgElem<float> {
+	static __device__ __forceinline__ float get(float x) { return x; }
+	static __device__ __forceinline__ float put(float x) { return x; }
+};
+template <> struct PgElem<__half> {
+	static __device__ __forceinline__ float get(__half x) { return __half2float(x); }
+	static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
+};
+template <> struct PgElem<__nv_bfloat16> {
+	static __device__ __forceinline__ float get(__nv_bfloat16 x) { return __bfloat162float(x); }
+	static __device__ __forceinline__ __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
+};
+
+// paged.cu: checks a description and fills the device view. `who` opens the error text.
+int pg_cache(const char *who, const tg_cuda_kv *c, PgCache *out);
+enum { PG_USE_Q = 1, PG_USE_K = 2, PG_USE_V = 4 };
+int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, int use, int most, PgDrafts *out);
+// The device's number and SM count, and the address of its status word; EDEVICE when a kernel
+// of an earlier call reported something.
+int pg_device(const char *who, int *sms, int **status);
+static inline int pg_size(int type) { return type == TG_CUDA_F32 ? 4 : 2; }
+
+} // namespace tgc
