@@ -10,20 +10,33 @@ constexpr int PG_DEVICES = 64;
 static std::mutex g_pg_mu;
 static struct { int sms; int *host, *dev; } g_pg[PG_DEVICES];
 
+int pg_sms(const char *who, int *dev, int *sms)
+{
+	cudaError_t e = cudaGetDevice(dev);
+	if (e != cudaSuccess) return set_err(TG_CUDA_ENODEV, "%s: cudaGetDevice: %s", who, cudaGetErrorString(e));
+	if (*dev < 0 || *dev >= PG_DEVICES) return set_err(TG_CUDA_EINVAL, "%s: device ordinal %d", who, *dev);
+	std::lock_guard<std::mutex> lk(g_pg_mu);
+	auto &g = g_pg[*dev];
+	if (!g.sms) {
+		int n = 0;
+		TGC_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev));
+		g.sms = n;
+	}
+	*sms = g.sms;
+	return TG_CUDA_OK;
+}
+
 int pg_device(const char *who, int *sms, int **status)
 {
-	int dev = -1;
-	cudaError_t e = cudaGetDevice(&dev);
-	if (e != cudaSuccess) return set_err(TG_CUDA_ENODEV, "%s: cudaGetDevice: %s", who, cudaGetErrorString(e));
-	if (dev < 0 || dev >= PG_DEVICES) return set_err(TG_CUDA_EINVAL, "%s: device ordinal %d", who, dev);
+	int dev = -1, rc = pg_sms(who, &dev, sms);
+	if (rc) return rc;
 	std::lock_guard<std::mutex> lk(g_pg_mu);
 	auto &g = g_pg[dev];
 	if (!g.host) {
-		TGC_CUDA(cudaDeviceGetAttribute(&g.sms, cudaDevAttrMultiProcessorCount, dev));
 		int *h = nullptr;
 		TGC_CUDA(cudaHostAlloc((void **)&h, PG_WORDS * sizeof(int), cudaHostAllocMapped));
 		for (int i = 0; i < PG_WORDS; i++) h[i] = 0;
-		e = cudaHostGetDevicePointer((void **)&g.dev, h, 0);
+		cudaError_t e = cudaHostGetDevicePointer((void **)&g.dev, h, 0);
 		if (e != cudaSuccess) {
 			cudaFreeHost(h);
 			return set_err(TG_CUDA_ECUDA, "%s: cudaHostGetDevicePointer: %s", who, cudaGetErrorString(e));
@@ -37,7 +50,6 @@ int pg_device(const char *who, int *sms, int **status)
 			       met[PG_LEN] ? " a len outside [0, max_len];" : "", met[PG_PAGE] ? " a page number outside the pool;" : "",
 			       met[PG_PATH] ? " a path entry outside the drafted tokens;" : "",
 			       met[PG_ROOM] ? " a row past the table or the weights;" : "");
-	*sms = g.sms;
 	*status = g.dev;
 	return TG_CUDA_OK;
 }

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace tgc {
@@ -65,15 +67,28 @@ template <class T> struct PgElem;
 template <> struct PgElem<float> {
 	static __device__ __forceinline__ float get(float x) { return x; }
 	static __device__ __forceinline__ float put(float x) { return x; }
+	// whether a word of elements holds an infinity or a NaN
+	static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
 };
 template <> struct PgElem<__half> {
 	static __device__ __forceinline__ float get(__half x) { return __half2float(x); }
 	static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
+	static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
 };
 template <> struct PgElem<__nv_bfloat16> {
 	static __device__ __forceinline__ float get(__nv_bfloat16 x) { return __bfloat162float(x); }
 	static __device__ __forceinline__ __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
+	static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 };
+
+// Dynamic shared memory of a kernel, allowed once per device: `done` is the kernel's own set of devices.
+template <class K> static inline int pg_smem(K kernel, int bytes, int dev, std::atomic<unsigned long long> &done)
+{
+	if (done.load(std::memory_order_acquire) >> dev & 1) return TG_CUDA_OK;
+	TGC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+	done.fetch_or(1ull << dev, std::memory_order_release);
+	return TG_CUDA_OK;
+}
 
 // paged.cu: checks a description and fills the device view. `who` opens the error text.
 int pg_cache(const char *who, const tg_cuda_kv *c, PgCache *out);
@@ -82,6 +97,7 @@ int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, int
 // The device's number and SM count, and the address of its status word; EDEVICE when a kernel
 // of an earlier call reported something.
 int pg_device(const char *who, int *sms, int **status);
+int pg_sms(const char *who, int *dev, int *sms); // the current device and its SM count alone
 static inline int pg_size(int type) { return type == TG_CUDA_F32 ? 4 : 2; }
 
 } // namespace tgc

@@ -1,0 +1,481 @@
+// tree_attn.cuh -- attention of drafted tokens over a paged cache: the kernel for few query rows, and
+// the join of partial results. One source per element type instantiates it (tree_attn_*.cu).
+#pragma once
+
+#include "common.cuh"
+#include "mma_sync.cuh"
+#include "paged.cuh"
+
+namespace tgc {
+
+struct AttnArgs {
+	PgCache c;
+	PgDrafts d;
+	char *out;
+	long long out_seq, out_tok, out_head; // bytes
+	float *lse;
+	int seqs;
+	int row_tiles;   // tiles of 16 * MT query rows per (sequence, kv head)
+	int whole;       // 1: a CTA per unit; 0: equal shares of the units' tiles
+	int least;       // shares: tiles per CTA at least
+	float *part;     // shares: partial results, two slots per CTA
+	int4 *split;     // shares: per CTA, the unit that begins in its share and ends in a later one
+};
+
+// The kernel for few query rows. Per (sequence b, kv head h) the query rows are r = t * group + g
+// (token t, query head h * group + g): every head of the group and every drafted token meet a key
+// while it is in shared memory, so the cache is read once for up to 16 * MT rows.
+//
+// Unit = (b, h, tile of 16 * MT rows); its keys are the cached positions in tiles of 4 * KW, then the
+// drafted tokens in as many tiles as they need. A CTA's four warps each take KW keys of a tile and
+// work on their own: a ring of NST stages of cp.async copies per warp (K and V rows, XOR-swizzled),
+// S = Q K^T on the tensor cores, p = 2^(z - mr) with z = scale log2(e) s, and O += P V with O in
+// registers. mr is a running reference for each row, raised (O and l rescaled) only when a score
+// exceeds it by RAISE, so the usual step needs no maximum across lanes; p stays below 2^(RAISE + SHIFT)
+// and the quotient O / l is the softmax's whatever mr is. At a unit's end the four warps' O are
+// brought to one reference and summed in warp order through the stage each of them has free.
+//
+// What bounds it: the cache's bytes. Lengths differ and units are few or many, so the CTAs of one
+// wave take equal shares of all units' tiles, in order; the ring runs on across unit boundaries. A
+// unit that ends in its CTA's share is written out; of one that spans several, each CTA leaves
+// (O, mr, l), and k_attn_join adds them in CTA order: results do not depend on timing.
+template <class T> struct AttnScale; // SHIFT: exponent given to probabilities near 1
+template <> struct AttnScale<float> { static constexpr float SHIFT = 0, RAISE = 8; };
+template <> struct AttnScale<__nv_bfloat16> { static constexpr float SHIFT = 0, RAISE = 8; };
+// f16 has 5 exponent bits: probabilities from 2^-24 to 2^5 of the reference must be normal numbers
+template <> struct AttnScale<__half> { static constexpr float SHIFT = 10, RAISE = 5; };
+
+template <class T, int DP, int MT> struct AttnTile {
+	static constexpr int KW = sizeof(T) == 4 ? 8 : 16, NT = KW / 8, TK = 4 * KW, RT = 16 * MT;
+	static constexpr int P = DP * (int)sizeof(T), CH = P / 16;
+	static constexpr int STAGE = 2 * KW * P; // also 16 x DP floats, what the end of a unit needs
+	static constexpr int NST = DP == 256 || (DP == 128 && MT == 2 && sizeof(T) == 4) ? 2 : 3; // two CTAs per SM up to 128 dimensions
+	static constexpr int Q = 0, RING = RT * P, MASK = RING + 4 * NST * STAGE, ML = MASK + RT * 8, SCAN = ML + 4 * RT * 8;
+	static constexpr int SMEM = SCAN + 64;
+	static constexpr int SLOT = RT * DP + 2 * RT; // floats of a partial result
+};
+
+// A place in the list of tiles.
+struct AttnCursor {
+	int b, h, r, tile, ctx, n, all; // ctx: tiles of cached positions, all: with the drafted ones
+};
+
+template <int TK>
+__device__ __forceinline__ void cursor_seq(const AttnArgs &p, AttnCursor &c, int extra)
+{
+	c.n = p.c.length(c.b);
+	c.ctx = (int)(((long long)c.n + TK - 1) / TK);
+	c.all = c.ctx + extra;
+}
+
+template <int TK>
+__device__ __forceinline__ void cursor_next(const AttnArgs &p, AttnCursor &c, int extra)
+{
+	if (++c.tile < c.all) return;
+	c.tile = 0;
+	if (++c.r < p.row_tiles) return;
+	c.r = 0;
+	if (++c.h < p.c.nkv) return;
+	c.h = 0;
+	if (++c.b < p.seqs) cursor_seq<TK>(p, c, extra);
+}
+
+// Sum of a value over the CTA's 128 threads, and the sum over the threads before this one.
+__device__ __forceinline__ long long scan128(long long v, long long *s, long long &before)
+{
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	long long x = v;
+#pragma unroll
+	for (int o = 1; o < 32; o <<= 1) {
+		const long long y = __shfl_up_sync(~0u, x, o);
+		if (lane >= o) x += y;
+	}
+	__syncthreads();
+	if (lane == 31) s[warp] = x;
+	__syncthreads();
+	before = x - v;
+	long long all = 0;
+#pragma unroll
+	for (int w = 0; w < 4; w++) {
+		if (w < warp) before += s[w];
+		all += s[w];
+	}
+	return all;
+}
+
+// o (already over l, or a partial's) of 4 columns
+__device__ __forceinline__ void store4(float *d, float4 v) { *(float4 *)d = v; }
+__device__ __forceinline__ void store4(__half *d, float4 v) { *(uint2 *)d = make_uint2(pack16(v.x, v.y, __half()), pack16(v.z, v.w, __half())); }
+__device__ __forceinline__ void store4(__nv_bfloat16 *d, float4 v)
+{
+	*(uint2 *)d = make_uint2(pack16(v.x, v.y, __nv_bfloat16()), pack16(v.z, v.w, __nv_bfloat16()));
+}
+
+// A row's result: a token past the count, or one that saw nothing, has 0 and -infinity.
+template <class T>
+__device__ __forceinline__ void store_row4(const AttnArgs &p, int b, int h, int row, int col, int cnt, float4 o, float mr, float l)
+{
+	const int t = row / p.d.group, j = h * p.d.group + row % p.d.group;
+	const bool none = t >= cnt || l == 0;
+	const float f = none ? 0 : 1 / l;
+	if (none) o = make_float4(0, 0, 0, 0);
+	o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+	if (col < p.c.dim) store4((T *)(p.out + b * p.out_seq + t * p.out_tok + j * p.out_head) + col, o);
+	if (col == 0) p.lse[((long long)b * p.d.tokens + t) * p.d.nq + j] = none ? -INFINITY : (mr + log2f(l)) * 0.69314718056f;
+}
+
+template <class T, int DP, int MT>
+__global__ void __launch_bounds__(128) k_tree_attn(const AttnArgs p)
+{
+	using A = AttnTile<T, DP, MT>;
+	constexpr int KW = A::KW, NT = A::NT, TK = A::TK, RT = A::RT, P = A::P, CH = A::CH, NST = A::NST;
+	constexpr float SHIFT = AttnScale<T>::SHIFT, RAISE = AttnScale<T>::RAISE;
+	extern __shared__ __align__(128) char smem[];
+	unsigned long long *s_mask = (unsigned long long *)(smem + A::MASK);
+	float2 *s_ml = (float2 *)(smem + A::ML);
+	long long *s_scan = (long long *)(smem + A::SCAN);
+	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+	const uint32_t s0 = smem_u32(smem), ring = s0 + A::RING + warp * NST * A::STAGE;
+	const int extra = (p.d.tokens + TK - 1) / TK, rows = p.d.tokens * p.d.group, chunks = p.c.dim * (int)sizeof(T) / 16;
+	const float zs = p.d.scale * 1.4426950408889634f;
+	pdl_launch();
+	pdl_wait();
+
+	// ---- this CTA's share
+	AttnCursor c; // the tile being worked on; f, below: the next to be fetched
+	long long left, pos = 0, share = 0;
+	if (p.whole) {
+		c.r = blockIdx.x % p.row_tiles;
+		c.h = blockIdx.x / p.row_tiles % p.c.nkv;
+		c.b = blockIdx.x / p.row_tiles / p.c.nkv;
+		c.tile = 0;
+		cursor_seq<TK>(p, c, extra);
+		left = c.all;
+	} else {
+		const int per = p.c.nkv * p.row_tiles;
+		auto weight = [&](int b) -> long long { return b < p.seqs ? (((long long)p.c.length(b) + TK - 1) / TK + extra) * per : 0; };
+		long long mine = 0, before, all;
+		for (int b = tid; b < p.seqs; b += 128) mine += weight(b);
+		all = scan128(mine, s_scan, before);
+		share = (all + gridDim.x - 1) / gridDim.x;
+		if (share < p.least) share = p.least;
+		pos = share * blockIdx.x;
+		if (tid == 0) p.split[blockIdx.x].x = -1;
+		if (pos >= all) return;
+		left = all - pos < share ? all - pos : share;
+		long long base = 0;
+		for (int b0 = 0;; b0 += 128) { // ends: pos < all
+			const long long w = weight(b0 + tid), sum = scan128(w, s_scan, before);
+			if (pos >= base + before && pos < base + before + w) s_scan[4] = b0 + tid, s_scan[5] = base + before;
+			base += sum;
+			if (pos < base) break;
+		}
+		__syncthreads();
+		c.b = (int)s_scan[4];
+		cursor_seq<TK>(p, c, extra);
+		const long long off = pos - s_scan[5], u = off / c.all;
+		c.tile = (int)(off - u * c.all);
+		c.h = (int)(u / p.row_tiles), c.r = (int)(u % p.row_tiles);
+	}
+
+	// ---- fetching: lane i < KW holds the address of the tile's row i
+	AttnCursor f = c;
+	long long fetched = 0;
+	auto fetch = [&](int stage) {
+		if (fetched < left) {
+			fetched++;
+			const char *kp = nullptr, *vp = nullptr;
+			if (lane < KW) {
+				if (f.tile < f.ctx) {
+					const long long x = (long long)f.tile * TK + warp * KW + lane;
+					const long long at = x < f.n ? p.c.row(p.c.table + (long long)f.b * p.c.cols, (int)x) : -1;
+					if (at >= 0) kp = p.c.k + at + f.h * p.c.head_b, vp = p.c.v + at + f.h * p.c.head_b;
+				} else {
+					const int u = (f.tile - f.ctx) * TK + warp * KW + lane;
+					const long long at = (long long)f.b * p.d.kv_seq + (long long)u * p.d.kv_tok + f.h * p.d.kv_head;
+					if (u < p.d.drafted(f.b)) kp = p.d.k + at, vp = p.d.v + at;
+				}
+			}
+			const uint32_t sk = ring + stage * A::STAGE, sv = sk + KW * P;
+#pragma unroll
+			for (int i = 0; i < KW * CH / 32; i++) {
+				const int x = i * 32 + lane, row = x / CH, ch = x % CH;
+				const unsigned long long kr = __shfl_sync(~0u, (unsigned long long)kp, row), vr = __shfl_sync(~0u, (unsigned long long)vp, row);
+				const uint32_t o = row * P + ((ch ^ (row & 7)) << 4);
+				const bool have = kr && ch < chunks;
+				cp16(sk + o, have ? (const char *)kr + ch * 16 : p.d.k, have);
+				cp16(sv + o, have ? (const char *)vr + ch * 16 : p.d.v, have);
+			}
+			cursor_next<TK>(p, f, extra);
+		}
+		cp_commit();
+	};
+
+	float o[MT][DP / 8][4], mr[MT][2], l[MT][2];
+	int cnt = 0;
+	bool first = true, from_start = true; // from_start: this CTA has the unit's first tile
+	int stage = 0;
+#pragma unroll
+	for (int i = 0; i < NST - 1; i++) fetch(i);
+
+	for (long long i = 0; i < left; i++) {
+		if (first) { // a unit begins here, or goes on from the CTA before
+			first = false;
+			from_start = c.tile == 0;
+			cnt = p.d.drafted(c.b);
+			for (int x = tid; x < RT * CH; x += 128) {
+				const int row = x / CH, ch = x % CH, r = c.r * RT + row, t = r / p.d.group;
+				uint4 v = make_uint4(0, 0, 0, 0);
+				if (r < rows && ch < chunks)
+					v = *(const uint4 *)(p.d.q + (long long)c.b * p.d.q_seq + (long long)t * p.d.q_tok + (long long)(c.h * p.d.group + r % p.d.group) * p.d.q_head + ch * 16);
+				*(uint4 *)(smem + row * P + ((ch ^ (row & 7)) << 4)) = v;
+			}
+			if (tid < RT) {
+				const int t = (c.r * RT + tid) / p.d.group;
+				s_mask[tid] = t < cnt ? p.d.sees(c.b, t, cnt) : 0;
+			}
+#pragma unroll
+			for (int m = 0; m < MT; m++) {
+				mr[m][0] = mr[m][1] = -INFINITY, l[m][0] = l[m][1] = 0;
+#pragma unroll
+				for (int d = 0; d < DP / 8; d++) o[m][d][0] = o[m][d][1] = o[m][d][2] = o[m][d][3] = 0;
+			}
+			__syncthreads();
+		}
+		fetch((stage + NST - 1) % NST); // into the stage of the tile before
+		cp_wait<NST - 1>();
+		__syncwarp();
+		const uint32_t sk = ring + stage * A::STAGE, sv = sk + KW * P;
+		const bool drafted = c.tile >= c.ctx;
+		float s[MT][NT][4];
+#pragma unroll
+		for (int m = 0; m < MT; m++)
+#pragma unroll
+			for (int x = 0; x < NT; x++) s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = 0;
+		qk_tile<T, DP, MT, NT>(s, s0, sk, lane);
+#pragma unroll
+		for (int m = 0; m < MT; m++)
+#pragma unroll
+			for (int x = 0; x < NT; x++)
+#pragma unroll
+				for (int e = 0; e < 4; e++) s[m][x][e] *= zs;
+		if (drafted || c.tile == c.ctx - 1) { // the mask's bits, or the end of the cache
+			const long long at = (long long)(drafted ? c.tile - c.ctx : c.tile) * TK + warp * KW;
+#pragma unroll
+			for (int m = 0; m < MT; m++)
+#pragma unroll
+				for (int x = 0; x < NT; x++)
+#pragma unroll
+					for (int e = 0; e < 4; e++) {
+						const long long key = at + x * 8 + 2 * t4 + (e & 1);
+						const bool ok = drafted ? s_mask[m * 16 + g + (e >> 1) * 8] >> key & 1 : key < c.n;
+						if (!ok) s[m][x][e] = -INFINITY;
+					}
+		}
+		// raise the references?
+		bool up = false;
+#pragma unroll
+		for (int m = 0; m < MT; m++)
+#pragma unroll
+			for (int x = 0; x < NT; x++)
+#pragma unroll
+				for (int e = 0; e < 4; e++) up |= s[m][x][e] > mr[m][e >> 1] + (SHIFT + RAISE);
+		if (__any_sync(~0u, up)) {
+#pragma unroll
+			for (int m = 0; m < MT; m++)
+#pragma unroll
+				for (int e = 0; e < 2; e++) {
+					float top = s[m][0][2 * e];
+#pragma unroll
+					for (int x = 0; x < NT; x++) top = fmaxf(top, fmaxf(s[m][x][2 * e], s[m][x][2 * e + 1]));
+					top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+					top = fmaxf(top, __shfl_xor_sync(~0u, top, 2)) - SHIFT;
+					if (top > mr[m][e]) {
+						const float a = ex2(mr[m][e] - top);
+						mr[m][e] = top, l[m][e] *= a;
+#pragma unroll
+						for (int d = 0; d < DP / 8; d++) o[m][d][2 * e] *= a, o[m][d][2 * e + 1] *= a;
+					}
+				}
+		}
+#pragma unroll
+		for (int m = 0; m < MT; m++)
+#pragma unroll
+			for (int e = 0; e < 2; e++) {
+				const float ref = mr[m][e] == -INFINITY ? 0 : mr[m][e]; // nothing seen yet: 2^-infinity
+#pragma unroll
+				for (int x = 0; x < NT; x++)
+#pragma unroll
+					for (int y = 2 * e; y < 2 * e + 2; y++) l[m][e] += s[m][x][y] = ex2(s[m][x][y] - ref);
+			}
+		bool plain = true;
+		if (drafted) { // a row that some token does not see may hold anything: 0 * infinity must not reach O
+			bool odd = false;
+			for (int x = lane; x < KW * CH; x += 32) {
+				const uint4 v = *(const uint4 *)(smem + (sv - s0) + x * 16);
+				const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+				for (int y = 0; y < 4; y++) odd |= PgElem<T>::odd(w[y]);
+			}
+			plain = !__any_sync(~0u, odd);
+		}
+		if (plain) pv_tile<T, DP, MT, NT>(o, s, sv, lane);
+		else {
+#pragma unroll
+			for (int x = 0; x < NT; x++)
+				for (int kk = 0; kk < 4; kk++) // the four lanes that hold keys 2 kk and 2 kk + 1
+#pragma unroll
+					for (int y = 0; y < 2; y++) {
+						const int key = x * 8 + kk * 2 + y;
+						float pr[MT][2];
+#pragma unroll
+						for (int m = 0; m < MT; m++)
+#pragma unroll
+							for (int e = 0; e < 2; e++) pr[m][e] = __shfl_sync(~0u, s[m][x][2 * e + y], (lane & ~3) | kk);
+#pragma unroll
+						for (int d = 0; d < DP / 8; d++)
+#pragma unroll
+							for (int z = 0; z < 2; z++) {
+								const int col = (d * 8 + 2 * t4 + z) * (int)sizeof(T);
+								const float v = PgElem<T>::get(*(const T *)(smem + (sv - s0) + key * P + (((col >> 4) ^ (key & 7)) << 4) + (col & 15)));
+#pragma unroll
+								for (int m = 0; m < MT; m++)
+#pragma unroll
+									for (int e = 0; e < 2; e++)
+										if (pr[m][e] != 0) o[m][d][2 * e + z] += pr[m][e] * v;
+							}
+					}
+		}
+		const bool end = c.tile == c.all - 1, last = i == left - 1;
+		if (end || last) {
+			// ---- the unit's end, or the share's: join the four warps
+#pragma unroll
+			for (int m = 0; m < MT; m++)
+#pragma unroll
+				for (int e = 0; e < 2; e++) {
+					l[m][e] += __shfl_xor_sync(~0u, l[m][e], 1);
+					l[m][e] += __shfl_xor_sync(~0u, l[m][e], 2);
+					if (t4 == 0) s_ml[warp * RT + m * 16 + e * 8 + g] = make_float2(mr[m][e], l[m][e]);
+				}
+			__syncthreads();
+			const bool complete = end && from_start;
+			float *slot = complete ? nullptr : p.part + (2ll * blockIdx.x + (from_start ? 1 : 0)) * A::SLOT;
+			const int b = c.b, h = c.h, r0 = c.r * RT;
+#pragma unroll
+			for (int m = 0; m < MT; m++) {
+				float *mine = (float *)(smem + (sk - s0)); // the stage just worked on
+#pragma unroll
+				for (int e = 0; e < 2; e++) {
+					const int row = e * 8 + g;
+					float top = -INFINITY;
+#pragma unroll
+					for (int w = 0; w < 4; w++) top = fmaxf(top, s_ml[w * RT + m * 16 + row].x);
+					const float a = mr[m][e] == -INFINITY ? 0 : ex2(mr[m][e] - top);
+#pragma unroll
+					for (int d = 0; d < DP / 8; d++)
+						*(float2 *)(mine + row * DP + ((d * 8) ^ (g * 8)) + 2 * t4) = make_float2(a == 0 ? 0 : o[m][d][2 * e] * a, a == 0 ? 0 : o[m][d][2 * e + 1] * a);
+				}
+				__syncthreads();
+				for (int x = tid; x < 16 * DP / 4; x += 128) {
+					const int row = x / (DP / 4), col = x % (DP / 4) * 4, r = m * 16 + row;
+					float top = -INFINITY, sum = 0;
+#pragma unroll
+					for (int w = 0; w < 4; w++) top = fmaxf(top, s_ml[w * RT + r].x);
+					float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+					for (int w = 0; w < 4; w++) {
+						const float2 ml = s_ml[w * RT + r];
+						sum += ml.x == -INFINITY ? ml.y : ml.y * ex2(ml.x - top);
+						const float4 y = *(const float4 *)(smem + (ring - s0) + ((w - warp) * NST + stage) * A::STAGE + (row * DP + (col ^ ((row & 7) * 8))) * 4);
+						v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+					}
+					if (complete) {
+						if (r0 + r < rows) store_row4<T>(p, b, h, r0 + r, col, cnt, v, top, sum);
+					} else {
+						*(float4 *)(slot + r * DP + col) = v;
+						if (col == 0) slot[RT * DP + r] = top, slot[RT * DP + RT + r] = sum;
+					}
+				}
+				__syncthreads();
+			}
+			if (!end && from_start && tid == 0) // the unit goes on in the CTAs after this one
+				p.split[blockIdx.x] = make_int4(b, h, c.r, (int)((pos + i + (c.all - 1 - c.tile)) / share));
+			first = true;
+		}
+		__syncwarp(); // every lane is done with this stage
+		stage = (stage + 1) % NST;
+		cursor_next<TK>(p, c, extra);
+	}
+	cp_wait<0>();
+}
+
+// The parts of the units that several CTAs shared: a warp per row, the parts in CTA order.
+template <class T, int DP, int RT>
+__global__ void __launch_bounds__(128) k_attn_join(const AttnArgs p)
+{
+	constexpr int SLOT = RT * DP + 2 * RT, N = DP / 128 ? DP / 128 : 1;
+	pdl_launch();
+	pdl_wait();
+	const int4 s = p.split[blockIdx.x];
+	if (s.x < 0) return;
+	const int lane = threadIdx.x & 31, rows = p.d.tokens * p.d.group, cnt = p.d.drafted(s.x);
+	const int parts = s.w - (int)blockIdx.x + 1;
+	auto part = [&](int i) { return p.part + (2ll * (blockIdx.x + i) + (i == 0)) * SLOT; };
+	for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < RT && s.z * RT + r < rows; r += gridDim.y * 4) {
+		float top = -INFINITY, l = 0;
+		for (int i = lane; i < parts; i += 32) top = fmaxf(top, part(i)[RT * DP + r]);
+#pragma unroll
+		for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+		float4 v[N];
+#pragma unroll
+		for (int x = 0; x < N; x++) v[x] = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+		for (int i = 0; i < parts; i++) {
+			const float *q = part(i);
+			const float m = q[RT * DP + r], a = m == -INFINITY ? 0 : ex2(m - top);
+			l += m == -INFINITY ? q[RT * DP + RT + r] : q[RT * DP + RT + r] * a;
+#pragma unroll
+			for (int x = 0; x < N; x++) {
+				const int col = x * 128 + lane * 4;
+				if (col >= DP || a == 0) continue;
+				const float4 y = *(const float4 *)(q + r * DP + col);
+				v[x].x += y.x * a, v[x].y += y.y * a, v[x].z += y.z * a, v[x].w += y.w * a;
+			}
+		}
+#pragma unroll
+		for (int x = 0; x < N; x++)
+			if (x * 128 + lane * 4 < DP) store_row4<T>(p, s.x, s.y, s.z * RT + r, x * 128 + lane * 4, cnt, v[x], top, l);
+	}
+}
+
+// How a call is cut.
+struct AttnPlan {
+	int dp, mt, row_tiles, whole, least, grid, sms, dev;
+	size_t slot; // bytes of a partial result
+	size_t bytes() const { return whole ? 0 : (size_t)grid * (2 * slot + sizeof(int4)); }
+};
+
+// Launches a planned call; T is the element type.
+template <class T> int attn_type(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st);
+
+template <class T, int DP, int MT>
+static int attn_run(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
+{
+	using A = AttnTile<T, DP, MT>;
+	static std::atomic<unsigned long long> done{0};
+	int rc = pg_smem(k_tree_attn<T, DP, MT>, A::SMEM, pl.dev, done);
+	if (rc) return rc;
+	TGC_CUDA(launch_pdl(k_tree_attn<T, DP, MT>, dim3(pl.grid), dim3(128), A::SMEM, st, p));
+	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT / 4), dim3(128), 0, st, p));
+	return TG_CUDA_OK;
+}
+
+template <class T>
+int attn_type(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
+{
+	if (pl.dp == 256) return attn_run<T, 256, 1>(p, pl, st);
+	if (pl.dp == 128) return pl.mt == 1 ? attn_run<T, 128, 1>(p, pl, st) : attn_run<T, 128, 2>(p, pl, st);
+	return pl.mt == 1 ? attn_run<T, 64, 1>(p, pl, st) : attn_run<T, 64, 2>(p, pl, st);
+}
+
+} // namespace tgc
