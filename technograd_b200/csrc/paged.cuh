@@ -11,9 +11,9 @@
 
 namespace tgc {
 
-// What a paged-cache kernel can meet in device data: each has a word of its own in mapped host
+// What a paged-cache kernel can meet in device data, or a wait of its own that gave up: each has a word of its own in mapped host
 // memory, set by a plain store (no read-modify-write over the bus) and cleared by the next call.
-enum : int { PG_LEN, PG_PAGE, PG_PATH, PG_ROOM, PG_WORDS };
+enum : int { PG_LEN, PG_PAGE, PG_PATH, PG_ROOM, PG_WAIT, PG_WORDS };
 
 // A pool in bytes: positions are table lookups, so every offset is 64-bit.
 struct PgCache {

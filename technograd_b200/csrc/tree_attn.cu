@@ -7,23 +7,27 @@ extern template int attn_type<float>(const AttnArgs &, const AttnPlan &, cudaStr
 extern template int attn_type<__half>(const AttnArgs &, const AttnPlan &, cudaStream_t);
 extern template int attn_type<__nv_bfloat16>(const AttnArgs &, const AttnPlan &, cudaStream_t);
 
-constexpr int ATTN_WHOLE = 4; // tiles: a unit of at most so many is one CTA's (below: their shares would be smaller than a CTA's set-up)
+// A unit of at most so many keys is one CTA's: smaller shares would cost more in set-up and joining.
+constexpr int ATTN_WHOLE = 256;
+// From so many query rows per key head on, 16-bit caches take the 128-row tiles of tree_attn_tc.cuh.
+constexpr int ATTN_TC_ROWS = 32;
 
 static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o)
 {
 	int rc = pg_sms(who, &o->dev, &o->sms);
 	if (rc) return rc;
-	const int rows = d.tokens * d.group, tk = c->type == TG_CUDA_F32 ? 32 : 64;
+	const int rows = d.tokens * d.group;
 	o->dp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+	o->tc = c->type != TG_CUDA_F32 && o->dp <= 128 && rows > ATTN_TC_ROWS;
 	o->mt = rows <= 16 || o->dp == 256 ? 1 : 2; // 256 dimensions of 32 rows do not fit in registers
-	const int rt = 16 * o->mt;
+	const int rt = o->tc ? 128 : 16 * o->mt, tk = o->tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
 	o->row_tiles = (rows + rt - 1) / rt;
 	const long long units = (long long)c->seqs * c->nkv * o->row_tiles;
 	const long long tiles = (c->max_len + tk - 1) / tk + (d.tokens + tk - 1) / tk;
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
-	o->whole = tiles <= ATTN_WHOLE, o->least = 2;
+	o->whole = tiles * tk <= ATTN_WHOLE, o->least = 128 / tk;
 	o->slot = (size_t)(rt * o->dp + 2 * rt) * 4;
-	const long long shares = (units * tiles + o->least - 1) / o->least, wave = (long long)o->sms * (o->dp == 256 ? 1 : 2);
+	const long long shares = (units * tiles + o->least - 1) / o->least, wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : 2);
 	o->grid = (int)(o->whole ? units : shares < wave ? shares : wave);
 	return TG_CUDA_OK;
 }

@@ -80,8 +80,9 @@ __device__ __forceinline__ void cursor_next(const AttnArgs &p, AttnCursor &c, in
 	if (++c.b < p.seqs) cursor_seq<TK>(p, c, extra);
 }
 
-// Sum of a value over the CTA's 128 threads, and the sum over the threads before this one.
-__device__ __forceinline__ long long scan128(long long v, long long *s, long long &before)
+// Sum of a value over the CTA's NW warps, and the sum over the threads before this one.
+template <int NW>
+__device__ __forceinline__ long long block_scan(long long v, long long *s, long long &before)
 {
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 	long long x = v;
@@ -96,11 +97,52 @@ __device__ __forceinline__ long long scan128(long long v, long long *s, long lon
 	before = x - v;
 	long long all = 0;
 #pragma unroll
-	for (int w = 0; w < 4; w++) {
+	for (int w = 0; w < NW; w++) {
 		if (w < warp) before += s[w];
 		all += s[w];
 	}
 	return all;
+}
+
+// What a CTA works on: `left` tiles from place c of the list. s: NW + 2 words of shared memory.
+// False: nothing. share and pos are for shares only: tiles per CTA, and c's place in the whole list.
+template <int TK, int NW>
+__device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int extra, AttnCursor &c, long long &left, long long &pos, long long &share)
+{
+	if (p.whole) {
+		c.r = blockIdx.x % p.row_tiles;
+		c.h = blockIdx.x / p.row_tiles % p.c.nkv;
+		c.b = blockIdx.x / p.row_tiles / p.c.nkv;
+		c.tile = 0;
+		cursor_seq<TK>(p, c, extra);
+		left = c.all, pos = 0, share = 1;
+		return true;
+	}
+	const int per = p.c.nkv * p.row_tiles;
+	auto weight = [&](int b) -> long long { return b < p.seqs ? (((long long)p.c.length(b) + TK - 1) / TK + extra) * per : 0; };
+	long long mine = 0, before, all;
+	for (int b = threadIdx.x; b < p.seqs; b += 32 * NW) mine += weight(b);
+	all = block_scan<NW>(mine, s, before);
+	share = (all + gridDim.x - 1) / gridDim.x;
+	if (share < p.least) share = p.least;
+	pos = share * blockIdx.x;
+	if (threadIdx.x == 0) p.split[blockIdx.x].x = -1;
+	if (pos >= all) return false;
+	left = all - pos < share ? all - pos : share;
+	long long base = 0;
+	for (int b0 = 0;; b0 += 32 * NW) { // ends: pos < all
+		const long long w = weight(b0 + threadIdx.x), sum = block_scan<NW>(w, s, before);
+		if (pos >= base + before && pos < base + before + w) s[NW] = b0 + threadIdx.x, s[NW + 1] = base + before;
+		base += sum;
+		if (pos < base) break;
+	}
+	__syncthreads();
+	c.b = (int)s[NW];
+	cursor_seq<TK>(p, c, extra);
+	const long long off = pos - s[NW + 1], u = off / c.all;
+	c.tile = (int)(off - u * c.all);
+	c.h = (int)(u / p.row_tiles), c.r = (int)(u % p.row_tiles);
+	return true;
 }
 
 // o (already over l, or a partial's) of 4 columns
@@ -141,42 +183,9 @@ __global__ void __launch_bounds__(128) k_tree_attn(const AttnArgs p)
 	pdl_launch();
 	pdl_wait();
 
-	// ---- this CTA's share
 	AttnCursor c; // the tile being worked on; f, below: the next to be fetched
-	long long left, pos = 0, share = 0;
-	if (p.whole) {
-		c.r = blockIdx.x % p.row_tiles;
-		c.h = blockIdx.x / p.row_tiles % p.c.nkv;
-		c.b = blockIdx.x / p.row_tiles / p.c.nkv;
-		c.tile = 0;
-		cursor_seq<TK>(p, c, extra);
-		left = c.all;
-	} else {
-		const int per = p.c.nkv * p.row_tiles;
-		auto weight = [&](int b) -> long long { return b < p.seqs ? (((long long)p.c.length(b) + TK - 1) / TK + extra) * per : 0; };
-		long long mine = 0, before, all;
-		for (int b = tid; b < p.seqs; b += 128) mine += weight(b);
-		all = scan128(mine, s_scan, before);
-		share = (all + gridDim.x - 1) / gridDim.x;
-		if (share < p.least) share = p.least;
-		pos = share * blockIdx.x;
-		if (tid == 0) p.split[blockIdx.x].x = -1;
-		if (pos >= all) return;
-		left = all - pos < share ? all - pos : share;
-		long long base = 0;
-		for (int b0 = 0;; b0 += 128) { // ends: pos < all
-			const long long w = weight(b0 + tid), sum = scan128(w, s_scan, before);
-			if (pos >= base + before && pos < base + before + w) s_scan[4] = b0 + tid, s_scan[5] = base + before;
-			base += sum;
-			if (pos < base) break;
-		}
-		__syncthreads();
-		c.b = (int)s_scan[4];
-		cursor_seq<TK>(p, c, extra);
-		const long long off = pos - s_scan[5], u = off / c.all;
-		c.tile = (int)(off - u * c.all);
-		c.h = (int)(u / p.row_tiles), c.r = (int)(u % p.row_tiles);
-	}
+	long long left, pos, share;
+	if (!attn_share<TK, 4>(p, s_scan, extra, c, left, pos, share)) return;
 
 	// ---- fetching: lane i < KW holds the address of the tile's row i
 	AttnCursor f = c;
@@ -450,32 +459,12 @@ __global__ void __launch_bounds__(128) k_attn_join(const AttnArgs p)
 
 // How a call is cut.
 struct AttnPlan {
-	int dp, mt, row_tiles, whole, least, grid, sms, dev;
+	int dp, mt, row_tiles, whole, least, grid, sms, dev, tc; // mt: 16-row products of a tile; tc: 128-row tiles on tcgen05
 	size_t slot; // bytes of a partial result
 	size_t bytes() const { return whole ? 0 : (size_t)grid * (2 * slot + sizeof(int4)); }
 };
 
 // Launches a planned call; T is the element type.
 template <class T> int attn_type(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st);
-
-template <class T, int DP, int MT>
-static int attn_run(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
-{
-	using A = AttnTile<T, DP, MT>;
-	static std::atomic<unsigned long long> done{0};
-	int rc = pg_smem(k_tree_attn<T, DP, MT>, A::SMEM, pl.dev, done);
-	if (rc) return rc;
-	TGC_CUDA(launch_pdl(k_tree_attn<T, DP, MT>, dim3(pl.grid), dim3(128), A::SMEM, st, p));
-	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT / 4), dim3(128), 0, st, p));
-	return TG_CUDA_OK;
-}
-
-template <class T>
-int attn_type(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
-{
-	if (pl.dp == 256) return attn_run<T, 256, 1>(p, pl, st);
-	if (pl.dp == 128) return pl.mt == 1 ? attn_run<T, 128, 1>(p, pl, st) : attn_run<T, 128, 2>(p, pl, st);
-	return pl.mt == 1 ? attn_run<T, 64, 1>(p, pl, st) : attn_run<T, 64, 2>(p, pl, st);
-}
 
 } // namespace tgc

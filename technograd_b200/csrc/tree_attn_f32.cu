@@ -1,5 +1,5 @@
 // tree_attn_f32.cu -- attention of drafted tokens, f32 caches.
-#include "tree_attn.cuh"
+#include "tree_attn_run.cuh"
 
 namespace tgc {
 template int attn_type<float>(const AttnArgs &, const AttnPlan &, cudaStream_t);

@@ -1,0 +1,44 @@
+// tree_attn_run.cuh -- the launches of a planned attention call, instantiated per element type.
+#pragma once
+
+#include "tree_attn.cuh"
+#include "tree_attn_tc.cuh"
+
+namespace tgc {
+
+template <class T, int DP, int MT>
+static int attn_run(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
+{
+	using A = AttnTile<T, DP, MT>;
+	static std::atomic<unsigned long long> done{0};
+	int rc = pg_smem(k_tree_attn<T, DP, MT>, A::SMEM, pl.dev, done);
+	if (rc) return rc;
+	TGC_CUDA(launch_pdl(k_tree_attn<T, DP, MT>, dim3(pl.grid), dim3(128), A::SMEM, st, p));
+	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT / 4), dim3(128), 0, st, p));
+	return TG_CUDA_OK;
+}
+
+template <class T, int DP>
+static int attn_run_tc(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
+{
+	using A = TaTile<DP>;
+	static std::atomic<unsigned long long> done{0};
+	int rc = pg_smem(k_tree_attn_tc<T, DP>, A::SMEM, pl.dev, done);
+	if (rc) return rc;
+	TGC_CUDA(launch_pdl(k_tree_attn_tc<T, DP>, dim3(pl.grid), dim3(A::THREADS), A::SMEM, st, p));
+	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT / 4), dim3(128), 0, st, p));
+	return TG_CUDA_OK;
+}
+
+template <class T>
+int attn_type(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
+{
+	if constexpr (sizeof(T) == 2) {
+		if (pl.tc) return pl.dp == 128 ? attn_run_tc<T, 128>(p, pl, st) : attn_run_tc<T, 64>(p, pl, st);
+	}
+	if (pl.dp == 256) return attn_run<T, 256, 1>(p, pl, st);
+	if (pl.dp == 128) return pl.mt == 1 ? attn_run<T, 128, 1>(p, pl, st) : attn_run<T, 128, 2>(p, pl, st);
+	return pl.mt == 1 ? attn_run<T, 64, 1>(p, pl, st) : attn_run<T, 64, 2>(p, pl, st);
+}
+
+} // namespace tgc

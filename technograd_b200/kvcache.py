@@ -27,17 +27,28 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _tensor(name: str, x, dtype, shape, device, contiguous: bool = True) -> None:
-    """x is a tensor of this type, shape (None = any extent) and device."""
-    if x.dtype is not dtype or x.device != device or len(x.shape) != len(shape) or \
-            any(w is not None and w != n for w, n in zip(shape, x.shape)) or (contiguous and not x.is_contiguous()):
-        raise ValueError(f"{name}: expected {'a contiguous' if contiguous else 'a'} {dtype} tensor {tuple(shape)} on {device}, got "
-                         f"{x.dtype} {tuple(x.shape)} strides {x.stride()} on {x.device}")
+def _check(name: str, x, dtype, shape, index: int) -> None:
+    """x is a contiguous tensor of this type and shape on CUDA device `index`."""
+    if x.dtype is not dtype or x.shape != shape or x.get_device() != index or not x.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on cuda:{index}, got {x.dtype} "
+                         f"{tuple(x.shape)} strides {x.stride()} on {x.device}")
 
 
-def _stream(device) -> int:
-    _need(device.index == torch.cuda.current_device(), f"the tensors are on {device}, which is not the current device")
-    return torch.cuda.current_stream().cuda_stream
+def _weights(name: str, x, cache: "PagedKV", least: int) -> tuple:
+    """x is f32 [seqs, nkv, >= least] on the cache's device, rows contiguous; its strides."""
+    n = x.shape
+    if x.dtype is not torch.float32 or x.get_device() != cache.index or len(n) != 3 or n[0] != cache.seqs or n[1] != cache.nkv or \
+            n[2] < least or (n[2] > 1 and x.stride(2) != 1):
+        raise ValueError(f"{name}: expected a float32 tensor [{cache.seqs}, {cache.nkv}, at least {least}] on cuda:{cache.index} with contiguous "
+                         f"rows, got {x.dtype} {tuple(n)} strides {x.stride()} on {x.device}")
+    return x.stride()
+
+
+def _stream(cache: "PagedKV") -> int:
+    """The current stream of the cache's device, which has to be the current one."""
+    if cache.index != torch.cuda.current_device():
+        raise ValueError(f"the cache is on cuda:{cache.index}, which is not the current device")
+    return torch._C._cuda_getCurrentRawStream(cache.index)  # torch.cuda.current_stream's handle without its object
 
 
 class PagedKV:
@@ -51,17 +62,21 @@ class PagedKV:
         _need(k.shape[3] <= 1 or k.stride(3) == 1, "k: the head dimension must be contiguous")
         _need(v.dtype is k.dtype and v.device == k.device and v.shape == k.shape and v.stride() == k.stride(),
               "v: expected k's type, device, shape and strides")
-        _tensor("table", table, torch.int32, (None, None), k.device)
-        _tensor("lens", lens, torch.int32, (table.shape[0],), k.device)
+        self.index = k.get_device()
+        _need(table.dim() == 2, "table: expected [seqs, cols]")
+        _check("table", table, torch.int32, table.shape, self.index)
+        _check("lens", lens, torch.int32, table.shape[:1], self.index)
         self.k, self.v, self.table, self.lens = k, v, table, lens
         self.device, self.dtype = k.device, k.dtype
         self.seqs, cols = table.shape
         pages, self.nkv, self.page, self.head_dim = k.shape
+        self.scale = 1 / math.sqrt(self.head_dim) if self.head_dim else 1.0  # of the scores, where a call gives none
         self.max_len = self.page * cols if max_len is None else int(max_len)
         s = _lib.Kv(_TYPES[k.dtype], self.seqs, self.nkv, self.head_dim, self.page, pages, cols, self.max_len,
                     k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), table.data_ptr(), lens.data_ptr())
         self._struct = s
         self._at = C.addressof(s)
+        self._work = {}  # (tokens, nq) -> bytes of tree_attention's scratch
 
     def with_lens(self, lens: torch.Tensor, max_len: int | None = None) -> "PagedKV":
         """The same pages with other lengths (what `commit` returned)."""
@@ -69,30 +84,28 @@ class PagedKV:
 
 
 def _drafts(cache: PagedKV, q, k, v, mask, count, scale):
-    B, T = k.shape[0], k.shape[1]
-    nkv, dim, dt, dev = cache.nkv, cache.head_dim, cache.dtype, cache.device
-    _tensor("k", k, dt, (cache.seqs, None, nkv, dim), dev, False)
-    kb, kt, kh, kd = k.stride()
-    _need(kd == 1 or dim == 1, "k: the head dimension must be contiguous")
-    d = _lib.Drafts()
-    d.tokens, d.k, d.kv_seq, d.kv_tok, d.kv_head = T, k.data_ptr(), kb, kt, kh
-    if v is not None:
-        _tensor("v", v, dt, k.shape, dev, False)
-        _need(v.stride() == (kb, kt, kh, kd), "v: expected k's strides")
-        d.v = v.data_ptr()
+    """The C description of drafted tokens, checked."""
+    index, dt, n, dim = cache.index, cache.dtype, k.shape, cache.head_dim
+    sk = k.stride()
+    if k.dtype is not dt or k.get_device() != index or len(n) != 4 or n[0] != cache.seqs or n[2] != cache.nkv or n[3] != dim or sk[3] != 1:
+        raise ValueError(f"k: expected a {dt} tensor [{cache.seqs}, tokens, {cache.nkv}, {dim}] on cuda:{index} with contiguous rows, got {k.dtype} "
+                         f"{tuple(n)} strides {sk} on {k.device}")
+    if v is not None and (v.dtype is not dt or v.get_device() != index or v.shape != n or v.stride() != sk):
+        raise ValueError(f"v: expected k's type, device, shape and strides, got {v.dtype} {tuple(v.shape)} strides {v.stride()} on {v.device}")
+    nq, sq = 0, (0, 0, 0, 1)
     if q is not None:
-        _tensor("q", q, dt, (B, T, None, dim), dev, False)
-        d.nq, d.q = q.shape[2], q.data_ptr()
-        d.q_seq, d.q_tok, d.q_head, qd = q.stride()
-        _need(qd == 1 or dim == 1, "q: the head dimension must be contiguous")
+        m, sq = q.shape, q.stride()
+        if q.dtype is not dt or q.get_device() != index or len(m) != 4 or m[0] != n[0] or m[1] != n[1] or m[3] != dim or sq[3] != 1:
+            raise ValueError(f"q: expected a {dt} tensor [{n[0]}, {n[1]}, heads, {dim}] on cuda:{index} with contiguous rows, got {q.dtype} "
+                             f"{tuple(m)} strides {sq} on {q.device}")
+        nq = m[2]
     if mask is not None:
-        _tensor("mask", mask, torch.int64, (B, T), dev)
-        d.mask = mask.data_ptr()
+        _check("mask", mask, torch.int64, n[:2], index)
     if count is not None:
-        _tensor("count", count, torch.int32, (B,), dev)
-        d.count = count.data_ptr()
-    d.scale = 1 / math.sqrt(dim) if scale is None else scale
-    return d
+        _check("count", count, torch.int32, n[:1], index)
+    return _lib.Drafts(n[1], nq, cache.scale if scale is None else scale, None if q is None else q.data_ptr(), sq[0], sq[1], sq[2],
+                       k.data_ptr(), None if v is None else v.data_ptr(), sk[0], sk[1], sk[2],
+                       None if mask is None else mask.data_ptr(), None if count is None else count.data_ptr())
 
 
 def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float | None = None):
@@ -102,17 +115,20 @@ def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float 
     tokens. mask int64 [seqs, tokens]: bit u of an entry = the token attends to drafted token u (None:
     a chain). count int32 [seqs]: tokens drafted (None: all). Returns (out as q, lse f32 [seqs, tokens,
     nq]); a token that sees nothing has out 0 and lse -inf."""
-    d = _drafts(cache, q, k, v, mask, count, scale)
-    stream, L = _stream(cache.device), _lib.lib()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    at = C.byref(d)
-    size = L.tg_cuda_tree_attn_workspace(cache._at, at)
-    if size < 0:
-        _lib.check(size)
-    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    ob, ot, oh, _ = out.stride()
-    _lib.check(L.tg_cuda_tree_attn(cache._at, at, out.data_ptr(), ob, ot, oh, lse.data_ptr(), work.data_ptr() if size else None, size, stream))
+    d = C.byref(_drafts(cache, q, k, v, mask, count, scale))
+    stream, L, shape = _stream(cache), _lib.lib(), q.shape
+    out = torch.empty_like(q)
+    lse = q.new_empty(shape[:3], dtype=torch.float32)
+    so = out.stride()
+    size = cache._work.get(shape[1:3])
+    if size is None:
+        size = L.tg_cuda_tree_attn_workspace(cache._at, d)
+        if size < 0:
+            _lib.check(size)
+        cache._work[shape[1:3]] = size
+    work = q.new_empty(size, dtype=torch.uint8) if size else None
+    _lib.check(L.tg_cuda_tree_attn(cache._at, d, out.data_ptr(), so[0], so[1], so[2], lse.data_ptr(), work.data_ptr() if size else None,
+                                   size, stream))
     return out, lse
 
 
@@ -123,22 +139,17 @@ def attention_weights(cache: PagedKV, q, k, lse, mask=None, count=None, select=N
     tokens that count, as bits (None: all). acc f32 [seqs, nkv, >= max_len]: what the cached
     positions had before (None: zeros). Returns (acc + weight [seqs, nkv, max_len], zero past a
     sequence's length; the drafted tokens' own weight [seqs, nkv, tokens])."""
-    d = _drafts(cache, q, k, None, mask, count, scale)
-    B, T, nq = q.shape[:3]
-    dev = cache.device
-    _tensor("lse", lse, torch.float32, (B, T, nq), dev)
+    d = C.byref(_drafts(cache, q, k, None, mask, count, scale))
+    n = q.shape
+    _check("lse", lse, torch.float32, n[:3], cache.index)
     if select is not None:
-        _tensor("select", select, torch.int64, (B,), dev)
-    ab = ah = 0
-    if acc is not None:
-        _tensor("acc", acc, torch.float32, (B, cache.nkv, None), dev, False)
-        _need(acc.shape[2] >= cache.max_len and (acc.shape[2] <= 1 or acc.stride(2) == 1), "acc: expected contiguous rows of at least max_len")
-        ab, ah, _ = acc.stride()
-    out = torch.empty((B, cache.nkv, cache.max_len), dtype=torch.float32, device=dev)
-    fresh = torch.empty((B, cache.nkv, T), dtype=torch.float32, device=dev)
-    _lib.check(_lib.lib().tg_cuda_attn_weights(cache._at, C.byref(d), lse.data_ptr(), select.data_ptr() if select is not None else None,
-                                               acc.data_ptr() if acc is not None else None, ab, ah, out.data_ptr(), fresh.data_ptr(),
-                                               _stream(dev)))
+        _check("select", select, torch.int64, n[:1], cache.index)
+    sa = (0, 0) if acc is None else _weights("acc", acc, cache, cache.max_len)
+    out = lse.new_empty((n[0], cache.nkv, cache.max_len))
+    fresh = lse.new_empty((n[0], cache.nkv, n[1]))
+    _lib.check(_lib.lib().tg_cuda_attn_weights(cache._at, d, lse.data_ptr(), None if select is None else select.data_ptr(),
+                                               None if acc is None else acc.data_ptr(), sa[0], sa[1], out.data_ptr(), fresh.data_ptr(),
+                                               _stream(cache)))
     return out, fresh
 
 
@@ -147,22 +158,19 @@ def commit(cache: PagedKV, k, v, count, path=None, new=None, acc=None):
     path[b, i] (path int32 [seqs, tokens]; None: row i) for i < count[b]. With new (the drafted tokens'
     weight from attention_weights) and acc f32 [seqs, nkv, cols], acc[b, h, lens + i] = new[b, h, path[b, i]] too.
     Returns the new lengths; the pages and acc are written in place. Any number of tokens."""
-    d = _drafts(cache, None, k, v, None, count, 1.0)
-    dev, T = cache.device, k.shape[1]
+    d = C.byref(_drafts(cache, None, k, v, None, count, 1.0))
+    T = k.shape[1]
     if path is not None:
-        _tensor("path", path, torch.int32, (cache.seqs, T), dev)
+        _check("path", path, torch.int32, (cache.seqs, T), cache.index)
     _need((new is None) == (acc is None), "new and acc: both or neither")
-    ab = ah = cols = 0
+    sa = (0, 0)
     if acc is not None:
-        _tensor("new", new, torch.float32, (cache.seqs, cache.nkv, T), dev)
-        _tensor("acc", acc, torch.float32, (cache.seqs, cache.nkv, None), dev, False)
-        cols = acc.shape[2]
-        _need(cols <= 1 or acc.stride(2) == 1, "acc: expected contiguous rows")
-        ab, ah, _ = acc.stride()
+        _check("new", new, torch.float32, (cache.seqs, cache.nkv, T), cache.index)
+        sa = _weights("acc", acc, cache, 0)
     lens = torch.empty_like(cache.lens)
-    _lib.check(_lib.lib().tg_cuda_kv_commit(cache._at, C.byref(d), path.data_ptr() if path is not None else None, lens.data_ptr(),
-                                            new.data_ptr() if acc is not None else None, acc.data_ptr() if acc is not None else None,
-                                            ab, ah, cols, _stream(dev)))
+    _lib.check(_lib.lib().tg_cuda_kv_commit(cache._at, d, None if path is None else path.data_ptr(), lens.data_ptr(),
+                                            None if acc is None else new.data_ptr(), None if acc is None else acc.data_ptr(), sa[0], sa[1],
+                                            0 if acc is None else acc.shape[2], _stream(cache)))
     return lens
 
 
@@ -172,16 +180,13 @@ def evict(cache: PagedKV, dst: PagedKV, acc, budget: int, recent: int = 0, sink:
     the lower position; NaN last). dst: pages that cache's sequences do not hold, of the same or other
     pools. Returns (kept positions int32 [seqs, nkv, budget], -1 past the last; their acc, 0 past
     the last; the lengths in dst)."""
-    dev = cache.device
-    _need(dst.device == dev and dst.dtype is cache.dtype, "dst: expected the cache's type and device")
-    _tensor("acc", acc, torch.float32, (cache.seqs, cache.nkv, None), dev, False)
-    _need(acc.shape[2] >= cache.max_len and (acc.shape[2] <= 1 or acc.stride(2) == 1), "acc: expected contiguous rows of at least max_len")
+    _need(dst.index == cache.index and dst.dtype is cache.dtype, "dst: expected the cache's type and device")
     _need(budget > 0, "budget: expected at least 1")
+    sa = _weights("acc", acc, cache, cache.max_len)
     shape = (cache.seqs, cache.nkv, budget)
-    keep = torch.empty(shape, dtype=torch.int32, device=dev)
-    out = torch.empty(shape, dtype=torch.float32, device=dev)
+    keep = cache.lens.new_empty(shape)
+    out = acc.new_empty(shape)
     lens = torch.empty_like(cache.lens)
-    ab, ah, _ = acc.stride()
-    _lib.check(_lib.lib().tg_cuda_kv_evict(cache._at, dst._at, acc.data_ptr(), ab, ah, budget, recent, sink, keep.data_ptr(), out.data_ptr(),
-                                           lens.data_ptr(), _stream(dev)))
+    _lib.check(_lib.lib().tg_cuda_kv_evict(cache._at, dst._at, acc.data_ptr(), sa[0], sa[1], budget, recent, sink, keep.data_ptr(), out.data_ptr(),
+                                           lens.data_ptr(), _stream(cache)))
     return keep, out, lens
