@@ -72,6 +72,11 @@ int pg_cache(const char *who, const tg_cuda_kv *c, PgCache *o)
 		return set_err(TG_CUDA_EINVAL, "%s: NULL pointer in the cache", who);
 	if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) || ((c->page_stride | c->head_stride | c->pos_stride) * e & 15))
 		return set_err(TG_CUDA_EINVAL, "%s: cache rows must start on 16-byte boundaries", who);
+	if (c->page_stride < 0 || c->head_stride < 0 || c->pos_stride < 0) return set_err(TG_CUDA_EINVAL, "%s: negative strides", who);
+	o->shift = 4;
+	while (o->shift < 30 && !(((c->page_stride | c->pos_stride) * e) >> o->shift & 1)) o->shift++;
+	if (c->pages && ((unsigned __int128)c->page_stride * (c->pages - 1) + (unsigned __int128)c->pos_stride * (c->page - 1)) * e >> o->shift >= PG_NONE)
+		return set_err(TG_CUDA_EINVAL, "%s: a pool of 2^32 rows' alignments of %d bytes or more", who, 1 << o->shift);
 	o->k = (char *)c->k, o->v = (char *)c->v, o->table = c->table, o->len = c->len;
 	o->page_b = c->page_stride * e, o->head_b = c->head_stride * e, o->pos_b = c->pos_stride * e;
 	o->page = c->page, o->pages = c->table && c->k && c->v ? c->pages : 0, o->cols = c->table_cols, o->max_len = c->max_len;

@@ -15,12 +15,15 @@ namespace tgc {
 // memory, set by a plain store (no read-modify-write over the bus) and cleared by the next call.
 enum : int { PG_LEN, PG_PAGE, PG_PATH, PG_ROOM, PG_WAIT, PG_WORDS };
 
+constexpr uint32_t PG_NONE = 0xffffffffu;
+
 // A pool in bytes: positions are table lookups, so every offset is 64-bit.
 struct PgCache {
 	char *k, *v;
 	const int *table, *len;
 	long long page_b, head_b, pos_b; // strides in bytes
 	int page, pages, cols, max_len, nkv, dim;
+	int shift;                       // rows lie at multiples of 2^shift bytes (at least 16)
 	int *status;                     // PG_WORDS words, written only on an error
 
 	__device__ __forceinline__ void report(int what) const { *(volatile int *)(status + what) = 1; }
@@ -33,12 +36,19 @@ struct PgCache {
 	// byte offset of a sequence's row (head 0) at position p, -1 where the page number is not one
 	__device__ __forceinline__ long long row(const int *tab, int p) const
 	{
-		const int c = p / page, g = tab[c];
+		const int c = p / page;
+		const uint32_t o = at(tab[c], p - c * page);
+		return o == PG_NONE ? -1 : (long long)((unsigned long long)o << shift);
+	}
+	// the same in units of 2^shift bytes for row r of page number g, which the host has checked to fit 32 bits
+	// in the whole pool, PG_NONE for none: half a register pair's price where lanes pass addresses on
+	__device__ __forceinline__ uint32_t at(int g, int r) const
+	{
 		if ((unsigned)g >= (unsigned)pages) {
 			report(PG_PAGE);
-			return -1;
+			return PG_NONE;
 		}
-		return (long long)g * page_b + (long long)(p - c * page) * pos_b;
+		return (uint32_t)(((long long)g * page_b + (long long)r * pos_b) >> shift);
 	}
 };
 

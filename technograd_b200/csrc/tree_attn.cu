@@ -12,6 +12,8 @@ constexpr int ATTN_WHOLE = 256;
 // From so many query rows per key head on, 16-bit caches take the 128-row tiles of tree_attn_tc.cuh.
 constexpr int ATTN_TC_ROWS = 32;
 
+constexpr int ATTN_BEGIN = 2; // what beginning a unit costs, in tiles
+
 static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o)
 {
 	int rc = pg_sms(who, &o->dev, &o->sms);
@@ -27,7 +29,7 @@ static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, At
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
 	o->whole = tiles * tk <= ATTN_WHOLE, o->least = 128 / tk;
 	o->slot = (size_t)(rt * o->dp + 2 * rt) * 4;
-	const long long shares = (units * tiles + o->least - 1) / o->least, wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : 2);
+	const long long shares = (units * (tiles + ATTN_BEGIN) + o->least + ATTN_BEGIN - 1) / (o->least + ATTN_BEGIN), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : 2);
 	o->grid = (int)(o->whole ? units : shares < wave ? shares : wave);
 	return TG_CUDA_OK;
 }
@@ -68,7 +70,7 @@ extern "C" int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, v
 	if (need && (!work || work_bytes < (long long)need || ((uintptr_t)work & 15)))
 		return set_err(TG_CUDA_EINVAL, "%s: needs %zu bytes of 16-byte aligned scratch", who, need);
 	p.out = (char *)out, p.out_seq = out_seq * e, p.out_tok = out_tok * e, p.out_head = out_head * e, p.lse = lse;
-	p.seqs = c->seqs, p.row_tiles = pl.row_tiles, p.whole = pl.whole, p.least = pl.least;
+	p.seqs = c->seqs, p.row_tiles = pl.row_tiles, p.whole = pl.whole, p.least = pl.least, p.begin = ATTN_BEGIN;
 	p.split = (int4 *)work, p.part = (float *)((char *)work + (size_t)pl.grid * sizeof(int4));
 	cudaStream_t st = (cudaStream_t)stream;
 	return c->type == TG_CUDA_F32 ? attn_type<float>(p, pl, st) : c->type == TG_CUDA_F16 ? attn_type<__half>(p, pl, st) : attn_type<__nv_bfloat16>(p, pl, st);

@@ -18,6 +18,7 @@ struct AttnArgs {
 	int row_tiles;   // tiles of 16 * MT query rows per (sequence, kv head)
 	int whole;       // 1: a CTA per unit; 0: equal shares of the units' tiles
 	int least;       // shares: tiles per CTA at least
+	int begin;       // shares: what beginning a unit costs, in tiles
 	float *part;     // shares: partial results, two slots per CTA
 	int4 *split;     // shares: per CTA, the unit that begins in its share and ends in a later one
 };
@@ -104,8 +105,9 @@ __device__ __forceinline__ long long block_scan(long long v, long long *s, long 
 	return all;
 }
 
-// What a CTA works on: `left` tiles from place c of the list. s: NW + 2 words of shared memory.
-// False: nothing. share and pos are for shares only: tiles per CTA, and c's place in the whole list.
+// What a CTA works on: `left` tiles from place c of the list. s: NW + 4 words of shared memory.
+// False: nothing. A unit counts its tiles and p.begin more, spent before its first tile; the CTAs' shares of
+// the total are equal, share and pos being one's size and beginning.
 template <int TK, int NW>
 __device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int extra, AttnCursor &c, long long &left, long long &pos, long long &share)
 {
@@ -119,30 +121,41 @@ __device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int 
 		return true;
 	}
 	const int per = p.c.nkv * p.row_tiles;
-	auto weight = [&](int b) -> long long { return b < p.seqs ? (((long long)p.c.length(b) + TK - 1) / TK + extra) * per : 0; };
+	auto weight = [&](int b) -> long long { return b < p.seqs ? (((long long)p.c.length(b) + TK - 1) / TK + extra + p.begin) * per : 0; };
 	long long mine = 0, before, all;
 	for (int b = threadIdx.x; b < p.seqs; b += 32 * NW) mine += weight(b);
 	all = block_scan<NW>(mine, s, before);
 	share = (all + gridDim.x - 1) / gridDim.x;
-	if (share < p.least) share = p.least;
+	if (share < p.least + p.begin) share = p.least + p.begin;
 	pos = share * blockIdx.x;
 	if (threadIdx.x == 0) p.split[blockIdx.x].x = -1;
 	if (pos >= all) return false;
-	left = all - pos < share ? all - pos : share;
+	const long long to = all - pos < share ? all : pos + share; // the place after the share
 	long long base = 0;
-	for (int b0 = 0;; b0 += 32 * NW) { // ends: pos < all
-		const long long w = weight(b0 + threadIdx.x), sum = block_scan<NW>(w, s, before);
-		if (pos >= base + before && pos < base + before + w) s[NW] = b0 + threadIdx.x, s[NW + 1] = base + before;
+	for (int b0 = 0;; b0 += 32 * NW) { // ends: pos < to <= all
+		const int b = b0 + threadIdx.x;
+		const long long w = weight(b), sum = block_scan<NW>(w, s, before);
+		if (pos >= base + before && pos < base + before + w) s[NW] = b, s[NW + 1] = base + before;
+		if (to - 1 >= base + before && to - 1 < base + before + w) s[NW + 2] = b, s[NW + 3] = base + before;
 		base += sum;
-		if (pos < base) break;
+		if (to <= base) break;
 	}
 	__syncthreads();
-	c.b = (int)s[NW];
-	cursor_seq<TK>(p, c, extra);
-	const long long off = pos - s[NW + 1], u = off / c.all;
-	c.tile = (int)(off - u * c.all);
-	c.h = (int)(u / p.row_tiles), c.r = (int)(u % p.row_tiles);
-	return true;
+	// tiles before the place `off` into sequence b's units, whose units begin at place `first`
+	int u, t, in;
+	auto tiles = [&](long long b, long long first, long long off) {
+		c.b = (int)b;
+		cursor_seq<TK>(p, c, extra);
+		u = (int)(off / (c.all + p.begin));
+		in = (int)(off - (long long)u * (c.all + p.begin));
+		t = in < p.begin ? 0 : in - p.begin;
+		return first - b * per * p.begin + (long long)u * c.all + t;
+	};
+	left = tiles(s[NW + 2], s[NW + 3], to - 1 - s[NW + 3]);
+	if (in >= p.begin) left++; // the last place is a tile's
+	left -= tiles(s[NW], s[NW + 1], pos - s[NW + 1]);
+	c.tile = t, c.h = u / p.row_tiles, c.r = u % p.row_tiles;
+	return left > 0;
 }
 
 // o (already over l, or a partial's) of 4 columns
@@ -153,17 +166,31 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *d, float4 v)
 	*(uint2 *)d = make_uint2(pack16(v.x, v.y, __nv_bfloat16()), pack16(v.z, v.w, __nv_bfloat16()));
 }
 
-// A row's result: a token past the count, or one that saw nothing, has 0 and -infinity.
-template <class T>
-__device__ __forceinline__ void store_row4(const AttnArgs &p, int b, int h, int row, int col, int cnt, float4 o, float mr, float l)
+// Where a row's result goes, and what it is divided by: a token past the count, or one that saw nothing, has
+// 0 and -infinity.
+struct AttnRow {
+	char *out;
+	float *lse;
+	float f; // 1 / l, 0 for none
+	bool none;
+};
+__device__ __forceinline__ AttnRow attn_row(const AttnArgs &p, int b, int h, int row, int cnt, float l)
 {
-	const int t = row / p.d.group, j = h * p.d.group + row % p.d.group;
-	const bool none = t >= cnt || l == 0;
-	const float f = none ? 0 : 1 / l;
-	if (none) o = make_float4(0, 0, 0, 0);
-	o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-	if (col < p.c.dim) store4((T *)(p.out + b * p.out_seq + t * p.out_tok + j * p.out_head) + col, o);
-	if (col == 0) p.lse[((long long)b * p.d.tokens + t) * p.d.nq + j] = none ? -INFINITY : (mr + log2f(l)) * 0.69314718056f;
+	const int t = row / p.d.group, j = h * p.d.group + (row - t * p.d.group);
+	AttnRow x;
+	x.out = p.out + b * p.out_seq + t * p.out_tok + j * p.out_head;
+	x.lse = p.lse + ((long long)b * p.d.tokens + t) * p.d.nq + j;
+	x.none = t >= cnt || l == 0;
+	x.f = x.none ? 0 : 1 / l;
+	return x;
+}
+__device__ __forceinline__ void store_lse(const AttnRow &x, float mr, float l) { *x.lse = x.none ? -INFINITY : (mr + log2f(l)) * 0.69314718056f; }
+template <class T>
+__device__ __forceinline__ void store_row4(const AttnArgs &p, const AttnRow &x, int col, float4 o)
+{
+	if (col >= p.c.dim) return;
+	if (x.none) o = make_float4(0, 0, 0, 0);
+	store4((T *)x.out + col, make_float4(o.x * x.f, o.y * x.f, o.z * x.f, o.w * x.f));
 }
 
 template <class T, int DP, int MT>
@@ -187,38 +214,47 @@ __global__ void __launch_bounds__(128) k_tree_attn(const AttnArgs p)
 	long long left, pos, share;
 	if (!attn_share<TK, 4>(p, s_scan, extra, c, left, pos, share)) return;
 
-	// ---- fetching: lane i < KW holds the address of the tile's row i
+	// ---- fetching: lane i < KW holds the place of the tile's row i, looked up while the tile before is fetched
 	AttnCursor f = c;
 	long long fetched = 0;
+	uint32_t at = PG_NONE;
+	auto find = [&]() {
+		at = PG_NONE;
+		if (lane >= KW || fetched >= left) return;
+		if (f.tile < f.ctx) {
+			const int x = f.tile * TK + warp * KW + lane;
+			if (x < f.n) {
+				const int page = x / p.c.page;
+				at = p.c.at(p.c.table[(long long)f.b * p.c.cols + page], x - page * p.c.page);
+			}
+		} else {
+			const int u = (f.tile - f.ctx) * TK + warp * KW + lane;
+			if (u < p.d.drafted(f.b)) at = (uint32_t)(u * p.d.kv_tok >> 4);
+		}
+	};
 	auto fetch = [&](int stage) {
 		if (fetched < left) {
+			const bool ctx = f.tile < f.ctx;
+			const int sh = ctx ? p.c.shift : 4;
+			const long long head = (ctx ? f.h * p.c.head_b : f.b * p.d.kv_seq + f.h * p.d.kv_head);
+			const char *kp = (ctx ? p.c.k : p.d.k) + head, *vp = (ctx ? p.c.v : p.d.v) + head;
+			const uint32_t sk = ring + stage * A::STAGE, sv = sk + KW * P, mine = at;
+			cursor_next<TK>(p, f, extra);
 			fetched++;
-			const char *kp = nullptr, *vp = nullptr;
-			if (lane < KW) {
-				if (f.tile < f.ctx) {
-					const long long x = (long long)f.tile * TK + warp * KW + lane;
-					const long long at = x < f.n ? p.c.row(p.c.table + (long long)f.b * p.c.cols, (int)x) : -1;
-					if (at >= 0) kp = p.c.k + at + f.h * p.c.head_b, vp = p.c.v + at + f.h * p.c.head_b;
-				} else {
-					const int u = (f.tile - f.ctx) * TK + warp * KW + lane;
-					const long long at = (long long)f.b * p.d.kv_seq + (long long)u * p.d.kv_tok + f.h * p.d.kv_head;
-					if (u < p.d.drafted(f.b)) kp = p.d.k + at, vp = p.d.v + at;
-				}
-			}
-			const uint32_t sk = ring + stage * A::STAGE, sv = sk + KW * P;
+			find();
 #pragma unroll
 			for (int i = 0; i < KW * CH / 32; i++) {
-				const int x = i * 32 + lane, row = x / CH, ch = x % CH;
-				const unsigned long long kr = __shfl_sync(~0u, (unsigned long long)kp, row), vr = __shfl_sync(~0u, (unsigned long long)vp, row);
-				const uint32_t o = row * P + ((ch ^ (row & 7)) << 4);
-				const bool have = kr && ch < chunks;
-				cp16(sk + o, have ? (const char *)kr + ch * 16 : p.d.k, have);
-				cp16(sv + o, have ? (const char *)vr + ch * 16 : p.d.v, have);
+				const int row = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
+				const uint32_t r = __shfl_sync(~0u, mine, row), o = row * P + ((ch ^ (row & 7)) << 4);
+				const bool have = r != PG_NONE && ch < chunks;
+				const unsigned long long off = ((unsigned long long)r << sh) + ch * 16;
+				cp16(sk + o, have ? kp + off : p.d.k, have);
+				cp16(sv + o, have ? vp + off : p.d.v, have);
 			}
-			cursor_next<TK>(p, f, extra);
 		}
 		cp_commit();
 	};
+	find();
 
 	float o[MT][DP / 8][4], mr[MT][2], l[MT][2];
 	int cnt = 0;
@@ -399,7 +435,11 @@ __global__ void __launch_bounds__(128) k_tree_attn(const AttnArgs p)
 						v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
 					}
 					if (complete) {
-						if (r0 + r < rows) store_row4<T>(p, b, h, r0 + r, col, cnt, v, top, sum);
+						if (r0 + r < rows) {
+							const AttnRow to = attn_row(p, b, h, r0 + r, cnt, sum);
+							store_row4<T>(p, to, col, v);
+							if (col == 0) store_lse(to, top, sum);
+						}
 					} else {
 						*(float4 *)(slot + r * DP + col) = v;
 						if (col == 0) slot[RT * DP + r] = top, slot[RT * DP + RT + r] = sum;
@@ -408,7 +448,7 @@ __global__ void __launch_bounds__(128) k_tree_attn(const AttnArgs p)
 				__syncthreads();
 			}
 			if (!end && from_start && tid == 0) // the unit goes on in the CTAs after this one
-				p.split[blockIdx.x] = make_int4(b, h, c.r, (int)((pos + i + (c.all - 1 - c.tile)) / share));
+				p.split[blockIdx.x] = make_int4(b, h, c.r, (int)((pos + share + (c.all - 2 - c.tile)) / share));
 			first = true;
 		}
 		__syncwarp(); // every lane is done with this stage
@@ -451,9 +491,10 @@ __global__ void __launch_bounds__(128) k_attn_join(const AttnArgs p)
 				v[x].x += y.x * a, v[x].y += y.y * a, v[x].z += y.z * a, v[x].w += y.w * a;
 			}
 		}
+		const AttnRow to = attn_row(p, s.x, s.y, s.z * RT + r, cnt, l);
 #pragma unroll
-		for (int x = 0; x < N; x++)
-			if (x * 128 + lane * 4 < DP) store_row4<T>(p, s.x, s.y, s.z * RT + r, x * 128 + lane * 4, cnt, v[x], top, l);
+		for (int x = 0; x < N; x++) store_row4<T>(p, to, x * 128 + lane * 4, v[x]);
+		if (lane == 0) store_lse(to, top, l);
 	}
 }
 

@@ -3,20 +3,24 @@
 //
 // The 128 rows of a unit's tile (k_tree_attn's unit, shares and partial results, tree_attn.cuh) are
 // the M of both products, 128 keys a tile: S = Q K^T into one of two TMEM score buffers, P in
-// shared memory, O += P V in TMEM. Warps:
-//   0-3   softmax, a query row per thread (TMEM lane = row): the running reference mr, p = 2^(z - mr)
-//         to P; where a score exceeds mr by more than RAISE, O is rescaled in TMEM, which is rare
-//         after the first tiles. At a unit's end the thread holds its row's O, l and mr.
-//   4     issue of the MMAs, each as soon as its operands are there: S of the next tile overlaps the
+// shared memory, O += P V in TMEM. The two halves of a tile's keys have a reference, a sum and an O
+// of their own, so their softmax warps need nothing of each other before the unit's end. Warps:
+//   0-7   softmax, a query row per thread (TMEM lane = row), warps 4-7 for the tile's second 64 keys:
+//         the running reference mr, p = 2^(z - mr) to P; where a score exceeds mr by more than RAISE,
+//         O is rescaled in TMEM, which is rare after the first tiles. At a unit's end the two
+//         halves exchange mr and l, and each joins and writes half of the row's dimensions.
+//   16    issue of the MMAs, each as soon as its operands are there: S of the next tile overlaps the
 //         softmax of this one.
-//   5-12  fetching, two warps each for K and V of even and of odd tiles: rows come by 16-byte
+//   8-15  fetching, two warps each for K and V of even and of odd tiles: rows come by 16-byte
 //         cp.async through the page table into the 128-byte-swizzled operand layout (K rows = N,
 //         K-major; V rows = the product's k, so V is read MN-major). Pages of any size and stride
 //         are thus alike, which TMA boxes of a page would not give. A tile's stage is signalled
-//         when it has landed, apart from when the next is asked for.
+//         when it has landed, apart from when the next is asked for; the next tile's table entries
+//         are looked up while this one's rows are on their way.
 // What bounds it: with up to 128 rows the cache's bytes (a 64 KB tile pair takes 2850 cycles of the
-// measured HBM rate; its MMAs about 2000, its softmax 1300). Every wait is bounded (tc.cuh): a
-// timeout sets the status word and all roles leave.
+// measured HBM rate). Of the 544 x 96 registers of the launch the fetching warps give 32 each to
+// the softmax warps, which hold 64 scores. Every wait is bounded (tc.cuh): a timeout sets the status word and all roles
+// leave.
 #pragma once
 
 #include <type_traits>
@@ -27,19 +31,23 @@
 namespace tgc {
 
 struct TaBars {
-	uint64_t kfull[2], kfree[2], vfull[2], vfree[2], s_full[2], s_free[2], p_full, p_empty, done;
+	uint64_t kfull[2], kfree[2], vfull[2], vfree[2], s_full[2], s_free[2]; // by the tile's parity
+	uint64_t p_full[2][2], p_empty[2][2];                                 // by half, then by the tile's parity
+	uint64_t x_full, o_free, done;                                        // per unit: mr and l exchanged, O read
 	uint32_t tmem;
 	int abort;
 	int odd[4][2]; // drafted tile: a V row held something not finite (tile & 3; half of its rows)
-	long long scan[16];
+	long long scan[24];
+	float2 ml[2][128];
 };
 
 template <int DP> struct TaTile {
-	static constexpr int TK = 128, RT = 128, THREADS = 416, NW = 13, CH = DP / 8;
+	static constexpr int TK = 128, RT = 128, NW = 17, THREADS = 32 * NW, CH = DP / 8;
 	static constexpr int OP = 128 * DP * 2;                               // bytes of a Q, K or V tile
-	static constexpr int Q = 0, K = OP, V = 3 * OP, P = 5 * OP, BARS = P + 128 * 128 * 2;
+	static constexpr int Q = 0, K = OP, V = 3 * OP, P = 5 * OP, PB = 128 * 128 * 2, BARS = P + 2 * PB;
 	static constexpr int SMEM = BARS + (int)sizeof(TaBars);
 	static constexpr int SLOT = RT * DP + 2 * RT;
+	static_assert(SMEM <= 232448, "shared memory of a CTA");
 };
 
 __device__ __forceinline__ bool ta_test(uint64_t *bar, uint32_t parity)
@@ -118,7 +126,7 @@ __device__ __forceinline__ uint64_t ta_mn_desc(uint32_t saddr, uint32_t lbo)
 __device__ __forceinline__ uint32_t ta_at(int r, int c) { return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
 template <class T, int DP>
-__global__ void __launch_bounds__(416, 1) k_tree_attn_tc(const AttnArgs p)
+__global__ void __launch_bounds__(544, 1) k_tree_attn_tc(const AttnArgs p)
 {
 	using A = TaTile<DP>;
 	constexpr int TK = A::TK, RT = A::RT, CH = A::CH;
@@ -134,10 +142,11 @@ __global__ void __launch_bounds__(416, 1) k_tree_attn_tc(const AttnArgs p)
 	if (tid == 0) {
 		for (int i = 0; i < 2; i++) {
 			mbar_init(&B->kfull[i], 2), mbar_init(&B->vfull[i], 2);
-			mbar_init(&B->kfree[i], 1), mbar_init(&B->vfree[i], 1);
-			mbar_init(&B->s_full[i], 1), mbar_init(&B->s_free[i], 4);
+			mbar_init(&B->kfree[i], 1), mbar_init(&B->vfree[i], 2);
+			mbar_init(&B->s_full[i], 1), mbar_init(&B->s_free[i], 8);
+			for (int k = 0; k < 2; k++) mbar_init(&B->p_full[i][k], 4), mbar_init(&B->p_empty[i][k], 1);
 		}
-		mbar_init(&B->p_full, 4), mbar_init(&B->p_empty, 1), mbar_init(&B->done, 1);
+		mbar_init(&B->x_full, 8), mbar_init(&B->o_free, 8), mbar_init(&B->done, 1);
 		B->abort = 0;
 		fence_barrier_init();
 	}
@@ -148,49 +157,74 @@ __global__ void __launch_bounds__(416, 1) k_tree_attn_tc(const AttnArgs p)
 	long long left_, pos, share;
 	if (!attn_share<TK, A::NW>(p, B->scan, 1, c, left_, pos, share)) return; // the whole CTA
 	const int left = (int)left_;
-	if (warp == 4) tmem_alloc(&B->tmem, 512); // S buffers at columns 0 and 128, O at 256
+	if (warp == 16) tmem_alloc(&B->tmem, 512); // S buffers at columns 0 and 128, the halves' O at 256 and 256 + DP
 	tc_fence_before();
 	__syncthreads();
 	tc_fence_after();
 	const uint32_t tmem = B->tmem;
 
-	if (warp > 4) {
+	if (warp >= 8 && warp < 16) {
 		// ---------------- fetching ----------------
-		const int role = warp - 5, isv = role & 1, par = role >> 1 & 1, half = role >> 2;
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+		const int role = warp - 8, isv = role & 1, par = role >> 1 & 1, half = role >> 2;
 		uint64_t *full = isv ? &B->vfull[par] : &B->kfull[par], *free_ = isv ? &B->vfree[par] : &B->kfree[par];
 		uint8_t *dst = sm + (isv ? A::V : A::K) + par * A::OP;
 		const uint32_t sd = smem_u32(dst), sq = smem_u32(sm + A::Q);
-		for (int j = 0; j < left; j++, cursor_next<TK>(p, c, 1)) {
-			if ((j & 1) != par) continue;
+		const int ch = lane % CH; // this lane's piece of the rows it copies
+		uint32_t at[2];           // this lane's rows half * 64 + lane and + 32 more: their places, looked up a tile ahead
+		auto find = [&]() {
 			const bool drafted = c.tile >= c.ctx;
-			const char *base = drafted ? (isv ? p.d.v : p.d.k) + (long long)c.b * p.d.kv_seq + c.h * p.d.kv_head : (isv ? p.c.v : p.c.k) + c.h * p.c.head_b;
-			// lane's rows half * 64 + lane and + 32 more
-			long long at[2];
 #pragma unroll
 			for (int i = 0; i < 2; i++) {
-				const long long x = (long long)(drafted ? 0 : c.tile) * TK + half * 64 + i * 32 + lane;
-				if (drafted) at[i] = x < p.d.drafted(c.b) ? x * p.d.kv_tok : -1;
-				else at[i] = x < c.n ? p.c.row(p.c.table + (long long)c.b * p.c.cols, (int)x) : -1;
+				const int x = (drafted ? 0 : c.tile * TK) + half * 64 + i * 32 + lane;
+				at[i] = PG_NONE;
+				if (drafted) {
+					if (x < p.d.drafted(c.b)) at[i] = (uint32_t)(x * p.d.kv_tok >> 4);
+				} else if (x < c.n) {
+					const int page = x / p.c.page;
+					at[i] = p.c.at(p.c.table[(long long)c.b * p.c.cols + page], x - page * p.c.page);
+				}
 			}
+		};
+		if (par < left) {
+			if (par) cursor_next<TK>(p, c, 1);
+			find();
+		}
+		for (int j = par; j < left; j += 2) {
+			const bool drafted = c.tile >= c.ctx, begin = j == 0 || c.tile == 0;
+			const int sh = drafted ? 4 : p.c.shift;
+			const char *base = (drafted ? (isv ? p.d.v : p.d.k) + (long long)c.b * p.d.kv_seq + c.h * p.d.kv_head : (isv ? p.c.v : p.c.k) + c.h * p.c.head_b) + ch * 16;
 			if (j >= 2 && !ta_wait(B, free_, ((j >> 1) - 1) & 1, p.c)) break;
 #pragma unroll
 			for (int i = 0; i < 2; i++)
 #pragma unroll 8
 				for (int y = 0; y < CH; y++) { // 32 / CH rows an instruction
-					const int z = y * 32 + lane, r = z / CH, ch = z % CH;
-					const long long o = __shfl_sync(~0u, at[i], r);
-					const bool have = o >= 0 && ch < chunks;
-					cp16(sd + ta_at(half * 64 + i * 32 + r, ch), have ? base + o + ch * 16 : p.d.k, have);
+					const int r = y * (32 / CH) + lane / CH;
+					const uint32_t o = __shfl_sync(~0u, at[i], r);
+					const bool have = o != PG_NONE && ch < chunks;
+					cp16(sd + ta_at(half * 64 + i * 32 + r, ch), have ? base + ((unsigned long long)o << sh) : p.d.k, have);
 				}
-			if (!isv && (j == 0 || c.tile == 0)) { // a unit begins: its Q, once the last S of the unit before is done
+			if (!isv && begin) { // the unit's Q, once the last S of the unit before is done
 				if (j > 0 && !ta_wait(B, &B->kfree[(j - 1) & 1], ((j - 1) >> 1) & 1, p.c)) break;
-				for (int z = lane; z < 64 * CH; z += 32) {
-					const int row = half * 64 + z / CH, ch = z % CH, r = c.r * RT + row, t = r / p.d.group;
-					const bool have = r < rows && ch < chunks;
-					cp16(sq + ta_at(row, ch), have ? p.d.q + (long long)c.b * p.d.q_seq + (long long)t * p.d.q_tok + (long long)(c.h * p.d.group + r % p.d.group) * p.d.q_head + ch * 16 : p.d.k, have);
+				const char *qb = p.d.q + (long long)c.b * p.d.q_seq + (long long)c.h * p.d.group * p.d.q_head + ch * 16;
+#pragma unroll
+				for (int i = 0; i < 2; i++) {
+					const int r = c.r * RT + half * 64 + i * 32 + lane, t = r / p.d.group;
+					const long long mine = r < rows ? (long long)t * p.d.q_tok + (long long)(r - t * p.d.group) * p.d.q_head : -1;
+#pragma unroll 4
+					for (int y = 0; y < CH; y++) {
+						const long long o = __shfl_sync(~0u, mine, y * (32 / CH) + lane / CH);
+						const bool have = o >= 0 && ch < chunks;
+						cp16(sq + ta_at(half * 64 + i * 32 + y * (32 / CH) + lane / CH, ch), have ? qb + o : p.d.k, have);
+					}
 				}
 			}
 			cp_commit();
+			if (j + 2 < left) {
+				cursor_next<TK>(p, c, 1);
+				cursor_next<TK>(p, c, 1);
+				find();
+			}
 			cp_wait<0>();
 			if (isv && drafted) {
 				// a row that some token does not see may hold anything, and 0 * infinity must not reach O: what is not
@@ -198,10 +232,9 @@ __global__ void __launch_bounds__(416, 1) k_tree_attn_tc(const AttnArgs p)
 				bool odd = false;
 #pragma unroll
 				for (int i = 0; i < 2; i++)
-#pragma unroll
+#pragma unroll 1
 					for (int y = 0; y < CH; y++) {
-						const int z = y * 32 + lane;
-						uint32_t *w = (uint32_t *)(dst + ta_at(half * 64 + i * 32 + z / CH, z % CH));
+						uint32_t *w = (uint32_t *)(dst + ta_at(half * 64 + i * 32 + y * (32 / CH) + lane / CH, ch));
 #pragma unroll
 						for (int x = 0; x < 4; x++)
 							if (PgElem<T>::odd(w[x])) {
@@ -217,16 +250,17 @@ __global__ void __launch_bounds__(416, 1) k_tree_attn_tc(const AttnArgs p)
 			mbar_arrive_warp(full);
 		}
 		cp_wait<0>();
-	} else if (warp == 4) {
+	} else if (warp == 16) {
 		// ---------------- MMA issue ----------------
 		if (lane == 0) {
 			const uint32_t id = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(RT >> 4) << 24); // f32 += f16 or bf16 products
 			const uint32_t idS = id | ((uint32_t)(TK >> 3) << 17), idO = id | ((uint32_t)(DP >> 3) << 17) | (1u << 16); // V MN-major
 			const uint32_t base = smem_u32(sm);
-			int ns = 0, npv = 0;
+			AttnCursor at[2] = {c, c}; // of the halves' next P V
+			int ns = 0, npv[2] = {0, 0}, units[2] = {0, 0};
 			bool ok = true;
 			long long idle0 = clock64();
-			for (uint32_t spins = 0; ok && npv < left;) {
+			for (uint32_t spins = 0; ok && (npv[0] < left || npv[1] < left);) {
 				bool did = false;
 				if (ns < left && ta_test(&B->kfull[ns & 1], (ns >> 1) & 1) && (ns < 2 || ta_test(&B->s_free[ns & 1], ((ns >> 1) - 1) & 1))) {
 					tc_fence_after();
@@ -240,18 +274,22 @@ __global__ void __launch_bounds__(416, 1) k_tree_attn_tc(const AttnArgs p)
 					ns++;
 					did = true;
 				}
-				if (npv < ns && ta_test(&B->vfull[npv & 1], (npv >> 1) & 1) && ta_test(&B->p_full, npv & 1)) {
-					tc_fence_after();
-					const uint32_t pa = base + A::P, v = base + A::V + (npv & 1) * A::OP;
-					const bool first = npv == 0 || c.tile == 0;
 #pragma unroll
-					for (int kk = 0; kk < TK / 16; kk++)
-						tc_mma_f16(tmem + 256, sw128_kmajor_desc(pa + (kk >> 2) * 16384 + (kk & 3) * 32), ta_mn_desc(v + kk * 2048, 16384), idO,
-							   !first || kk > 0);
-					tc_commit(&B->p_empty);
-					tc_commit(&B->vfree[npv & 1]);
-					npv++;
-					cursor_next<TK>(p, c, 1);
+				for (int f = 0; f < 2; f++) {
+					const int j = npv[f];
+					if (j >= ns || !ta_test(&B->p_full[f][j & 1], (j >> 1) & 1) || !ta_test(&B->vfull[j & 1], (j >> 1) & 1)) continue;
+					const bool first = j == 0 || at[f].tile == 0;
+					if (first && j > 0 && !ta_test(&B->o_free, (units[f] - 1) & 1)) continue; // the unit before has been read
+					if (first) units[f]++;
+					tc_fence_after();
+					const uint32_t pa = base + A::P + (j & 1) * A::PB + f * 16384, v = base + A::V + (j & 1) * A::OP + f * 8192;
+#pragma unroll
+					for (int kk = 0; kk < 4; kk++)
+						tc_mma_f16(tmem + 256 + f * DP, sw128_kmajor_desc(pa + kk * 32), ta_mn_desc(v + kk * 2048, 16384), idO, !first || kk > 0);
+					tc_commit(&B->p_empty[f][j & 1]);
+					tc_commit(&B->vfree[j & 1]);
+					npv[f]++;
+					cursor_next<TK>(p, at[f], 1);
 					did = true;
 				}
 				if (did) {
@@ -272,102 +310,97 @@ __global__ void __launch_bounds__(416, 1) k_tree_attn_tc(const AttnArgs p)
 		__syncwarp();
 	} else {
 		// ---------------- softmax ----------------
-		const int row = tid;
-		const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+		const int row = tid & 127, hf = warp >> 2;
+		const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), mine = lanes + 256 + hf * DP;
 		const float zs = p.d.scale * 1.4426950408889634f;
 		float mr = -INFINITY, l = 0;
 		unsigned long long see = 0;
-		int cnt = 0;
+		int cnt = 0, unit = 0;
 		bool from_start = true;
 		for (int j = 0; j < left; j++) {
-			if (j == 0 || c.tile == 0) { // a unit begins, or goes on from the CTA before
+			const bool fresh = j == 0 || c.tile == 0, drafted = c.tile >= c.ctx;
+			if (fresh) { // a unit begins, or goes on from the CTA before
 				from_start = c.tile == 0;
 				cnt = p.d.drafted(c.b);
 				const int t = (c.r * RT + row) / p.d.group;
 				see = t < cnt ? p.d.sees(c.b, t, cnt) : 0;
 				mr = -INFINITY, l = 0;
 			}
-			const bool fresh = j == 0 || c.tile == 0, drafted = c.tile >= c.ctx;
-			// which of the tile's keys count
-			uint32_t ok[4] = {~0u, ~0u, ~0u, ~0u};
-			const bool masked = drafted || c.tile == c.ctx - 1;
-			if (masked) {
-				const int n = drafted ? 0 : (int)(c.n - (long long)c.tile * TK);
-#pragma unroll
-				for (int w = 0; w < 4; w++)
-					ok[w] = drafted ? (w == 0 ? (uint32_t)see : w == 1 ? (uint32_t)(see >> 32) : 0u) : n >= 32 * w + 32 ? ~0u : n <= 32 * w ? 0u : (1u << (n - 32 * w)) - 1;
-			}
 			if (!ta_wait(B, &B->s_full[j & 1], (j >> 1) & 1, p.c)) break;
 			tc_fence_after();
-			const uint32_t ts = lanes + (j & 1) * TK;
-			float v[32], top = -INFINITY;
+			float z[64];
+			tmem_ld32(lanes + (j & 1) * TK + hf * 64, *(float (*)[32])z);
+			tmem_ld32(lanes + (j & 1) * TK + hf * 64 + 32, *(float (*)[32])(z + 32));
+			tc_fence_before();
+			mbar_arrive_warp(&B->s_free[j & 1]);
 #pragma unroll
-			for (int w = 0; w < 4; w++) {
-				tmem_ld32(ts + w * 32, v);
-				float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-				if (masked) {
+			for (int e = 0; e < 64; e++) z[e] *= zs;
+			if (drafted || c.tile == c.ctx - 1) { // the mask's bits, or the end of the cache
+				const int n = drafted ? 0 : (int)(c.n - (long long)c.tile * TK) - hf * 64;
+				const unsigned long long ok = drafted ? (hf ? 0ull : see) : n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+				const uint32_t lo = (uint32_t)ok, hi = (uint32_t)(ok >> 32);
 #pragma unroll
-					for (int e = 0; e < 32; e++) x[e & 3] = fmaxf(x[e & 3], ok[w] >> e & 1 ? v[e] * zs : -INFINITY);
-				} else {
-#pragma unroll
-					for (int e = 0; e < 32; e++) x[e & 3] = fmaxf(x[e & 3], v[e] * zs);
-				}
-				top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+				for (int e = 0; e < 64; e++)
+					if (!((e < 32 ? lo : hi) >> (e & 31) & 1)) z[e] = -INFINITY;
 			}
-			if (j > 0 && !ta_wait(B, &B->p_empty, (j - 1) & 1, p.c)) break; // P V of the tile before is done
-			const bool raise = top > mr + (SHIFT + RAISE);
-			const float ref0 = mr;
+			float x[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+			for (int e = 4; e < 64; e++) x[e & 3] = fmaxf(x[e & 3], z[e]);
+			const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), ref0 = mr;
+			const bool raise = top > mr + (SHIFT + RAISE), scale = raise && ref0 != -INFINITY;
 			if (raise) mr = top - SHIFT;
-			const bool scale = raise && ref0 != -INFINITY;
-			if (__any_sync(~0u, scale)) {
+			if (j > 1 && !ta_wait(B, &B->p_empty[hf][j & 1], ((j >> 1) - 1) & 1, p.c)) break; // this P buffer's product is done
+			if (__any_sync(~0u, scale)) { // O waits for that of the tile before, too (scale: there is one)
+				if (!ta_wait(B, &B->p_empty[hf][(j - 1) & 1], ((j - 1) >> 1) & 1, p.c)) break;
 				const float f = scale ? ex2(ref0 - mr) : 1;
 				l *= f;
-				if (!fresh) {
-					tc_fence_after();
+				tc_fence_after();
 #pragma unroll 1
-					for (int w = 0; w < DP / 32; w++) {
-						tmem_ld32(lanes + 256 + w * 32, v);
+				for (int w = 0; w < DP / 32; w++) {
+					float v[32];
+					tmem_ld32(mine + w * 32, v);
 #pragma unroll
-						for (int e = 0; e < 32; e++) v[e] *= f;
-						tmem_st32(lanes + 256 + w * 32, v);
-					}
+					for (int e = 0; e < 32; e++) v[e] *= f;
+					tmem_st32(mine + w * 32, v);
 				}
 			}
 			const float ref = mr == -INFINITY ? 0 : mr;
 			float sum[4] = {0, 0, 0, 0};
 #pragma unroll
-			for (int w = 0; w < 4; w++) {
-				tmem_ld32(ts + w * 32, v);
-				if (masked) {
+			for (int i = 0; i < 8; i++) {
 #pragma unroll
-					for (int e = 0; e < 32; e++) v[e] = ok[w] >> e & 1 ? ex2(v[e] * zs - ref) : 0;
-				} else {
-#pragma unroll
-					for (int e = 0; e < 32; e++) v[e] = ex2(v[e] * zs - ref);
-				}
-#pragma unroll
-				for (int e = 0; e < 32; e++) sum[e & 3] += v[e];
-#pragma unroll
-				for (int i = 0; i < 4; i++)
-					*(uint4 *)(sm + A::P + ta_at(row, w * 4 + i)) = make_uint4(pack16(v[8 * i], v[8 * i + 1], T()), pack16(v[8 * i + 2], v[8 * i + 3], T()),
-												   pack16(v[8 * i + 4], v[8 * i + 5], T()), pack16(v[8 * i + 6], v[8 * i + 7], T()));
+				for (int e = 8 * i; e < 8 * i + 8; e++) sum[e & 3] += z[e] = ex2(z[e] - ref);
+				*(uint4 *)(sm + A::P + (j & 1) * A::PB + ta_at(row, hf * 8 + i)) = make_uint4(pack16(z[8 * i], z[8 * i + 1], T()), pack16(z[8 * i + 2], z[8 * i + 3], T()),
+											pack16(z[8 * i + 4], z[8 * i + 5], T()), pack16(z[8 * i + 6], z[8 * i + 7], T()));
 			}
 			l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 			tc_fence_before();
 			fence_async_smem();
-			mbar_arrive_warp(&B->s_free[j & 1]);
-			mbar_arrive_warp(&B->p_full);
+			mbar_arrive_warp(&B->p_full[hf][j & 1]);
 
 			const bool end = c.tile == c.all - 1;
 			if (end || j == left - 1) {
-				if (!ta_wait(B, &B->p_empty, j & 1, p.c)) break;
+				B->ml[hf][row] = make_float2(mr, l);
+				mbar_arrive_warp(&B->x_full);
+				if (!ta_wait(B, &B->x_full, unit & 1, p.c) || !ta_wait(B, &B->p_empty[0][j & 1], (j >> 1) & 1, p.c) ||
+				    !ta_wait(B, &B->p_empty[1][j & 1], (j >> 1) & 1, p.c))
+					break;
 				tc_fence_after();
+				const float2 a = B->ml[0][row], d = B->ml[1][row];
+				const float both = fmaxf(a.x, d.x), fa = a.x == -INFINITY ? 0 : ex2(a.x - both), fd = d.x == -INFINITY ? 0 : ex2(d.x - both);
+				const float sl = (a.x == -INFINITY ? a.y : a.y * fa) + (d.x == -INFINITY ? d.y : d.y * fd);
 				const int r = c.r * RT + row, b = c.b, h = c.h;
 				const bool complete = end && from_start, odd = drafted && (*(volatile int *)&B->odd[j & 3][0] | *(volatile int *)&B->odd[j & 3][1]);
 				float *slot = complete ? nullptr : p.part + (2ll * blockIdx.x + (from_start ? 1 : 0)) * A::SLOT;
+				const AttnRow to = attn_row(p, b, h, r < rows ? r : 0, cnt, sl);
 #pragma unroll 1
-				for (int w = 0; w < DP / 32; w++) {
+				for (int w = hf * (DP / 64); w < (hf + 1) * (DP / 64); w++) {
+					float v[32], u[32];
 					tmem_ld32(lanes + 256 + w * 32, v);
+					tmem_ld32(lanes + 256 + DP + w * 32, u);
+#pragma unroll
+					for (int e = 0; e < 32; e++) v[e] = (fa == 0 ? 0 : v[e] * fa) + (fd == 0 ? 0 : u[e] * fd);
 					if (odd && r < rows)
 						for (unsigned long long m = see; m; m &= m - 1) {
 							const T *vr = (const T *)(p.d.v + (long long)b * p.d.kv_seq + (long long)(__ffsll((long long)m) - 1) * p.d.kv_tok + h * p.d.kv_head) + w * 32;
@@ -381,19 +414,23 @@ __global__ void __launch_bounds__(416, 1) k_tree_attn_tc(const AttnArgs p)
 					for (int e = 0; e < 32; e += 4) {
 						const float4 y = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
 						if (!complete) *(float4 *)(slot + row * DP + w * 32 + e) = y;
-						else if (r < rows) store_row4<T>(p, b, h, r, w * 32 + e, cnt, y, mr, l);
+						else if (r < rows) store_row4<T>(p, to, w * 32 + e, y);
 					}
 				}
-				if (!complete) slot[RT * DP + row] = mr, slot[RT * DP + RT + row] = l;
+				if (complete && hf == 0 && r < rows) store_lse(to, both, sl);
+				if (!complete && hf == 0) slot[RT * DP + row] = both, slot[RT * DP + RT + row] = sl;
 				if (!end && from_start && tid == 0) // the unit goes on in the CTAs after this one
-					p.split[blockIdx.x] = make_int4(b, h, c.r, (int)((pos + j + (c.all - 1 - c.tile)) / share));
+					p.split[blockIdx.x] = make_int4(b, h, c.r, (int)((pos + share + (c.all - 2 - c.tile)) / share));
+				tc_fence_before();
+				mbar_arrive_warp(&B->o_free);
+				unit++;
 			}
 			cursor_next<TK>(p, c, 1);
 		}
 	}
 	tc_fence_before();
 	__syncthreads();
-	if (warp == 4) {
+	if (warp == 16) {
 		tc_fence_after();
 		tmem_dealloc(tmem, 512);
 	}
