@@ -185,6 +185,21 @@ __device__ __forceinline__ AttnRow attn_row(const AttnArgs &p, int b, int h, int
 	return x;
 }
 __device__ __forceinline__ void store_lse(const AttnRow &x, float mr, float l) { *x.lse = x.none ? -INFINITY : (mr + log2f(l)) * 0.69314718056f; }
+// 8 columns of a row: whole 16-byte pieces for 16-bit elements
+template <class T>
+__device__ __forceinline__ void store_row8(const AttnArgs &p, const AttnRow &x, int col, const float *o)
+{
+	if (col >= p.c.dim) return;
+	float v[8];
+#pragma unroll
+	for (int i = 0; i < 8; i++) v[i] = x.none ? 0 : o[i] * x.f;
+	if constexpr (sizeof(T) == 2)
+		*(uint4 *)((T *)x.out + col) = make_uint4(pack16(v[0], v[1], T()), pack16(v[2], v[3], T()), pack16(v[4], v[5], T()), pack16(v[6], v[7], T()));
+	else {
+		store4((T *)x.out + col, make_float4(v[0], v[1], v[2], v[3]));
+		if (col + 4 < p.c.dim) store4((T *)x.out + col + 4, make_float4(v[4], v[5], v[6], v[7]));
+	}
+}
 template <class T>
 __device__ __forceinline__ void store_row4(const AttnArgs &p, const AttnRow &x, int col, float4 o)
 {
@@ -458,43 +473,43 @@ __global__ void __launch_bounds__(128) k_tree_attn(const AttnArgs p)
 	cp_wait<0>();
 }
 
-// The parts of the units that several CTAs shared: a warp per row, the parts in CTA order.
+// A partial result's place of 4 columns of a row (then come the rows' mr and l): as the kernel that
+// leaves it writes whole lines, a row's columns together from k_tree_attn, the rows of 4 columns together
+// from the row per thread of 128-row tiles.
+template <int DP, int RT> __device__ __forceinline__ int slot_at(int row, int col) { return RT == 128 ? (col / 4 * RT + row) * 4 : row * DP + col; }
+
+// The parts of the units that several CTAs shared, added in CTA order: a thread has a row and 8 of its
+// columns, and the threads of a warp what lies together in a part.
 template <class T, int DP, int RT>
 __global__ void __launch_bounds__(128) k_attn_join(const AttnArgs p)
 {
-	constexpr int SLOT = RT * DP + 2 * RT, N = DP / 128 ? DP / 128 : 1;
+	constexpr int SLOT = RT * DP + 2 * RT, RW = RT == 128 ? 32 : 1; // rows side by side in a warp
 	pdl_launch();
 	pdl_wait();
 	const int4 s = p.split[blockIdx.x];
 	if (s.x < 0) return;
-	const int lane = threadIdx.x & 31, rows = p.d.tokens * p.d.group, cnt = p.d.drafted(s.x);
-	const int parts = s.w - (int)blockIdx.x + 1;
-	auto part = [&](int i) { return p.part + (2ll * (blockIdx.x + i) + (i == 0)) * SLOT; };
-	for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < RT && s.z * RT + r < rows; r += gridDim.y * 4) {
-		float top = -INFINITY, l = 0;
-		for (int i = lane; i < parts; i += 32) top = fmaxf(top, part(i)[RT * DP + r]);
-#pragma unroll
-		for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-		float4 v[N];
-#pragma unroll
-		for (int x = 0; x < N; x++) v[x] = make_float4(0, 0, 0, 0);
+	const int rows = p.d.tokens * p.d.group, cnt = p.d.drafted(s.x), parts = s.w - (int)blockIdx.x + 1;
+	const float *first = p.part + (2ll * blockIdx.x + 1) * SLOT, *rest = p.part + 2ll * blockIdx.x * SLOT;
+	auto part = [&](int i) { return i ? rest + 2ll * i * SLOT : first; };
+	for (int x = blockIdx.y * 128 + threadIdx.x; x < RT * DP / 8; x += gridDim.y * 128) {
+		const int r = x / (RW * DP / 8) * RW + x % RW, col = x / RW % (DP / 8) * 8;
+		if (s.z * RT + r >= rows) continue;
+		float top = -INFINITY, l = 0, v[8] = {};
+#pragma unroll 4
+		for (int i = 0; i < parts; i++) top = fmaxf(top, part(i)[RT * DP + r]);
 #pragma unroll 4
 		for (int i = 0; i < parts; i++) {
 			const float *q = part(i);
 			const float m = q[RT * DP + r], a = m == -INFINITY ? 0 : ex2(m - top);
 			l += m == -INFINITY ? q[RT * DP + RT + r] : q[RT * DP + RT + r] * a;
-#pragma unroll
-			for (int x = 0; x < N; x++) {
-				const int col = x * 128 + lane * 4;
-				if (col >= DP || a == 0) continue;
-				const float4 y = *(const float4 *)(q + r * DP + col);
-				v[x].x += y.x * a, v[x].y += y.y * a, v[x].z += y.z * a, v[x].w += y.w * a;
-			}
+			const float4 y = *(const float4 *)(q + slot_at<DP, RT>(r, col)), z = *(const float4 *)(q + slot_at<DP, RT>(r, col + 4));
+			if (a == 0) continue;
+			v[0] += y.x * a, v[1] += y.y * a, v[2] += y.z * a, v[3] += y.w * a;
+			v[4] += z.x * a, v[5] += z.y * a, v[6] += z.z * a, v[7] += z.w * a;
 		}
 		const AttnRow to = attn_row(p, s.x, s.y, s.z * RT + r, cnt, l);
-#pragma unroll
-		for (int x = 0; x < N; x++) store_row4<T>(p, to, x * 128 + lane * 4, v[x]);
-		if (lane == 0) store_lse(to, top, l);
+		store_row8<T>(p, to, col, v);
+		if (col == 0) store_lse(to, top, l);
 	}
 }
 

@@ -14,7 +14,7 @@ static int attn_run(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 	int rc = pg_smem(k_tree_attn<T, DP, MT>, A::SMEM, pl.dev, done);
 	if (rc) return rc;
 	TGC_CUDA(launch_pdl(k_tree_attn<T, DP, MT>, dim3(pl.grid), dim3(128), A::SMEM, st, p));
-	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT / 4), dim3(128), 0, st, p));
+	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT * DP / 1024), dim3(128), 0, st, p));
 	return TG_CUDA_OK;
 }
 
@@ -26,7 +26,7 @@ static int attn_run_tc(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 	int rc = pg_smem(k_tree_attn_tc<T, DP>, A::SMEM, pl.dev, done);
 	if (rc) return rc;
 	TGC_CUDA(launch_pdl(k_tree_attn_tc<T, DP>, dim3(pl.grid), dim3(A::THREADS), A::SMEM, st, p));
-	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT / 4), dim3(128), 0, st, p));
+	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT * DP / 1024), dim3(128), 0, st, p));
 	return TG_CUDA_OK;
 }
 

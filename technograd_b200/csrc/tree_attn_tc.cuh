@@ -2,15 +2,16 @@
 // (drafted tokens x heads of a key head's group) and 16-bit caches.
 //
 // The 128 rows of a unit's tile (k_tree_attn's unit, shares and partial results, tree_attn.cuh) are
-// the M of both products, 128 keys a tile: S = Q K^T into one of two TMEM score buffers, P in
-// shared memory, O += P V in TMEM. The two halves of a tile's keys have a reference, a sum and an O
+// the M of both products, 128 keys a tile: S = Q K^T into one of two TMEM score buffers, P over S in
+// the type of V (the operand of O += P V that comes from TMEM), O in TMEM. The two halves of a tile's keys have a reference, a sum and an O
 // of their own, so their softmax warps need nothing of each other before the unit's end. Warps:
 //   0-7   softmax, a query row per thread (TMEM lane = row), warps 4-7 for the tile's second 64 keys:
 //         the running reference mr, p = 2^(z - mr) to P; where a score exceeds mr by more than RAISE,
 //         O is rescaled in TMEM, which is rare after the first tiles. At a unit's end the two
 //         halves exchange mr and l, and each joins and writes half of the row's dimensions.
-//   16    issue of the MMAs, each as soon as its operands are there: S of the next tile overlaps the
-//         softmax of this one.
+//   16-18 issue of the MMAs, one thread each for S and the halves' P V, as soon as the operands are there: S
+//         of the next tiles overlaps the softmax of this one. (One thread for all was busy 3200 cycles a
+//         tile with its barriers, commits and issues, more than the tile's bytes take.)
 //   8-15  fetching, two warps each for K and V of even and of odd tiles: rows come by 16-byte
 //         cp.async through the page table into the 128-byte-swizzled operand layout (K rows = N,
 //         K-major; V rows = the product's k, so V is read MN-major). Pages of any size and stride
@@ -18,7 +19,7 @@
 //         when it has landed, apart from when the next is asked for; the next tile's table entries
 //         are looked up while this one's rows are on their way.
 // What bounds it: with up to 128 rows the cache's bytes (a 64 KB tile pair takes 2850 cycles of the
-// measured HBM rate). Of the 544 x 96 registers of the launch the fetching warps give 32 each to
+// measured HBM rate). Of the 608 x 96 registers of the launch the fetching warps give 32 each to
 // the softmax warps, which hold 64 scores. Every wait is bounded (tc.cuh): a timeout sets the status word and all roles
 // leave.
 #pragma once
@@ -31,8 +32,8 @@
 namespace tgc {
 
 struct TaBars {
-	uint64_t kfull[2], kfree[2], vfull[2], vfree[2], s_full[2], s_free[2]; // by the tile's parity
-	uint64_t p_full[2][2], p_empty[2][2];                                 // by half, then by the tile's parity
+	uint64_t kfull[3], kfree[3], vfull[3], vfree[3]; // by stage
+	uint64_t s_full[2], p_full[2][2], p_empty[2][2]; // by the tile's parity (P: by half, then parity)
 	uint64_t x_full, o_free, done;                                        // per unit: mr and l exchanged, O read
 	uint32_t tmem;
 	int abort;
@@ -42,9 +43,9 @@ struct TaBars {
 };
 
 template <int DP> struct TaTile {
-	static constexpr int TK = 128, RT = 128, NW = 17, THREADS = 32 * NW, CH = DP / 8;
+	static constexpr int TK = 128, RT = 128, NW = 19, THREADS = 32 * NW, CH = DP / 8;
 	static constexpr int OP = 128 * DP * 2;                               // bytes of a Q, K or V tile
-	static constexpr int Q = 0, K = OP, V = 3 * OP, P = 5 * OP, PB = 128 * 128 * 2, BARS = P + 2 * PB;
+	static constexpr int NST = 3, Q = 0, K = OP, V = (1 + NST) * OP, BARS = (1 + 2 * NST) * OP;
 	static constexpr int SMEM = BARS + (int)sizeof(TaBars);
 	static constexpr int SLOT = RT * DP + 2 * RT;
 	static_assert(SMEM <= 232448, "shared memory of a CTA");
@@ -60,30 +61,25 @@ __device__ __forceinline__ bool ta_test(uint64_t *bar, uint32_t parity)
 	return ok != 0;
 }
 
-// Bounded wait of a whole warp; false after the CTA's abort flag or the cycle budget, which sets it.
-__device__ __forceinline__ bool ta_wait(TaBars *B, uint64_t *bar, uint32_t parity, const PgCache &c)
+// Bounded wait; false after the CTA's abort flag or the cycle budget, which sets it.
+__device__ __forceinline__ bool ta_poll(TaBars *B, uint64_t *bar, uint32_t parity, const PgCache &c)
 {
-	bool ok = true;
-	if (!ta_test(bar, parity)) {
-		const long long t0 = clock64();
-		for (uint32_t i = 1;; i++) {
-			if (ta_test(bar, parity)) break;
-			if ((i & 63) == 0) {
-				if (*(volatile int *)&B->abort) {
-					ok = false;
-					break;
-				}
-				if (clock64() - t0 > WAIT_CYCLES) {
-					c.report(PG_WAIT);
-					*(volatile int *)&B->abort = 1;
-					ok = false;
-					break;
-				}
+	if (ta_test(bar, parity)) return true;
+	const long long t0 = clock64();
+	for (uint32_t i = 1;; i++) {
+		if (ta_test(bar, parity)) return true;
+		if ((i & 63) == 0) {
+			if (*(volatile int *)&B->abort) return false;
+			if (clock64() - t0 > WAIT_CYCLES) {
+				c.report(PG_WAIT);
+				*(volatile int *)&B->abort = 1;
+				return false;
 			}
 		}
 	}
-	return __all_sync(~0u, ok);
 }
+// ... of a whole warp, which leaves together
+__device__ __forceinline__ bool ta_wait(TaBars *B, uint64_t *bar, uint32_t parity, const PgCache &c) { return __all_sync(~0u, ta_poll(B, bar, parity, c)); }
 
 // 32 lanes x 32 columns of TMEM
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32])
@@ -102,9 +98,9 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32])
 	for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32])
+__device__ __forceinline__ void ta_st32(uint32_t taddr, const uint32_t (&v)[32])
 {
-#define R(i) "r"(__float_as_uint(v[i]))
+#define R(i) "r"(v[i])
 	asm volatile(
 		"tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
 		"%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
@@ -113,6 +109,22 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32])
 		: "memory");
 #undef R
 	asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// D[tmem] (+)= A[tmem] B[smem], A 128 rows (lanes) of 16-bit pairs (columns)
+__device__ __forceinline__ void ta_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+	asm volatile(
+		"{\n\t.reg .pred p;\n\t"
+		"setp.ne.b32 p, %4, 0;\n\t"
+		"tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+		: "memory");
+}
+
+// An arrival of this thread on bar (counted in its initial count) once all its cp.async copies so far have landed
+__device__ __forceinline__ void cp_arrive(uint64_t *bar)
+{
+	asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // MN-major operand, 128-byte swizzle: rows of 64 elements along MN, 8 rows of k 1024 bytes apart (sbo),
@@ -126,7 +138,7 @@ __device__ __forceinline__ uint64_t ta_mn_desc(uint32_t saddr, uint32_t lbo)
 __device__ __forceinline__ uint32_t ta_at(int r, int c) { return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
 template <class T, int DP>
-__global__ void __launch_bounds__(544, 1) k_tree_attn_tc(const AttnArgs p)
+__global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p)
 {
 	using A = TaTile<DP>;
 	constexpr int TK = A::TK, RT = A::RT, CH = A::CH;
@@ -140,13 +152,15 @@ __global__ void __launch_bounds__(544, 1) k_tree_attn_tc(const AttnArgs p)
 		return;
 	}
 	if (tid == 0) {
-		for (int i = 0; i < 2; i++) {
-			mbar_init(&B->kfull[i], 2), mbar_init(&B->vfull[i], 2);
+		for (int i = 0; i < A::NST; i++) {
+			mbar_init(&B->kfull[i], 64), mbar_init(&B->vfull[i], 64);
 			mbar_init(&B->kfree[i], 1), mbar_init(&B->vfree[i], 2);
-			mbar_init(&B->s_full[i], 1), mbar_init(&B->s_free[i], 8);
+		}
+		for (int i = 0; i < 2; i++) {
+			mbar_init(&B->s_full[i], 1);
 			for (int k = 0; k < 2; k++) mbar_init(&B->p_full[i][k], 4), mbar_init(&B->p_empty[i][k], 1);
 		}
-		mbar_init(&B->x_full, 8), mbar_init(&B->o_free, 8), mbar_init(&B->done, 1);
+		mbar_init(&B->x_full, 8), mbar_init(&B->o_free, 8), mbar_init(&B->done, 3);
 		B->abort = 0;
 		fence_barrier_init();
 	}
@@ -167,74 +181,83 @@ __global__ void __launch_bounds__(544, 1) k_tree_attn_tc(const AttnArgs p)
 		// ---------------- fetching ----------------
 		asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
 		const int role = warp - 8, isv = role & 1, par = role >> 1 & 1, half = role >> 2;
-		uint64_t *full = isv ? &B->vfull[par] : &B->kfull[par], *free_ = isv ? &B->vfree[par] : &B->kfree[par];
-		uint8_t *dst = sm + (isv ? A::V : A::K) + par * A::OP;
-		const uint32_t sd = smem_u32(dst), sq = smem_u32(sm + A::Q);
-		const int ch = lane % CH; // this lane's piece of the rows it copies
-		uint32_t at[2];           // this lane's rows half * 64 + lane and + 32 more: their places, looked up a tile ahead
-		auto find = [&]() {
+		constexpr int RI = 32 / CH;  // rows an instruction copies
+		const int ch = lane % CH; // this lane's piece of them
+		// its place in a tile: row lane / CH of the warp's half, before the swizzle of the rows after it
+		const uint32_t d0 = smem_u32(sm) + (uint32_t)((ch >> 3) * 16384 + (half * 64 + lane / CH) * 128), x0 = (uint32_t)((ch & 7) ^ (lane / CH)) << 4;
+		const bool piece = ch < chunks;
+		// this lane's rows half * 64 + lane and + 32 more: the table's entries, then the rows' places
+		int entry[2], in_page[2];
+		uint32_t at[2];
+		auto look = [&]() {
 			const bool drafted = c.tile >= c.ctx;
 #pragma unroll
 			for (int i = 0; i < 2; i++) {
 				const int x = (drafted ? 0 : c.tile * TK) + half * 64 + i * 32 + lane;
-				at[i] = PG_NONE;
+				in_page[i] = -1;
 				if (drafted) {
-					if (x < p.d.drafted(c.b)) at[i] = (uint32_t)(x * p.d.kv_tok >> 4);
+					if (x < p.d.drafted(c.b)) in_page[i] = x;
 				} else if (x < c.n) {
 					const int page = x / p.c.page;
-					at[i] = p.c.at(p.c.table[(long long)c.b * p.c.cols + page], x - page * p.c.page);
+					in_page[i] = x - page * p.c.page;
+					entry[i] = p.c.table[(long long)c.b * p.c.cols + page];
 				}
 			}
 		};
 		if (par < left) {
 			if (par) cursor_next<TK>(p, c, 1);
-			find();
+			look();
 		}
 		for (int j = par; j < left; j += 2) {
 			const bool drafted = c.tile >= c.ctx, begin = j == 0 || c.tile == 0;
 			const int sh = drafted ? 4 : p.c.shift;
 			const char *base = (drafted ? (isv ? p.d.v : p.d.k) + (long long)c.b * p.d.kv_seq + c.h * p.d.kv_head : (isv ? p.c.v : p.c.k) + c.h * p.c.head_b) + ch * 16;
-			if (j >= 2 && !ta_wait(B, free_, ((j >> 1) - 1) & 1, p.c)) break;
+			const int st = j % A::NST;
+			const char *qb = p.d.q + (long long)c.b * p.d.q_seq + (long long)c.h * p.d.group * p.d.q_head + ch * 16;
+			const int r0 = c.r * RT + half * 64 + lane;
 #pragma unroll
 			for (int i = 0; i < 2; i++)
-#pragma unroll 8
-				for (int y = 0; y < CH; y++) { // 32 / CH rows an instruction
-					const int r = y * (32 / CH) + lane / CH;
-					const uint32_t o = __shfl_sync(~0u, at[i], r);
-					const bool have = o != PG_NONE && ch < chunks;
-					cp16(sd + ta_at(half * 64 + i * 32 + r, ch), have ? base + ((unsigned long long)o << sh) : p.d.k, have);
-				}
-			if (!isv && begin) { // the unit's Q, once the last S of the unit before is done
-				if (j > 0 && !ta_wait(B, &B->kfree[(j - 1) & 1], ((j - 1) >> 1) & 1, p.c)) break;
-				const char *qb = p.d.q + (long long)c.b * p.d.q_seq + (long long)c.h * p.d.group * p.d.q_head + ch * 16;
-#pragma unroll
-				for (int i = 0; i < 2; i++) {
-					const int r = c.r * RT + half * 64 + i * 32 + lane, t = r / p.d.group;
-					const long long mine = r < rows ? (long long)t * p.d.q_tok + (long long)(r - t * p.d.group) * p.d.q_head : -1;
-#pragma unroll 4
-					for (int y = 0; y < CH; y++) {
-						const long long o = __shfl_sync(~0u, mine, y * (32 / CH) + lane / CH);
-						const bool have = o >= 0 && ch < chunks;
-						cp16(sq + ta_at(half * 64 + i * 32 + y * (32 / CH) + lane / CH, ch), have ? qb + o : p.d.k, have);
-					}
-				}
-			}
-			cp_commit();
+				at[i] = in_page[i] < 0 ? PG_NONE : drafted ? (uint32_t)(in_page[i] * p.d.kv_tok >> 4) : p.c.at(entry[i], in_page[i]);
 			if (j + 2 < left) {
 				cursor_next<TK>(p, c, 1);
 				cursor_next<TK>(p, c, 1);
-				find();
+				look();
 			}
-			cp_wait<0>();
+			const int tile = (isv ? A::V : A::K) + st * A::OP;
+			if (j >= A::NST && !ta_wait(B, isv ? &B->vfree[st] : &B->kfree[st], (j / A::NST - 1) & 1, p.c)) break;
+#pragma unroll
+			for (int i = 0; i < 2; i++)
+#pragma unroll 4
+				for (int y = 0; y < CH; y++) {
+					const uint32_t o = __shfl_sync(~0u, at[i], y * RI + lane / CH);
+					const bool have = o != PG_NONE && piece;
+					cp16(d0 + tile + (i * 32 + y * RI) * 128 + (x0 ^ ((y * RI & 7) << 4)), base + ((unsigned long long)(have ? o : 0) << sh), have);
+				}
+			if (!isv && begin) { // the unit's Q, once the last S of the unit before is done
+				if (j > 0 && !ta_wait(B, &B->kfree[(j - 1) % A::NST], (j - 1) / A::NST & 1, p.c)) break;
+#pragma unroll 1
+				for (int i = 0; i < 2; i++) {
+					const int r = r0 + i * 32, t = r / p.d.group;
+					const uint32_t mine = r < rows ? (uint32_t)(((long long)t * p.d.q_tok + (long long)(r - t * p.d.group) * p.d.q_head) >> 4) : PG_NONE;
+#pragma unroll 4
+					for (int y = 0; y < CH; y++) {
+						const uint32_t o = __shfl_sync(~0u, mine, y * RI + lane / CH);
+						const bool have = o != PG_NONE && piece;
+						cp16(d0 + A::Q + (i * 32 + y * RI) * 128 + (x0 ^ ((y * RI & 7) << 4)), qb + ((unsigned long long)(have ? o : 0) << 4), have);
+					}
+				}
+			}
 			if (isv && drafted) {
 				// a row that some token does not see may hold anything, and 0 * infinity must not reach O: what is not
 				// finite is taken out here and put back for the tokens that see it when O is read
+				cp_commit();
+				cp_wait<0>();
 				bool odd = false;
 #pragma unroll
 				for (int i = 0; i < 2; i++)
 #pragma unroll 1
 					for (int y = 0; y < CH; y++) {
-						uint32_t *w = (uint32_t *)(dst + ta_at(half * 64 + i * 32 + y * (32 / CH) + lane / CH, ch));
+						uint32_t *w = (uint32_t *)(sm + tile + ta_at(half * 64 + i * 32 + y * RI + lane / CH, ch));
 #pragma unroll
 						for (int x = 0; x < 4; x++)
 							if (PgElem<T>::odd(w[x])) {
@@ -245,62 +268,48 @@ __global__ void __launch_bounds__(544, 1) k_tree_attn_tc(const AttnArgs p)
 					}
 				odd = __any_sync(~0u, odd);
 				if (lane == 0) *(volatile int *)&B->odd[j & 3][half] = odd;
-			}
-			fence_async_smem();
-			mbar_arrive_warp(full);
+				mbar_arrive(&B->vfull[st]); // of this thread's copies and of what it wrote itself
+			} else
+				cp_arrive(isv ? &B->vfull[st] : &B->kfull[st]);
 		}
+		cp_commit();
 		cp_wait<0>();
-	} else if (warp == 16) {
+	} else if (warp >= 16) {
 		// ---------------- MMA issue ----------------
 		if (lane == 0) {
 			const uint32_t id = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(RT >> 4) << 24); // f32 += f16 or bf16 products
-			const uint32_t idS = id | ((uint32_t)(TK >> 3) << 17), idO = id | ((uint32_t)(DP >> 3) << 17) | (1u << 16); // V MN-major
 			const uint32_t base = smem_u32(sm);
-			AttnCursor at[2] = {c, c}; // of the halves' next P V
-			int ns = 0, npv[2] = {0, 0}, units[2] = {0, 0};
-			bool ok = true;
-			long long idle0 = clock64();
-			for (uint32_t spins = 0; ok && (npv[0] < left || npv[1] < left);) {
-				bool did = false;
-				if (ns < left && ta_test(&B->kfull[ns & 1], (ns >> 1) & 1) && (ns < 2 || ta_test(&B->s_free[ns & 1], ((ns >> 1) - 1) & 1))) {
+			if (warp == 16) {
+				const uint32_t idS = id | ((uint32_t)(TK >> 3) << 17), q = base + A::Q;
+				for (int j = 0; j < left; j++) {
+					// over the P of two tiles before, once that has been used
+					if (j >= 2 && (!ta_poll(B, &B->p_empty[0][j & 1], ((j >> 1) - 1) & 1, p.c) || !ta_poll(B, &B->p_empty[1][j & 1], ((j >> 1) - 1) & 1, p.c))) break;
+					if (!ta_poll(B, &B->kfull[j % A::NST], j / A::NST & 1, p.c)) break;
+					fence_async_smem();
 					tc_fence_after();
-					const uint32_t q = base + A::Q, k = base + A::K + (ns & 1) * A::OP;
+					const uint32_t k = base + A::K + j % A::NST * A::OP;
 #pragma unroll
 					for (int kk = 0; kk < DP / 16; kk++)
-						tc_mma_f16(tmem + (ns & 1) * TK, sw128_kmajor_desc(q + (kk >> 2) * 16384 + (kk & 3) * 32),
+						tc_mma_f16(tmem + (j & 1) * TK, sw128_kmajor_desc(q + (kk >> 2) * 16384 + (kk & 3) * 32),
 							   sw128_kmajor_desc(k + (kk >> 2) * 16384 + (kk & 3) * 32), idS, kk > 0);
-					tc_commit(&B->s_full[ns & 1]);
-					tc_commit(&B->kfree[ns & 1]);
-					ns++;
-					did = true;
+					tc_commit(&B->s_full[j & 1]);
+					tc_commit(&B->kfree[j % A::NST]);
 				}
-#pragma unroll
-				for (int f = 0; f < 2; f++) {
-					const int j = npv[f];
-					if (j >= ns || !ta_test(&B->p_full[f][j & 1], (j >> 1) & 1) || !ta_test(&B->vfull[j & 1], (j >> 1) & 1)) continue;
-					const bool first = j == 0 || at[f].tile == 0;
-					if (first && j > 0 && !ta_test(&B->o_free, (units[f] - 1) & 1)) continue; // the unit before has been read
-					if (first) units[f]++;
+			} else {
+				const int f = warp - 17; // the half of the tile's keys
+				const uint32_t idO = id | ((uint32_t)(DP >> 3) << 17) | (1u << 16); // V MN-major
+				int unit = 0;
+				for (int j = 0; j < left; j++, cursor_next<TK>(p, c, 1)) {
+					const bool first = j == 0 || c.tile == 0;
+					if (first && unit++ && !ta_poll(B, &B->o_free, unit & 1, p.c)) break; // the unit before has been read
+					if (!ta_poll(B, &B->vfull[j % A::NST], j / A::NST & 1, p.c) || !ta_poll(B, &B->p_full[f][j & 1], (j >> 1) & 1, p.c)) break;
+					fence_async_smem();
 					tc_fence_after();
-					const uint32_t pa = base + A::P + (j & 1) * A::PB + f * 16384, v = base + A::V + (j & 1) * A::OP + f * 8192;
+					const uint32_t pa = tmem + (j & 1) * TK + f * 64, v = base + A::V + j % A::NST * A::OP + f * 8192;
 #pragma unroll
-					for (int kk = 0; kk < 4; kk++)
-						tc_mma_f16(tmem + 256 + f * DP, sw128_kmajor_desc(pa + kk * 32), ta_mn_desc(v + kk * 2048, 16384), idO, !first || kk > 0);
+					for (int kk = 0; kk < 4; kk++) ta_mma_ts(tmem + 256 + f * DP, pa + kk * 8, ta_mn_desc(v + kk * 2048, 16384), idO, !first || kk > 0);
 					tc_commit(&B->p_empty[f][j & 1]);
-					tc_commit(&B->vfree[j & 1]);
-					npv[f]++;
-					cursor_next<TK>(p, at[f], 1);
-					did = true;
-				}
-				if (did) {
-					idle0 = clock64(), spins = 0;
-				} else if ((++spins & 63) == 0) {
-					if (*(volatile int *)&B->abort) ok = false;
-					else if (clock64() - idle0 > WAIT_CYCLES) {
-						p.c.report(PG_WAIT);
-						*(volatile int *)&B->abort = 1;
-						ok = false;
-					}
+					tc_commit(&B->vfree[j % A::NST]);
 				}
 			}
 			// every MMA issued has completed before TMEM is released (also after an abort)
@@ -332,8 +341,6 @@ __global__ void __launch_bounds__(544, 1) k_tree_attn_tc(const AttnArgs p)
 			float z[64];
 			tmem_ld32(lanes + (j & 1) * TK + hf * 64, *(float (*)[32])z);
 			tmem_ld32(lanes + (j & 1) * TK + hf * 64 + 32, *(float (*)[32])(z + 32));
-			tc_fence_before();
-			mbar_arrive_warp(&B->s_free[j & 1]);
 #pragma unroll
 			for (int e = 0; e < 64; e++) z[e] *= zs;
 			if (drafted || c.tile == c.ctx - 1) { // the mask's bits, or the end of the cache
@@ -350,8 +357,7 @@ __global__ void __launch_bounds__(544, 1) k_tree_attn_tc(const AttnArgs p)
 			const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), ref0 = mr;
 			const bool raise = top > mr + (SHIFT + RAISE), scale = raise && ref0 != -INFINITY;
 			if (raise) mr = top - SHIFT;
-			if (j > 1 && !ta_wait(B, &B->p_empty[hf][j & 1], ((j >> 1) - 1) & 1, p.c)) break; // this P buffer's product is done
-			if (__any_sync(~0u, scale)) { // O waits for that of the tile before, too (scale: there is one)
+			if (__any_sync(~0u, scale)) { // once the product of the tile before is done (scale: there is one)
 				if (!ta_wait(B, &B->p_empty[hf][(j - 1) & 1], ((j - 1) >> 1) & 1, p.c)) break;
 				const float f = scale ? ex2(ref0 - mr) : 1;
 				l *= f;
@@ -359,24 +365,23 @@ __global__ void __launch_bounds__(544, 1) k_tree_attn_tc(const AttnArgs p)
 #pragma unroll 1
 				for (int w = 0; w < DP / 32; w++) {
 					float v[32];
+					uint32_t u[32];
 					tmem_ld32(mine + w * 32, v);
 #pragma unroll
-					for (int e = 0; e < 32; e++) v[e] *= f;
-					tmem_st32(mine + w * 32, v);
+					for (int e = 0; e < 32; e++) u[e] = __float_as_uint(v[e] * f);
+					ta_st32(mine + w * 32, u);
 				}
 			}
 			const float ref = mr == -INFINITY ? 0 : mr;
 			float sum[4] = {0, 0, 0, 0};
+			uint32_t pw[32];
 #pragma unroll
-			for (int i = 0; i < 8; i++) {
+			for (int e = 0; e < 64; e++) sum[e & 3] += z[e] = ex2(z[e] - ref);
 #pragma unroll
-				for (int e = 8 * i; e < 8 * i + 8; e++) sum[e & 3] += z[e] = ex2(z[e] - ref);
-				*(uint4 *)(sm + A::P + (j & 1) * A::PB + ta_at(row, hf * 8 + i)) = make_uint4(pack16(z[8 * i], z[8 * i + 1], T()), pack16(z[8 * i + 2], z[8 * i + 3], T()),
-											pack16(z[8 * i + 4], z[8 * i + 5], T()), pack16(z[8 * i + 6], z[8 * i + 7], T()));
-			}
+			for (int i = 0; i < 32; i++) pw[i] = pack16(z[2 * i], z[2 * i + 1], T());
+			ta_st32(lanes + (j & 1) * TK + hf * 64, pw); // 64 keys in 32 columns
 			l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 			tc_fence_before();
-			fence_async_smem();
 			mbar_arrive_warp(&B->p_full[hf][j & 1]);
 
 			const bool end = c.tile == c.all - 1;
@@ -410,11 +415,12 @@ __global__ void __launch_bounds__(544, 1) k_tree_attn_tc(const AttnArgs p)
 								if (!isfinite(y)) v[e] += y;
 							}
 						}
+					if (!complete) {
 #pragma unroll
-					for (int e = 0; e < 32; e += 4) {
-						const float4 y = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-						if (!complete) *(float4 *)(slot + row * DP + w * 32 + e) = y;
-						else if (r < rows) store_row4<T>(p, to, w * 32 + e, y);
+						for (int e = 0; e < 32; e += 4) *(float4 *)(slot + slot_at<DP, RT>(row, w * 32 + e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+					} else if (r < rows) {
+#pragma unroll
+						for (int e = 0; e < 32; e += 8) store_row8<T>(p, to, w * 32 + e, v + e);
 					}
 				}
 				if (complete && hf == 0 && r < rows) store_lse(to, both, sl);
