@@ -427,8 +427,8 @@ int tg_cuda_kv_commit(const tg_cuda_kv *c, const tg_cuda_drafts *d, const int *p
  * ascending order. A sequence of at most budget positions keeps all; a longer one keeps its
  * first `sink` and last `recent` and, of those between, the budget - sink - recent with the
  * largest acc (ties: the lower position; NaN counts below every number). keep [seqs][nkv]
- * [budget] = the kept positions, -1 past the last; acc_out, alike, their acc, 0 past the
- * last; len_out[b] = min(len, budget). dst's pages (of src's pools or others) may not be
+ * [budget] = the kept positions, -1 past the last; acc_out, alike, their acc (-0 may become 0), 0
+ * past the last; len_out[b] = min(len, budget). dst's pages (of src's pools or others) may not be
  * among the pages src's sequences hold; dst->len and dst->max_len are not read. A kept row
  * past dst's table is not written and is reported like a bad page. */
 int tg_cuda_kv_evict(const tg_cuda_kv *src, const tg_cuda_kv *dst, const float *acc, long long acc_seq, long long acc_head,

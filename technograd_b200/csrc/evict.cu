@@ -1,5 +1,7 @@
 // evict.cu -- tg_cuda_kv_evict: the positions of a paged cache to keep by their accumulated
 // attention weight, and their rows' copy to other pages.
+#include <cooperative_groups.h>
+
 #include "paged.cuh"
 
 namespace tgc {
@@ -12,107 +14,251 @@ struct EvictArgs {
 	int *keep;
 	float *acc_out;
 	int *len_out;
-	int chunks; // 16-byte pieces of a row
-	long long heads; // sequences times kv heads
+	int pieces, lg;   // 16-byte pieces of a row's K and V together, and its logarithm where it is a power of two, else -1
+	long long heads;  // sequences times kv heads
 };
 
 // A weight's place in the order: unsigned, larger = kept first. Negative numbers reverse, -0 is 0,
-// NaN is below -infinity (whose key is 0x007fffff).
+// NaN (1) is below -infinity (whose key is 0x007fffff). EV_NONE is a position that does not compete.
+constexpr uint32_t EV_NONE = 0;
 __device__ __forceinline__ uint32_t evict_key(float x)
 {
-	if (isnan(x)) return 0;
+	if (isnan(x)) return 1;
 	const uint32_t u = __float_as_uint(x == 0 ? 0.0f : x);
 	return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+// The weight of a key (a zero is +0, a NaN any).
+__device__ __forceinline__ float evict_weight(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// Sum over the CTA's 1024 threads, to every thread.
-__device__ __forceinline__ int block_sum(int v, int *s)
-{
-	v = __reduce_add_sync(~0u, v);
-	__syncthreads();
-	if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-	__syncthreads();
-	return __reduce_add_sync(~0u, s[threadIdx.x & 31]);
-}
+constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32, EV_CLUSTER = 8, EV_LIST = 512;
 
-// One CTA per (sequence, kv head): the threshold key by bisection over its 32 bits, then one pass
-// in order that takes every position above it and the first ones that equal it.
-__global__ void __launch_bounds__(1024) k_evict_select(const EvictArgs p)
+// What the CTAs of a cluster exchange.
+struct EvictShared {
+	int part[2][EV_WARPS];    // a warp's counts
+	int count[2][EV_CLUSTER]; // the CTAs' counts, in turns
+	int sure[EV_CLUSTER], ties[EV_CLUSTER];
+	uint32_t thr;
+	int above, least, n_list;
+	uint32_t list[EV_LIST];
+};
+
+// One cluster of CTAs per (sequence, kv head). A CTA has an equal run of the positions, a warp a run of that
+// one, and a thread holds KPT of their keys in registers (0: any number, read again from L2 each time).
+// The threshold is the want-th largest key, found bit by bit: count the keys that reach a candidate, over
+// the cluster. Once few enough keys share the threshold's prefix (after about ten bits),
+// the first CTA's first warp finishes alone on their list. Every position above the threshold is kept, and the first
+// ones that equal it; ballots over the runs give each its place.
+// What bounds it: latency. The weights come in one round of loads, a count is 2 KPT instructions a
+// thread and a barrier or two.
+template <int KPT>
+__global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p)
 {
-	__shared__ int s[32], sa[32], sb[32];
-	const int h = blockIdx.x % p.src.nkv, b = blockIdx.x / p.src.nkv, tid = threadIdx.x;
+	namespace cg = cooperative_groups;
+	__shared__ EvictShared s;
+	cg::cluster_group cluster = cg::this_cluster();
+	const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+	pdl_launch();
+	pdl_wait();
+	const long long head = blockIdx.x / ranks;
+	const int h = (int)(head % p.src.nkv), b = (int)(head / p.src.nkv), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	const int n = p.src.length(b);
 	const float *acc = p.acc + b * p.acc_seq + h * p.acc_head;
-	int *keep = p.keep + (long long)blockIdx.x * p.budget;
-	float *out = p.acc_out + (long long)blockIdx.x * p.budget;
-	const int kept = min(n, p.budget);
-	if (h == 0 && tid == 0) p.len_out[b] = kept;
-	for (int i = kept + tid; i < p.budget; i += 1024) keep[i] = -1, out[i] = 0;
-	if (n <= p.budget) {
-		for (int i = tid; i < n; i += 1024) keep[i] = i, out[i] = acc[i];
+	int *keep = p.keep + head * p.budget;
+	float *out = p.acc_out + head * p.budget;
+	const int kept = min(n, p.budget), all = ranks * EV_THREADS, me = rank * EV_THREADS + tid;
+	if (h == 0 && me == 0) p.len_out[b] = kept;
+	for (int i = kept + me; i < p.budget; i += all) keep[i] = -1, out[i] = 0;
+	if (n <= p.budget) { // of the whole cluster
+		for (int i = me; i < n; i += all) keep[i] = i, out[i] = acc[i];
 		return;
 	}
+	// the first and last positions have their places; want of those between compete for theirs
 	const int lo = p.sink, hi = n - p.recent, want = p.budget - p.sink - p.recent; // 0 <= want < hi - lo
-	uint32_t thr = 0;                                                             // the want-th largest key
-	for (int bit = 31; bit >= 0; bit--) {
-		const uint32_t c = thr | 1u << bit;
+	for (int i = me; i < lo; i += all) keep[i] = i, out[i] = acc[i];
+	for (int i = hi + me; i < n; i += all) keep[i - n + p.budget] = i, out[i - n + p.budget] = acc[i];
+	if (want == 0) return; // of the whole cluster
+	keep += lo, out += lo;
+	// the warp's positions, `per` from w0 on: all whole warps' worth
+	const int per = KPT ? KPT * 32 : (int)(((long long)n + ranks * EV_WARPS * 32 - 1) / (ranks * EV_WARPS * 32)) * 32;
+	const int w0 = (rank * EV_WARPS + warp) * per; // within int: at most 8192 past n
+	auto fresh = [&](int i) { // (every lane loads, so that the loads go out together)
+		const uint32_t x = evict_key(acc[min(i, n - 1)]);
+		return i < lo || i >= hi ? EV_NONE : x;
+	};
+	uint32_t k[KPT ? KPT : 1];
+	if constexpr (KPT > 0) {
+		float a[KPT];
+#pragma unroll
+		for (int u = 0; u < KPT; u++) a[u] = acc[min(w0 + u * 32 + lane, n - 1)];
+#pragma unroll
+		for (int u = 0; u < KPT; u++) {
+			const int i = w0 + u * 32 + lane;
+			k[u] = i < lo || i >= hi ? EV_NONE : evict_key(a[u]);
+		}
+	}
+	// f(position, key) for the thread's positions, in order, the warp's lanes together
+	auto each = [&](auto f) {
+		if constexpr (KPT > 0) {
+#pragma unroll
+			for (int u = 0; u < KPT; u++) f(w0 + u * 32 + lane, k[u]);
+		} else
+			for (int i = w0; i < w0 + per && i < n; i += 32) f(i + lane, fresh(i + lane));
+	};
+	auto sync = [&]() {
+		if (ranks > 1) cluster.sync();
+		else __syncthreads();
+	};
+	int turn = 0;
+	// the cluster's total of a count, to every thread of it
+	auto total = [&](int v) {
+		v = __reduce_add_sync(~0u, v);
+		if (lane == 0) s.part[turn][warp] = v;
+		__syncthreads();
+		v = __reduce_add_sync(~0u, s.part[turn][lane]);
+		if (ranks > 1) {
+			if (tid < ranks) *cluster.map_shared_rank(&s.count[turn][rank], tid) = v;
+			cluster.sync();
+			v = 0;
+			for (int r = 0; r < ranks; r++) v += s.count[turn][r];
+		}
+		turn ^= 1; // the next count's words are read by nobody any more
+		return v;
+	};
+	auto reach = [&](uint32_t c) { // keys >= c, this thread's
 		int m = 0;
-		for (int i = lo + tid; i < hi; i += 1024) m += evict_key(acc[i]) >= c;
-		if (block_sum(m, s) >= want) thr = c;
+		each([&](int, uint32_t x) { m += x >= c; });
+		return m;
+	};
+	uint32_t thr = 0;        // its bits so far
+	int bit = 31, above = 0, least = hi - lo; // keys above every one that shares thr's bits; keys that reach thr, at most
+	auto step = [&]() {
+		const uint32_t c = thr | 1u << bit;
+		const int m = total(reach(c));
+		if (m >= want) thr = c, least = m;
+		else above = m;
+		bit--;
+	};
+	// the last bits of thr, by the first warp alone: c keys on its list
+	auto finish = [&](int c) {
+		uint32_t x[EV_LIST / 32];
+#pragma unroll
+		for (int u = 0; u < EV_LIST / 32; u++) x[u] = u * 32 + lane < c ? s.list[u * 32 + lane] : EV_NONE;
+		auto those = [&](uint32_t from) {
+			int m = 0;
+#pragma unroll
+			for (int u = 0; u < EV_LIST / 32; u++) m += x[u] >= from;
+			return above + __reduce_add_sync(~0u, m);
+		};
+		for (; bit >= 0; bit--)
+			if (those(thr | 1u << bit) >= want) thr |= 1u << bit;
+		least = those(thr);
+		above = those(thr + 1);
+		if (lane == 0) s.thr = thr, s.above = above, s.least = least;
+	};
+	if (KPT == 1 && ranks == 1 && n <= EV_LIST) { // all on the list at once
+		if (tid < EV_LIST) s.list[tid] = fresh(tid);
+		__syncthreads();
+		if (warp == 0) finish(n);
+		__syncthreads();
+		thr = s.thr, above = s.above, least = s.least;
+	} else {
+		while (bit >= 0 && least - above > EV_LIST) step();
+		if (bit >= 0) {
+			// the keys that share the prefix, on the first CTA's list
+			if (rank == 0 && tid == 0) s.n_list = 0;
+			sync();
+			const uint32_t end = thr + (2u << bit) - 1; // the last key with the prefix
+			EvictShared *first = ranks > 1 ? cluster.map_shared_rank(&s, 0) : &s;
+			each([&](int, uint32_t x) {
+				if (x >= thr && x <= end && x != EV_NONE) first->list[atomicAdd(&first->n_list, 1)] = x; // any order: only counts are taken of it
+			});
+			sync();
+			if (rank == 0 && warp == 0) finish(s.n_list);
+			sync();
+			thr = first->thr, above = first->above, least = first->least;
+		} else above = total(reach(thr + 1));
 	}
-	int above = 0;
-	for (int i = lo + tid; i < hi; i += 1024) above += evict_key(acc[i]) > thr;
-	int ties = want - block_sum(above, s); // of the positions equal to thr, the first so many
-	if (want == 0) thr = 0xffffffffu, ties = 0;
-	int done = 0, tied = 0;
-	for (int i0 = 0; i0 < n; i0 += 1024) {
-		const int i = i0 + tid;
-		const bool mid = i >= lo && i < hi;
-		const uint32_t k = mid ? evict_key(acc[i]) : 0;
-		const bool tie = mid && k == thr, sure = i < n && (!mid || k > thr);
-		const unsigned bt = __ballot_sync(~0u, tie), below = (1u << (tid & 31)) - 1;
-		__syncthreads();
-		if ((tid & 31) == 0) sa[tid >> 5] = __popc(bt);
-		__syncthreads();
-		int rank = tied + __popc(bt & below);
-		for (int w = 0; w < 32; w++) {
-			if (w < tid >> 5) rank += sa[w];
-			tied += sa[w];
+	int ties = want - above; // of the positions that equal thr, the first so many
+	if (least == want) thr--, ties = 0; // all of them
+	// ---- in order: counts of each warp's run, then each writes its own
+	int n_sure = 0, n_tie = 0;
+	each([&](int, uint32_t x) {
+		n_sure += x > thr;
+		if (ties) n_tie += x == thr;
+	});
+	n_sure = __reduce_add_sync(~0u, n_sure), n_tie = __reduce_add_sync(~0u, n_tie);
+	__syncthreads();
+	if (lane == 0) s.part[0][warp] = n_sure, s.part[1][warp] = n_tie;
+	__syncthreads();
+	const int ps = s.part[0][lane], pt = s.part[1][lane];
+	int done = __reduce_add_sync(~0u, lane < warp ? ps : 0), tied = __reduce_add_sync(~0u, lane < warp ? pt : 0);
+	if (ranks > 1) {
+		const int as = __reduce_add_sync(~0u, ps), at = __reduce_add_sync(~0u, pt);
+		if (tid < ranks) {
+			EvictShared *o = cluster.map_shared_rank(&s, tid);
+			o->sure[rank] = as, o->ties[rank] = at;
 		}
-		const bool take = sure || (tie && rank < ties);
+		cluster.sync();
+		for (int r = 0; r < rank; r++) done += s.sure[r], tied += s.ties[r];
+	}
+	done += min(tied, ties);
+	const unsigned below = (1u << lane) - 1;
+	each([&](int i, uint32_t x) {
+		bool take = x > thr;
+		if (ties) { // the first `ties` of those that equal the threshold
+			const bool t = x == thr;
+			const unsigned bt = __ballot_sync(~0u, t);
+			take |= t && tied + __popc(bt & below) < ties;
+			tied += __popc(bt);
+		}
 		const unsigned bk = __ballot_sync(~0u, take);
-		if ((tid & 31) == 0) sb[tid >> 5] = __popc(bk);
-		__syncthreads();
-		int at = done + __popc(bk & below);
-		for (int w = 0; w < 32; w++) {
-			if (w < tid >> 5) at += sb[w];
-			done += sb[w];
+		if (take) {
+			const int at = done + __popc(bk & below);
+			keep[at] = i, out[at] = evict_weight(x); // (a load here would wait for the stores of the step before)
 		}
-		if (take) keep[at] = i, out[at] = acc[i];
-	}
+		done += __popc(bk);
+	});
 }
 
-// One warp per (kept position, kv head, sequence): the row's 16-byte pieces of K, then of V.
+// The copy, bound by HBM: a warp takes 32 kept positions of a head; a lane finds the places of one of them,
+// then the warp moves the rows' 16-byte pieces, K and V, eight loads in flight a lane.
 __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs p)
 {
-	const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-	const int lane = threadIdx.x & 31;
-	const long long bh = w / p.budget;
-	const int i = (int)(w - bh * p.budget), h = (int)(bh % p.src.nkv);
-	const long long b = bh / p.src.nkv;
+	pdl_launch();
+	pdl_wait();
+	const int groups = (p.budget + 31) / 32, lane = threadIdx.x & 31;
+	const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), bh = w / groups;
 	if (bh >= p.heads) return;
-	const int from = p.keep[bh * p.budget + i];
-	if (from < 0) return;
-	if (i >= (long long)p.dst.page * p.dst.cols) {
-		if (lane == 0) p.dst.report(PG_ROOM);
-		return;
+	const int i = (int)(w - bh * groups) * 32 + lane, h = (int)(bh % p.src.nkv);
+	const long long b = bh / p.src.nkv;
+	const int from = i < p.budget ? p.keep[bh * p.budget + i] : -1;
+	uint32_t s = PG_NONE, t = PG_NONE; // places, PG_NONE: zeros; no copy
+	if (from >= 0) {
+		if (i >= (long long)p.dst.page * p.dst.cols) p.dst.report(PG_ROOM);
+		else {
+			const int a = from / p.src.page, d = i / p.dst.page;
+			t = p.dst.at(p.dst.table[b * p.dst.cols + d], i - d * p.dst.page);
+			s = p.src.at(p.src.table[b * p.src.cols + a], from - a * p.src.page);
+		}
 	}
-	const long long s = p.src.row(p.src.table + b * p.src.cols, from), t = p.dst.row(p.dst.table + b * p.dst.cols, i);
-	if (t < 0) return;
-	for (int x = lane; x < 2 * p.chunks; x += 32) {
-		const int o = (x < p.chunks ? x : x - p.chunks) * 16;
-		const char *a = (x < p.chunks ? p.src.k : p.src.v) + s + h * p.src.head_b + o;
-		*(uint4 *)((x < p.chunks ? p.dst.k : p.dst.v) + t + h * p.dst.head_b + o) = s < 0 ? make_uint4(0, 0, 0, 0) : *(const uint4 *)a;
+	const int rows = 32 - __clz(__ballot_sync(~0u, t != PG_NONE)), pieces = p.pieces, half = pieces / 2;
+	const char *sk = p.src.k + h * p.src.head_b, *sv = p.src.v + h * p.src.head_b;
+	char *tk = p.dst.k + h * p.dst.head_b, *tv = p.dst.v + h * p.dst.head_b;
+	for (int x0 = 0; x0 < rows * pieces; x0 += 32 * 8) {
+		uint4 v[8];
+		char *to[8];
+#pragma unroll
+		for (int u = 0; u < 8; u++) {
+			const int x = x0 + u * 32 + lane, row = p.lg >= 0 ? x >> p.lg : x / pieces, c = x - row * pieces;
+			const uint32_t a = __shfl_sync(~0u, s, row & 31), d = __shfl_sync(~0u, t, row & 31);
+			const int o = (c < half ? c : c - half) * 16;
+			to[u] = row < rows && d != PG_NONE ? (c < half ? tk : tv) + ((unsigned long long)d << p.dst.shift) + o : nullptr;
+			v[u] = make_uint4(0, 0, 0, 0);
+			if (to[u] && a != PG_NONE) v[u] = __ldcs((const uint4 *)((c < half ? sk : sv) + ((unsigned long long)a << p.src.shift) + o));
+		}
+#pragma unroll
+		for (int u = 0; u < 8; u++)
+			if (to[u]) *(uint4 *)to[u] = v[u];
 	}
 }
 
@@ -140,14 +286,26 @@ extern "C" int tg_cuda_kv_evict(const tg_cuda_kv *src, const tg_cuda_kv *dst, co
 	if ((rc = pg_device(who, &sms, &p.src.status)) || src->seqs == 0) return rc;
 	p.dst.status = p.src.status;
 	p.acc = acc, p.acc_seq = acc_seq, p.acc_head = acc_head, p.budget = budget, p.recent = recent, p.sink = sink;
-	p.keep = keep, p.acc_out = acc_out, p.len_out = len_out, p.chunks = src->head_dim * pg_size(src->type) / 16;
-	const long long heads = (long long)src->seqs * src->nkv, blocks = (heads * budget + 7) / 8;
-	p.heads = heads;
-	if (blocks > 0x7fffffff || heads > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences, budget %d", who, src->seqs, budget);
+	p.keep = keep, p.acc_out = acc_out, p.len_out = len_out, p.pieces = src->head_dim * pg_size(src->type) / 8;
+	p.lg = -1;
+	if (!(p.pieces & (p.pieces - 1)))
+		for (p.lg = 0; 1 << p.lg < p.pieces;) p.lg++;
+	p.heads = (long long)src->seqs * src->nkv;
+	const long long blocks = (p.heads * ((budget + 31ll) / 32) + 7) / 8;
+	if (blocks > 0x7fffffff || p.heads * EV_CLUSTER > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences, budget %d", who, src->seqs, budget);
+	// a head's CTAs: as many as hold its keys in registers, and more where heads are fewer than SMs and the runs stay of
+	// some length (below 4096 keys a cluster's barriers cost more than the shorter passes give)
+	int ranks = 1;
+	while (ranks < EV_CLUSTER && (src->max_len > 32ll * EV_THREADS * ranks || (p.heads * ranks * 2 <= sms && src->max_len > 4096 * 2 * ranks))) ranks *= 2;
+	const long long run = ((long long)src->max_len + ranks - 1) / ranks;
 	cudaStream_t st = (cudaStream_t)stream;
-	k_evict_select<<<(unsigned)heads, 1024, 0, st>>>(p);
-	TGC_LAUNCH_CHECK();
-	k_evict_copy<<<(unsigned)blocks, 256, 0, st>>>(p);
-	TGC_LAUNCH_CHECK();
+	cudaLaunchConfig_t cfg = {};
+	cudaLaunchAttribute attr[2];
+	cfg.gridDim = dim3((unsigned)(p.heads * ranks)), cfg.blockDim = dim3(EV_THREADS), cfg.stream = st;
+	attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
+	attr[1].id = cudaLaunchAttributeClusterDimension, attr[1].val.clusterDim.x = ranks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+	cfg.attrs = attr, cfg.numAttrs = ranks > 1 ? 2 : 1;
+	TGC_CUDA(cudaLaunchKernelEx(&cfg, run <= EV_THREADS ? k_evict_select<1> : run <= 8 * EV_THREADS ? k_evict_select<8> : run <= 32 * EV_THREADS ? k_evict_select<32> : k_evict_select<0>, p));
+	TGC_CUDA(launch_pdl(k_evict_copy, dim3((unsigned)blocks), dim3(256), 0, st, p));
 	return TG_CUDA_OK;
 }

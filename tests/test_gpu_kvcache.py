@@ -460,3 +460,31 @@ def test_device_data_out_of_range_is_reported(cuda):
     assert "past the table" in reported(good)
     kvcache.commit(c.cache.with_lens(torch.tensor([0, 0], dtype=torch.int32, device="cuda"), 40), k, v, n, path=torch.full((2, 3), 3, dtype=torch.int32, device="cuda"))
     assert "path" in reported(good)
+
+
+@pytest.mark.parametrize("lens,nkv,budget,recent,sink,kind", [
+    ([131072], 1, 4000, 100, 4, "random"), ([131071, 40000], 2, 60000, 0, 0, "ties"), ([100000], 1, 5, 2, 3, "random"), ([450001], 1, 70000, 9, 1, "random"),
+    ([60000], 1, 59999, 0, 0, "same"), ([9000] * 3, 1, 4500, 0, 0, "same"), ([30000], 1, 29000, 0, 0, "nan")])
+def test_evict_long(cuda, lens, nkv, budget, recent, sink, kind):
+    """Heads whose weights span several CTAs, fit no shared memory, or are all alike."""
+    c = Case(lens, nkv, 1, 8, 64, "head", BF16, 1, spare=len(lens) * (-(-budget // 64)))
+    g = torch.Generator().manual_seed(12)
+    acc = torch.rand(len(lens), nkv, max(lens), generator=g)
+    if kind == "ties":
+        acc = (acc * 50).floor() / 50
+    if kind == "same":
+        acc[:] = 0.25
+    if kind == "nan":
+        acc[:, :, 100:] = math.nan
+    cols = -(-budget // 64)
+    dst = kvcache.PagedKV(c.pk, c.pv, c.free[:len(lens) * cols].view(len(lens), cols).int().cuda(), torch.zeros_like(c.len), max_len=0)
+    keep, out, _ = kvcache.evict(c.cache, dst, acc.cuda(), budget, recent, sink)
+    for b, n in enumerate(lens):
+        for h in range(nkv):
+            want = plain_keep(acc[b, h, :n].tolist(), n, budget, recent, sink)
+            assert keep[b, h].tolist() == want + [-1] * (budget - len(want))
+            w = torch.tensor(want)
+            assert torch.equal(torch.nan_to_num(out[b, h, :len(want)].cpu(), 7), torch.nan_to_num(acc[b, h][w], 7))
+            i = torch.arange(len(want))
+            at = dst.table[b].cpu()[i // 64].long().cuda(), h, (i % 64).cuda()
+            assert torch.equal(c.pk[at].cpu(), c.k[b][w, h]) and torch.equal(c.pv[at].cpu(), c.v[b][w, h])
