@@ -24,19 +24,19 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a)
 // d += a b: a 16 x 16 (16 x 8 for tf32) row-major fragments, b 16 x 8 (8 x 8) column-major
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16)
 {
-	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+	asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
 		     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
 		     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half)
 {
-	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+	asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
 		     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
 		     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-	asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+	asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
 		     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
 		     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -115,6 +115,66 @@ __device__ __forceinline__ void qk_tile(float (&s)[MT][NT][4], uint32_t sq, uint
 					mma8(s[m][0], al, bh[2 * e], bh[2 * e + 1]);
 					mma8(s[m][0], ah, bl[2 * e], bl[2 * e + 1]);
 					mma8(s[m][0], ah, bh[2 * e], bh[2 * e + 1]);
+				}
+		}
+	}
+}
+
+// A tile of KW keys as the operand of Q K^T, in registers: for many query rows, which then each
+// take their own loads only. f32: hi and lo parts.
+template <class T, int DP> struct KeyFrag { uint32_t r[DP / 16][sizeof(T) == 2 ? 4 : 8]; };
+
+template <class T, int DP>
+__device__ __forceinline__ void load_keys(KeyFrag<T, DP> &f, uint32_t sk, int lane)
+{
+	constexpr int P = DP * (int)sizeof(T);
+	const int l7 = lane & 7, mi = lane >> 3;
+#pragma unroll
+	for (int k = 0; k < DP / 16; k++) {
+		if constexpr (sizeof(T) == 2) ldsm4(f.r[k], sk + ((mi >> 1) * 8 + l7) * P + (((2 * k + (mi & 1)) ^ l7) << 4));
+		else {
+			uint32_t b[4];
+			ldsm4(b, sk + l7 * P + (((4 * k + mi) ^ l7) << 4));
+#pragma unroll
+			for (int i = 0; i < 4; i++) tf32_split(b[i], f.r[k][i], f.r[k][4 + i]);
+		}
+	}
+}
+
+// S[MT x 16 rows, KW keys] = Q K^T, Q's rows from sq on; the MT tiles' products are independent
+template <class T, int DP, int MT, int NT>
+__device__ __forceinline__ void qk_keys(float (&s)[MT][NT][4], const KeyFrag<T, DP> &f, uint32_t sq, int lane)
+{
+	constexpr int P = DP * (int)sizeof(T);
+	const int l7 = lane & 7, mi = lane >> 3;
+	const uint32_t qrow = sq + ((mi & 1) * 8 + l7) * P;
+#pragma unroll
+	for (int m = 0; m < MT; m++)
+#pragma unroll
+		for (int x = 0; x < NT; x++) s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = 0;
+#pragma unroll
+	for (int k = 0; k < DP / 16; k++) {
+		if constexpr (sizeof(T) == 2) {
+			uint32_t a[MT][4];
+#pragma unroll
+			for (int m = 0; m < MT; m++) ldsm4(a[m], qrow + m * 16 * P + (((2 * k + (mi >> 1)) ^ l7) << 4));
+#pragma unroll
+			for (int m = 0; m < MT; m++) {
+				mma16(s[m][0], a[m], f.r[k][0], f.r[k][1], T());
+				mma16(s[m][1], a[m], f.r[k][2], f.r[k][3], T());
+			}
+		} else {
+#pragma unroll
+			for (int e = 0; e < 2; e++)
+#pragma unroll
+				for (int m = 0; m < MT; m++) {
+					uint32_t a[4], ah[4], al[4];
+					ldsm4(a, qrow + m * 16 * P + (((4 * k + 2 * e + (mi >> 1)) ^ l7) << 4));
+#pragma unroll
+					for (int i = 0; i < 4; i++) tf32_split(a[i], ah[i], al[i]);
+					mma8(s[m][0], al, f.r[k][2 * e], f.r[k][2 * e + 1]);
+					mma8(s[m][0], ah, f.r[k][4 + 2 * e], f.r[k][4 + 2 * e + 1]);
+					mma8(s[m][0], ah, f.r[k][2 * e], f.r[k][2 * e + 1]);
 				}
 		}
 	}

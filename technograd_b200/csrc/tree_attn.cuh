@@ -128,7 +128,7 @@ __device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int 
 	share = (all + gridDim.x - 1) / gridDim.x;
 	if (share < p.least + p.begin) share = p.least + p.begin;
 	pos = share * blockIdx.x;
-	if (threadIdx.x == 0) p.split[blockIdx.x].x = -1;
+	if (threadIdx.x == 0 && p.split) p.split[blockIdx.x].x = -1;
 	if (pos >= all) return false;
 	const long long to = all - pos < share ? all : pos + share; // the place after the share
 	long long base = 0;
