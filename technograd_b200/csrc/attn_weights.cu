@@ -1,16 +1,9 @@
 // attn_weights.cu -- tg_cuda_attn_weights: the attention weight that a paged cache's positions receive.
 #include <type_traits>
 
-#include "tree_attn.cuh"
+#include "attn_weights_tc.cuh"
 
 namespace tgc {
-
-struct WeightArgs : AttnArgs { // its lse is the input; out and part are not used
-	const unsigned long long *select;
-	const float *acc;
-	long long acc_seq, acc_head;
-	float *acc_out, *fresh;
-};
 
 // The weights' kernel goes through the keys as k_tree_attn does (tree_attn.cuh): equal shares of all
 // (sequence, kv head) units' tiles, a ring of asynchronous copies per warp, drafted tokens after the cached
@@ -19,7 +12,8 @@ struct WeightArgs : AttnArgs { // its lse is the input; out and part are not use
 // registers and, at the tile's end, over lanes. Every key is one warp's, so nothing is joined and results
 // do not depend on timing. Up to QR rows stay in shared memory for a unit; more are taken in turns at
 // every tile.
-// What bounds it: HBM while the rows are few; the tensor cores (mma.sync) from about 64 rows on.
+// What bounds it: HBM while the rows are few, then instruction issue (about 540 a warp for 16 keys and 64 rows);
+// 16-bit caches of more rows take attn_weights_tc.cuh.
 template <class T, int DP> struct WeightTile {
 	// eight warps where the keys' registers allow two such CTAs per SM: the products' latencies need them
 	static constexpr int NW = sizeof(T) == 2 && DP <= 128 ? 8 : 4, THREADS = 32 * NW;
@@ -42,8 +36,6 @@ __global__ void __launch_bounds__(WeightTile<T, DP>::THREADS, 2) k_attn_weights(
 	const int extra = (p.d.tokens + TK - 1) / TK, rows = p.d.tokens * p.d.group, chunks = p.c.dim * (int)sizeof(T) / 16;
 	const int turns = (rows + QR - 1) / QR;
 	const float zs = p.d.scale * 1.4426950408889634f;
-	pdl_launch();
-	pdl_wait();
 	AttnCursor c;
 	long long left, pos, share;
 	if (!attn_share<TK, W::NW>(p, (long long *)(smem + W::SCAN), extra, c, left, pos, share)) return;
@@ -208,13 +200,38 @@ static int weights_run(WeightArgs &p, int sms, int dev, cudaStream_t st, const c
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences", who, p.seqs);
 	p.row_tiles = 1, p.whole = 0, p.least = W::TK < 128 ? 128 / W::TK : 1, p.begin = 1, p.split = nullptr;
 	const long long shares = (units * (tiles + p.begin) + p.least + p.begin - 1) / (p.least + p.begin), wave = 2ll * sms;
-	TGC_CUDA(launch_pdl(k_attn_weights<T, DP>, dim3((unsigned)(shares < wave ? shares : wave)), dim3(W::THREADS), W::SMEM, st, p));
+	k_attn_weights<T, DP><<<(unsigned)(shares < wave ? shares : wave), W::THREADS, W::SMEM, st>>>(p);
+	TGC_LAUNCH_CHECK();
 	return TG_CUDA_OK;
 }
+
+template <class T, int DP>
+static int weights_run_tc(WeightArgs &p, int sms, int dev, cudaStream_t st, const char *who)
+{
+	using W = TwTile<DP>;
+	static std::atomic<unsigned long long> done{0};
+	int rc = pg_smem(k_attn_weights_tc<T, DP>, W::SMEM, dev, done);
+	if (rc) return rc;
+	const long long units = (long long)p.seqs * p.c.nkv, tiles = (p.c.max_len + W::TK - 1) / W::TK + 1;
+	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences", who, p.seqs);
+	p.row_tiles = 1, p.whole = 0, p.least = 1, p.begin = 2, p.split = nullptr;
+	const long long shares = (units * (tiles + p.begin) + p.begin) / (1 + p.begin);
+	k_attn_weights_tc<T, DP><<<(unsigned)(shares < sms ? shares : sms), W::THREADS, W::SMEM, st>>>(p);
+	TGC_LAUNCH_CHECK();
+	return TG_CUDA_OK;
+}
+
+// From so many query rows per key head on (and up to TW_ROWS), 16-bit caches take attn_weights_tc.cuh.
+constexpr int WEIGHTS_TC_ROWS = 32;
 
 template <class T>
 static int weights_type(WeightArgs &p, int sms, int dev, cudaStream_t st, const char *who)
 {
+	if constexpr (sizeof(T) == 2) {
+		const int rows = p.d.tokens * p.d.group;
+		if (p.c.dim <= 128 && rows > WEIGHTS_TC_ROWS && rows <= TW_ROWS)
+			return p.c.dim > 64 ? weights_run_tc<T, 128>(p, sms, dev, st, who) : weights_run_tc<T, 64>(p, sms, dev, st, who);
+	}
 	if (p.c.dim > 128) return weights_run<T, 256>(p, sms, dev, st, who);
 	return p.c.dim > 64 ? weights_run<T, 128>(p, sms, dev, st, who) : weights_run<T, 64>(p, sms, dev, st, who);
 }

@@ -12,7 +12,11 @@ constexpr int ATTN_WHOLE = 256;
 // From so many query rows per key head on, 16-bit caches take the 128-row tiles of tree_attn_tc.cuh.
 constexpr int ATTN_TC_ROWS = 32;
 
-constexpr int ATTN_BEGIN = 2; // what beginning a unit costs, in tiles
+// What beginning a unit costs, in tiles. The 128-row tiles' is about 6 (their chain of products and the output), but
+// where shares are short every CTA has such a start of its own and counting it only makes them uneven: 48
+// sequences of up to 6001 positions, 90 tiles a CTA, take 187 us at 6 and 211 at 2; 8 of up to 1280, 4 tiles
+// a CTA, 33 and 27.
+constexpr int ATTN_BEGIN = 2, ATTN_TC_BEGIN = 6, ATTN_LONG = 24;
 
 static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o)
 {
@@ -27,9 +31,9 @@ static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, At
 	const long long units = (long long)c->seqs * c->nkv * o->row_tiles;
 	const long long tiles = (c->max_len + tk - 1) / tk + (d.tokens + tk - 1) / tk;
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
-	o->whole = tiles * tk <= ATTN_WHOLE, o->least = 128 / tk;
+	o->whole = tiles * tk <= ATTN_WHOLE, o->least = 128 / tk, o->begin = o->tc && units * tiles > (long long)ATTN_LONG * o->sms ? ATTN_TC_BEGIN : ATTN_BEGIN;
 	o->slot = (size_t)(rt * o->dp + 2 * rt) * 4;
-	const long long shares = (units * (tiles + ATTN_BEGIN) + o->least + ATTN_BEGIN - 1) / (o->least + ATTN_BEGIN), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : 2);
+	const long long shares = (units * (tiles + o->begin) + o->least + o->begin - 1) / (o->least + o->begin), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : 2);
 	o->grid = (int)(o->whole ? units : shares < wave ? shares : wave);
 	return TG_CUDA_OK;
 }
@@ -70,7 +74,7 @@ extern "C" int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, v
 	if (need && (!work || work_bytes < (long long)need || ((uintptr_t)work & 15)))
 		return set_err(TG_CUDA_EINVAL, "%s: needs %zu bytes of 16-byte aligned scratch", who, need);
 	p.out = (char *)out, p.out_seq = out_seq * e, p.out_tok = out_tok * e, p.out_head = out_head * e, p.lse = lse;
-	p.seqs = c->seqs, p.row_tiles = pl.row_tiles, p.whole = pl.whole, p.least = pl.least, p.begin = ATTN_BEGIN;
+	p.seqs = c->seqs, p.row_tiles = pl.row_tiles, p.whole = pl.whole, p.least = pl.least, p.begin = pl.begin;
 	p.split = (int4 *)work, p.part = (float *)((char *)work + (size_t)pl.grid * sizeof(int4));
 	cudaStream_t st = (cudaStream_t)stream;
 	return c->type == TG_CUDA_F32 ? attn_type<float>(p, pl, st) : c->type == TG_CUDA_F16 ? attn_type<__half>(p, pl, st) : attn_type<__nv_bfloat16>(p, pl, st);

@@ -23,6 +23,13 @@ struct AttnArgs {
 	int4 *split;     // shares: per CTA, the unit that begins in its share and ends in a later one
 };
 
+struct WeightArgs : AttnArgs { // its lse is the input; out and part are not used
+	const unsigned long long *select;
+	const float *acc;
+	long long acc_seq, acc_head;
+	float *acc_out, *fresh;
+};
+
 // The kernel for few query rows. Per (sequence b, kv head h) the query rows are r = t * group + g
 // (token t, query head h * group + g): every head of the group and every drafted token meet a key
 // while it is in shared memory, so the cache is read once for up to 16 * MT rows.
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(128) k_attn_join(const AttnArgs p)
 
 // How a call is cut.
 struct AttnPlan {
-	int dp, mt, row_tiles, whole, least, grid, sms, dev, tc; // mt: 16-row products of a tile; tc: 128-row tiles on tcgen05
+	int dp, mt, row_tiles, whole, least, begin, grid, sms, dev, tc; // mt: 16-row products of a tile; tc: 128-row tiles on tcgen05
 	size_t slot; // bytes of a partial result
 	size_t bytes() const { return whole ? 0 : (size_t)grid * (2 * slot + sizeof(int4)); }
 };

@@ -13,8 +13,13 @@ static int attn_run(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 	static std::atomic<unsigned long long> done{0};
 	int rc = pg_smem(k_tree_attn<T, DP, MT>, A::SMEM, pl.dev, done);
 	if (rc) return rc;
+	if (pl.whole) { // one kernel: the plain launch is the cheaper one for the host
+		k_tree_attn<T, DP, MT><<<pl.grid, 128, A::SMEM, st>>>(p);
+		TGC_LAUNCH_CHECK();
+		return TG_CUDA_OK;
+	}
 	TGC_CUDA(launch_pdl(k_tree_attn<T, DP, MT>, dim3(pl.grid), dim3(128), A::SMEM, st, p));
-	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT * DP / 1024), dim3(128), 0, st, p));
+	TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT * DP / 1024), dim3(128), 0, st, p));
 	return TG_CUDA_OK;
 }
 

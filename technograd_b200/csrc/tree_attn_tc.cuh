@@ -62,7 +62,8 @@ __device__ __forceinline__ bool ta_test(uint64_t *bar, uint32_t parity)
 }
 
 // Bounded wait; false after the CTA's abort flag or the cycle budget, which sets it.
-__device__ __forceinline__ bool ta_poll(TaBars *B, uint64_t *bar, uint32_t parity, const PgCache &c)
+template <class BARS>
+__device__ __forceinline__ bool ta_poll(BARS *B, uint64_t *bar, uint32_t parity, const PgCache &c)
 {
 	if (ta_test(bar, parity)) return true;
 	const long long t0 = clock64();
@@ -79,7 +80,8 @@ __device__ __forceinline__ bool ta_poll(TaBars *B, uint64_t *bar, uint32_t parit
 	}
 }
 // ... of a whole warp, which leaves together
-__device__ __forceinline__ bool ta_wait(TaBars *B, uint64_t *bar, uint32_t parity, const PgCache &c) { return __all_sync(~0u, ta_poll(B, bar, parity, c)); }
+template <class BARS>
+__device__ __forceinline__ bool ta_wait(BARS *B, uint64_t *bar, uint32_t parity, const PgCache &c) { return __all_sync(~0u, ta_poll(B, bar, parity, c)); }
 
 // 32 lanes x 32 columns of TMEM
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32])

@@ -14,10 +14,15 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import torch
 
 from . import _lib
+
+# tg_cuda_drafts as bytes, which ctypes passes by address: cheaper than filling a Structure each call
+_pack_drafts = struct.Struct("@2if4xP3q2P3q2P").pack
+assert struct.calcsize("@2if4xP3q2P3q2P") == C.sizeof(_lib.Drafts)
 
 _TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
@@ -76,7 +81,8 @@ class PagedKV:
                     k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), table.data_ptr(), lens.data_ptr())
         self._struct = s
         self._at = C.addressof(s)
-        self._work = {}  # (tokens, nq) -> bytes of tree_attention's scratch
+        self._plans = {}  # (tokens, nq) -> bytes of tree_attention's scratch, and a shape to make its lse like
+        self._one = torch.empty(1, dtype=torch.float32, device=k.device)
 
     def with_lens(self, lens: torch.Tensor, max_len: int | None = None) -> "PagedKV":
         """The same pages with other lengths (what `commit` returned)."""
@@ -84,7 +90,7 @@ class PagedKV:
 
 
 def _drafts(cache: PagedKV, q, k, v, mask, count, scale):
-    """The C description of drafted tokens, checked."""
+    """The C description of drafted tokens (tg_cuda_drafts), checked."""
     index, dt, n, dim = cache.index, cache.dtype, k.shape, cache.head_dim
     sk = k.stride()
     if k.dtype is not dt or k.get_device() != index or len(n) != 4 or n[0] != cache.seqs or n[2] != cache.nkv or n[3] != dim or sk[3] != 1:
@@ -103,9 +109,9 @@ def _drafts(cache: PagedKV, q, k, v, mask, count, scale):
         _check("mask", mask, torch.int64, n[:2], index)
     if count is not None:
         _check("count", count, torch.int32, n[:1], index)
-    return _lib.Drafts(n[1], nq, cache.scale if scale is None else scale, None if q is None else q.data_ptr(), sq[0], sq[1], sq[2],
-                       k.data_ptr(), None if v is None else v.data_ptr(), sk[0], sk[1], sk[2],
-                       None if mask is None else mask.data_ptr(), None if count is None else count.data_ptr())
+    return _pack_drafts(n[1], nq, cache.scale if scale is None else scale, 0 if q is None else q.data_ptr(), sq[0], sq[1], sq[2],
+                        k.data_ptr(), 0 if v is None else v.data_ptr(), sk[0], sk[1], sk[2],
+                        0 if mask is None else mask.data_ptr(), 0 if count is None else count.data_ptr())
 
 
 def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float | None = None):
@@ -115,20 +121,19 @@ def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float 
     tokens. mask int64 [seqs, tokens]: bit u of an entry = the token attends to drafted token u (None:
     a chain). count int32 [seqs]: tokens drafted (None: all). Returns (out as q, lse f32 [seqs, tokens,
     nq]); a token that sees nothing has out 0 and lse -inf."""
-    d = C.byref(_drafts(cache, q, k, v, mask, count, scale))
-    stream, L, shape = _stream(cache), _lib.lib(), q.shape
-    out = torch.empty_like(q)
-    lse = q.new_empty(shape[:3], dtype=torch.float32)
-    so = out.stride()
-    size = cache._work.get(shape[1:3])
-    if size is None:
-        size = L.tg_cuda_tree_attn_workspace(cache._at, d)
+    d = _drafts(cache, q, k, v, mask, count, scale)
+    stream, shape = _stream(cache), q.shape
+    plan = cache._plans.get(shape[1:3])
+    if plan is None:
+        size = _lib.lib().tg_cuda_tree_attn_workspace(cache._at, d)
         if size < 0:
             _lib.check(size)
-        cache._work[shape[1:3]] = size
-    work = q.new_empty(size, dtype=torch.uint8) if size else None
-    _lib.check(L.tg_cuda_tree_attn(cache._at, d, out.data_ptr(), so[0], so[1], so[2], lse.data_ptr(), work.data_ptr() if size else None,
-                                   size, stream))
+        plan = cache._plans[shape[1:3]] = size, cache._one.expand(shape[:3])
+    size, like = plan
+    out, lse = torch.empty_like(q), torch.empty_like(like)
+    work = q.new_empty(size, dtype=torch.uint8).data_ptr() if size else None  # kept by the allocator for this stream until the call has run
+    so = out.stride()
+    _lib.check(_lib.lib().tg_cuda_tree_attn(cache._at, d, out.data_ptr(), so[0], so[1], so[2], lse.data_ptr(), work, size, stream))
     return out, lse
 
 
@@ -139,7 +144,7 @@ def attention_weights(cache: PagedKV, q, k, lse, mask=None, count=None, select=N
     tokens that count, as bits (None: all). acc f32 [seqs, nkv, >= max_len]: what the cached
     positions had before (None: zeros). Returns (acc + weight [seqs, nkv, max_len], zero past a
     sequence's length; the drafted tokens' own weight [seqs, nkv, tokens])."""
-    d = C.byref(_drafts(cache, q, k, None, mask, count, scale))
+    d = _drafts(cache, q, k, None, mask, count, scale)
     n = q.shape
     _check("lse", lse, torch.float32, n[:3], cache.index)
     if select is not None:
@@ -158,7 +163,7 @@ def commit(cache: PagedKV, k, v, count, path=None, new=None, acc=None):
     path[b, i] (path int32 [seqs, tokens]; None: row i) for i < count[b]. With new (the drafted tokens'
     weight from attention_weights) and acc f32 [seqs, nkv, cols], acc[b, h, lens + i] = new[b, h, path[b, i]] too.
     Returns the new lengths; the pages and acc are written in place. Any number of tokens."""
-    d = C.byref(_drafts(cache, None, k, v, None, count, 1.0))
+    d = _drafts(cache, None, k, v, None, count, 1.0)
     T = k.shape[1]
     if path is not None:
         _check("path", path, torch.int32, (cache.seqs, T), cache.index)

@@ -304,14 +304,10 @@ def test_weights_in_place_and_masked_rows(cuda):
     assert torch.allclose(total, torch.tensor([[6.0], [6.0]], device="cuda").expand(2, 2), atol=1e-4)
     acc = one.clone()
     two, _ = kvcache.attention_weights(c.cache, q, kn, lse, mask.cuda(), acc=acc)
-    d = _lib.Drafts
-    drafts = kvcache._drafts(c.cache, q, kn, None, mask.cuda(), None, None)
-    assert isinstance(drafts, d)
     m = mask.cuda()
-    drafts.mask = m.data_ptr()
+    drafts = kvcache._drafts(c.cache, q, kn, None, m, None, None)
     fresh2 = torch.empty_like(fresh)
-    import ctypes
-    _lib.check(cuda.tg_cuda_attn_weights(c.cache._at, ctypes.byref(drafts), lse.data_ptr(), None, acc.data_ptr(), acc.stride(0), acc.stride(1),
+    _lib.check(cuda.tg_cuda_attn_weights(c.cache._at, drafts, lse.data_ptr(), None, acc.data_ptr(), acc.stride(0), acc.stride(1),
                                          acc.data_ptr(), fresh2.data_ptr(), torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()
     assert torch.equal(acc, two) and torch.equal(fresh, fresh2)
