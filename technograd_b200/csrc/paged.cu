@@ -1,5 +1,8 @@
 // paged.cu -- descriptions of a paged key/value cache, checked on the host, and
 // tg_cuda_kv_commit.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
 #include <mutex>
 
 #include "paged.cuh"
@@ -107,6 +110,29 @@ int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, int
 	o->mask = d->mask, o->count = d->count, o->tokens = d->tokens, o->scale = d->scale;
 	o->nq = use & PG_USE_Q ? d->nq : c->nkv, o->group = o->nq / c->nkv;
 	return TG_CUDA_OK;
+}
+
+bool pg_map(CUtensorMap *m, const PgCache &c, const void *pool, bool f16, int rows, PgBox *box)
+{
+	static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+	static std::once_flag once;
+	std::call_once(once, [] {
+		cudaDriverEntryPointQueryResult q;
+		void *fn = nullptr;
+		if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+			encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+	});
+	box->rows = std::min(rows, c.page), box->swap = c.head_b < c.pos_b;
+	const long long first = std::min(c.head_b, c.pos_b), second = std::max(c.head_b, c.pos_b);
+	if (!encode || c.pages <= 0 || c.page % 8 || (rows % c.page && c.page % rows) || first <= 0 || second % first || c.page_b % second || c.page_b <= 0 ||
+	    c.page_b >= 1ll << 40)
+		return false;
+	const cuuint64_t dims[4] = { (cuuint64_t)c.dim, (cuuint64_t)(box->swap ? c.nkv : c.page), (cuuint64_t)(box->swap ? c.page : c.nkv), (cuuint64_t)c.pages };
+	const cuuint64_t strides[3] = { (cuuint64_t)first, (cuuint64_t)second, (cuuint64_t)c.page_b };
+	const cuuint32_t size[4] = { 64, (cuuint32_t)(box->swap ? 1 : box->rows), (cuuint32_t)(box->swap ? box->rows : 1), 1 }, es[4] = { 1, 1, 1, 1 };
+	return encode(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void *)pool, dims, strides, size, es,
+		      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+		      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // ---- commit -------------------------------------------------------------------------------

@@ -2,6 +2,7 @@
 // address of a row, the status word, element types and the host's checks of a description.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -108,6 +109,13 @@ int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, int
 // of an earlier call reported something.
 int pg_device(const char *who, int *sms, int **status);
 int pg_sms(const char *who, int *dev, int *sms); // the current device and its SM count alone
+// A TMA map of a pool of 16-bit elements, for boxes of 64 dimensions x as many rows of a page as `rows` and the page
+// allow, 128-byte swizzle. Coordinates: dimension, then row and head (head and row with `swap`: TMA wants
+// ascending strides), then page. False where the pages or strides do not suit boxes of whole 8-row atoms.
+struct PgBox {
+	int rows, swap;
+};
+bool pg_map(CUtensorMap *m, const PgCache &c, const void *pool, bool f16, int rows, PgBox *box);
 static inline int pg_size(int type) { return type == TG_CUDA_F32 ? 4 : 2; }
 
 } // namespace tgc

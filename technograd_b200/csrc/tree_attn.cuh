@@ -19,6 +19,7 @@ struct AttnArgs {
 	int whole;       // 1: a CTA per unit; 0: equal shares of the units' tiles
 	int least;       // shares: tiles per CTA at least
 	int begin;       // shares: what beginning a unit costs, in tiles
+	PgBox box;       // of the pools' TMA maps; rows 0: none
 	float *part;     // shares: partial results, two slots per CTA
 	int4 *split;     // shares: per CTA, the unit that begins in its share and ends in a later one
 };

@@ -30,7 +30,11 @@ static int attn_run_tc(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 	static std::atomic<unsigned long long> done{0};
 	int rc = pg_smem(k_tree_attn_tc<T, DP>, A::SMEM, pl.dev, done);
 	if (rc) return rc;
-	TGC_CUDA(launch_pdl(k_tree_attn_tc<T, DP>, dim3(pl.grid), dim3(A::THREADS), A::SMEM, st, p));
+	AttnArgs a = p;
+	CUtensorMap maps[2] = {};
+	const bool f16 = std::is_same<T, __half>::value;
+	if (!pg_map(&maps[0], p.c, p.c.k, f16, 64, &a.box) || !pg_map(&maps[1], p.c, p.c.v, f16, 64, &a.box)) a.box.rows = 0;
+	TGC_CUDA(launch_pdl(k_tree_attn_tc<T, DP>, dim3(pl.grid), dim3(A::THREADS), A::SMEM, st, a, maps[0], maps[1]));
 	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT * DP / 1024), dim3(128), 0, st, p));
 	return TG_CUDA_OK;
 }

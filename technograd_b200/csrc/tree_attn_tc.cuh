@@ -123,6 +123,18 @@ __device__ __forceinline__ void ta_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint
 		: "memory");
 }
 
+// Box of a 4D map into shared memory, its bytes counted on bar; x a multiple of 8, places outside the map are zeros
+__device__ __forceinline__ void ta_box(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int x, int c1, int c2, int c3)
+{
+	asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+		     "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(c1), "r"(c2), "r"(c3)
+		     : "memory");
+}
+__device__ __forceinline__ void ta_expect(uint64_t *bar, uint32_t bytes)
+{
+	asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
 // An arrival of this thread on bar (counted in its initial count) once all its cp.async copies so far have landed
 __device__ __forceinline__ void cp_arrive(uint64_t *bar)
 {
@@ -136,11 +148,31 @@ __device__ __forceinline__ uint64_t ta_mn_desc(uint32_t saddr, uint32_t lbo)
 	return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
+// packed f32 arithmetic, two elements an instruction, and the largest of three
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+	unsigned long long d;
+	asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b), "l"(*(unsigned long long *)&c));
+	return *(float2 *)&d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+	unsigned long long d;
+	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
+	return *(float2 *)&d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+	float d;
+	asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+	return d;
+}
+
 // 16-byte chunk c of row r of an operand tile of 128 rows
 __device__ __forceinline__ uint32_t ta_at(int r, int c) { return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
 template <class T, int DP>
-__global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p)
+__global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
 {
 	using A = TaTile<DP>;
 	constexpr int TK = A::TK, RT = A::RT, CH = A::CH;
@@ -191,15 +223,19 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p)
 		// this lane's rows half * 64 + lane and + 32 more: the table's entries, then the rows' places
 		int entry[2], in_page[2];
 		uint32_t at[2];
+		// by TMA, lane i has box i / (DP / 64) of its half's 64 rows, and 64 of its dimensions
+		constexpr int ND = DP / 64;
+		const int boxes = p.box.rows ? 64 / p.box.rows : 0;
+		auto by_box = [&]() { return boxes && c.tile < c.ctx - isv; };
 		auto look = [&]() {
-			const bool drafted = c.tile >= c.ctx;
+			const bool drafted = c.tile >= c.ctx, box = by_box();
 #pragma unroll
 			for (int i = 0; i < 2; i++) {
-				const int x = (drafted ? 0 : c.tile * TK) + half * 64 + i * 32 + lane;
+				const int x = (drafted ? 0 : c.tile * TK) + half * 64 + (box ? lane / ND * p.box.rows : i * 32 + lane);
 				in_page[i] = -1;
 				if (drafted) {
 					if (x < p.d.drafted(c.b)) in_page[i] = x;
-				} else if (x < c.n) {
+				} else if (x < c.n && !(box && (i || lane >= boxes * ND))) {
 					const int page = x / p.c.page;
 					in_page[i] = x - page * p.c.page;
 					entry[i] = p.c.table[(long long)c.b * p.c.cols + page];
@@ -210,8 +246,10 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p)
 			if (par) cursor_next<TK>(p, c, 1);
 			look();
 		}
+		int last = -1; // tile asked for
 		for (int j = par; j < left; j += 2) {
-			const bool drafted = c.tile >= c.ctx, begin = j == 0 || c.tile == 0;
+			const bool drafted = c.tile >= c.ctx, begin = j == 0 || c.tile == 0, box = by_box();
+			const int kvh = c.h;
 			const int sh = drafted ? 4 : p.c.shift;
 			const char *base = (drafted ? (isv ? p.d.v : p.d.k) + (long long)c.b * p.d.kv_seq + c.h * p.d.kv_head : (isv ? p.c.v : p.c.k) + c.h * p.c.head_b) + ch * 16;
 			const int st = j % A::NST;
@@ -219,7 +257,8 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p)
 			const int r0 = c.r * RT + half * 64 + lane;
 #pragma unroll
 			for (int i = 0; i < 2; i++)
-				at[i] = in_page[i] < 0 ? PG_NONE : drafted ? (uint32_t)(in_page[i] * p.d.kv_tok >> 4) : p.c.at(entry[i], in_page[i]);
+				at[i] = in_page[i] < 0 ? PG_NONE : box ? (uint32_t)((unsigned)entry[i] < (unsigned)p.c.pages ? in_page[i] : (p.c.report(PG_PAGE), -1)) : drafted ? (uint32_t)(in_page[i] * p.d.kv_tok >> 4) : p.c.at(entry[i], in_page[i]);
+			const int page = entry[0];
 			if (j + 2 < left) {
 				cursor_next<TK>(p, c, 1);
 				cursor_next<TK>(p, c, 1);
@@ -227,6 +266,17 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p)
 			}
 			const int tile = (isv ? A::V : A::K) + st * A::OP;
 			if (j >= A::NST && !ta_wait(B, isv ? &B->vfree[st] : &B->kfree[st], (j / A::NST - 1) & 1, p.c)) break;
+			uint64_t *full = isv ? &B->vfull[st] : &B->kfull[st];
+			last = j;
+			if (box) {
+				if (lane == 0) ta_expect(full, 64 * DP * 2);
+				__syncwarp();
+				if (lane < boxes * ND) {
+					const int r = at[0] == PG_NONE ? 0 : (int)at[0], g = at[0] == PG_NONE ? -1 : page; // -1: zeros
+					ta_box(smem_u32(sm) + tile + lane % ND * 16384 + (half * 64 + lane / ND * p.box.rows) * 128, isv ? &vmap : &kmap, full, lane % ND * 64,
+					       p.box.swap ? kvh : r, p.box.swap ? r : kvh, g);
+				}
+			} else
 #pragma unroll
 			for (int i = 0; i < 2; i++)
 #pragma unroll 4
@@ -270,12 +320,17 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p)
 					}
 				odd = __any_sync(~0u, odd);
 				if (lane == 0) *(volatile int *)&B->odd[j & 3][half] = odd;
-				mbar_arrive(&B->vfull[st]); // of this thread's copies and of what it wrote itself
+				mbar_arrive(full); // of this thread's copies and of what it wrote itself
 			} else
-				cp_arrive(isv ? &B->vfull[st] : &B->kfull[st]);
+				cp_arrive(full);
 		}
 		cp_commit();
 		cp_wait<0>();
+		// boxes still on their way land before the CTA's shared memory is released: those of this warp's last
+		// tile, and of the one before where no other warp has waited for it
+		auto landed = [&](int j) { mbar_wait(isv ? &B->vfull[j % A::NST] : &B->kfull[j % A::NST], j / A::NST & 1, nullptr, 0); };
+		if (last >= 0) landed(last);
+		if (last >= 2 && last + 1 >= left) landed(last - 2);
 	} else if (warp >= 16) {
 		// ---------------- MMA issue ----------------
 		if (lane == 0) {
@@ -343,20 +398,26 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p)
 			float z[64];
 			tmem_ld32(lanes + (j & 1) * TK + hf * 64, *(float (*)[32])z);
 			tmem_ld32(lanes + (j & 1) * TK + hf * 64 + 32, *(float (*)[32])(z + 32));
-#pragma unroll
-			for (int e = 0; e < 64; e++) z[e] *= zs;
+			float mul = zs; // what turns z into the exponent
 			if (drafted || c.tile == c.ctx - 1) { // the mask's bits, or the end of the cache
 				const int n = drafted ? 0 : (int)(c.n - (long long)c.tile * TK) - hf * 64;
 				const unsigned long long ok = drafted ? (hf ? 0ull : see) : n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
 				const uint32_t lo = (uint32_t)ok, hi = (uint32_t)(ok >> 32);
 #pragma unroll
-				for (int e = 0; e < 64; e++)
-					if (!((e < 32 ? lo : hi) >> (e & 31) & 1)) z[e] = -INFINITY;
+				for (int e = 0; e < 64; e++) z[e] = (e < 32 ? lo : hi) >> (e & 31) & 1 ? z[e] * zs : -INFINITY;
+				mul = 1;
 			}
-			float x[4] = {z[0], z[1], z[2], z[3]};
+			float x[4] = {z[0], z[1], z[2], z[3]}, top;
+			if (mul >= 0) {
 #pragma unroll
-			for (int e = 4; e < 64; e++) x[e & 3] = fmaxf(x[e & 3], z[e]);
-			const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), ref0 = mr;
+				for (int e = 4; e < 64; e += 2) x[e >> 1 & 3] = max3(x[e >> 1 & 3], z[e], z[e + 1]);
+				top = max3(x[0], x[1], fmaxf(x[2], x[3])) * mul;
+			} else {
+#pragma unroll
+				for (int e = 4; e < 64; e++) x[e & 3] = fminf(x[e & 3], z[e]);
+				top = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])) * mul;
+			}
+			const float ref0 = mr;
 			const bool raise = top > mr + (SHIFT + RAISE), scale = raise && ref0 != -INFINITY;
 			if (raise) mr = top - SHIFT;
 			if (__any_sync(~0u, scale)) { // once the product of the tile before is done (scale: there is one)
@@ -375,14 +436,17 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p)
 				}
 			}
 			const float ref = mr == -INFINITY ? 0 : mr;
-			float sum[4] = {0, 0, 0, 0};
+			float2 sum[2] = {make_float2(0, 0), make_float2(0, 0)};
 			uint32_t pw[32];
 #pragma unroll
-			for (int e = 0; e < 64; e++) sum[e & 3] += z[e] = ex2(z[e] - ref);
-#pragma unroll
-			for (int i = 0; i < 32; i++) pw[i] = pack16(z[2 * i], z[2 * i + 1], T());
+			for (int i = 0; i < 32; i++) {
+				const float2 y = fma2(make_float2(z[2 * i], z[2 * i + 1]), make_float2(mul, mul), make_float2(-ref, -ref));
+				const float2 q = make_float2(ex2(y.x), ex2(y.y));
+				sum[i & 1] = add2(sum[i & 1], q);
+				pw[i] = pack16(q.x, q.y, T());
+			}
 			ta_st32(lanes + (j & 1) * TK + hf * 64, pw); // 64 keys in 32 columns
-			l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+			l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 			tc_fence_before();
 			mbar_arrive_warp(&B->p_full[hf][j & 1]);
 

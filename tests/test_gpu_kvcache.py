@@ -484,3 +484,27 @@ def test_evict_long(cuda, lens, nkv, budget, recent, sink, kind):
             i = torch.arange(len(want))
             at = dst.table[b].cpu()[i // 64].long().cuda(), h, (i % 64).cuda()
             assert torch.equal(c.pk[at].cpu(), c.k[b][w, h]) and torch.equal(c.pv[at].cpu(), c.v[b][w, h])
+
+
+@pytest.mark.parametrize("page,order", [(8, "head"), (16, "pos"), (32, "head"), (64, "pos"), (128, "head"), (192, "pos"), (256, "head"), (40, "pos"), (4, "head")])
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (BF16, 72)])
+def test_many_rows_over_pages(cuda, page, order, dtype, dim):
+    """Tiles of many rows read pages in boxes or row by row; what lies past a sequence's end is NaN."""
+    c = Case([1, 127, 128, 129, 700, 0], 2, 3, dim, page, order, dtype, 33)
+    mask = random_mask(6, 33, 7)
+    out, lse, want = check_attend(c, mask)
+    acc, fresh = kvcache.attention_weights(c.cache, c.q.cuda(), c.kn.cuda(), want[1].float().cuda(), mask.cuda())
+    rows = (want[1] > -INF).sum(1).view(6, 2, 3).sum(2)  # each row that sees something spreads a weight of 1
+    assert (acc.sum(2).cpu() + fresh.sum(2).cpu() - rows).abs().max() < 1e-3
+
+
+def test_negative_and_zero_scale(cuda):
+    for tokens in (2, 40):
+        c = Case([300, 9], 2, 2, 128, 16, "head", BF16, tokens)
+        for scale in (-0.1, 0.0):
+            out, lse = attend(c, scale=scale)
+            flip = Case([300, 9], 2, 2, 128, 16, "head", BF16, tokens)
+            flip.q = -flip.q if scale < 0 else flip.q * 0
+            want = plain(flip, scale=abs(scale) or 0.1)
+            near(out, want[0], want[2], "out")
+            near(lse, want[1], want[3], "lse")
