@@ -35,6 +35,7 @@ static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, At
 	o->slot = (size_t)(rt * o->dp + 2 * rt) * 4;
 	const long long shares = (units * (tiles + o->begin) + o->least + o->begin - 1) / (o->least + o->begin), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : 2);
 	o->grid = (int)(o->whole ? units : shares < wave ? shares : wave);
+	o->units = (int)units, o->by_unit = !o->whole && units <= o->grid;
 	return TG_CUDA_OK;
 }
 
@@ -74,7 +75,7 @@ extern "C" int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, v
 	if (need && (!work || work_bytes < (long long)need || ((uintptr_t)work & 15)))
 		return set_err(TG_CUDA_EINVAL, "%s: needs %zu bytes of 16-byte aligned scratch", who, need);
 	p.out = (char *)out, p.out_seq = out_seq * e, p.out_tok = out_tok * e, p.out_head = out_head * e, p.lse = lse;
-	p.seqs = c->seqs, p.row_tiles = pl.row_tiles, p.whole = pl.whole, p.least = pl.least, p.begin = pl.begin;
+	p.seqs = c->seqs, p.row_tiles = pl.row_tiles, p.whole = pl.whole, p.least = pl.least, p.begin = pl.begin, p.by_unit = pl.by_unit;
 	p.split = (int4 *)work, p.part = (float *)((char *)work + (size_t)pl.grid * sizeof(int4));
 	cudaStream_t st = (cudaStream_t)stream;
 	return c->type == TG_CUDA_F32 ? attn_type<float>(p, pl, st) : c->type == TG_CUDA_F16 ? attn_type<__half>(p, pl, st) : attn_type<__nv_bfloat16>(p, pl, st);

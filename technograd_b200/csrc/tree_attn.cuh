@@ -21,7 +21,9 @@ struct AttnArgs {
 	int begin;       // shares: what beginning a unit costs, in tiles
 	PgBox box;       // of the pools' TMA maps; rows 0: none
 	float *part;     // shares: partial results, two slots per CTA
-	int4 *split;     // shares: per CTA, the unit that begins in its share and ends in a later one
+	int by_unit;     // shares: split's entries are the units', else the CTAs'
+	int4 *split;     // shares: of a unit that begins in a CTA's share and ends in a later one, the two CTAs, its
+	                 // sequence and head, and its row tile; x = -1: none, or nothing to join
 };
 
 struct WeightArgs : AttnArgs { // its lse is the input; out and part are not used
@@ -136,7 +138,7 @@ __device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int 
 	share = (all + gridDim.x - 1) / gridDim.x;
 	if (share < p.least + p.begin) share = p.least + p.begin;
 	pos = share * blockIdx.x;
-	if (threadIdx.x == 0 && p.split) p.split[blockIdx.x].x = -1;
+	if (threadIdx.x == 0 && p.split && !p.by_unit) p.split[blockIdx.x].x = -1;
 	if (pos >= all) return false;
 	const long long to = all - pos < share ? all : pos + share; // the place after the share
 	long long base = 0;
@@ -164,6 +166,15 @@ __device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int 
 	left -= tiles(s[NW], s[NW + 1], pos - s[NW + 1]);
 	c.tile = t, c.h = u / p.row_tiles, c.r = u % p.row_tiles;
 	return left > 0;
+}
+
+// Notes, at the end of the part of a unit that has its first tile, whether other CTAs have the rest. c: the part's last tile.
+__device__ __forceinline__ void attn_note(const AttnArgs &p, const AttnCursor &c, bool whole, long long pos, long long share)
+{
+	if (p.whole || (whole && !p.by_unit)) return;
+	const int head = c.b * p.c.nkv + c.h;
+	p.split[p.by_unit ? (long long)head * p.row_tiles + c.r : blockIdx.x] =
+		whole ? make_int4(-1, 0, 0, 0) : make_int4(blockIdx.x, (int)((pos + share + (c.all - 2 - c.tile)) / share), head, c.r);
 }
 
 // o (already over l, or a partial's) of 4 columns
@@ -470,8 +481,7 @@ __global__ void __launch_bounds__(128) k_tree_attn(const AttnArgs p)
 				}
 				__syncthreads();
 			}
-			if (!end && from_start && tid == 0) // the unit goes on in the CTAs after this one
-				p.split[blockIdx.x] = make_int4(b, h, c.r, (int)((pos + share + (c.all - 2 - c.tile)) / share));
+			if (from_start && tid == 0) attn_note(p, c, end, pos, share);
 			first = true;
 		}
 		__syncwarp(); // every lane is done with this stage
@@ -486,44 +496,62 @@ __global__ void __launch_bounds__(128) k_tree_attn(const AttnArgs p)
 // from the row per thread of 128-row tiles.
 template <int DP, int RT> __device__ __forceinline__ int slot_at(int row, int col) { return RT == 128 ? (col / 4 * RT + row) * 4 : row * DP + col; }
 
-// The parts of the units that several CTAs shared, added in CTA order: a thread has a row and 8 of its
-// columns, and the threads of a warp what lies together in a part.
-template <class T, int DP, int RT>
-__global__ void __launch_bounds__(128) k_attn_join(const AttnArgs p)
+// The parts of the units that several CTAs shared. A thread has a row and 8 of its columns, and the threads of a
+// warp what lies together in a part; the NG warps of a block take the parts in turn (each with a running
+// reference), and the first adds up what they have, in their order. Many parts (one long sequence) would be a
+// chain of loads for one warp: 37 parts took it 28 us.
+template <class T, int DP, int RT, int NG>
+__global__ void __launch_bounds__(32 * NG) k_attn_join(const AttnArgs p)
 {
 	constexpr int SLOT = RT * DP + 2 * RT, RW = RT == 128 ? 32 : 1; // rows side by side in a warp
+	__shared__ float s[NG > 1 ? NG : 1][10][32];
 	pdl_launch();
 	pdl_wait();
-	const int4 s = p.split[blockIdx.x];
-	if (s.x < 0) return;
-	const int rows = p.d.tokens * p.d.group, cnt = p.d.drafted(s.x), parts = s.w - (int)blockIdx.x + 1;
-	const float *first = p.part + (2ll * blockIdx.x + 1) * SLOT, *rest = p.part + 2ll * blockIdx.x * SLOT;
-	auto part = [&](int i) { return i ? rest + 2ll * i * SLOT : first; };
-	for (int x = blockIdx.y * 128 + threadIdx.x; x < RT * DP / 8; x += gridDim.y * 128) {
-		const int r = x / (RW * DP / 8) * RW + x % RW, col = x / RW % (DP / 8) * 8;
-		if (s.z * RT + r >= rows) continue;
-		float top = -INFINITY, l = 0, v[8] = {};
+	const int4 u = p.split[blockIdx.x];
+	if (u.x < 0) return;
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = u.z / p.c.nkv, h = u.z - b * p.c.nkv;
+	const int rows = p.d.tokens * p.d.group, cnt = p.d.drafted(b), parts = u.y - u.x + 1;
+	const int x = blockIdx.y * 32 + lane, r = x / (RW * DP / 8) * RW + x % RW, col = x / RW % (DP / 8) * 8;
+	if (u.w * RT + (RT == 128 ? r - lane : r) >= rows) return; // of the whole block: a warp has 32 rows or one
+	float top = -INFINITY, l = 0, v[8] = {};
+	auto add = [&](float m, float n, const float *y) {
+		const float t = fmaxf(top, m), f = top == -INFINITY ? 0 : ex2(top - t), a = m == -INFINITY ? 0 : ex2(m - t);
+		l = (top == -INFINITY ? l : l * f) + (m == -INFINITY ? n : n * a); // sums keep a NaN
+#pragma unroll
+		for (int i = 0; i < 8; i++) v[i] = (f == 0 ? 0 : v[i] * f) + (a == 0 ? 0 : y[i] * a);
+		top = t;
+	};
 #pragma unroll 4
-		for (int i = 0; i < parts; i++) top = fmaxf(top, part(i)[RT * DP + r]);
-#pragma unroll 4
-		for (int i = 0; i < parts; i++) {
-			const float *q = part(i);
-			const float m = q[RT * DP + r], a = m == -INFINITY ? 0 : ex2(m - top);
-			l += m == -INFINITY ? q[RT * DP + RT + r] : q[RT * DP + RT + r] * a;
-			const float4 y = *(const float4 *)(q + slot_at<DP, RT>(r, col)), z = *(const float4 *)(q + slot_at<DP, RT>(r, col + 4));
-			if (a == 0) continue;
-			v[0] += y.x * a, v[1] += y.y * a, v[2] += y.z * a, v[3] += y.w * a;
-			v[4] += z.x * a, v[5] += z.y * a, v[6] += z.z * a, v[7] += z.w * a;
-		}
-		const AttnRow to = attn_row(p, s.x, s.y, s.z * RT + r, cnt, l);
-		store_row8<T>(p, to, col, v);
-		if (col == 0) store_lse(to, top, l);
+	for (int i = warp; i < parts; i += NG) {
+		const float *q = p.part + (2ll * (u.x + i) + (i == 0)) * SLOT;
+		const float4 y = *(const float4 *)(q + slot_at<DP, RT>(r, col)), z = *(const float4 *)(q + slot_at<DP, RT>(r, col + 4));
+		const float w[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+		add(q[RT * DP + r], q[RT * DP + RT + r], w);
 	}
+	if constexpr (NG > 1) {
+		if (warp) {
+			s[warp][8][lane] = top, s[warp][9][lane] = l;
+#pragma unroll
+			for (int i = 0; i < 8; i++) s[warp][i][lane] = v[i];
+		}
+		__syncthreads();
+		if (warp) return;
+		for (int g = 1; g < NG && g < parts; g++) {
+			float w[8];
+#pragma unroll
+			for (int i = 0; i < 8; i++) w[i] = s[g][i][lane];
+			add(s[g][8][lane], s[g][9][lane], w);
+		}
+	}
+	if (u.w * RT + r >= rows) return;
+	const AttnRow to = attn_row(p, b, h, u.w * RT + r, cnt, l);
+	store_row8<T>(p, to, col, v);
+	if (col == 0) store_lse(to, top, l);
 }
 
 // How a call is cut.
 struct AttnPlan {
-	int dp, mt, row_tiles, whole, least, begin, grid, sms, dev, tc; // mt: 16-row products of a tile; tc: 128-row tiles on tcgen05
+	int dp, mt, row_tiles, whole, least, begin, grid, by_unit, units, sms, dev, tc; // mt: 16-row products of a tile; tc: 128-row tiles on tcgen05
 	size_t slot; // bytes of a partial result
 	size_t bytes() const { return whole ? 0 : (size_t)grid * (2 * slot + sizeof(int4)); }
 };

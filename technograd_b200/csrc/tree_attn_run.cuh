@@ -6,6 +6,15 @@
 
 namespace tgc {
 
+// Units shared by many CTAs (few units) have many parts each: eight warps a block for them.
+template <class T, int DP, int RT>
+static int attn_join(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
+{
+	if (pl.grid >= 4ll * pl.units) TGC_CUDA(launch_pdl(k_attn_join<T, DP, RT, 8>, dim3(pl.by_unit ? pl.units : pl.grid, RT * DP / 256), dim3(256), 0, st, p));
+	else TGC_CUDA(launch_pdl(k_attn_join<T, DP, RT, 1>, dim3(pl.by_unit ? pl.units : pl.grid, RT * DP / 256), dim3(32), 0, st, p));
+	return TG_CUDA_OK;
+}
+
 template <class T, int DP, int MT>
 static int attn_run(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 {
@@ -19,8 +28,7 @@ static int attn_run(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 		return TG_CUDA_OK;
 	}
 	TGC_CUDA(launch_pdl(k_tree_attn<T, DP, MT>, dim3(pl.grid), dim3(128), A::SMEM, st, p));
-	TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT * DP / 1024), dim3(128), 0, st, p));
-	return TG_CUDA_OK;
+	return attn_join<T, DP, A::RT>(p, pl, st);
 }
 
 template <class T, int DP>
@@ -35,8 +43,7 @@ static int attn_run_tc(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 	const bool f16 = std::is_same<T, __half>::value;
 	if (!pg_map(&maps[0], p.c, p.c.k, f16, 64, &a.box) || !pg_map(&maps[1], p.c, p.c.v, f16, 64, &a.box)) a.box.rows = 0;
 	TGC_CUDA(launch_pdl(k_tree_attn_tc<T, DP>, dim3(pl.grid), dim3(A::THREADS), A::SMEM, st, a, maps[0], maps[1]));
-	if (!pl.whole) TGC_CUDA(launch_pdl(k_attn_join<T, DP, A::RT>, dim3(pl.grid, A::RT * DP / 1024), dim3(128), 0, st, p));
-	return TG_CUDA_OK;
+	return pl.whole ? TG_CUDA_OK : attn_join<T, DP, A::RT>(p, pl, st);
 }
 
 template <class T>

@@ -491,8 +491,7 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 				}
 				if (complete && hf == 0 && r < rows) store_lse(to, both, sl);
 				if (!complete && hf == 0) slot[RT * DP + row] = both, slot[RT * DP + RT + row] = sl;
-				if (!end && from_start && tid == 0) // the unit goes on in the CTAs after this one
-					p.split[blockIdx.x] = make_int4(b, h, c.r, (int)((pos + share + (c.all - 2 - c.tile)) / share));
+				if (from_start && tid == 0) attn_note(p, c, end, pos, share);
 				tc_fence_before();
 				mbar_arrive_warp(&B->o_free);
 				unit++;
