@@ -214,7 +214,9 @@ static int weights_run_tc(WeightArgs &p, int sms, int dev, cudaStream_t st, cons
 	if (rc) return rc;
 	const long long units = (long long)p.seqs * p.c.nkv, tiles = (p.c.max_len + W::TK - 1) / W::TK + 1;
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences", who, p.seqs);
-	p.row_tiles = 1, p.whole = 0, p.least = 1, p.begin = 2, p.split = nullptr;
+	// a unit's start is worth about 6 tiles, except where every CTA has one of its own anyway (the window case: 120 us at 2,
+	// 84 at 4, 82 at 8)
+	p.row_tiles = 1, p.whole = 0, p.least = 1, p.begin = units * tiles > 24ll * sms ? 6 : 2, p.split = nullptr;
 	const long long shares = (units * (tiles + p.begin) + p.begin) / (1 + p.begin);
 	k_attn_weights_tc<T, DP><<<(unsigned)(shares < sms ? shares : sms), W::THREADS, W::SMEM, st>>>(p);
 	TGC_LAUNCH_CHECK();

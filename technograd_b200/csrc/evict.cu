@@ -16,6 +16,7 @@ struct EvictArgs {
 	int *len_out;
 	int pieces, lg;   // 16-byte pieces of a row's K and V together, and its logarithm where it is a power of two, else -1
 	long long heads;  // sequences times kv heads
+	int fused;        // the selecting CTA copies its rows itself
 };
 
 // A weight's place in the order: unsigned, larger = kept first. Negative numbers reverse, -0 is 0,
@@ -30,7 +31,54 @@ __device__ __forceinline__ uint32_t evict_key(float x)
 // The weight of a key (a zero is +0, a NaN any).
 __device__ __forceinline__ float evict_weight(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
+// The copy, bound by HBM: a warp takes 32 kept positions of a head; a lane finds the places of one of them,
+// then the warp moves the rows' 16-byte pieces, K and V, eight loads in flight a lane.
+__device__ __forceinline__ void evict_copy32(const EvictArgs &p, long long bh, int group)
+{
+	const int lane = threadIdx.x & 31, i = group * 32 + lane, h = (int)(bh % p.src.nkv);
+	const long long b = bh / p.src.nkv;
+	const int from = i < p.budget ? p.keep[bh * p.budget + i] : -1;
+	uint32_t s = PG_NONE, t = PG_NONE; // places, PG_NONE: zeros; no copy
+	if (from >= 0) {
+		if (i >= (long long)p.dst.page * p.dst.cols) p.dst.report(PG_ROOM);
+		else {
+			const int a = from / p.src.page, d = i / p.dst.page;
+			t = p.dst.at(p.dst.table[b * p.dst.cols + d], i - d * p.dst.page);
+			s = p.src.at(p.src.table[b * p.src.cols + a], from - a * p.src.page);
+		}
+	}
+	const int rows = 32 - __clz(__ballot_sync(~0u, t != PG_NONE)), pieces = p.pieces, half = pieces / 2;
+	const char *sk = p.src.k + h * p.src.head_b, *sv = p.src.v + h * p.src.head_b;
+	char *tk = p.dst.k + h * p.dst.head_b, *tv = p.dst.v + h * p.dst.head_b;
+	for (int x0 = 0; x0 < rows * pieces; x0 += 32 * 8) {
+		uint4 v[8];
+		char *to[8];
+#pragma unroll
+		for (int u = 0; u < 8; u++) {
+			const int x = x0 + u * 32 + lane, row = p.lg >= 0 ? x >> p.lg : x / pieces, c = x - row * pieces;
+			const uint32_t a = __shfl_sync(~0u, s, row & 31), d = __shfl_sync(~0u, t, row & 31);
+			const int o = (c < half ? c : c - half) * 16;
+			to[u] = row < rows && d != PG_NONE ? (c < half ? tk : tv) + ((unsigned long long)d << p.dst.shift) + o : nullptr;
+			v[u] = make_uint4(0, 0, 0, 0);
+			if (to[u] && a != PG_NONE) v[u] = __ldcs((const uint4 *)((c < half ? sk : sv) + ((unsigned long long)a << p.src.shift) + o));
+		}
+#pragma unroll
+		for (int u = 0; u < 8; u++)
+			if (to[u]) *(uint4 *)to[u] = v[u];
+	}
+}
+
+__global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs p)
+{
+	pdl_launch();
+	pdl_wait();
+	const int groups = (p.budget + 31) / 32;
+	const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), bh = w / groups;
+	if (bh < p.heads) evict_copy32(p, bh, (int)(w - bh * groups));
+}
+
 constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32, EV_CLUSTER = 8, EV_LIST = 512;
+constexpr long long EV_FUSED = 128 * 1024; // bytes of a head's kept rows
 
 // What the CTAs of a cluster exchange.
 struct EvictShared {
@@ -51,14 +99,11 @@ struct EvictShared {
 // What bounds it: latency. The weights come in one round of loads, a count is 2 KPT instructions a
 // thread and a barrier or two.
 template <int KPT>
-__global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p)
+__device__ __forceinline__ void evict_select(const EvictArgs &p, EvictShared &s)
 {
 	namespace cg = cooperative_groups;
-	__shared__ EvictShared s;
 	cg::cluster_group cluster = cg::this_cluster();
 	const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-	pdl_launch();
-	pdl_wait();
 	const long long head = blockIdx.x / ranks;
 	const int h = (int)(head % p.src.nkv), b = (int)(head / p.src.nkv), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	const int n = p.src.length(b);
@@ -220,46 +265,16 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p)
 	});
 }
 
-// The copy, bound by HBM: a warp takes 32 kept positions of a head; a lane finds the places of one of them,
-// then the warp moves the rows' 16-byte pieces, K and V, eight loads in flight a lane.
-__global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs p)
+template <int KPT>
+__global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p)
 {
+	__shared__ EvictShared s;
 	pdl_launch();
 	pdl_wait();
-	const int groups = (p.budget + 31) / 32, lane = threadIdx.x & 31;
-	const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), bh = w / groups;
-	if (bh >= p.heads) return;
-	const int i = (int)(w - bh * groups) * 32 + lane, h = (int)(bh % p.src.nkv);
-	const long long b = bh / p.src.nkv;
-	const int from = i < p.budget ? p.keep[bh * p.budget + i] : -1;
-	uint32_t s = PG_NONE, t = PG_NONE; // places, PG_NONE: zeros; no copy
-	if (from >= 0) {
-		if (i >= (long long)p.dst.page * p.dst.cols) p.dst.report(PG_ROOM);
-		else {
-			const int a = from / p.src.page, d = i / p.dst.page;
-			t = p.dst.at(p.dst.table[b * p.dst.cols + d], i - d * p.dst.page);
-			s = p.src.at(p.src.table[b * p.src.cols + a], from - a * p.src.page);
-		}
-	}
-	const int rows = 32 - __clz(__ballot_sync(~0u, t != PG_NONE)), pieces = p.pieces, half = pieces / 2;
-	const char *sk = p.src.k + h * p.src.head_b, *sv = p.src.v + h * p.src.head_b;
-	char *tk = p.dst.k + h * p.dst.head_b, *tv = p.dst.v + h * p.dst.head_b;
-	for (int x0 = 0; x0 < rows * pieces; x0 += 32 * 8) {
-		uint4 v[8];
-		char *to[8];
-#pragma unroll
-		for (int u = 0; u < 8; u++) {
-			const int x = x0 + u * 32 + lane, row = p.lg >= 0 ? x >> p.lg : x / pieces, c = x - row * pieces;
-			const uint32_t a = __shfl_sync(~0u, s, row & 31), d = __shfl_sync(~0u, t, row & 31);
-			const int o = (c < half ? c : c - half) * 16;
-			to[u] = row < rows && d != PG_NONE ? (c < half ? tk : tv) + ((unsigned long long)d << p.dst.shift) + o : nullptr;
-			v[u] = make_uint4(0, 0, 0, 0);
-			if (to[u] && a != PG_NONE) v[u] = __ldcs((const uint4 *)((c < half ? sk : sv) + ((unsigned long long)a << p.src.shift) + o));
-		}
-#pragma unroll
-		for (int u = 0; u < 8; u++)
-			if (to[u]) *(uint4 *)to[u] = v[u];
-	}
+	evict_select<KPT>(p, s);
+	if (!p.fused) return;
+	__syncthreads(); // the CTA's kept positions are written
+	for (int g = threadIdx.x >> 5; g < (p.budget + 31) / 32; g += EV_WARPS) evict_copy32(p, blockIdx.x, g);
 }
 
 } // namespace tgc
@@ -298,6 +313,8 @@ extern "C" int tg_cuda_kv_evict(const tg_cuda_kv *src, const tg_cuda_kv *dst, co
 	int ranks = 1;
 	while (ranks < EV_CLUSTER && (src->max_len > 32ll * EV_THREADS * ranks || (p.heads * ranks * 2 <= sms && src->max_len > 4096 * 2 * ranks))) ranks *= 2;
 	const long long run = ((long long)src->max_len + ranks - 1) / ranks;
+	// little to copy: a second kernel would take longer than the selecting CTAs do (200 positions of 64 bytes: 15 us a call against 12)
+	p.fused = ranks == 1 && p.heads <= sms && (long long)budget * p.pieces * 16 <= EV_FUSED;
 	cudaStream_t st = (cudaStream_t)stream;
 	cudaLaunchConfig_t cfg = {};
 	cudaLaunchAttribute attr[2];
@@ -306,6 +323,6 @@ extern "C" int tg_cuda_kv_evict(const tg_cuda_kv *src, const tg_cuda_kv *dst, co
 	attr[1].id = cudaLaunchAttributeClusterDimension, attr[1].val.clusterDim.x = ranks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
 	cfg.attrs = attr, cfg.numAttrs = ranks > 1 ? 2 : 1;
 	TGC_CUDA(cudaLaunchKernelEx(&cfg, run <= EV_THREADS ? k_evict_select<1> : run <= 8 * EV_THREADS ? k_evict_select<8> : run <= 32 * EV_THREADS ? k_evict_select<32> : k_evict_select<0>, p));
-	TGC_CUDA(launch_pdl(k_evict_copy, dim3((unsigned)blocks), dim3(256), 0, st, p));
+	if (!p.fused) TGC_CUDA(launch_pdl(k_evict_copy, dim3((unsigned)blocks), dim3(256), 0, st, p));
 	return TG_CUDA_OK;
 }

@@ -33,7 +33,7 @@ static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, At
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
 	o->whole = tiles * tk <= ATTN_WHOLE, o->least = 128 / tk, o->begin = o->tc && units * tiles > (long long)ATTN_LONG * o->sms ? ATTN_TC_BEGIN : ATTN_BEGIN;
 	o->slot = (size_t)(rt * o->dp + 2 * rt) * 4;
-	const long long shares = (units * (tiles + o->begin) + o->least + o->begin - 1) / (o->least + o->begin), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : 2);
+	const long long shares = (units * (tiles + o->begin) + o->least + o->begin - 1) / (o->least + o->begin), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : o->mt == 1 && c->type != TG_CUDA_F32 ? 3 : 2); // AttnTile's CTAS
 	o->grid = (int)(o->whole ? units : shares < wave ? shares : wave);
 	o->units = (int)units, o->by_unit = !o->whole && units <= o->grid;
 	return TG_CUDA_OK;

@@ -60,7 +60,10 @@ template <class T, int DP, int MT> struct AttnTile {
 	static constexpr int KW = sizeof(T) == 4 ? 8 : 16, NT = KW / 8, TK = 4 * KW, RT = 16 * MT;
 	static constexpr int P = DP * (int)sizeof(T), CH = P / 16;
 	static constexpr int STAGE = 2 * KW * P; // also 16 x DP floats, what the end of a unit needs
-	static constexpr int NST = DP == 256 || (DP == 128 && MT == 2 && sizeof(T) == 4) ? 2 : 3; // two CTAs per SM up to 128 dimensions
+	// 16 rows of 16-bit elements: three CTAs per SM with a stage ahead each, 167 us for a 256-sequence decode wave
+	// against 184 of two CTAs with two ahead; the others' registers allow two
+	static constexpr int CTAS = DP == 256 ? 1 : MT == 1 && sizeof(T) == 2 ? 3 : 2;
+	static constexpr int NST = CTAS == 3 || DP == 256 || (DP == 128 && MT == 2 && sizeof(T) == 4) ? 2 : 3;
 	static constexpr int Q = 0, RING = RT * P, MASK = RING + 4 * NST * STAGE, ML = MASK + RT * 8, SCAN = ML + 4 * RT * 8;
 	static constexpr int SMEM = SCAN + 64;
 	static constexpr int SLOT = RT * DP + 2 * RT; // floats of a partial result
@@ -228,7 +231,7 @@ __device__ __forceinline__ void store_row4(const AttnArgs &p, const AttnRow &x, 
 }
 
 template <class T, int DP, int MT>
-__global__ void __launch_bounds__(128) k_tree_attn(const AttnArgs p)
+__global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(const AttnArgs p)
 {
 	using A = AttnTile<T, DP, MT>;
 	constexpr int KW = A::KW, NT = A::NT, TK = A::TK, RT = A::RT, P = A::P, CH = A::CH, NST = A::NST;
