@@ -71,7 +71,7 @@ int pg_cache(const char *who, const tg_cuda_kv *c, PgCache *o)
 	if (c->max_len > (long long)c->page * c->table_cols)
 		return set_err(TG_CUDA_EINVAL, "%s: max_len %d is more than %d pages of %d hold", who, c->max_len, c->table_cols, c->page);
 	if (c->max_len > 0x7fff0000) return set_err(TG_CUDA_EINVAL, "%s: max_len %d", who, c->max_len);
-	if (c->seqs && (!c->len || ((!c->table || !c->k || !c->v) && c->table_cols > 0 && c->pages > 0)))
+	if (c->seqs && (!c->len || (!c->table && c->table_cols > 0) || ((!c->k || !c->v) && c->pages > 0)))
 		return set_err(TG_CUDA_EINVAL, "%s: NULL pointer in the cache", who);
 	if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) || ((c->page_stride | c->head_stride | c->pos_stride) * e & 15))
 		return set_err(TG_CUDA_EINVAL, "%s: cache rows must start on 16-byte boundaries", who);
@@ -82,7 +82,7 @@ int pg_cache(const char *who, const tg_cuda_kv *c, PgCache *o)
 		return set_err(TG_CUDA_EINVAL, "%s: a pool of 2^32 rows' alignments of %d bytes or more", who, 1 << o->shift);
 	o->k = (char *)c->k, o->v = (char *)c->v, o->table = c->table, o->len = c->len;
 	o->page_b = c->page_stride * e, o->head_b = c->head_stride * e, o->pos_b = c->pos_stride * e;
-	o->page = c->page, o->pages = c->table && c->k && c->v ? c->pages : 0, o->cols = c->table_cols, o->max_len = c->max_len;
+	o->page = c->page, o->pages = c->pages, o->cols = c->table_cols, o->max_len = c->max_len;
 	o->nkv = c->nkv, o->dim = c->head_dim;
 	return TG_CUDA_OK;
 }
@@ -93,8 +93,8 @@ int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, int
 	if (d->tokens <= 0 || (most && d->tokens > most)) return set_err(TG_CUDA_EINVAL, "%s: %d tokens per sequence", who, d->tokens);
 	const int e = pg_size(c->type);
 	if (use & PG_USE_Q) {
-		if (d->nq <= 0 || d->nq % c->nkv)
-			return set_err(TG_CUDA_EINVAL, "%s: nq %d is not a multiple of nkv %d", who, d->nq, c->nkv);
+		if (d->nq <= 0 || d->nq > 1 << 20 || d->nq % c->nkv)
+			return set_err(TG_CUDA_EINVAL, "%s: nq %d is not a multiple of nkv %d, or over 2^20", who, d->nq, c->nkv);
 		if (c->seqs && !d->q) return set_err(TG_CUDA_EINVAL, "%s: NULL q", who);
 		if (((uintptr_t)d->q & 15) || ((d->q_seq | d->q_tok | d->q_head) * e & 15))
 			return set_err(TG_CUDA_EINVAL, "%s: q rows must start on 16-byte boundaries", who);
@@ -104,6 +104,12 @@ int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, int
 	if (((use & PG_USE_K) && ((uintptr_t)d->k & 15)) || ((use & PG_USE_V) && ((uintptr_t)d->v & 15)) ||
 	    ((d->kv_seq | d->kv_tok | d->kv_head) * e & 15))
 		return set_err(TG_CUDA_EINVAL, "%s: drafted k and v rows must start on 16-byte boundaries", who);
+	if (((use & PG_USE_Q) && (d->q_seq < 0 || d->q_tok < 0 || d->q_head < 0)) || d->kv_seq < 0 || d->kv_tok < 0 || d->kv_head < 0)
+		return set_err(TG_CUDA_EINVAL, "%s: negative strides", who);
+	// attention passes on places within a sequence's drafted rows in 32 bits of 16 bytes
+	if (most && (((unsigned __int128)d->kv_tok * d->tokens * e >> 4) >= PG_NONE ||
+		     (((unsigned __int128)d->q_tok * d->tokens + (unsigned __int128)d->q_head * d->nq) * e >> 4) >= PG_NONE))
+		return set_err(TG_CUDA_EINVAL, "%s: a sequence's drafted rows span 64 GB", who);
 	o->q = (const char *)d->q, o->k = (const char *)d->k, o->v = (const char *)d->v;
 	o->q_seq = d->q_seq * e, o->q_tok = d->q_tok * e, o->q_head = d->q_head * e;
 	o->kv_seq = d->kv_seq * e, o->kv_tok = d->kv_tok * e, o->kv_head = d->kv_head * e;

@@ -75,7 +75,7 @@ extern "C" int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, v
 	if (need && (!work || work_bytes < (long long)need || ((uintptr_t)work & 15)))
 		return set_err(TG_CUDA_EINVAL, "%s: needs %zu bytes of 16-byte aligned scratch", who, need);
 	p.out = (char *)out, p.out_seq = out_seq * e, p.out_tok = out_tok * e, p.out_head = out_head * e, p.lse = lse;
-	p.seqs = c->seqs, p.row_tiles = pl.row_tiles, p.whole = pl.whole, p.least = pl.least, p.begin = pl.begin, p.by_unit = pl.by_unit;
+	p.seqs = c->seqs, p.row_tiles = pl.row_tiles, p.whole = pl.whole, p.least = pl.least, p.begin = pl.begin, p.by_unit = pl.by_unit, p.ctas = pl.grid;
 	p.split = (int4 *)work, p.part = (float *)((char *)work + (size_t)pl.grid * sizeof(int4));
 	cudaStream_t st = (cudaStream_t)stream;
 	return c->type == TG_CUDA_F32 ? attn_type<float>(p, pl, st) : c->type == TG_CUDA_F16 ? attn_type<__half>(p, pl, st) : attn_type<__nv_bfloat16>(p, pl, st);

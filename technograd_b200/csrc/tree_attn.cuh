@@ -21,6 +21,7 @@ struct AttnArgs {
 	int begin;       // shares: what beginning a unit costs, in tiles
 	PgBox box;       // of the pools' TMA maps; rows 0: none
 	float *part;     // shares: partial results, two slots per CTA
+	int ctas;        // of the launch
 	int by_unit;     // shares: split's entries are the units', else the CTAs'
 	int4 *split;     // shares: of a unit that begins in a CTA's share and ends in a later one, the two CTAs, its
 	                 // sequence and head, and its row tile; x = -1: none, or nothing to join
@@ -511,7 +512,8 @@ __global__ void __launch_bounds__(32 * NG) k_attn_join(const AttnArgs p)
 	pdl_launch();
 	pdl_wait();
 	const int4 u = p.split[blockIdx.x];
-	if (u.x < 0) return;
+	// (after a wait that gave up the entry may not have been written)
+	if (u.x < 0 || u.y < u.x || u.y >= p.ctas || u.z < 0 || u.z / p.c.nkv >= p.seqs || u.w < 0 || u.w >= p.row_tiles) return;
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = u.z / p.c.nkv, h = u.z - b * p.c.nkv;
 	const int rows = p.d.tokens * p.d.group, cnt = p.d.drafted(b), parts = u.y - u.x + 1;
 	const int x = blockIdx.y * 32 + lane, r = x / (RW * DP / 8) * RW + x % RW, col = x / RW % (DP / 8) * 8;

@@ -31,9 +31,9 @@ def drafts(**kw):
 BAD_CACHE = [dict(type=3), dict(type=-1), dict(seqs=-1), dict(nkv=0), dict(page=0), dict(pages=-1), dict(table_cols=-1), dict(max_len=-1), dict(max_len=65),
              dict(head_dim=0), dict(head_dim=264), dict(head_dim=60), dict(k=0x10008), dict(v=0x20002), dict(page_stride=2044), dict(head_stride=1023),
              dict(pos_stride=-64), dict(k=0), dict(v=0), dict(table=0), dict(len=0), dict(type=_lib.F32, head_dim=66),
-             dict(pages=2 ** 31 - 1, page_stride=2 ** 40 + 8)]
+             dict(pages=2 ** 31 - 1, page_stride=2 ** 40 + 8), dict(pages=0, table=0)]
 BAD_DRAFTS = [dict(tokens=0), dict(tokens=65), dict(nq=0), dict(nq=3), dict(q=0), dict(q=0x30008), dict(q_tok=252), dict(k=0), dict(k=0x40004),
-              dict(kv_head=60)]
+              dict(kv_head=60), dict(kv_tok=-128), dict(q_seq=-768), dict(kv_tok=2 ** 34), dict(q_tok=2 ** 34), dict(nq=2 ** 21)]
 
 
 def refused(rc):
