@@ -49,6 +49,10 @@ __device__ __forceinline__ void tf32_split(uint32_t x, uint32_t &hi, uint32_t &l
 	asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(__uint_as_float(x) - __uint_as_float(hi)));
 }
 
+// A tensor core's accumulation truncates, and thousands of keys add that up to 1e-5 of an f32 output: f32 caches
+// leave it only a few products and add those to the sums in f32, rounded to nearest.
+__device__ __forceinline__ void add4(float (&d)[4], const float (&t)[4]) { d[0] += t[0], d[1] += t[1], d[2] += t[2], d[3] += t[3]; }
+
 __device__ __forceinline__ uint32_t pack16(float a, float b, __nv_bfloat16)
 {
 	const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -105,17 +109,20 @@ __device__ __forceinline__ void qk_tile(float (&s)[MT][NT][4], uint32_t sq, uint
 #pragma unroll
 			for (int i = 0; i < 4; i++) tf32_split(b[i], bh[i], bl[i]);
 #pragma unroll
-			for (int m = 0; m < MT; m++)
+			for (int m = 0; m < MT; m++) {
+				float t[4] = {0, 0, 0, 0};
 #pragma unroll
 				for (int e = 0; e < 2; e++) {
 					uint32_t a[4], ah[4], al[4];
 					ldsm4(a, qrow + m * 16 * P + (((4 * k + 2 * e + (mi >> 1)) ^ l7) << 4));
 #pragma unroll
 					for (int i = 0; i < 4; i++) tf32_split(a[i], ah[i], al[i]);
-					mma8(s[m][0], al, bh[2 * e], bh[2 * e + 1]);
-					mma8(s[m][0], ah, bl[2 * e], bl[2 * e + 1]);
-					mma8(s[m][0], ah, bh[2 * e], bh[2 * e + 1]);
+					mma8(t, al, bh[2 * e], bh[2 * e + 1]);
+					mma8(t, ah, bl[2 * e], bl[2 * e + 1]);
+					mma8(t, ah, bh[2 * e], bh[2 * e + 1]);
 				}
+				add4(s[m][0], t);
+			}
 		}
 	}
 }
@@ -152,12 +159,21 @@ __device__ __forceinline__ void qk_keys(float (&s)[MT][NT][4], const KeyFrag<T, 
 	for (int m = 0; m < MT; m++)
 #pragma unroll
 		for (int x = 0; x < NT; x++) s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = 0;
+	float whole[MT][NT][4] = {}; // past 128 dimensions of 16 bits
 #pragma unroll
 	for (int k = 0; k < DP / 16; k++) {
 		if constexpr (sizeof(T) == 2) {
 			uint32_t a[MT][4];
 #pragma unroll
 			for (int m = 0; m < MT; m++) ldsm4(a[m], qrow + m * 16 * P + (((2 * k + (mi >> 1)) ^ l7) << 4));
+			if (k && k % 8 == 0) { // see add4: a weight is an f32 output
+#pragma unroll
+				for (int m = 0; m < MT; m++)
+#pragma unroll
+					for (int x = 0; x < NT; x++)
+#pragma unroll
+						for (int i = 0; i < 4; i++) whole[m][x][i] += s[m][x][i], s[m][x][i] = 0;
+			}
 #pragma unroll
 			for (int m = 0; m < MT; m++) {
 				mma16(s[m][0], a[m], f.r[k][0], f.r[k][1], T());
@@ -165,18 +181,27 @@ __device__ __forceinline__ void qk_keys(float (&s)[MT][NT][4], const KeyFrag<T, 
 			}
 		} else {
 #pragma unroll
-			for (int e = 0; e < 2; e++)
+			for (int m = 0; m < MT; m++) {
+				float t[4] = {0, 0, 0, 0};
 #pragma unroll
-				for (int m = 0; m < MT; m++) {
+				for (int e = 0; e < 2; e++) {
 					uint32_t a[4], ah[4], al[4];
 					ldsm4(a, qrow + m * 16 * P + (((4 * k + 2 * e + (mi >> 1)) ^ l7) << 4));
 #pragma unroll
 					for (int i = 0; i < 4; i++) tf32_split(a[i], ah[i], al[i]);
-					mma8(s[m][0], al, f.r[k][2 * e], f.r[k][2 * e + 1]);
-					mma8(s[m][0], ah, f.r[k][4 + 2 * e], f.r[k][4 + 2 * e + 1]);
-					mma8(s[m][0], ah, f.r[k][2 * e], f.r[k][2 * e + 1]);
+					mma8(t, al, f.r[k][2 * e], f.r[k][2 * e + 1]);
+					mma8(t, ah, f.r[k][4 + 2 * e], f.r[k][4 + 2 * e + 1]);
+					mma8(t, ah, f.r[k][2 * e], f.r[k][2 * e + 1]);
 				}
+				add4(s[m][0], t);
+			}
 		}
+	}
+	if constexpr (sizeof(T) == 2 && DP > 128) {
+#pragma unroll
+		for (int m = 0; m < MT; m++)
+#pragma unroll
+			for (int x = 0; x < NT; x++) add4(s[m][x], whole[m][x]);
 	}
 }
 
@@ -221,9 +246,11 @@ __device__ __forceinline__ void pv_tile(float (&o)[MT][DP / 8][4], const float (
 			tf32_split(b0, h0, l0), tf32_split(b1, h1, l1);
 #pragma unroll
 			for (int m = 0; m < MT; m++) {
-				mma8(o[m][d], al[m], h0, h1);
-				mma8(o[m][d], ah[m], l0, l1);
-				mma8(o[m][d], ah[m], h0, h1);
+				float t[4] = {0, 0, 0, 0};
+				mma8(t, al[m], h0, h1);
+				mma8(t, ah[m], l0, l1);
+				mma8(t, ah[m], h0, h1);
+				add4(o[m][d], t);
 			}
 		}
 	}

@@ -20,7 +20,9 @@
 //         are looked up while this one's rows are on their way.
 // What bounds it: with up to 128 rows the cache's bytes (a 64 KB tile pair takes 2850 cycles of the
 // measured HBM rate). Of the 608 x 96 registers of the launch the fetching warps give 32 each to
-// the softmax warps, which hold 64 scores. Every wait is bounded (tc.cuh): a timeout sets the status word and all roles
+// the softmax warps, which hold 64 scores. Measured: 48 sequences of up to 6001 positions with 64 drafted tokens
+// (16 query heads over 8, bf16) 187 us in short runs, 218 us in a long one, which draws 995 W and runs at 1550 MHz; 131009
+// positions with 5 tokens of 8 heads per key head (f16) 70 us, 3.8 TB/s. Every wait is bounded (tc.cuh): a timeout sets the status word and all roles
 // leave.
 #pragma once
 

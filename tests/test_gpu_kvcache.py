@@ -508,3 +508,14 @@ def test_negative_and_zero_scale(cuda):
             want = plain(flip, scale=abs(scale) or 0.1)
             near(out, want[0], want[2], "out")
             near(lse, want[1], want[3], "lse")
+
+
+def test_f32_sums_over_many_keys_do_not_drift(cuda):
+    """60000 keys: products rounded to nearest keep the output within sqrt(steps) * 2^-24 of the definition (about
+    2^-19 here); sums that truncate would be off by 2^-16."""
+    c = Case([60000], 1, 4, 64, 64, "head", F32, 2)
+    c.q *= 0.25
+    out, lse = attend(c)
+    want = plain(c)
+    assert ((out.cpu().double() - want[0]).norm() / want[0].norm()).item() < 2.0 ** -18
+    assert (lse.cpu().double() - want[1]).abs().max() < 2.0 ** -20 * 16
