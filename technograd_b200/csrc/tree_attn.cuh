@@ -121,6 +121,9 @@ __device__ __forceinline__ long long block_scan(long long v, long long *s, long 
 	return all;
 }
 
+// a / b of numbers that nearly always fit 32 bits (a 64-bit division is a long chain of instructions)
+__device__ __forceinline__ long long quotient(long long a, unsigned b) { return a >> 32 ? a / b : (long long)((unsigned)a / b); }
+
 // What a CTA works on: `left` tiles from place c of the list. s: NW + 4 words of shared memory.
 // False: nothing. A unit counts its tiles and p.begin more, spent before its first tile; the CTAs' shares of
 // the total are equal, share and pos being one's size and beginning.
@@ -138,10 +141,11 @@ __device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int 
 	}
 	const int per = p.c.nkv * p.row_tiles;
 	auto weight = [&](int b) -> long long { return b < p.seqs ? (((long long)p.c.length(b) + TK - 1) / TK + extra + p.begin) * per : 0; };
+	const bool once = p.seqs <= 32 * NW; // a thread per sequence: one pass over the lengths
 	long long mine = 0, before, all;
 	for (int b = threadIdx.x; b < p.seqs; b += 32 * NW) mine += weight(b);
 	all = block_scan<NW>(mine, s, before);
-	share = (all + gridDim.x - 1) / gridDim.x;
+	share = quotient(all + gridDim.x - 1, gridDim.x);
 	if (share < p.least + p.begin) share = p.least + p.begin;
 	pos = share * blockIdx.x;
 	if (threadIdx.x == 0 && p.split && !p.by_unit) p.split[blockIdx.x].x = -1;
@@ -150,7 +154,7 @@ __device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int 
 	long long base = 0;
 	for (int b0 = 0;; b0 += 32 * NW) { // ends: pos < to <= all
 		const int b = b0 + threadIdx.x;
-		const long long w = weight(b), sum = block_scan<NW>(w, s, before);
+		const long long w = once ? mine : weight(b), sum = once ? all : block_scan<NW>(w, s, before);
 		if (pos >= base + before && pos < base + before + w) s[NW] = b, s[NW + 1] = base + before;
 		if (to - 1 >= base + before && to - 1 < base + before + w) s[NW + 2] = b, s[NW + 3] = base + before;
 		base += sum;
@@ -162,7 +166,7 @@ __device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int 
 	auto tiles = [&](long long b, long long first, long long off) {
 		c.b = (int)b;
 		cursor_seq<TK>(p, c, extra);
-		u = (int)(off / (c.all + p.begin));
+		u = (int)quotient(off, c.all + p.begin);
 		in = (int)(off - (long long)u * (c.all + p.begin));
 		t = in < p.begin ? 0 : in - p.begin;
 		return first - b * per * p.begin + (long long)u * c.all + t;
