@@ -72,6 +72,20 @@ __device__ __forceinline__ float ex2(float x)
 	return y;
 }
 
+// packed f32 arithmetic, two elements an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+	unsigned long long d;
+	asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b), "l"(*(unsigned long long *)&c));
+	return *(float2 *)&d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+	unsigned long long d;
+	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
+	return *(float2 *)&d;
+}
+
 // 16 bytes from global to shared memory, or 16 zero bytes
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool have)
 {

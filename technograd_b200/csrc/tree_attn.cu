@@ -27,14 +27,15 @@ static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, At
 	o->dp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
 	o->tc = c->type != TG_CUDA_F32 && o->dp <= 128 && rows > ATTN_TC_ROWS;
 	o->mt = rows <= 16 || o->dp == 256 ? 1 : 2; // 256 dimensions of 32 rows do not fit in registers
-	const int rt = o->tc ? 128 : 16 * o->mt, tk = o->tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
+	o->fma = c->type == TG_CUDA_F32 && rows <= 8 ? rows <= 4 ? 4 : 8 : 0;
+	const int rt = o->tc ? 128 : o->fma ? o->fma : 16 * o->mt, tk = o->tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
 	o->row_tiles = (rows + rt - 1) / rt;
 	const long long units = (long long)c->seqs * c->nkv * o->row_tiles;
 	const long long tiles = (c->max_len + tk - 1) / tk + (d.tokens + tk - 1) / tk;
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
 	o->whole = tiles * tk <= ATTN_WHOLE, o->least = 128 / tk, o->begin = o->tc && units * tiles > (long long)ATTN_LONG * o->sms ? ATTN_TC_BEGIN : ATTN_BEGIN;
 	o->slot = (size_t)(rt * o->dp + 2 * rt) * 4;
-	const long long shares = (units * (tiles + o->begin) + o->least + o->begin - 1) / (o->least + o->begin), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : o->mt == 1 && c->type != TG_CUDA_F32 ? 3 : 2); // AttnTile's CTAS
+	const long long shares = (units * (tiles + o->begin) + o->least + o->begin - 1) / (o->least + o->begin), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : o->fma || (o->mt == 1 && c->type != TG_CUDA_F32) ? 3 : 2); // the tiles' CTAS
 	o->grid = (int)(o->whole ? units : shares < wave ? shares : wave);
 	o->units = (int)units, o->by_unit = !o->whole && units <= o->grid;
 	return TG_CUDA_OK;

@@ -237,6 +237,63 @@ __device__ __forceinline__ void store_row4(const AttnArgs &p, const AttnRow &x, 
 	store4((T *)x.out + col, make_float4(o.x * x.f, o.y * x.f, o.z * x.f, o.w * x.f));
 }
 
+// A warp's fetching of its rows of the tiles to come, K and V: lane i < KW holds the place of the tile's row i, looked up
+// while the tile before is fetched.
+template <class T, int DP, class A> struct AttnFetch {
+	const AttnArgs &p;
+	AttnCursor f;
+	long long left, fetched = 0;
+	uint32_t at = PG_NONE, ring;
+	int extra, chunks;
+
+	__device__ __forceinline__ AttnFetch(const AttnArgs &args, const AttnCursor &c, long long n, uint32_t stages, int drafted_tiles, int row_chunks)
+		: p(args), f(c), left(n), ring(stages), extra(drafted_tiles), chunks(row_chunks)
+	{
+		find();
+	}
+	__device__ __forceinline__ void find()
+	{
+		const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+		at = PG_NONE;
+		if (lane >= A::KW || fetched >= left) return;
+		if (f.tile < f.ctx) {
+			const int x = f.tile * A::TK + warp * A::KW + lane;
+			if (x < f.n) {
+				const int page = x / p.c.page;
+				at = p.c.at(p.c.table[(long long)f.b * p.c.cols + page], x - page * p.c.page);
+			}
+		} else {
+			const int u = (f.tile - f.ctx) * A::TK + warp * A::KW + lane;
+			if (u < p.d.drafted(f.b)) at = (uint32_t)(u * p.d.kv_tok >> 4);
+		}
+	}
+	// the next tile, if there is one, into a stage; always one group of copies
+	__device__ __forceinline__ void fetch(int stage)
+	{
+		if (fetched < left) {
+			const int lane = threadIdx.x & 31;
+			const bool ctx = f.tile < f.ctx;
+			const int sh = ctx ? p.c.shift : 4;
+			const long long head = ctx ? f.h * p.c.head_b : f.b * p.d.kv_seq + f.h * p.d.kv_head;
+			const char *kp = (ctx ? p.c.k : p.d.k) + head, *vp = (ctx ? p.c.v : p.d.v) + head;
+			const uint32_t sk = ring + stage * A::STAGE, sv = sk + A::KW * A::P, mine = at;
+			cursor_next<A::TK>(p, f, extra);
+			fetched++;
+			find();
+#pragma unroll
+			for (int i = 0; i < A::KW * A::CH / 32; i++) {
+				const int row = (i * 32 + lane) / A::CH, ch = (i * 32 + lane) % A::CH;
+				const uint32_t r = __shfl_sync(~0u, mine, row), o = row * A::P + ((ch ^ (row & 7)) << 4);
+				const bool have = r != PG_NONE && ch < chunks;
+				const unsigned long long off = ((unsigned long long)r << sh) + ch * 16;
+				cp16(sk + o, have ? kp + off : p.d.k, have);
+				cp16(sv + o, have ? vp + off : p.d.v, have);
+			}
+		}
+		cp_commit();
+	}
+};
+
 template <class T, int DP, int MT>
 __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(const AttnArgs p)
 {
@@ -258,47 +315,8 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 	long long left, pos, share;
 	if (!attn_share<TK, 4>(p, s_scan, extra, c, left, pos, share)) return;
 
-	// ---- fetching: lane i < KW holds the place of the tile's row i, looked up while the tile before is fetched
-	AttnCursor f = c;
-	long long fetched = 0;
-	uint32_t at = PG_NONE;
-	auto find = [&]() {
-		at = PG_NONE;
-		if (lane >= KW || fetched >= left) return;
-		if (f.tile < f.ctx) {
-			const int x = f.tile * TK + warp * KW + lane;
-			if (x < f.n) {
-				const int page = x / p.c.page;
-				at = p.c.at(p.c.table[(long long)f.b * p.c.cols + page], x - page * p.c.page);
-			}
-		} else {
-			const int u = (f.tile - f.ctx) * TK + warp * KW + lane;
-			if (u < p.d.drafted(f.b)) at = (uint32_t)(u * p.d.kv_tok >> 4);
-		}
-	};
-	auto fetch = [&](int stage) {
-		if (fetched < left) {
-			const bool ctx = f.tile < f.ctx;
-			const int sh = ctx ? p.c.shift : 4;
-			const long long head = (ctx ? f.h * p.c.head_b : f.b * p.d.kv_seq + f.h * p.d.kv_head);
-			const char *kp = (ctx ? p.c.k : p.d.k) + head, *vp = (ctx ? p.c.v : p.d.v) + head;
-			const uint32_t sk = ring + stage * A::STAGE, sv = sk + KW * P, mine = at;
-			cursor_next<TK>(p, f, extra);
-			fetched++;
-			find();
-#pragma unroll
-			for (int i = 0; i < KW * CH / 32; i++) {
-				const int row = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
-				const uint32_t r = __shfl_sync(~0u, mine, row), o = row * P + ((ch ^ (row & 7)) << 4);
-				const bool have = r != PG_NONE && ch < chunks;
-				const unsigned long long off = ((unsigned long long)r << sh) + ch * 16;
-				cp16(sk + o, have ? kp + off : p.d.k, have);
-				cp16(sv + o, have ? vp + off : p.d.v, have);
-			}
-		}
-		cp_commit();
-	};
-	find();
+	AttnFetch<T, DP, A> f(p, c, left, ring, extra, chunks);
+	auto fetch = [&](int stage) { f.fetch(stage); };
 
 	float o[MT][DP / 8][4], mr[MT][2], l[MT][2];
 	int cnt = 0;
@@ -562,7 +580,7 @@ __global__ void __launch_bounds__(32 * NG) k_attn_join(const AttnArgs p)
 
 // How a call is cut.
 struct AttnPlan {
-	int dp, mt, row_tiles, whole, least, begin, grid, by_unit, units, sms, dev, tc; // mt: 16-row products of a tile; tc: 128-row tiles on tcgen05
+	int dp, mt, row_tiles, whole, least, begin, grid, by_unit, units, sms, dev, tc, fma; // fma: rows of tree_attn_fma.cuh, 0: another kernel; mt: 16-row products of a tile; tc: 128-row tiles on tcgen05
 	size_t slot; // bytes of a partial result
 	size_t bytes() const { return whole ? 0 : (size_t)grid * (2 * slot + sizeof(int4)); }
 };

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "tree_attn.cuh"
+#include "tree_attn_fma.cuh"
 #include "tree_attn_tc.cuh"
 
 namespace tgc {
@@ -31,6 +32,22 @@ static int attn_run(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 	return attn_join<T, DP, A::RT>(p, pl, st);
 }
 
+template <int DP, int R>
+static int attn_run_fma(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
+{
+	using A = FmaTile<DP, R>;
+	static std::atomic<unsigned long long> done{0};
+	int rc = pg_smem(k_tree_attn_fma<DP, R>, A::SMEM, pl.dev, done);
+	if (rc) return rc;
+	if (pl.whole) {
+		k_tree_attn_fma<DP, R><<<pl.grid, 128, A::SMEM, st>>>(p);
+		TGC_LAUNCH_CHECK();
+		return TG_CUDA_OK;
+	}
+	TGC_CUDA(launch_pdl(k_tree_attn_fma<DP, R>, dim3(pl.grid), dim3(128), A::SMEM, st, p));
+	return attn_join<float, DP, R>(p, pl, st);
+}
+
 template <class T, int DP>
 static int attn_run_tc(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 {
@@ -51,6 +68,10 @@ int attn_type(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 {
 	if constexpr (sizeof(T) == 2) {
 		if (pl.tc) return pl.dp == 128 ? attn_run_tc<T, 128>(p, pl, st) : attn_run_tc<T, 64>(p, pl, st);
+	}
+	if constexpr (sizeof(T) == 4) {
+		if (pl.fma == 4) return pl.dp == 256 ? attn_run_fma<256, 4>(p, pl, st) : pl.dp == 128 ? attn_run_fma<128, 4>(p, pl, st) : attn_run_fma<64, 4>(p, pl, st);
+		if (pl.fma == 8) return pl.dp == 256 ? attn_run_fma<256, 8>(p, pl, st) : pl.dp == 128 ? attn_run_fma<128, 8>(p, pl, st) : attn_run_fma<64, 8>(p, pl, st);
 	}
 	if (pl.dp == 256) return attn_run<T, 256, 1>(p, pl, st);
 	if (pl.dp == 128) return pl.mt == 1 ? attn_run<T, 128, 1>(p, pl, st) : attn_run<T, 128, 2>(p, pl, st);

@@ -150,19 +150,7 @@ __device__ __forceinline__ uint64_t ta_mn_desc(uint32_t saddr, uint32_t lbo)
 	return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-// packed f32 arithmetic, two elements an instruction, and the largest of three
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-	unsigned long long d;
-	asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b), "l"(*(unsigned long long *)&c));
-	return *(float2 *)&d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
-{
-	unsigned long long d;
-	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
-	return *(float2 *)&d;
-}
+// the largest of three
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
 	float d;

@@ -519,3 +519,12 @@ def test_f32_sums_over_many_keys_do_not_drift(cuda):
     want = plain(c)
     assert ((out.cpu().double() - want[0]).norm() / want[0].norm()).item() < 2.0 ** -18
     assert (lse.cpu().double() - want[1]).abs().max() < 2.0 ** -20 * 16
+
+
+@pytest.mark.parametrize("dim", [4, 64, 68, 128, 252, 256])
+@pytest.mark.parametrize("tokens,nkv,group", [(1, 2, 1), (1, 1, 3), (2, 2, 2), (5, 1, 1), (2, 1, 4), (3, 1, 3), (4, 1, 4)])
+def test_f32_with_few_rows(cuda, dim, tokens, nkv, group):
+    """1 to 16 rows per key head, on the FMA units up to 8."""
+    for lens in ([70, 0, 1, 259], [2000]):
+        c = Case(lens, nkv, group, dim, 16, "pos", F32, tokens)
+        check_attend(c, random_mask(len(lens), tokens, 3), [tokens, tokens, (tokens + 1) // 2, 0][:len(lens)])
