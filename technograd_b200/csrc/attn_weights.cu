@@ -219,7 +219,9 @@ static int weights_run_tc(WeightArgs &p, int sms, int dev, cudaStream_t st, cons
 	// 84 at 4, 82 at 8)
 	p.row_tiles = 1, p.whole = 0, p.least = 1, p.begin = units * tiles > 24ll * sms ? 6 : 2, p.split = nullptr;
 	const long long shares = (units * (tiles + p.begin) + p.begin) / (1 + p.begin);
-	k_attn_weights_tc<T, DP><<<(unsigned)(shares < sms ? shares : sms), W::THREADS, W::SMEM, st>>>(p);
+	CUtensorMap map = {};
+	if (!pg_map(&map, p.c, p.c.k, std::is_same<T, __half>::value, 32, &p.box)) p.box.rows = 0;
+	k_attn_weights_tc<T, DP><<<(unsigned)(shares < sms ? shares : sms), W::THREADS, W::SMEM, st>>>(p, map);
 	TGC_LAUNCH_CHECK();
 	return TG_CUDA_OK;
 }

@@ -6,8 +6,8 @@
 //   0-3  a key per thread: sum over the rows' columns of 2^(z - lse log2(e)); what the key had, and the result,
 //        are one coalesced access each
 //   4    MMA issue, into one of two TMEM score buffers
-//   5-8  fetching: the tile's keys through the page table into the operand layout (four stages), and at
-//        a unit's beginning its q
+//   5-8  fetching: the tile's keys through the page table into the operand layout (four stages), by TMA boxes
+//        where the pages suit them (k_tree_attn_tc), and at a unit's beginning its q
 // What bounds it: HBM up to about 128 rows (a tile's 32 KB take 1425 cycles of the measured rate, its exponentials
 // 8 cycles a row), then the exponentials. Measured: windows of 32 tokens (64 rows) over 16 sequences of up to 16001
 // positions 85 us, 3.9 TB/s. Every wait is bounded (tc.cuh).
@@ -35,7 +35,7 @@ template <int DP> struct TwTile {
 };
 
 template <class T, int DP>
-__global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p)
+__global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p, const __grid_constant__ CUtensorMap kmap)
 {
 	using W = TwTile<DP>;
 	constexpr int TK = W::TK, CH = W::CH, NST = W::NST, RI = 32 / CH;
@@ -72,14 +72,17 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p)
 		const uint32_t dk = s0 + W::K + (uint32_t)((ch >> 3) * 16384 + (part * 32 + lane / CH) * 128);
 		const uint32_t dq = s0 + (uint32_t)((ch >> 3) * (TW_ROWS * 128) + (lane / CH) * 128);
 		const bool piece = ch < chunks;
-		int entry = 0, in_page = -1;
-		auto look = [&]() { // the table's entry of this lane's key
-			const bool drafted = c.tile >= c.ctx;
-			const int x = (drafted ? 0 : c.tile * TK) + part * 32 + lane;
+		int entry = 0, in_page = -1, last = -1;
+		// by TMA, lane i has box i / (DP / 64) of its warp's 32 keys, and 64 of the dimensions; keys past the end are not looked at
+		constexpr int ND = DP / 64;
+		const int boxes = p.box.rows ? 32 / p.box.rows : 0;
+		auto look = [&]() { // the table's entry of this lane's key or box
+			const bool drafted = c.tile >= c.ctx, box = boxes && !drafted;
+			const int x = (drafted ? 0 : c.tile * TK) + part * 32 + (box ? lane / ND * p.box.rows : lane);
 			in_page = -1;
 			if (drafted) {
 				if (x < p.d.drafted(c.b)) in_page = x;
-			} else if (x < c.n) {
+			} else if (x < c.n && !(box && lane >= boxes * ND)) {
 				const int page = x / p.c.page;
 				in_page = x - page * p.c.page;
 				entry = p.c.table[(long long)c.b * p.c.cols + page];
@@ -87,16 +90,26 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p)
 		};
 		look();
 		for (int j = 0; j < left; j++) {
-			const bool drafted = c.tile >= c.ctx, begin = j == 0 || c.tile == 0;
-			const int sh = drafted ? 4 : p.c.shift, st = j % NST;
+			const bool drafted = c.tile >= c.ctx, begin = j == 0 || c.tile == 0, box = boxes && !drafted;
+			const int sh = drafted ? 4 : p.c.shift, st = j % NST, kvh = c.h, page = entry;
 			const char *base = (drafted ? p.d.k + (long long)c.b * p.d.kv_seq + c.h * p.d.kv_head : p.c.k + c.h * p.c.head_b) + ch * 16;
 			const char *qb = p.d.q + (long long)c.b * p.d.q_seq + (long long)c.h * p.d.group * p.d.q_head + ch * 16;
-			const uint32_t at = in_page < 0 ? PG_NONE : drafted ? (uint32_t)(in_page * p.d.kv_tok >> 4) : p.c.at(entry, in_page);
+			const uint32_t at = in_page < 0 ? PG_NONE : box ? (uint32_t)((unsigned)entry < (unsigned)p.c.pages ? in_page : (p.c.report(PG_PAGE), -1)) : drafted ? (uint32_t)(in_page * p.d.kv_tok >> 4) : p.c.at(entry, in_page);
 			if (j + 1 < left) {
 				cursor_next<TK>(p, c, 1);
 				look();
 			}
 			if (j >= NST && !ta_wait(B, &B->kfree[st], (j / NST - 1) & 1, p.c)) break;
+			last = j;
+			if (box) {
+				if (lane == 0) ta_expect(&B->kfull[st], 32 * DP * 2);
+				__syncwarp();
+				if (lane < boxes * ND) {
+					const int r = at == PG_NONE ? 0 : (int)at, g = at == PG_NONE ? -1 : page; // -1: zeros
+					ta_box(s0 + W::K + st * W::KB + lane % ND * 16384 + (part * 32 + lane / ND * p.box.rows) * 128, &kmap, &B->kfull[st], lane % ND * 64,
+					       p.box.swap ? kvh : r, p.box.swap ? r : kvh, g);
+				}
+			} else
 #pragma unroll 8
 			for (int y = 0; y < CH; y++) {
 				const uint32_t o = __shfl_sync(~0u, at, y * RI + lane / CH);
@@ -120,6 +133,8 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p)
 		}
 		cp_commit();
 		cp_wait<0>();
+		// boxes still on their way land before the CTA's shared memory is released
+		for (int j = last > NST - 1 ? last - NST + 1 : 0; j <= last; j++) mbar_wait(&B->kfull[j % NST], j / NST & 1, nullptr, 0);
 	} else if (warp == 4) {
 		// ---------------- MMA issue ----------------
 		if (lane == 0) {
