@@ -215,8 +215,8 @@ static int weights_run_tc(WeightArgs &p, int sms, int dev, cudaStream_t st, cons
 	if (rc) return rc;
 	const long long units = (long long)p.seqs * p.c.nkv, tiles = (p.c.max_len + W::TK - 1) / W::TK + 1;
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences", who, p.seqs);
-	// a unit's start is worth about 6 tiles, except where every CTA has one of its own anyway (the window case: 120 us at 2,
-	// 84 at 4, 82 at 8)
+	// a unit's start is worth about 6 tiles, except where every CTA has one of its own anyway (32-token windows over 16
+	// sequences of up to 16001 positions: 120 us at 2, 84 at 4, 82 at 8)
 	p.row_tiles = 1, p.whole = 0, p.least = 1, p.begin = units * tiles > 24ll * sms ? 6 : 2, p.split = nullptr;
 	const long long shares = (units * (tiles + p.begin) + p.begin) / (1 + p.begin);
 	CUtensorMap map = {};
@@ -226,7 +226,7 @@ static int weights_run_tc(WeightArgs &p, int sms, int dev, cudaStream_t st, cons
 	return TG_CUDA_OK;
 }
 
-// From so many query rows per key head on (and up to TW_ROWS), 16-bit caches take attn_weights_tc.cuh (64 rows: 85 us
+// From so many query rows per key head on (and up to TW_ROWS), 16-bit caches take attn_weights_tc.cuh (64 rows: 81 us
 // against 136).
 constexpr int WEIGHTS_TC_ROWS = 32;
 

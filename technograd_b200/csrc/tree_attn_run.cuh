@@ -53,6 +53,11 @@ static int attn_run_tc(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 {
 	using A = TaTile<DP>;
 	static std::atomic<unsigned long long> done{0};
+	if (!(done.load(std::memory_order_acquire) >> pl.dev & 1)) { // the roles' registers must be the launch's: a warp would wait for ever for others
+		cudaFuncAttributes at;
+		TGC_CUDA(cudaFuncGetAttributes(&at, k_tree_attn_tc<T, DP>));
+		if (at.numRegs < TA_REGS) return set_err(TG_CUDA_EUNSUPPORTED, "tree attention kernel built with %d registers, not %d", at.numRegs, TA_REGS);
+	}
 	int rc = pg_smem(k_tree_attn_tc<T, DP>, A::SMEM, pl.dev, done);
 	if (rc) return rc;
 	AttnArgs a = p;
