@@ -8,7 +8,7 @@ namespace tgc {
 // The weights' kernel goes through the keys as k_tree_attn does (tree_attn.cuh): equal shares of all
 // (sequence, kv head) units' tiles, a ring of asynchronous copies per warp, drafted tokens after the cached
 // ones. A warp takes its tile's keys into registers as the product's operand and meets all query rows
-// with them, 16 at a time from shared memory: S = Q K^T, then 2^(z - lse log2(e)) summed over the rows in
+// with them, 16 at a time from shared memory: S = Q K^T, then exp(scale s - lse) summed over the rows in
 // registers and, at the tile's end, over lanes. Every key is one warp's, so nothing is joined and results
 // do not depend on timing. Up to QR rows stay in shared memory for a unit; more are taken in turns at
 // every tile.
@@ -36,7 +36,6 @@ __global__ void __launch_bounds__(WeightTile<T, DP>::THREADS, 2) k_attn_weights(
 	const uint32_t s0 = smem_u32(smem), ring = s0 + W::RING + warp * NST * W::STAGE;
 	const int extra = (p.d.tokens + TK - 1) / TK, rows = p.d.tokens * p.d.group, chunks = p.c.dim * (int)sizeof(T) / 16;
 	const int turns = (rows + QR - 1) / QR;
-	const float zs = p.d.scale * 1.4426950408889634f;
 	AttnCursor c;
 	long long left, pos, share;
 	if (!attn_share<TK, W::NW>(p, (long long *)(smem + W::SCAN), extra, c, left, pos, share)) return;
@@ -82,7 +81,7 @@ __global__ void __launch_bounds__(WeightTile<T, DP>::THREADS, 2) k_attn_weights(
 #pragma unroll
 	for (int i = 0; i < NST - 1; i++) fetch(i);
 
-	// rows r0 .. r0 + QR of unit c into shared memory: q, lse log2(e), and the drafted tokens each counts for
+	// rows r0 .. r0 + QR of unit c into shared memory: q, lse, and the drafted tokens each counts for
 	// (cached positions: all bits or none)
 	auto load_rows = [&](int r0) {
 		const int cnt = p.d.drafted(c.b), in = min(QR, (rows - r0 + 15) & ~15);
@@ -97,7 +96,7 @@ __global__ void __launch_bounds__(WeightTile<T, DP>::THREADS, 2) k_attn_weights(
 			const int r = r0 + x, t = r / p.d.group;
 			const bool on = r < rows && t < cnt && (sel >> t & 1);
 			const float lse = on ? p.lse[((long long)c.b * p.d.tokens + t) * p.d.nq + c.h * p.d.group + r - t * p.d.group] : -INFINITY;
-			s_lse[x] = lse * 1.4426950408889634f;
+			s_lse[x] = lse;
 			s_mask[x] = lse == -INFINITY ? 0 : p.d.sees(c.b, t, cnt);
 		}
 		cp_commit();
@@ -152,12 +151,12 @@ __global__ void __launch_bounds__(WeightTile<T, DP>::THREADS, 2) k_attn_weights(
 #pragma unroll
 							for (int x = 0; x < NT; x++)
 #pragma unroll
-								for (int y = 0; y < 2; y++) acc[x][y] += ok >> (x * 8 + y) & 1 ? ex2(s[m][x][2 * e + y] * zs - ref) : 0;
+								for (int y = 0; y < 2; y++) acc[x][y] += ok >> (x * 8 + y) & 1 ? weight_of(s[m][x][2 * e + y], p.d.scale, ref) : 0;
 						} else {
 #pragma unroll
 							for (int x = 0; x < NT; x++)
 #pragma unroll
-								for (int y = 0; y < 2; y++) acc[x][y] += ref != -INFINITY ? ex2(s[m][x][2 * e + y] * zs - ref) : 0;
+								for (int y = 0; y < 2; y++) acc[x][y] += ref != -INFINITY ? weight_of(s[m][x][2 * e + y], p.d.scale, ref) : 0;
 						}
 					}
 			};

@@ -3,7 +3,7 @@
 // S^T = K Q^T: 128 keys are the product's M, the query rows (up to 256) its N, so that a key's scores lie in
 // one TMEM lane and its weight is one thread's sum over columns, with nothing to exchange. Units, shares and
 // tiles as in tree_attn.cuh. Warps:
-//   0-3  a key per thread: sum over the rows' columns of 2^(z - lse log2(e)); what the key had, and the result,
+//   0-3  a key per thread: sum over the rows' columns of exp(scale s - lse); what the key had, and the result,
 //        are one coalesced access each
 //   4    MMA issue, into one of two TMEM score buffers
 //   5-8  fetching: the tile's keys through the page table into the operand layout (four stages), by TMA boxes
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p, 
 	} else {
 		// ---------------- a key per thread ----------------
 		const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-		const float zs = p.d.scale * 1.4426950408889634f;
+		const float zs = p.d.scale * 1.4426950408889634f; // (the tensor core's sums of scores are no exacter than this form of the exponent)
 		int unit = -1;
 		for (int j = 0; j < left; j++, cursor_next<TK>(p, c, 1)) {
 			if (j == 0 || c.tile == 0) { // a unit's rows: their lse, and whom they count for

@@ -173,14 +173,14 @@ __device__ __forceinline__ void qk_keys(float (&s)[MT][NT][4], const KeyFrag<T, 
 	for (int m = 0; m < MT; m++)
 #pragma unroll
 		for (int x = 0; x < NT; x++) s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = 0;
-	float whole[MT][NT][4] = {}; // past 128 dimensions of 16 bits
+	float whole[MT][NT][4] = {}; // 64 dimensions of 16 bits at a time
 #pragma unroll
 	for (int k = 0; k < DP / 16; k++) {
 		if constexpr (sizeof(T) == 2) {
 			uint32_t a[MT][4];
 #pragma unroll
 			for (int m = 0; m < MT; m++) ldsm4(a[m], qrow + m * 16 * P + (((2 * k + (mi >> 1)) ^ l7) << 4));
-			if (k && k % 8 == 0) { // see add4: a weight is an f32 output
+			if (DP > 64 && k && k % 4 == 0) { // see add4: a weight is an f32 output
 #pragma unroll
 				for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -211,7 +211,7 @@ __device__ __forceinline__ void qk_keys(float (&s)[MT][NT][4], const KeyFrag<T, 
 			}
 		}
 	}
-	if constexpr (sizeof(T) == 2 && DP > 128) {
+	if constexpr (sizeof(T) == 2 && DP > 64) {
 #pragma unroll
 		for (int m = 0; m < MT; m++)
 #pragma unroll

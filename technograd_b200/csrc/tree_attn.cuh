@@ -34,6 +34,10 @@ struct WeightArgs : AttnArgs { // its lse is the input; out and part are not use
 	float *acc_out, *fresh;
 };
 
+// exp(scale s - lse). The difference is taken before anything is multiplied by log2(e): of a key with much weight it is
+// near 0, while scale s and lse may be tens, and their products' roundings would be errors of 1e-6 in the weight.
+__device__ __forceinline__ float weight_of(float s, float scale, float lse) { return ex2(fmaf(s, scale, -lse) * 1.4426950408889634f); }
+
 // The kernel for few query rows. Per (sequence b, kv head h) the query rows are r = t * group + g
 // (token t, query head h * group + g): every head of the group and every drafted token meet a key
 // while it is in shared memory, so the cache is read once for up to 16 * MT rows.

@@ -140,12 +140,13 @@ def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float 
 def attention_weights(cache: PagedKV, q, k, lse, mask=None, count=None, select=None, acc=None, scale: float | None = None):
     """The attention weight of the selected tokens on each position (tg_cuda_attn_weights).
 
-    q, k, mask, count, scale as in tree_attention, lse as it returned it. select int64 [seqs]: the
+    q, k, mask, count, scale as in tree_attention, lse as it returned it (or of any strides). select int64 [seqs]: the
     tokens that count, as bits (None: all). acc f32 [seqs, nkv, >= max_len]: what the cached
     positions had before (None: zeros). Returns (acc + weight [seqs, nkv, max_len], zero past a
     sequence's length; the drafted tokens' own weight [seqs, nkv, tokens])."""
     d = _drafts(cache, q, k, None, mask, count, scale)
     n = q.shape
+    lse = lse.contiguous()  # as tree_attention gives it, or a copy
     _check("lse", lse, torch.float32, n[:3], cache.index)
     if select is not None:
         _check("select", select, torch.int64, n[:1], cache.index)

@@ -528,3 +528,15 @@ def test_f32_with_few_rows(cuda, dim, tokens, nkv, group):
     for lens in ([70, 0, 1, 259], [2000]):
         c = Case(lens, nkv, group, dim, 16, "pos", F32, tokens)
         check_attend(c, random_mask(len(lens), tokens, 3), [tokens, tokens, (tokens + 1) // 2, 0][:len(lens)])
+
+
+def test_weights_take_any_strides(cuda):
+    """lse, q and k as views whose rows or tokens are not next to each other; acc as a slice of something wider."""
+    c = Case([150, 41], 1, 2, 64, 16, "head", BF16, 5)
+    q, kn, vn = c.q.cuda(), c.kn.cuda(), c.vn.cuda()
+    _, lse = kvcache.tree_attention(c.cache, q, kn, vn)
+    wide = torch.rand(2, 3, 200, device="cuda")
+    want = kvcache.attention_weights(c.cache, q, kn, lse, acc=wide[:, 1:2].contiguous())
+    turned = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, kn, lse)]
+    got = kvcache.attention_weights(c.cache, *turned, acc=wide[:, 1:2])
+    assert not turned[2].is_contiguous() and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
