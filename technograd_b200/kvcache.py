@@ -131,9 +131,11 @@ def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float 
         plan = cache._plans[shape[1:3]] = size, cache._one.expand(shape[:3])
     size, like = plan
     out, lse = torch.empty_like(q), torch.empty_like(like)
-    work = q.new_empty(size, dtype=torch.uint8).data_ptr() if size else None  # kept by the allocator for this stream until the call has run
+    # held until the kernels are launched: from then on the allocator gives its memory only to what comes after them on the stream
+    work = q.new_empty(size, dtype=torch.uint8) if size else None
     so = out.stride()
-    _lib.check(_lib.lib().tg_cuda_tree_attn(cache._at, d, out.data_ptr(), so[0], so[1], so[2], lse.data_ptr(), work, size, stream))
+    _lib.check(_lib.lib().tg_cuda_tree_attn(cache._at, d, out.data_ptr(), so[0], so[1], so[2], lse.data_ptr(),
+                                            work.data_ptr() if size else None, size, stream))
     return out, lse
 
 
