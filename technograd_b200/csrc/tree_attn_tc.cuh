@@ -446,6 +446,8 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 
 			const bool end = c.tile == c.all - 1;
 			if (end || j == left - 1) {
+				// over the unit before's, once the other half has read them too: a unit of one or two tiles needs nothing else of that half
+				if (unit && !ta_wait(B, &B->o_free, (unit - 1) & 1, p.c)) break;
 				B->ml[hf][row] = make_float2(mr, l);
 				mbar_arrive_warp(&B->x_full);
 				if (!ta_wait(B, &B->x_full, unit & 1, p.c) || !ta_wait(B, &B->p_empty[0][j & 1], (j >> 1) & 1, p.c) ||
