@@ -123,6 +123,7 @@ __device__ __forceinline__ void evict_select(const EvictArgs &p, EvictShared &s)
 	for (int i = me; i < lo; i += all) keep[i] = i, out[i] = acc[i];
 	for (int i = hi + me; i < n; i += all) keep[i - n + p.budget] = i, out[i - n + p.budget] = acc[i];
 	if (want == 0) return; // of the whole cluster
+	if (ranks > 1) cluster.barrier_arrive(); // a CTA's shared memory may be written to once the CTA has begun: waited for after the loads below
 	keep += lo, out += lo;
 	// the warp's positions, `per` from w0 on: all whole warps' worth
 	const int per = (int)(((long long)n + ranks * EV_WARPS * 32 - 1) / (ranks * EV_WARPS * 32)) * 32; // at most 32 KPT
@@ -142,6 +143,7 @@ __device__ __forceinline__ void evict_select(const EvictArgs &p, EvictShared &s)
 			k[u] = i < lo || i >= hi || u * 32 >= per ? EV_NONE : evict_key(a[u]);
 		}
 	}
+	if (ranks > 1) cluster.barrier_wait();
 	// f(position, key) for the thread's positions, in order, the warp's lanes together
 	auto each = [&](auto f) {
 		if constexpr (KPT > 0) {

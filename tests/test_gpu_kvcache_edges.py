@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from technograd_b200 import _lib, kvcache  # noqa: F401
-from test_gpu_kvcache import BF16, F16, F32, INF, UNIT, Case, attend, bits, check_attend, near, plain, random_mask  # noqa: F401
+from test_gpu_kvcache import BF16, F16, F32, INF, UNIT, Case, attend, bits, check_attend, near, plain, plain_keep, random_mask  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +31,28 @@ def test_short_units_after_each_other(cuda, lens, dtype, dim):
     for _ in range(20):
         again = attend(c, mask)
         assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+@pytest.mark.parametrize("heads,n,want", [(1, 70000, 20000), (2, 20000, 7000), (70, 40000, 5000), (3, 140001, 1000)])
+def test_evict_heads_of_several_ctas(cuda, heads, n, want):
+    """Heads whose keys span a cluster of CTAs, next to heads that end before they count anything (all kept) and that
+    compete for one place, many times over and beside other work."""
+    lens = [n, want, want + 1][:heads] + [n] * (heads - 3)
+    c = Case([1] * heads, 1, 1, 8, 64, "head", F32, 1)
+    acc = torch.rand(heads, 1, n, generator=torch.Generator().manual_seed(5))
+    src = kvcache.PagedKV(c.pk, c.pv, torch.zeros(heads, -(-n // 64), dtype=torch.int32, device="cuda"), torch.tensor(lens, dtype=torch.int32, device="cuda"), max_len=n)
+    cols = -(-want // 64)
+    pool = torch.empty(heads * cols, 1, 64, 8, device="cuda")
+    dst = kvcache.PagedKV(pool, torch.empty_like(pool), torch.arange(heads * cols, dtype=torch.int32, device="cuda").view(heads, cols), torch.zeros_like(src.lens), max_len=0)
+    dev = acc.cuda()
+    keep, out, _ = kvcache.evict(src, dst, dev, want, want // 8, 2)
+    for b in range(0, heads, 1 if heads < 4 else 13):
+        kept = plain_keep(acc[b, 0, :lens[b]].tolist(), lens[b], want, want // 8, 2)
+        assert keep[b, 0, :len(kept)].tolist() == kept and torch.equal(out[b, 0, :len(kept)].cpu(), acc[b, 0, kept])
+    side = torch.cuda.Stream()
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            pool.new_empty(1 << 26).zero_()
+        again, _, _ = kvcache.evict(src, dst, dev, want, want // 8, 2)
+        assert torch.equal(again, keep)
+    torch.cuda.synchronize()
