@@ -545,7 +545,9 @@ __global__ void __launch_bounds__(32 * NG) k_attn_join(const AttnArgs p)
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = u.z / p.c.nkv, h = u.z - b * p.c.nkv;
 	const int rows = p.d.tokens * p.d.group, cnt = p.d.drafted(b), parts = u.y - u.x + 1;
 	const int x = blockIdx.y * 32 + lane, r = x / (RW * DP / 8) * RW + x % RW, col = x / RW % (DP / 8) * 8;
-	if (u.w * RT + (RT == 128 ? r - lane : r) >= rows) return; // of the whole block: a warp has 32 rows or one
+	// nothing of the block's rows is there (a warp has 32 rows, or at 256, 128 and 64 dimensions one, two and four): the whole block
+	// leaves, since single lanes may not miss its barrier
+	if (u.w * RT + blockIdx.y * 32 / (RW * DP / 8) * RW >= rows) return;
 	float top = -INFINITY, l = 0, v[8] = {};
 	auto add = [&](float m, float n, const float *y) {
 		const float t = fmaxf(top, m), f = top == -INFINITY ? 0 : ex2(top - t), a = m == -INFINITY ? 0 : ex2(m - t);

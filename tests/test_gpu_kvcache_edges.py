@@ -56,3 +56,13 @@ def test_evict_heads_of_several_ctas(cuda, heads, n, want):
         again, _, _ = kvcache.evict(src, dst, dev, want, want // 8, 2)
         assert torch.equal(again, keep)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("tokens,group", [(1, 1), (1, 3), (3, 3), (13, 1), (18, 1)])
+def test_join_of_blocks_with_few_rows(cuda, dtype, dim, tokens, group):
+    """One long sequence: many partial results of rows that fill a block of the join only in part."""
+    c = Case([9001], 1, group, dim, 64, "head", dtype, tokens)
+    mask = random_mask(1, tokens, 4)
+    check(attend(c, mask), plain(c, mask), dtype)
