@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(WeightTile<T, DP>::THREADS, 2) k_attn_weights(
 						const int row = (m0 + m) * 16 + e * 8 + g;
 						const float ref = s_lse[row];
 						if (drafted) {
-							const unsigned long long ok = s_mask[row] >> (x0 + 2 * t4);
+							const unsigned long long ok = x0 < 64 ? s_mask[row] >> (x0 + 2 * t4) : 0; // (a mask's bits end at 64, a tile may not)
 #pragma unroll
 							for (int x = 0; x < NT; x++)
 #pragma unroll

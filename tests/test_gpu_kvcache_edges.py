@@ -18,6 +18,28 @@ def check(got, want, dtype):
     near(got[1], want[1], want[3], "lse")
 
 
+def check_weights(c, mask=None, count=None, select=None, acc=None):
+    """attention_weights key by key against plain()'s probabilities, given its lse rounded to f32."""
+    want = plain(c, mask, count)
+    lse = want[1].float()
+    dev = [None if x is None else x.cuda() for x in (mask, None if count is None else torch.tensor(count, dtype=torch.int32), select, acc)]
+    got, fresh = (x.cpu() for x in kvcache.attention_weights(c.cache, c.q.cuda(), c.kn.cuda(), lse.cuda(), *dev))
+    for b, n in enumerate(c.lens):
+        m = count[b] if count else c.T
+        on = torch.tensor([1 if select is None else int(select[b]) >> t & 1 for t in range(c.T)], dtype=torch.float64)
+        off = torch.nan_to_num((lse[b].double() - want[1][b]).abs(), 0, 0, 0)  # rounding of the lse it was given
+        for h in range(c.nkv):
+            w, tol = torch.zeros(n + m, dtype=torch.float64), torch.zeros(n + m, dtype=torch.float64)
+            for j in range(h * c.group, (h + 1) * c.group):
+                p, tp = want[4][b][j]
+                w += on @ p
+                tol += on @ (tp + 2 * p * off[:, j, None])
+            base = torch.zeros(n, dtype=torch.float64) if acc is None else acc[b, h, :n].double()
+            near(got[b, h, :n], base + w[:n], tol[:n] + 2.0 ** -23 * (base + w[:n]), "acc")
+            near(fresh[b, h, :m], w[n:], tol[n:] + 2.0 ** -23 * w[n:], "fresh")
+            assert not got[b, h, n:].any() and not fresh[b, h, m:].any()
+
+
 @pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
 @pytest.mark.parametrize("lens", [[0] * 200 + [700], [0, 1, 128, 129] * 60, [128] * 300])
 def test_short_units_after_each_other(cuda, lens, dtype, dim):
@@ -66,3 +88,12 @@ def test_join_of_blocks_with_few_rows(cuda, dtype, dim, tokens, group):
     c = Case([9001], 1, group, dim, 64, "head", dtype, tokens)
     mask = random_mask(1, tokens, 4)
     check(attend(c, mask), plain(c, mask), dtype)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (F32, 128), (BF16, 256)])
+@pytest.mark.parametrize("tokens,group", [(17, 1), (32, 1), (63, 5), (64, 5)])
+def test_drafted_weights_of_all_tokens(cuda, dtype, dim, tokens, group):
+    """A tile of keys may be wider than a mask: every drafted key has its own weight, the keys past the tokens none."""
+    c = Case([40, 0, 3], 1, group, dim, 16, "head", dtype, tokens)
+    check_weights(c, random_mask(3, tokens, 6), [tokens, tokens, tokens - 1])
+    check_weights(c)
