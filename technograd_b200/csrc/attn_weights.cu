@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(WeightTile<T, DP>::THREADS, 2) k_attn_weights(
 				constexpr int MT = decltype(mt)::value;
 				float s[MT][NT][4];
 				qk_keys<T, DP, MT, NT>(s, k, s0 + m0 * 16 * P, lane);
+				unsplit_scores<T, DP, MT, NT>(s, s0 + m0 * 16 * P, ring + stage * W::STAGE, lane);
 #pragma unroll
 				for (int m = 0; m < MT; m++)
 #pragma unroll

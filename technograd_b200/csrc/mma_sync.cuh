@@ -141,6 +141,46 @@ __device__ __forceinline__ void qk_tile(float (&s)[MT][NT][4], uint32_t sq, uint
 	}
 }
 
+// q . k of two f32 rows as above, in f32
+template <int DP> static __device__ __noinline__ float plain_score(uint32_t sq, int row, uint32_t sk, int key)
+{
+	constexpr int P = DP * 4;
+	float s = 0;
+#pragma unroll 1
+	for (int c = 0; c < P / 16; c++) {
+		float q[4], k[4];
+		asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(q[0]), "=f"(q[1]), "=f"(q[2]), "=f"(q[3]) : "r"(sq + row * P + ((c ^ (row & 7)) << 4)) : "memory");
+		asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(k[0]), "=f"(k[1]), "=f"(k[2]), "=f"(k[3]) : "r"(sk + key * P + ((c ^ (key & 7)) << 4)) : "memory");
+#pragma unroll
+		for (int i = 0; i < 4; i++) s = fmaf(q[i], k[i], s);
+	}
+	return s;
+}
+
+// An infinite element makes products of split operands NaN where the score may be an infinity (infinity has no low part, and 0 times
+// it is not 0): f32 scores that are NaN are taken again without splitting. sq: the first of S's rows.
+template <class T, int DP, int MT, int NT>
+__device__ __forceinline__ void unsplit_scores(float (&s)[MT][NT][4], uint32_t sq, uint32_t sk, int lane)
+{
+	if constexpr (sizeof(T) == 4) {
+		bool nan = false;
+#pragma unroll
+		for (int m = 0; m < MT; m++)
+#pragma unroll
+			for (int x = 0; x < NT; x++)
+#pragma unroll
+				for (int e = 0; e < 4; e++) nan |= isnan(s[m][x][e]);
+		if (!__any_sync(~0u, nan)) return;
+#pragma unroll
+		for (int m = 0; m < MT; m++)
+#pragma unroll
+			for (int x = 0; x < NT; x++)
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					if (isnan(s[m][x][e])) s[m][x][e] = plain_score<DP>(sq, m * 16 + (e >> 1) * 8 + (lane >> 2), sk, x * 8 + 2 * (lane & 3) + (e & 1));
+	}
+}
+
 // A tile of KW keys as the operand of Q K^T, in registers: for many query rows, which then each
 // take their own loads only. f32: hi and lo parts.
 template <class T, int DP> struct KeyFrag { uint32_t r[DP / 16][sizeof(T) == 2 ? 4 : 8]; };

@@ -364,6 +364,7 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 #pragma unroll
 			for (int x = 0; x < NT; x++) s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = 0;
 		qk_tile<T, DP, MT, NT>(s, s0, sk, lane);
+		unsplit_scores<T, DP, MT, NT>(s, s0, sk, lane);
 #pragma unroll
 		for (int m = 0; m < MT; m++)
 #pragma unroll

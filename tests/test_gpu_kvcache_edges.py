@@ -1,6 +1,7 @@
 """The paged key/value cache operators where their kernels' parts meet: short units next to each other, several CTAs on one
 head, few rows of a block (GPU). Cases, definitions in 64 bits and tolerances as in test_gpu_kvcache.py, and half of f16's
 least spacing (2^-24) more where an f16 output is below its normal numbers: u |o| is the rounding of normal ones only."""
+import copy
 import math
 
 import pytest
@@ -97,3 +98,31 @@ def test_drafted_weights_of_all_tokens(cuda, dtype, dim, tokens, group):
     c = Case([40, 0, 3], 1, group, dim, 16, "head", dtype, tokens)
     check_weights(c, random_mask(3, tokens, 6), [tokens, tokens, tokens - 1])
     check_weights(c)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,group", [(2, 2), (9, 1), (9, 2), (40, 1), (40, 4)])
+def test_keys_of_minus_infinity(cuda, dtype, tokens, group):
+    """Keys of -infinity against positive queries have scores of -infinity: no weight, in the cache and among the drafted; a
+    token that sees nothing else has 0 and -infinity."""
+    c = Case([0, 5, 300], 2, group, 64, 16, "head", dtype, tokens)
+    c.q[:] = c.q.abs() + 0.5
+    gone = [torch.zeros(n, dtype=torch.bool) for n in c.lens]
+    gone[1][:], gone[2][torch.arange(0, 300, 7)] = True, True
+    for b, n in enumerate(c.lens):
+        for p in gone[b].nonzero()[:, 0].tolist():
+            c.pk[int(c.table[b, p // c.page]), :, p % c.page] = -INF
+    c.kn[:, 1] = -INF
+    mask = bits([[2 if t == 0 else (2 << t) - 1 for t in range(tokens)]] * 3)
+    got = attend(c, mask)
+    rest = copy.copy(c)
+    rest.lens, rest.k, rest.v = [int((~x).sum()) for x in gone], [x[~y] for x, y in zip(c.k, gone)], [x[~y] for x, y in zip(c.v, gone)]
+    want = plain(rest, mask & ~2)
+    assert (want[1][:2, 0] == -INF).all()
+    check(got, want, dtype)
+    acc, fresh = kvcache.attention_weights(c.cache, c.q.cuda(), c.kn.cuda(), want[1].float().cuda(), mask.cuda())
+    assert torch.isfinite(acc).all() and torch.isfinite(fresh).all() and not fresh[:, :, 1].any()
+    for b, n in enumerate(c.lens):
+        assert not acc[b, :, :n][:, gone[b].cuda()].any()
+    rows = (want[1] > -INF).sum(1).view(3, 2, group).sum(2)
+    assert (acc.sum(2).cpu() + fresh.sum(2).cpu() - rows).abs().max() < 1e-3  # each row that sees something spreads a weight of 1
