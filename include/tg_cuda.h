@@ -395,7 +395,10 @@ typedef struct {
  * = softmax(scale q.k) v in the cache's type, lse [seqs][tokens][nq] = the natural log of
  * the sum of exp(scale q.k). A token that sees nothing, or only scores of -infinity, has
  * out 0 and lse -infinity, and so have tokens past count. What a masked row holds
- * (infinities and NaN too) does not matter. Scores, softmax and sums are f32; 16-bit
+ * (infinities and NaN too) does not matter, and a drafted row that a token sees with a
+ * probability of 0 in f32 adds nothing to it, whatever its v. An infinity or NaN in the v of
+ * a cached row makes that element of the outputs that see it an infinity or NaN (where the
+ * row's probability is 0, possibly). Scores, softmax and sums are f32; 16-bit
  * caches round each probability to the cache's type for its product with v. work: scratch
  * of at least tg_cuda_tree_attn_workspace bytes, 16-byte aligned, not shared with a call
  * that may run at the same time (NULL where that is 0). */

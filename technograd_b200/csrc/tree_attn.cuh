@@ -406,7 +406,8 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 						const float a = ex2(mr[m][e] - top);
 						mr[m][e] = top, l[m][e] *= a;
 #pragma unroll
-						for (int d = 0; d < DP / 8; d++) o[m][d][2 * e] *= a, o[m][d][2 * e + 1] *= a;
+						for (int d = 0; d < DP / 8; d++) // (what has lost its weight may be infinite)
+							o[m][d][2 * e] = a == 0 ? 0 : o[m][d][2 * e] * a, o[m][d][2 * e + 1] = a == 0 ? 0 : o[m][d][2 * e + 1] * a;
 					}
 				}
 		}

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(con
 					const float a = ex2(mr[r] - top);
 					mr[r] = top, l[r] *= a;
 #pragma unroll
-					for (int x = 0; x < NP; x++) o[r][x].x *= a, o[r][x].y *= a;
+					for (int x = 0; x < NP; x++) o[r][x] = a == 0 ? make_float2(0, 0) : make_float2(o[r][x].x * a, o[r][x].y * a); // (what has lost its weight may be infinite)
 				}
 			}
 		}

@@ -165,6 +165,18 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 // 16-byte chunk c of row r of an operand tile of 128 rows
 __device__ __forceinline__ uint32_t ta_at(int r, int c) { return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
+// Whether the probability of drafted token u for a query row (token t, head j) is not 0 in f32 against the row's reference
+template <class T>
+__device__ __forceinline__ bool ta_weighs(const AttnArgs &p, int b, int h, int t, int j, int u, float ref)
+{
+	const T *q = (const T *)(p.d.q + b * p.d.q_seq + t * p.d.q_tok + j * p.d.q_head);
+	const T *k = (const T *)(p.d.k + b * p.d.kv_seq + u * p.d.kv_tok + h * p.d.kv_head);
+	float s = 0;
+#pragma unroll 1
+	for (int i = 0; i < p.c.dim; i++) s = fmaf(PgElem<T>::get(q[i]), PgElem<T>::get(k[i]), s);
+	return !(s * p.d.scale * 1.4426950408889634f - ref < -126); // (a score that is NaN counts)
+}
+
 template <class T, int DP>
 __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
 {
@@ -425,7 +437,7 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 					uint32_t u[32];
 					tmem_ld32(mine + w * 32, v);
 #pragma unroll
-					for (int e = 0; e < 32; e++) u[e] = __float_as_uint(v[e] * f);
+					for (int e = 0; e < 32; e++) u[e] = __float_as_uint(f == 0 ? 0 : v[e] * f);
 					ta_st32(mine + w * 32, u);
 				}
 			}
@@ -468,9 +480,11 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 					tmem_ld32(lanes + 256 + DP + w * 32, u);
 #pragma unroll
 					for (int e = 0; e < 32; e++) v[e] = (fa == 0 ? 0 : v[e] * fa) + (fd == 0 ? 0 : u[e] * fd);
-					if (odd && r < rows)
+					if (odd && r < rows && fa != 0) // (the drafted keys are the first half's)
 						for (unsigned long long m = see; m; m &= m - 1) {
-							const T *vr = (const T *)(p.d.v + (long long)b * p.d.kv_seq + (long long)(__ffsll((long long)m) - 1) * p.d.kv_tok + h * p.d.kv_head) + w * 32;
+							const int key = __ffsll((long long)m) - 1, t = r / p.d.group;
+							if (!ta_weighs<T>(p, b, h, t, h * p.d.group + (r - t * p.d.group), key, a.x)) continue;
+							const T *vr = (const T *)(p.d.v + (long long)b * p.d.kv_seq + (long long)key * p.d.kv_tok + h * p.d.kv_head) + w * 32;
 #pragma unroll
 							for (int e = 0; e < 32; e++) {
 								const float y = w * 32 + e < p.c.dim ? PgElem<T>::get(vr[e]) : 0;

@@ -126,3 +126,37 @@ def test_keys_of_minus_infinity(cuda, dtype, tokens, group):
         assert not acc[b, :, :n][:, gone[b].cuda()].any()
     rows = (want[1] > -INF).sum(1).view(3, 2, group).sum(2)
     assert (acc.sum(2).cpu() + fresh.sum(2).cpu() - rows).abs().max() < 1e-3  # each row that sees something spreads a weight of 1
+
+
+def with_infinities(dtype, tokens, group):
+    """Token 0's value row holds an infinity and a NaN. Masks: every token sees itself and token 0; and itself alone."""
+    c = Case([0, 5, 300, 5000], 2, group, 64, 16, "head", dtype, tokens)
+    c.q[:] = c.q.abs() + 0.5  # so that a key of -60 has a score of -240 or less, and one of 60 one of 240 or more
+    c.vn[:, 0, :, 5], c.vn[:, 0, :, 6] = INF, math.nan
+    return c, bits([[1 << t | 1 for t in range(tokens)]] * 4), bits([[1 << t for t in range(tokens)]] * 4)
+
+
+ROWS = [(2, 2), (9, 2), (40, 1), (40, 2)]  # tokens and heads per key head: 4, 18, 40 and 80 rows
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,group", ROWS)
+@pytest.mark.parametrize("far", [-60.0, -INF])
+def test_infinities_of_no_weight(cuda, dtype, tokens, group, far):
+    """A drafted row that a token sees with a probability of 0 in f32 adds nothing to it, whatever it holds."""
+    c, mask, alone = with_infinities(dtype, tokens, group)
+    c.kn[:, 0] = far
+    got, want = attend(c, mask), plain(c, alone)
+    check([x[:, 1:] for x in got], [x[:, 1:] for x in want[:4]], dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,group", ROWS)
+def test_infinities_that_lose_their_weight(cuda, dtype, tokens, group):
+    """... also where only a later key takes its probability away; token 0, which sees nothing else drafted, gets them."""
+    c, mask, alone = with_infinities(dtype, tokens, group)
+    c.kn[:, 0], c.kn[:, 1:] = 0, 60
+    got, want = attend(c, mask), plain(c, alone)
+    check([x[:, 1:] for x in got], [x[:, 1:] for x in want[:4]], dtype)
+    out = got[0][:, 0].float()
+    assert torch.isinf(out[..., 5]).all() and torch.isnan(out[..., 6]).all() and torch.isfinite(out[..., :5]).all() and torch.isfinite(out[..., 7:]).all()
