@@ -161,7 +161,6 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p, 
 	} else {
 		// ---------------- a key per thread ----------------
 		const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-		const float zs = p.d.scale * 1.4426950408889634f; // (the tensor core's sums of scores are no exacter than this form of the exponent)
 		int unit = -1;
 		for (int j = 0; j < left; j++, cursor_next<TK>(p, c, 1)) {
 			if (j == 0 || c.tile == 0) { // a unit's rows: their lse, and whom they count for
@@ -172,7 +171,7 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p, 
 					const int t = r / p.d.group;
 					const bool on = r < rows && t < cnt && (sel >> t & 1);
 					const float lse = on ? p.lse[((long long)c.b * p.d.tokens + t) * p.d.nq + c.h * p.d.group + r - t * p.d.group] : -INFINITY;
-					B->lse[unit & 1][r] = lse * 1.4426950408889634f;
+					B->lse[unit & 1][r] = lse;
 					B->mask[unit & 1][r] = lse == -INFINITY ? 0 : p.d.sees(c.b, t, cnt);
 				}
 				mbar_arrive_warp(&B->rows_full);
@@ -192,10 +191,10 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p, 
 				if (drafted) {
 					const unsigned long long *mask = &B->mask[unit & 1][x];
 #pragma unroll
-					for (int e = 0; e < 32; e++) w[e & 3] += tid < 64 && mask[e] >> (tid & 63) & 1 ? ex2(v[e] * zs - lse[e]) : 0;
+					for (int e = 0; e < 32; e++) w[e & 3] += tid < 64 && mask[e] >> (tid & 63) & 1 ? weight_of(v[e], p.d.scale, lse[e]) : 0;
 				} else {
 #pragma unroll
-					for (int e = 0; e < 32; e++) w[e & 3] += lse[e] != -INFINITY ? ex2(v[e] * zs - lse[e]) : 0;
+					for (int e = 0; e < 32; e++) w[e & 3] += lse[e] != -INFINITY ? weight_of(v[e], p.d.scale, lse[e]) : 0;
 				}
 			}
 			tc_fence_before();

@@ -160,3 +160,33 @@ def test_infinities_that_lose_their_weight(cuda, dtype, tokens, group):
     check([x[:, 1:] for x in got], [x[:, 1:] for x in want[:4]], dtype)
     out = got[0][:, 0].float()
     assert torch.isinf(out[..., 5]).all() and torch.isnan(out[..., 6]).all() and torch.isfinite(out[..., :5]).all() and torch.isfinite(out[..., 7:]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,group", [(1, 2), (16, 2), (17, 2), (64, 4), (64, 5)])
+def test_weights_of_large_scores(cuda, dtype, tokens, group):
+    """Scores of thousands that f32 holds exactly: a weight is 2^((scale s - lse) log2 e), whose error follows the difference d
+    and not the score: 2^-24 |d| for it, its product and log2 e each, 2^-22 of the exponential, 2^-24 for each row of the sum."""
+    c = Case([150, 3], 1, group, 64, 16, "head", dtype, tokens)
+    g = torch.Generator().manual_seed(3)
+    c.q[:] = 0
+    c.q[..., 0] = 128
+    for b, n in enumerate(c.lens):
+        c.k[b][:] = 0
+        c.k[b][..., 0] = torch.randint(195, 201, (n, 1), generator=g).to(dtype)
+        for p in range(n):
+            c.pk[int(c.table[b, p // 16]), :, p % 16] = c.k[b][p].cuda()
+    c.kn[:] = 0
+    c.kn[..., 0] = torch.randint(195, 201, c.kn.shape[:3], generator=g).to(dtype)
+    lse = 3200 + 2 * torch.rand(2, tokens, group, generator=g)
+    acc, fresh = (x.cpu().double() for x in kvcache.attention_weights(c.cache, c.q.cuda(), c.kn.cuda(), lse.cuda(), scale=0.125))
+    for b, n in enumerate(c.lens):
+        k = torch.cat([c.k[b][:, 0, 0], c.kn[b, :, 0, 0]]).double()
+        d = 16 * k[None, None] - lse[b].double()[:, :, None]  # [token][head][key]
+        w = torch.exp(d)
+        tol = w * (3 * 2.0 ** -24 * d.abs() + 2.0 ** -22 + 2.0 ** -24 * tokens * group)
+        see = torch.ones(tokens, n + tokens)
+        see[:, n:].tril_()
+        w, tol = ((x * see[:, None]).sum((0, 1)) for x in (w, tol))
+        near(acc[b, 0, :n], w[:n], tol[:n], "acc")
+        near(fresh[b, 0], w[n:], tol[n:], "fresh")
