@@ -86,6 +86,31 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b)
 	return *(float2 *)&d;
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+	unsigned long long d;
+	asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
+	return *(float2 *)&d;
+}
+
+// Two probabilities as 16-bit high and low parts: within 2^-15 of the number (bf16), 2^-21 (f16), so that P V errs by far less than
+// the output's rounding. The high part is cut off a little below the number, so that a positive one has positive parts: an
+// infinite V element then stays what it is (but f16 has no low part of numbers below 2^-14).
+__device__ __forceinline__ void split16(float2 x, uint32_t &hi, uint32_t &lo, __nv_bfloat16)
+{
+	const float2 y = mul2(x, make_float2(1 - 0x1p-23f, 1 - 0x1p-23f));
+	hi = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632);
+	const float2 z = add2(x, make_float2(-__uint_as_float(__float_as_uint(y.x) & 0xffff0000u), -__uint_as_float(__float_as_uint(y.y) & 0xffff0000u)));
+	lo = pack16(z.x, z.y, __nv_bfloat16());
+}
+__device__ __forceinline__ void split16(float2 x, uint32_t &hi, uint32_t &lo, __half)
+{
+	const float2 y = mul2(x, make_float2(1 - 0x1p-23f, 1 - 0x1p-23f));
+	asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y.y), "f"(y.x));
+	const float2 z = fma2(__half22float2(*(const __half2 *)&hi), make_float2(-1, -1), x);
+	lo = pack16(z.x, z.y, __half());
+}
+
 // 16 bytes from global to shared memory, or 16 zero bytes
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool have)
 {
@@ -259,19 +284,21 @@ __device__ __forceinline__ void qk_keys(float (&s)[MT][NT][4], const KeyFrag<T, 
 	}
 }
 
-// O[16 rows x DP] += P V, P in the accumulator layout of qk_tile
+// O[16 rows x DP] += P V, P in the accumulator layout of qk_tile, 16 bits in two parts (split16). twin: rows 8 to 15 are rows 0 to 7
+// again, and take the low parts: the two halves of O add up to theirs.
 template <class T, int DP, int MT, int NT>
-__device__ __forceinline__ void pv_tile(float (&o)[MT][DP / 8][4], const float (&s)[MT][NT][4], uint32_t sv, int lane)
+__device__ __forceinline__ void pv_tile(float (&o)[MT][DP / 8][4], const float (&s)[MT][NT][4], uint32_t sv, int lane, bool twin)
 {
 	constexpr int P = DP * (int)sizeof(T);
 	if constexpr (sizeof(T) == 2) {
 		const int l7 = lane & 7, mi = lane >> 3;
 		const uint32_t vrow = sv + ((mi & 1) * 8 + l7) * P;
-		uint32_t a[MT][4];
+		uint32_t a[MT][4], lo[MT][4];
 #pragma unroll
 		for (int m = 0; m < MT; m++)
 #pragma unroll
-			for (int i = 0; i < 4; i++) a[m][i] = pack16(s[m][i >> 1][(i & 1) * 2], s[m][i >> 1][(i & 1) * 2 + 1], T());
+			for (int i = 0; i < 4; i++) split16(make_float2(s[m][i >> 1][(i & 1) * 2], s[m][i >> 1][(i & 1) * 2 + 1]), a[m][i], lo[m][i], T());
+		if (twin) a[0][1] = lo[0][0], a[0][3] = lo[0][2];
 #pragma unroll
 		for (int d = 0; d < DP / 16; d++) {
 			uint32_t b[4];
@@ -280,6 +307,13 @@ __device__ __forceinline__ void pv_tile(float (&o)[MT][DP / 8][4], const float (
 			for (int m = 0; m < MT; m++) {
 				mma16(o[m][2 * d], a[m], b[0], b[1], T());
 				mma16(o[m][2 * d + 1], a[m], b[2], b[3], T());
+			}
+			if (!twin) {
+#pragma unroll
+				for (int m = 0; m < MT; m++) {
+					mma16(o[m][2 * d], lo[m], b[0], b[1], T());
+					mma16(o[m][2 * d + 1], lo[m], b[2], b[3], T());
+				}
 			}
 		}
 	} else {

@@ -311,6 +311,7 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
 	const uint32_t s0 = smem_u32(smem), ring = s0 + A::RING + warp * NST * A::STAGE;
 	const int extra = (p.d.tokens + TK - 1) / TK, rows = p.d.tokens * p.d.group, chunks = p.c.dim * (int)sizeof(T) / 16;
+	const bool twin = MT == 1 && sizeof(T) == 2 && rows <= 8; // rows 8 to 15 are rows 0 to 7 again (pv_tile)
 	const float zs = p.d.scale * 1.4426950408889634f;
 	pdl_launch();
 	pdl_wait();
@@ -335,14 +336,14 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 			from_start = c.tile == 0;
 			cnt = p.d.drafted(c.b);
 			for (int x = tid; x < RT * CH; x += 128) {
-				const int row = x / CH, ch = x % CH, r = c.r * RT + row, t = r / p.d.group;
+				const int row = x / CH, ch = x % CH, r = c.r * RT + (twin ? row & 7 : row), t = r / p.d.group;
 				uint4 v = make_uint4(0, 0, 0, 0);
 				if (r < rows && ch < chunks)
 					v = *(const uint4 *)(p.d.q + (long long)c.b * p.d.q_seq + (long long)t * p.d.q_tok + (long long)(c.h * p.d.group + r % p.d.group) * p.d.q_head + ch * 16);
 				*(uint4 *)(smem + row * P + ((ch ^ (row & 7)) << 4)) = v;
 			}
 			if (tid < RT) {
-				const int t = (c.r * RT + tid) / p.d.group;
+				const int t = (c.r * RT + (twin ? tid & 7 : tid)) / p.d.group;
 				s_mask[tid] = t < cnt ? p.d.sees(c.b, t, cnt) : 0;
 			}
 #pragma unroll
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 			}
 			plain = !__any_sync(~0u, odd);
 		}
-		if (plain) pv_tile<T, DP, MT, NT>(o, s, sv, lane);
+		if (plain) pv_tile<T, DP, MT, NT>(o, s, sv, lane, twin);
 		else {
 #pragma unroll
 			for (int x = 0; x < NT; x++)
@@ -455,13 +456,17 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 								for (int m = 0; m < MT; m++)
 #pragma unroll
 									for (int e = 0; e < 2; e++)
-										if (pr[m][e] != 0) o[m][d][2 * e + z] += pr[m][e] * v;
+										if (pr[m][e] != 0 && !(twin && e)) o[m][d][2 * e + z] += pr[m][e] * v;
 							}
 					}
 		}
 		const bool end = c.tile == c.all - 1, last = i == left - 1;
 		if (end || last) {
 			// ---- the unit's end, or the share's: join the four warps
+			if (twin) {
+#pragma unroll
+				for (int d = 0; d < DP / 8; d++) o[0][d][0] += o[0][d][2], o[0][d][1] += o[0][d][3];
+			}
 #pragma unroll
 			for (int m = 0; m < MT; m++)
 #pragma unroll

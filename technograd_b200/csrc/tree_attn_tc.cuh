@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 					tc_fence_after();
 					const uint32_t pa = tmem + (j & 1) * TK + f * 64, v = base + A::V + j % A::NST * A::OP + f * 8192;
 #pragma unroll
-					for (int kk = 0; kk < 4; kk++) ta_mma_ts(tmem + 256 + f * DP, pa + kk * 8, ta_mn_desc(v + kk * 2048, 16384), idO, !first || kk > 0);
+					for (int kk = 0; kk < 8; kk++) // P's high parts, then its low ones
+						ta_mma_ts(tmem + 256 + f * DP, pa + kk * 8, ta_mn_desc(v + (kk & 3) * 2048, 16384), idO, !first || kk > 0);
 					tc_commit(&B->p_empty[f][j & 1]);
 					tc_commit(&B->vfree[j % A::NST]);
 				}
@@ -443,15 +444,16 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 			}
 			const float ref = mr == -INFINITY ? 0 : mr;
 			float2 sum[2] = {make_float2(0, 0), make_float2(0, 0)};
-			uint32_t pw[32];
+			uint32_t pw[32], lo[32];
 #pragma unroll
 			for (int i = 0; i < 32; i++) {
 				const float2 y = fma2(make_float2(z[2 * i], z[2 * i + 1]), make_float2(mul, mul), make_float2(-ref, -ref));
 				const float2 q = make_float2(ex2(y.x), ex2(y.y));
 				sum[i & 1] = add2(sum[i & 1], q);
-				pw[i] = pack16(q.x, q.y, T());
+				split16(q, pw[i], lo[i], T());
 			}
 			ta_st32(lanes + (j & 1) * TK + hf * 64, pw); // 64 keys in 32 columns
+			ta_st32(lanes + (j & 1) * TK + hf * 64 + 32, lo);
 			l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 			tc_fence_before();
 			mbar_arrive_warp(&B->p_full[hf][j & 1]);

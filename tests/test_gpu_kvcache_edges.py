@@ -190,3 +190,42 @@ def test_weights_of_large_scores(cuda, dtype, tokens, group):
         w, tol = ((x * see[:, None]).sum((0, 1)) for x in (w, tol))
         near(acc[b, 0, :n], w[:n], tol[:n], "acc")
         near(fresh[b, 0], w[n:], tol[n:], "fresh")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("tokens,group", [(1, 2), (4, 2), (3, 3), (16, 2), (20, 2), (64, 2)])
+@pytest.mark.parametrize("sharp", [1, 4])
+def test_16_bit_outputs_are_rounded_once(cuda, dtype, dim, tokens, group, sharp):
+    """An output's error is its own rounding and that of an f32 softmax, whether many keys share the weight or one has most of it:
+    probabilities keep 2^-15 (bf16) or 2^-20 (f16, with 2^-35 of the largest for each key, below its normal numbers) of theirs."""
+    c = Case([1, 0, 300, 2000], 2, group, dim, 16, "head", dtype, tokens)
+    c.q *= sharp
+    mask = random_mask(4, tokens, 9, empty=False)
+    got, want = attend(c, mask), plain(c, mask)
+    of = copy.copy(c)
+    of.v, of.vn = [x.abs() for x in c.v], c.vn.abs()
+    spread = plain(of, mask)[0]  # sum p |v|
+    kept = 2.0 ** -15 if dtype is BF16 else 2.0 ** -20
+    tol = want[2] - (UNIT[dtype] - kept) * spread
+    if dtype is F16:
+        tol += 2.0 ** -25 + torch.tensor([(n + tokens) * 2.0 ** -35 * 6 for n in c.lens])[:, None, None, None]
+    near(got[0], want[0], tol, "out")
+    near(got[1], want[1], want[3], "lse")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens,group", [(1, 2), (9, 1), (40, 1), (64, 2)])
+def test_infinite_cached_values(cuda, dtype, tokens, group):
+    """An infinite element of a cached value row with a probability (here 2^-14 or more) is infinite in the outputs, with its sign,
+    and nothing else is, though a probability is two parts to the tensor core."""
+    c = Case([200], 1, group, 64, 16, "head", dtype, tokens)
+    c.q *= 0.25
+    for i, p in enumerate((0, 17, 63, 64, 199)):
+        for at, x in ((i, INF), (20 + i, -INF)):
+            c.pv[int(c.table[0, p // 16]), 0, p % 16, at] = x
+    for zero in (False, True):  # and all scores alike: probabilities of one bit
+        out = attend(c)[0].float()
+        assert (out[..., :5] == INF).all() and (out[..., 20:25] == -INF).all()
+        assert torch.isfinite(out[..., 5:20]).all() and torch.isfinite(out[..., 25:]).all()
+        c.q *= 0
