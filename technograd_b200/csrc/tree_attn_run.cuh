@@ -48,24 +48,34 @@ static int attn_run_fma(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
 	return attn_join<float, DP, R>(p, pl, st);
 }
 
-template <class T, int DP>
-static int attn_run_tc(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
+template <class T, int DP, bool BOX>
+static int attn_run_tc(const AttnArgs &p, const AttnPlan &pl, const CUtensorMap *maps, cudaStream_t st)
 {
 	using A = TaTile<DP>;
 	static std::atomic<unsigned long long> done{0};
+	auto *kernel = k_tree_attn_tc<T, DP, BOX>;
 	if (!(done.load(std::memory_order_acquire) >> pl.dev & 1)) { // the roles' registers must be the launch's: a warp would wait for ever for others
 		cudaFuncAttributes at;
-		TGC_CUDA(cudaFuncGetAttributes(&at, k_tree_attn_tc<T, DP>));
+		TGC_CUDA(cudaFuncGetAttributes(&at, kernel));
 		if (at.numRegs < TA_REGS) return set_err(TG_CUDA_EUNSUPPORTED, "tree attention kernel built with %d registers, not %d", at.numRegs, TA_REGS);
 	}
-	int rc = pg_smem(k_tree_attn_tc<T, DP>, A::SMEM, pl.dev, done);
+	int rc = pg_smem(kernel, A::SMEM, pl.dev, done);
 	if (rc) return rc;
+	TGC_CUDA(launch_pdl(kernel, dim3(pl.grid), dim3(A::THREADS), A::SMEM, st, p, maps[0], maps[1]));
+	return pl.whole ? TG_CUDA_OK : attn_join<T, DP, A::RT>(p, pl, st);
+}
+
+// Pages that suit boxes have a kernel of their own: one kernel with both ways of fetching costs the other pages (24 rows, trees of
+// 21 tokens over 8 sequences of up to 1280 positions) 29.4 us where 26.8 do, and copies cost pages of 64 (48 sequences of up
+// to 6001 positions) 198 us where boxes took 187.
+template <class T, int DP>
+static int attn_run_tc(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st)
+{
 	AttnArgs a = p;
 	CUtensorMap maps[2] = {};
 	const bool f16 = std::is_same<T, __half>::value;
-	if (!pg_map(&maps[0], p.c, p.c.k, f16, 64, &a.box) || !pg_map(&maps[1], p.c, p.c.v, f16, 64, &a.box)) a.box.rows = 0;
-	TGC_CUDA(launch_pdl(k_tree_attn_tc<T, DP>, dim3(pl.grid), dim3(A::THREADS), A::SMEM, st, a, maps[0], maps[1]));
-	return pl.whole ? TG_CUDA_OK : attn_join<T, DP, A::RT>(p, pl, st);
+	if (pg_map(&maps[0], p.c, p.c.k, f16, 64, &a.box) && pg_map(&maps[1], p.c, p.c.v, f16, 64, &a.box)) return attn_run_tc<T, DP, true>(a, pl, maps, st);
+	return attn_run_tc<T, DP, false>(a, pl, maps, st);
 }
 
 template <class T>

@@ -177,7 +177,7 @@ __device__ __forceinline__ bool ta_weighs(const AttnArgs &p, int b, int h, int t
 	return !(s * p.d.scale * 1.4426950408889634f - ref < -126); // (a score that is NaN counts)
 }
 
-template <class T, int DP>
+template <class T, int DP, bool BOX>
 __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
 {
 	using A = TaTile<DP>;
@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 		uint32_t at[2];
 		// by TMA, lane i has box i / (DP / 64) of its half's 64 rows, and 64 of its dimensions
 		constexpr int ND = DP / 64;
-		const int boxes = p.box.rows ? 64 / p.box.rows : 0;
-		auto by_box = [&]() { return boxes && c.tile < c.ctx - isv; };
+		const int boxes = BOX ? 64 / p.box.rows : 0;
+		auto by_box = [&]() { return BOX && c.tile < c.ctx - isv; };
 		auto look = [&]() {
 			const bool drafted = c.tile >= c.ctx, box = by_box();
 #pragma unroll
