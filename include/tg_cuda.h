@@ -355,8 +355,9 @@ int tg_cuda_ssm_get_stats(const tg_cuda_ssm *g, tg_cuda_ssm_stats *out);
  * pointers on the current device; calls are asynchronous on `stream` (NULL = the legacy
  * default stream), allocate no device memory and keep nothing between calls. Every row
  * (cache, q, drafted k and v, out) starts on a 16-byte boundary and has a multiple of 16
- * bytes; head_dim is at most 256. Strides are not negative, and a pool is less than 2^32
- * times as long as its pages' and rows' common alignment (64 GB at 16 bytes).
+ * bytes; head_dim is at most 256. Strides are not negative (one along a single element is
+ * not looked at), and a pool is less than 2^32 times as long as its pages' and rows' common
+ * alignment (64 GB at 16 bytes).
  *
  * len and table are read by the kernels. A len outside [0, max_len] is taken as the
  * nearest of the two, rows of a page number outside [0, pages) read as zeros and are

@@ -57,9 +57,13 @@ int pg_device(const char *who, int *sms, int **status)
 	return TG_CUDA_OK;
 }
 
-int pg_cache(const char *who, const tg_cuda_kv *c, PgCache *o)
+// A stride along one element alone is never used, and need not suit
+static long long pg_stride(long long s, int n, int e) { return n <= 1 && (s < 0 || s * e & 15) ? 0 : s; }
+
+int pg_cache(const char *who, const tg_cuda_kv *desc, PgCache *o)
 {
-	if (!c) return set_err(TG_CUDA_EINVAL, "%s: NULL cache", who);
+	if (!desc) return set_err(TG_CUDA_EINVAL, "%s: NULL cache", who);
+	tg_cuda_kv copy = *desc, *c = &copy;
 	if (c->type != TG_CUDA_F32 && c->type != TG_CUDA_F16 && c->type != TG_CUDA_BF16)
 		return set_err(TG_CUDA_EINVAL, "%s: element type %d", who, c->type);
 	const int e = pg_size(c->type);
@@ -73,6 +77,7 @@ int pg_cache(const char *who, const tg_cuda_kv *c, PgCache *o)
 	if (c->max_len > 0x7fff0000) return set_err(TG_CUDA_EINVAL, "%s: max_len %d", who, c->max_len);
 	if (c->seqs && (!c->len || (!c->table && c->table_cols > 0) || ((!c->k || !c->v) && c->pages > 0)))
 		return set_err(TG_CUDA_EINVAL, "%s: NULL pointer in the cache", who);
+	c->page_stride = pg_stride(c->page_stride, c->pages, e), c->head_stride = pg_stride(c->head_stride, c->nkv, e), c->pos_stride = pg_stride(c->pos_stride, c->page, e);
 	if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) || ((c->page_stride | c->head_stride | c->pos_stride) * e & 15))
 		return set_err(TG_CUDA_EINVAL, "%s: cache rows must start on 16-byte boundaries", who);
 	if (c->page_stride < 0 || c->head_stride < 0 || c->pos_stride < 0) return set_err(TG_CUDA_EINVAL, "%s: negative strides", who);
@@ -87,11 +92,14 @@ int pg_cache(const char *who, const tg_cuda_kv *c, PgCache *o)
 	return TG_CUDA_OK;
 }
 
-int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, int use, int most, PgDrafts *o)
+int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *desc, int use, int most, PgDrafts *o)
 {
-	if (!d) return set_err(TG_CUDA_EINVAL, "%s: NULL drafted tokens", who);
+	if (!desc) return set_err(TG_CUDA_EINVAL, "%s: NULL drafted tokens", who);
+	tg_cuda_drafts copy = *desc, *d = &copy;
 	if (d->tokens <= 0 || (most && d->tokens > most)) return set_err(TG_CUDA_EINVAL, "%s: %d tokens per sequence", who, d->tokens);
 	const int e = pg_size(c->type);
+	d->q_seq = pg_stride(d->q_seq, c->seqs, e), d->q_tok = pg_stride(d->q_tok, d->tokens, e), d->q_head = pg_stride(d->q_head, d->nq, e);
+	d->kv_seq = pg_stride(d->kv_seq, c->seqs, e), d->kv_tok = pg_stride(d->kv_tok, d->tokens, e), d->kv_head = pg_stride(d->kv_head, c->nkv, e);
 	if (use & PG_USE_Q) {
 		if (d->nq <= 0 || d->nq > 1 << 20 || d->nq % c->nkv)
 			return set_err(TG_CUDA_EINVAL, "%s: nq %d is not a multiple of nkv %d, or over 2^20", who, d->nq, c->nkv);

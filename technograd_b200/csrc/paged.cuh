@@ -102,9 +102,9 @@ template <class K> static inline int pg_smem(K kernel, int bytes, int dev, std::
 }
 
 // paged.cu: checks a description and fills the device view. `who` opens the error text.
-int pg_cache(const char *who, const tg_cuda_kv *c, PgCache *out);
+int pg_cache(const char *who, const tg_cuda_kv *desc, PgCache *out);
 enum { PG_USE_Q = 1, PG_USE_K = 2, PG_USE_V = 4 };
-int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, int use, int most, PgDrafts *out);
+int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *desc, int use, int most, PgDrafts *out);
 // The device's number and SM count, and the address of its status word; EDEVICE when a kernel
 // of an earlier call reported something.
 int pg_device(const char *who, int *sms, int **status);

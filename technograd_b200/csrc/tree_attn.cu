@@ -70,6 +70,9 @@ extern "C" int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, v
 	if ((rc = pg_cache(who, c, &p.c)) || (rc = pg_drafts(who, c, d, PG_USE_Q | PG_USE_K | PG_USE_V, 64, &p.d))) return rc;
 	const int e = pg_size(c->type);
 	if (c->seqs && (!out || !lse)) return set_err(TG_CUDA_EINVAL, "%s: NULL output", who);
+	if (c->seqs <= 1) out_seq = 0; // strides along one element are not used
+	if (d->tokens <= 1) out_tok = 0;
+	if (d->nq <= 1) out_head = 0;
 	if (((uintptr_t)out & 15) || ((out_seq | out_tok | out_head) * e & 15))
 		return set_err(TG_CUDA_EINVAL, "%s: out rows must start on 16-byte boundaries", who);
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0 || (rc = attn_plan(who, c, p.d, &pl))) return rc;

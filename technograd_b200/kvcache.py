@@ -39,6 +39,11 @@ def _check(name: str, x, dtype, shape, index: int) -> None:
                          f"{tuple(x.shape)} strides {x.stride()} on {x.device}")
 
 
+def _alike(x, y) -> bool:
+    """Tensors of one shape whose strides are the same wherever there is more than one element along them."""
+    return x.stride() == y.stride() or all(n == 1 or a == b for n, a, b in zip(x.shape, x.stride(), y.stride()))
+
+
 def _weights(name: str, x, cache: "PagedKV", least: int) -> tuple:
     """x is f32 [seqs, nkv, >= least] on the cache's device, rows contiguous; its strides."""
     n = x.shape
@@ -65,7 +70,7 @@ class PagedKV:
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, max_len: int | None = None):
         _need(k.dim() == 4 and k.dtype in _TYPES and k.is_cuda, "k: expected an f32, f16 or bf16 CUDA tensor [pages, nkv, page, head_dim]")
         _need(k.shape[3] <= 1 or k.stride(3) == 1, "k: the head dimension must be contiguous")
-        _need(v.dtype is k.dtype and v.device == k.device and v.shape == k.shape and v.stride() == k.stride(),
+        _need(v.dtype is k.dtype and v.device == k.device and v.shape == k.shape and _alike(v, k),
               "v: expected k's type, device, shape and strides")
         self.index = k.get_device()
         _need(table.dim() == 2, "table: expected [seqs, cols]")
@@ -96,7 +101,7 @@ def _drafts(cache: PagedKV, q, k, v, mask, count, scale):
     if k.dtype is not dt or k.get_device() != index or len(n) != 4 or n[0] != cache.seqs or n[2] != cache.nkv or n[3] != dim or sk[3] != 1:
         raise ValueError(f"k: expected a {dt} tensor [{cache.seqs}, tokens, {cache.nkv}, {dim}] on cuda:{index} with contiguous rows, got {k.dtype} "
                          f"{tuple(n)} strides {sk} on {k.device}")
-    if v is not None and (v.dtype is not dt or v.get_device() != index or v.shape != n or v.stride() != sk):
+    if v is not None and (v.dtype is not dt or v.get_device() != index or v.shape != n or not _alike(v, k)):
         raise ValueError(f"v: expected k's type, device, shape and strides, got {v.dtype} {tuple(v.shape)} strides {v.stride()} on {v.device}")
     nq, sq = 0, (0, 0, 0, 1)
     if q is not None:

@@ -55,3 +55,35 @@ def test_scratch_lives_until_the_call_returns(library):
     for _ in range(2):  # the plan made, and the plan found
         kvcache.tree_attention(c, *drafted())
     assert held == [True, True]
+
+
+def test_strides_of_single_rows_do_not_matter(library):
+    """k and v of one token, head or sequence are the same rows whatever their strides along it."""
+    c = cache(seqs=1)
+    q, k, v = drafted(1, 1)
+    qkv = torch.zeros(1, 5, 8 * 64, dtype=BF16)[:, 2:3].unflatten(2, (8, 64))
+    assert qkv[:, :, 6:].stride() != k.stride()
+    kvcache.tree_attention(c, q, k, qkv[:, :, 6:])
+    kvcache.commit(c, k, qkv[:, :, 6:], torch.zeros(1, dtype=torch.int32))
+    assert [n for n, _ in library.calls[-2:]] == ["tg_cuda_tree_attn", "tg_cuda_kv_commit"]
+
+
+def test_strides_of_several_rows_do(library):
+    c = cache()
+    q, k, v = drafted()
+    with pytest.raises(ValueError):
+        kvcache.tree_attention(c, q, k, v.transpose(1, 2).contiguous().transpose(1, 2))
+    assert not library.calls
+
+
+def test_the_library_does_not_look_at_strides_of_single_rows():
+    """A stride along one element alone may be anything: past the checks only the device is missing here."""
+    import ctypes as C
+    from test_kvcache_abi import cache as kv, drafts
+    L, p = kvcache._lib.lib(), C.byref
+    one = dict(seqs=1, nkv=1, pages=1, page=64, table_cols=1)
+    for c, d in ((kv(**one, page_stride=7, head_stride=1), drafts(tokens=1, nq=1, q_seq=1, q_tok=3, q_head=-1, kv_seq=5, kv_tok=1, kv_head=1)),
+                 (kv(page=1, pages=64, table_cols=64, pos_stride=-1), drafts())):
+        assert L.tg_cuda_tree_attn_workspace(p(c), p(d)) != kvcache._lib.EINVAL
+    for c, d in ((kv(page_stride=7), drafts()), (kv(head_stride=1), drafts()), (kv(), drafts(q_seq=1)), (kv(), drafts(kv_tok=1)), (kv(), drafts(kv_head=-8))):
+        assert L.tg_cuda_tree_attn_workspace(p(c), p(d)) == kvcache._lib.EINVAL
