@@ -421,7 +421,8 @@ int tg_cuda_attn_weights(const tg_cuda_kv *c, const tg_cuda_drafts *d, const flo
 /* Accepted tokens into the cache: for i < count[b], cache row len[b] + i receives drafted
  * row path[b][i] (path [seqs][tokens]; NULL = row i), keys and values, and len_out[b] =
  * len[b] + count[b] (len_out may not be len). fresh and acc, both or neither: acc[b][h][len + i]
- * = fresh[b][h][path[b][i]], acc [seqs][nkv][acc_cols] with the given strides. tokens may be
+ * = fresh[b][h][path[b][i]], acc [seqs][nkv][acc_cols] with the given strides, at which no
+ * two rows may overlap (all of one dimension between two of the other's). tokens may be
  * any number here, d->q is not read, and max_len bounds len before the call. A row past the
  * table, a path entry outside [0, tokens) or a column past acc_cols is not written and is
  * reported like a bad page. No two rows written may share a page row. */

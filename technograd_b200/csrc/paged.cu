@@ -230,6 +230,18 @@ extern "C" int tg_cuda_kv_commit(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	if (c->seqs && (!len_out || !fresh != !acc)) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);
 	if (len_out == c->len && c->seqs) return set_err(TG_CUDA_EINVAL, "%s: len_out may not be the cache's len", who);
 	if (acc && acc_cols < 0) return set_err(TG_CUDA_EINVAL, "%s: acc_cols %d", who, acc_cols);
+	if (acc) { // rows that share elements would be written in any order: one dimension's outside the other's
+		const bool inner = acc_head <= acc_seq; // heads within sequences
+		__int128 span = acc_cols;
+		for (int i = 0; i < 2; i++) {
+			const bool head = inner == !i;
+			const long long stride = head ? acc_head : acc_seq;
+			const int n = head ? c->nkv : c->seqs;
+			if (n <= 1) continue;
+			if (stride < span) return set_err(TG_CUDA_EINVAL, "%s: acc's rows overlap (strides %lld, %lld, %d columns)", who, acc_seq, acc_head, acc_cols);
+			span += (__int128)stride * (n - 1);
+		}
+	}
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0) return rc;
 	p.path = path, p.len_out = len_out, p.fresh = fresh, p.acc = acc, p.acc_seq = acc_seq, p.acc_head = acc_head;
 	p.acc_cols = acc_cols, p.seqs = c->seqs, p.chunks = c->head_dim * pg_size(c->type) / 16;

@@ -1,4 +1,5 @@
 """The paged cache's Python calls, up to the library's entry points: a stand-in takes the place of the library (CPU)."""
+import ctypes as C
 import gc
 from types import SimpleNamespace
 
@@ -6,6 +7,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 from technograd_b200 import kvcache  # noqa: E402
+from test_kvcache_abi import cache as kv, drafts  # noqa: E402
 
 BF16 = torch.bfloat16
 
@@ -78,8 +80,6 @@ def test_strides_of_several_rows_do(library):
 
 def test_the_library_does_not_look_at_strides_of_single_rows():
     """A stride along one element alone may be anything: past the checks only the device is missing here."""
-    import ctypes as C
-    from test_kvcache_abi import cache as kv, drafts
     L, p = kvcache._lib.lib(), C.byref
     one = dict(seqs=1, nkv=1, pages=1, page=64, table_cols=1)
     for c, d in ((kv(**one, page_stride=7, head_stride=1), drafts(tokens=1, nq=1, q_seq=1, q_tok=3, q_head=-1, kv_seq=5, kv_tok=1, kv_head=1)),
@@ -87,3 +87,14 @@ def test_the_library_does_not_look_at_strides_of_single_rows():
         assert L.tg_cuda_tree_attn_workspace(p(c), p(d)) != kvcache._lib.EINVAL
     for c, d in ((kv(page_stride=7), drafts()), (kv(head_stride=1), drafts()), (kv(), drafts(q_seq=1)), (kv(), drafts(kv_tok=1)), (kv(), drafts(kv_head=-8))):
         assert L.tg_cuda_tree_attn_workspace(p(c), p(d)) == kvcache._lib.EINVAL
+
+
+@pytest.mark.parametrize("seq,head,cols,good", [(200, 100, 100, True), (100, 900, 100, True), (250, 120, 100, True), (200, 100, 101, False), (0, 100, 100, False),
+                                                (200, 0, 100, False), (100, 100, 100, False), (150, 100, 100, False), (100, 850, 100, False), (-200, 100, 100, False)])
+def test_commit_refuses_weights_whose_rows_overlap(seq, head, cols, good):
+    """Several warps would write one element. The description is one that no launch takes (too many tokens), since its addresses
+    are made up: past the checks only the device is missing here."""
+    if good and torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    rc = kvcache._lib.lib().tg_cuda_kv_commit(C.byref(kv(seqs=9)), C.byref(drafts(tokens=2 ** 31 - 1)), None, 0x70000, 0x80000, 0x90000, seq, head, cols, None)
+    assert (rc != kvcache._lib.EINVAL) == good
