@@ -356,7 +356,9 @@ int tg_cuda_ssm_get_stats(const tg_cuda_ssm *g, tg_cuda_ssm_stats *out);
  * default stream), allocate no device memory and keep nothing between calls. Every row
  * (cache, q, drafted k and v, out) starts on a 16-byte boundary and has a multiple of 16
  * bytes; head_dim is at most 256. Strides are not negative (one along a single element is
- * not looked at), and a pool is less than 2^32 times as long as its pages' and rows' common
+ * not looked at). Rows that a call writes (out, the pools of a commit and of an eviction's
+ * destination, a commit's acc) do not overlap: a stride spans all of the dimensions of smaller
+ * strides. A pool is less than 2^32 times as long as its pages' and rows' common
  * alignment (64 GB at 16 bytes).
  *
  * len and table are read by the kernels. A len outside [0, max_len] is taken as the
@@ -421,8 +423,7 @@ int tg_cuda_attn_weights(const tg_cuda_kv *c, const tg_cuda_drafts *d, const flo
 /* Accepted tokens into the cache: for i < count[b], cache row len[b] + i receives drafted
  * row path[b][i] (path [seqs][tokens]; NULL = row i), keys and values, and len_out[b] =
  * len[b] + count[b] (len_out may not be len). fresh and acc, both or neither: acc[b][h][len + i]
- * = fresh[b][h][path[b][i]], acc [seqs][nkv][acc_cols] with the given strides, at which no
- * two rows may overlap (all of one dimension between two of the other's). tokens may be
+ * = fresh[b][h][path[b][i]], acc [seqs][nkv][acc_cols] with the given strides. tokens may be
  * any number here, d->q is not read, and max_len bounds len before the call. A row past the
  * table, a path entry outside [0, tokens) or a column past acc_cols is not written and is
  * reported like a bad page. No two rows written may share a page row. */

@@ -297,6 +297,7 @@ extern "C" int tg_cuda_kv_evict(const tg_cuda_kv *src, const tg_cuda_kv *dst, co
 	if ((rc = pg_cache(who, src, &p.src)) || (rc = pg_cache(who, &to, &p.dst))) return rc;
 	if (to.type != src->type || to.seqs != src->seqs || to.nkv != src->nkv || to.head_dim != src->head_dim)
 		return set_err(TG_CUDA_EINVAL, "%s: the destination's type, seqs, nkv or head_dim differ", who);
+	if ((rc = pg_apart(who, "the destination", to.head_dim, {to.page_stride, to.head_stride, to.pos_stride}, {to.pages, to.nkv, to.page}))) return rc;
 	if (budget <= 0 || recent < 0 || sink < 0 || recent > budget - sink)
 		return set_err(TG_CUDA_EINVAL, "%s: budget %d, recent %d, sink %d", who, budget, recent, sink);
 	if (src->seqs && (!keep || !acc_out || !len_out || (!acc && src->max_len))) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <utility>
 
 #include "paged.cuh"
 
@@ -126,6 +127,20 @@ int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *desc, 
 	return TG_CUDA_OK;
 }
 
+int pg_apart(const char *who, const char *what, int row, std::array<long long, 3> stride, std::array<int, 3> n)
+{
+	for (int i = 0; i < 2; i++) // ascending strides
+		for (int k = 0; k < 2; k++)
+			if (stride[k] > stride[k + 1]) std::swap(stride[k], stride[k + 1]), std::swap(n[k], n[k + 1]);
+	__int128 span = row;
+	for (int i = 0; i < 3; i++) {
+		if (n[i] <= 1) continue;
+		if (stride[i] < span) return set_err(TG_CUDA_EINVAL, "%s: rows of %s overlap (a stride of %lld)", who, what, stride[i]);
+		span += (__int128)stride[i] * (n[i] - 1);
+	}
+	return TG_CUDA_OK;
+}
+
 bool pg_map(CUtensorMap *m, const PgCache &c, const void *pool, bool f16, int rows, PgBox *box)
 {
 	static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
@@ -230,18 +245,8 @@ extern "C" int tg_cuda_kv_commit(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	if (c->seqs && (!len_out || !fresh != !acc)) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);
 	if (len_out == c->len && c->seqs) return set_err(TG_CUDA_EINVAL, "%s: len_out may not be the cache's len", who);
 	if (acc && acc_cols < 0) return set_err(TG_CUDA_EINVAL, "%s: acc_cols %d", who, acc_cols);
-	if (acc) { // rows that share elements would be written in any order: one dimension's outside the other's
-		const bool inner = acc_head <= acc_seq; // heads within sequences
-		__int128 span = acc_cols;
-		for (int i = 0; i < 2; i++) {
-			const bool head = inner == !i;
-			const long long stride = head ? acc_head : acc_seq;
-			const int n = head ? c->nkv : c->seqs;
-			if (n <= 1) continue;
-			if (stride < span) return set_err(TG_CUDA_EINVAL, "%s: acc's rows overlap (strides %lld, %lld, %d columns)", who, acc_seq, acc_head, acc_cols);
-			span += (__int128)stride * (n - 1);
-		}
-	}
+	if (acc && (rc = pg_apart(who, "acc", acc_cols, {acc_seq, acc_head, 0}, {c->seqs, c->nkv, 1}))) return rc;
+	if ((rc = pg_apart(who, "the cache", c->head_dim, {c->page_stride, c->head_stride, c->pos_stride}, {c->pages, c->nkv, c->page}))) return rc;
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0) return rc;
 	p.path = path, p.len_out = len_out, p.fresh = fresh, p.acc = acc, p.acc_seq = acc_seq, p.acc_head = acc_head;
 	p.acc_cols = acc_cols, p.seqs = c->seqs, p.chunks = c->head_dim * pg_size(c->type) / 16;

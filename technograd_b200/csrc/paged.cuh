@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <array>
 #include <atomic>
 
 #include "common.cuh"
@@ -105,6 +106,9 @@ template <class K> static inline int pg_smem(K kernel, int bytes, int dev, std::
 int pg_cache(const char *who, const tg_cuda_kv *desc, PgCache *out);
 enum { PG_USE_Q = 1, PG_USE_K = 2, PG_USE_V = 4 };
 int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *desc, int use, int most, PgDrafts *out);
+// EINVAL where rows of `row` elements that a call writes overlap: they would be written in any order. They lie apart where each
+// dimension's stride spans all of the dimensions of smaller strides.
+int pg_apart(const char *who, const char *what, int row, std::array<long long, 3> stride, std::array<int, 3> n);
 // The device's number and SM count, and the address of its status word; EDEVICE when a kernel
 // of an earlier call reported something.
 int pg_device(const char *who, int *sms, int **status);

@@ -75,6 +75,7 @@ extern "C" int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, v
 	if (d->nq <= 1) out_head = 0;
 	if (((uintptr_t)out & 15) || ((out_seq | out_tok | out_head) * e & 15))
 		return set_err(TG_CUDA_EINVAL, "%s: out rows must start on 16-byte boundaries", who);
+	if ((rc = pg_apart(who, "out", c->head_dim, {out_seq, out_tok, out_head}, {c->seqs, d->tokens, d->nq}))) return rc;
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0 || (rc = attn_plan(who, c, p.d, &pl))) return rc;
 	const size_t need = pl.bytes();
 	if (need && (!work || work_bytes < (long long)need || ((uintptr_t)work & 15)))

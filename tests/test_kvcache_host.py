@@ -98,3 +98,18 @@ def test_commit_refuses_weights_whose_rows_overlap(seq, head, cols, good):
         pytest.skip("a GPU is present")
     rc = kvcache._lib.lib().tg_cuda_kv_commit(C.byref(kv(seqs=9)), C.byref(drafts(tokens=2 ** 31 - 1)), None, 0x70000, 0x80000, 0x90000, seq, head, cols, None)
     assert (rc != kvcache._lib.EINVAL) == good
+
+
+@pytest.mark.parametrize("bad", [dict(head_stride=0), dict(pos_stride=0), dict(page_stride=0), dict(page_stride=1024), dict(head_stride=64), dict(pos_stride=56)])
+def test_pools_whose_rows_overlap_are_not_written(bad):
+    """A broadcast pool may be read, but a commit or an eviction would write its rows in any order."""
+    L, p, c = kvcache._lib.lib(), C.byref, kv(**bad)
+    assert L.tg_cuda_kv_commit(p(c), p(drafts()), None, 0x70000, None, None, 0, 0, 0, None) == kvcache._lib.EINVAL
+    assert L.tg_cuda_kv_evict(p(kv()), p(c), 0x70000, 120, 60, 32, 4, 1, 0x80000, 0x90000, 0xA0000, None) == kvcache._lib.EINVAL
+    assert L.tg_cuda_tree_attn_workspace(p(c), p(drafts())) != kvcache._lib.EINVAL
+
+
+@pytest.mark.parametrize("out", [(0, 256, 64), (768, 0, 64), (768, 256, 0), (512, 256, 64), (768, 192, 64), (768, 256, 56), (-768, 256, 64)])
+def test_outputs_whose_rows_overlap_are_refused(out):
+    L, p = kvcache._lib.lib(), C.byref
+    assert L.tg_cuda_tree_attn(p(kv()), p(drafts()), 0x60000, *out, 0x70000, None, 0, None) == kvcache._lib.EINVAL
