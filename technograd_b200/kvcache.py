@@ -61,6 +61,18 @@ def _stream(cache: "PagedKV") -> int:
     return torch._C._cuda_getCurrentRawStream(cache.index)  # torch.cuda.current_stream's handle without its object
 
 
+class _ForwardOnly(torch.autograd.Function):
+    """out and lse as results of inputs that want a gradient: there is none, and asking for it is an error."""
+
+    @staticmethod
+    def forward(ctx, out, lse, *inputs):
+        return out.detach(), lse.detach()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("kvcache.tree_attention has no backward pass")
+
+
 class PagedKV:
     """One layer's cache: pools k and v, the table of pages [seqs, cols] and lengths [seqs] (int32).
 
@@ -125,7 +137,8 @@ def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float 
     q [seqs, tokens, nq, head_dim]; k, v [seqs, tokens, nkv, head_dim], not yet in the cache; at most 64
     tokens. mask int64 [seqs, tokens]: bit u of an entry = the token attends to drafted token u (None:
     a chain). count int32 [seqs]: tokens drafted (None: all). Returns (out as q, lse f32 [seqs, tokens,
-    nq]); a token that sees nothing has out 0 and lse -inf."""
+    nq]); a token that sees nothing has out 0 and lse -inf. Forward only: where q, k or v require a
+    gradient, a backward pass through the results is an error (the other calls' results never require one)."""
     d = _drafts(cache, q, k, v, mask, count, scale)
     stream, shape = _stream(cache), q.shape
     plan = cache._plans.get(shape[1:3])
@@ -141,6 +154,8 @@ def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float 
     so = out.stride()
     _lib.check(_lib.lib().tg_cuda_tree_attn(cache._at, d, out.data_ptr(), so[0], so[1], so[2], lse.data_ptr(),
                                             work.data_ptr() if size else None, size, stream))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _ForwardOnly.apply(out, lse, q, k, v)
     return out, lse
 
 

@@ -113,3 +113,16 @@ def test_pools_whose_rows_overlap_are_not_written(bad):
 def test_outputs_whose_rows_overlap_are_refused(out):
     L, p = kvcache._lib.lib(), C.byref
     assert L.tg_cuda_tree_attn(p(kv()), p(drafts()), 0x60000, *out, 0x70000, None, 0, None) == kvcache._lib.EINVAL
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_a_gradient_through_attention_is_an_error(library, which):
+    """... and not left out in silence; without autograd, and for inputs that want none, results are plain tensors."""
+    x = [y.requires_grad_(i == which) for i, y in enumerate(drafted())]
+    out, lse = kvcache.tree_attention(cache(), *x)
+    for y in (out, lse):
+        with pytest.raises(RuntimeError, match="no backward"):
+            (y.float().sum() + x[which].float().sum()).backward(retain_graph=True)
+    with torch.no_grad():
+        assert not any(y.requires_grad for y in kvcache.tree_attention(cache(), *x))
+    assert not any(y.requires_grad for y in kvcache.tree_attention(cache(), *drafted()))
