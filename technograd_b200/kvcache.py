@@ -32,6 +32,12 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _int32(**values: int) -> None:
+    """The library's ints: ctypes would keep the low 32 bits of more."""
+    for name, x in values.items():
+        _need(-(1 << 31) <= x < 1 << 31, f"{name}: {x} does not fit 32 bits")
+
+
 def _check(name: str, x, dtype, shape, index: int) -> None:
     """x is a contiguous tensor of this type and shape on CUDA device `index`."""
     if x.dtype is not dtype or x.shape != shape or x.get_device() != index or not x.is_contiguous():
@@ -94,6 +100,7 @@ class PagedKV:
         pages, self.nkv, self.page, self.head_dim = k.shape
         self.scale = 1 / math.sqrt(self.head_dim) if self.head_dim else 1.0  # of the scores, where a call gives none
         self.max_len = self.page * cols if max_len is None else int(max_len)
+        _int32(max_len=self.max_len, pages=pages, cols=cols, seqs=self.seqs)
         s = _lib.Kv(_TYPES[k.dtype], self.seqs, self.nkv, self.head_dim, self.page, pages, cols, self.max_len,
                     k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), table.data_ptr(), lens.data_ptr())
         self._struct = s
@@ -210,6 +217,7 @@ def evict(cache: PagedKV, dst: PagedKV, acc, budget: int, recent: int = 0, sink:
     the last; the lengths in dst)."""
     _need(dst.index == cache.index and dst.dtype is cache.dtype, "dst: expected the cache's type and device")
     _need(budget > 0, "budget: expected at least 1")
+    _int32(budget=budget, recent=recent, sink=sink)
     sa = _weights("acc", acc, cache, cache.max_len)
     shape = (cache.seqs, cache.nkv, budget)
     keep = cache.lens.new_empty(shape)

@@ -229,3 +229,13 @@ def test_infinite_cached_values(cuda, dtype, tokens, group):
         assert (out[..., :5] == INF).all() and (out[..., 20:25] == -INF).all()
         assert torch.isfinite(out[..., 5:20]).all() and torch.isfinite(out[..., 25:]).all()
         c.q *= 0
+
+
+def test_lengths_past_32_bits_are_refused(cuda):
+    """A max_len of 2^32 + 40 is not one of 40, nor is a table that holds more positions than an int numbers."""
+    c = Case([40], 1, 1, 64, 16, "head", BF16, 1)
+    with pytest.raises(ValueError, match="32 bits"):
+        kvcache.PagedKV(c.pk, c.pv, c.table, c.len, max_len=2 ** 32 + 40)
+    page = torch.zeros(1, 1, 1 << 20, 8, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="32 bits"):
+        kvcache.PagedKV(page, page, torch.zeros(1, 1 << 12, dtype=torch.int32, device="cuda"), c.len)

@@ -126,3 +126,14 @@ def test_a_gradient_through_attention_is_an_error(library, which):
     with torch.no_grad():
         assert not any(y.requires_grad for y in kvcache.tree_attention(cache(), *x))
     assert not any(y.requires_grad for y in kvcache.tree_attention(cache(), *drafted()))
+
+
+def test_numbers_past_32_bits_are_refused(library):
+    """ctypes would pass on their low bits: a budget of 2^32 + 8 as 8."""
+    acc = torch.zeros(2, 2, 40)
+    for kw in (dict(budget=2 ** 32 + 8), dict(budget=8, recent=2 ** 32), dict(budget=8, sink=2 ** 32 + 1), dict(budget=8, recent=-2 ** 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            kvcache.evict(cache(), cache(), acc, **kw)
+    assert not library.calls
+    kvcache.evict(cache(), cache(), acc, 8, 2, 1)
+    assert library.calls[-1][0] == "tg_cuda_kv_evict"
