@@ -78,6 +78,7 @@ int pg_cache(const char *who, const tg_cuda_kv *desc, PgCache *o)
 	if (c->max_len > 0x7fff0000) return set_err(TG_CUDA_EINVAL, "%s: max_len %d", who, c->max_len);
 	if (c->seqs && (!c->len || (!c->table && c->table_cols > 0) || ((!c->k || !c->v) && c->pages > 0)))
 		return set_err(TG_CUDA_EINVAL, "%s: NULL pointer in the cache", who);
+	if (((uintptr_t)c->table | (uintptr_t)c->len) & 3) return set_err(TG_CUDA_EINVAL, "%s: table or len is not on a 4-byte boundary", who);
 	c->page_stride = pg_stride(c->page_stride, c->pages, e), c->head_stride = pg_stride(c->head_stride, c->nkv, e), c->pos_stride = pg_stride(c->pos_stride, c->page, e);
 	if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) || ((c->page_stride | c->head_stride | c->pos_stride) * e & 15))
 		return set_err(TG_CUDA_EINVAL, "%s: cache rows must start on 16-byte boundaries", who);
@@ -115,6 +116,7 @@ int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *desc, 
 		return set_err(TG_CUDA_EINVAL, "%s: drafted k and v rows must start on 16-byte boundaries", who);
 	if (((use & PG_USE_Q) && (d->q_seq < 0 || d->q_tok < 0 || d->q_head < 0)) || d->kv_seq < 0 || d->kv_tok < 0 || d->kv_head < 0)
 		return set_err(TG_CUDA_EINVAL, "%s: negative strides", who);
+	if (((uintptr_t)d->mask & 7) || ((uintptr_t)d->count & 3)) return set_err(TG_CUDA_EINVAL, "%s: mask (8 bytes) or count (4) is not on a boundary of its type", who);
 	// attention passes on places within a sequence's drafted rows in 32 bits of 16 bytes
 	if (most && (((unsigned __int128)d->kv_tok * d->tokens * e >> 4) >= PG_NONE ||
 		     (((unsigned __int128)d->q_tok * d->tokens + (unsigned __int128)d->q_head * d->nq) * e >> 4) >= PG_NONE))
@@ -243,6 +245,7 @@ extern "C" int tg_cuda_kv_commit(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	int rc, sms;
 	if ((rc = pg_cache(who, c, &p.c)) || (rc = pg_drafts(who, c, d, PG_USE_K | PG_USE_V, 0, &p.d))) return rc;
 	if (c->seqs && (!len_out || !fresh != !acc)) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);
+	if (((uintptr_t)path | (uintptr_t)len_out | (uintptr_t)fresh | (uintptr_t)acc) & 3) return set_err(TG_CUDA_EINVAL, "%s: a pointer is not on a 4-byte boundary", who);
 	if (len_out == c->len && c->seqs) return set_err(TG_CUDA_EINVAL, "%s: len_out may not be the cache's len", who);
 	if (acc && acc_cols < 0) return set_err(TG_CUDA_EINVAL, "%s: acc_cols %d", who, acc_cols);
 	if (acc && (rc = pg_apart(who, "acc", acc_cols, {acc_seq, acc_head, 0}, {c->seqs, c->nkv, 1}))) return rc;

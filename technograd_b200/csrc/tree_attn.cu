@@ -73,6 +73,7 @@ extern "C" int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, v
 	if (c->seqs <= 1) out_seq = 0; // strides along one element are not used
 	if (d->tokens <= 1) out_tok = 0;
 	if (d->nq <= 1) out_head = 0;
+	if ((uintptr_t)lse & 3) return set_err(TG_CUDA_EINVAL, "%s: lse is not on a 4-byte boundary", who);
 	if (((uintptr_t)out & 15) || ((out_seq | out_tok | out_head) * e & 15))
 		return set_err(TG_CUDA_EINVAL, "%s: out rows must start on 16-byte boundaries", who);
 	if ((rc = pg_apart(who, "out", c->head_dim, {out_seq, out_tok, out_head}, {c->seqs, d->tokens, d->nq}))) return rc;

@@ -137,3 +137,26 @@ def test_numbers_past_32_bits_are_refused(library):
     assert not library.calls
     kvcache.evict(cache(), cache(), acc, 8, 2, 1)
     assert library.calls[-1][0] == "tg_cuda_kv_evict"
+
+
+def test_pointers_off_their_type_are_refused():
+    """A kernel that reads a word across its boundary would fault."""
+    L, p = kvcache._lib.lib(), C.byref
+    E = kvcache._lib.EINVAL
+    out = (0x60000, 768, 256, 64)
+    for c, d in ((kv(table=0x1002), drafts()), (kv(len=0x2001), drafts()), (kv(), drafts(mask=0x3004)), (kv(), drafts(count=0x3002))):
+        assert L.tg_cuda_tree_attn_workspace(p(c), p(d)) == E
+        assert L.tg_cuda_tree_attn(p(c), p(d), *out, 0x70000, None, 0, None) == E
+        assert L.tg_cuda_attn_weights(p(c), p(d), 0x70000, None, None, 0, 0, 0x80000, 0x90000, None) == E
+        assert L.tg_cuda_kv_commit(p(c), p(d), None, 0x70000, None, None, 0, 0, 0, None) == E
+    c, d = kv(), drafts()
+    assert L.tg_cuda_tree_attn(p(c), p(d), *out, 0x70002, None, 0, None) == E
+    for at in range(5):
+        w = [0x70000, 0xA0000, 0xB0000, 0x80000, 0x90000]  # lse, select, acc, acc_out, fresh
+        w[at] += 4 if at == 1 else 2
+        assert L.tg_cuda_attn_weights(p(c), p(d), w[0], w[1], w[2], 128, 64, w[3], w[4], None) == E
+    for at in range(4):
+        w = [0x70000, 0x80000, 0x90000, 0xA0000]  # path, len_out, fresh, acc; and acc, keep, acc_out, len_out
+        w[at] += 1
+        assert L.tg_cuda_kv_commit(p(c), p(d), w[0], w[1], w[2], w[3], 200, 100, 100, None) == E
+        assert L.tg_cuda_kv_evict(p(kv()), p(c), w[0], 120, 60, 32, 4, 1, w[1], w[2], w[3], None) == E
