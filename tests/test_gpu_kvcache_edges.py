@@ -239,3 +239,13 @@ def test_lengths_past_32_bits_are_refused(cuda):
     page = torch.zeros(1, 1, 1 << 20, 8, dtype=BF16, device="cuda")
     with pytest.raises(ValueError, match="32 bits"):
         kvcache.PagedKV(page, page, torch.zeros(1, 1 << 12, dtype=torch.int32, device="cuda"), c.len)
+
+
+@pytest.mark.parametrize("page,order", [(8, "head"), (16, "pos"), (24, "pos"), (32, "head"), (64, "pos"), (128, "head"), (192, "pos"), (40, "pos"), (4, "head")])
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (BF16, 72)])
+@pytest.mark.parametrize("tokens,group", [(33, 3), (64, 4)])
+def test_weights_of_every_key_over_pages(cuda, page, order, dtype, dim, tokens, group):
+    """Key by key, which a tile's keys in another order would not pass: boxes of pages, their two halves of the dimensions, several
+    heads; what lies past a sequence's end is NaN."""
+    c = Case([1, 127, 129, 700, 0], 2, group, dim, page, order, dtype, tokens)
+    check_weights(c, random_mask(5, tokens, 7), acc=torch.rand(5, 2, 700, generator=torch.Generator().manual_seed(1)))
