@@ -9,15 +9,19 @@ extern template int attn_type<__nv_bfloat16>(const AttnArgs &, const AttnPlan &,
 
 // A unit of at most so many keys is one CTA's: smaller shares would cost more in set-up and joining.
 constexpr int ATTN_WHOLE = 256;
-// From so many query rows per key head on, 16-bit caches take the 128-row tiles of tree_attn_tc.cuh (40 rows over 131009
-// positions: 70 us, against 126 of 32-row tiles that read the cache twice; 32 rows are one such tile).
-constexpr int ATTN_TC_ROWS = 32;
+// 16-bit caches take the 128-row tiles of tree_attn_tc.cuh for more than 32 query rows per key head, which 32-row tiles read the
+// cache twice for (34 rows: 8 sequences of up to 1280 positions 27.6 us against 33, 16 of up to 4001 65 against 123, 131009 positions
+// 115 against 225); and for 17 to 32 rows where a CTA has more than ATTN_LONG tiles (32 rows, us, 128-row against 32-row
+// tiles, 8 key heads of 128 dimensions, bf16: 27.3 and 27.1 at 5 tiles, 54.2 and 50.2 at 16, 62.5 and 63.7 at 19; 65.2 and 80.5 at 28,
+// 80 and 110 at 42, 115 and 126 at 55, 211 and 259 at 125; at 64 dimensions 36.8 and 32.9 at 16, 48.4 and 51.4 at 28, 150 and 172 at
+// 125). 16 rows are one 16-row tile, at 28 tiles a CTA 48 us against 65.
+constexpr int ATTN_TC_ROWS = 32, ATTN_TC_ROWS_LONG = 16, ATTN_LONG = 24;
 
 // What beginning a unit costs, in tiles. The 128-row tiles' is about 6 (their chain of products and the output), but
-// where shares are short every CTA has such a start of its own and counting it only makes them uneven: 48
-// sequences of up to 6001 positions, 90 tiles a CTA, take 187 us at 6 and 211 at 2; 8 of up to 1280, 4 tiles
-// a CTA, 33 and 27.
-constexpr int ATTN_BEGIN = 2, ATTN_TC_BEGIN = 6, ATTN_LONG = 24;
+// where shares are short every CTA has such a start of its own and counting it only makes them uneven. 64 rows, us at 2, 4, 6 and
+// 8: 27.5, 29.4, 31.5, 33.8 at 5 tiles a CTA (8 sequences of up to 1280 positions); 44.1, 40.6, 40.9, 40.5 at 10; 65, 65, 66.7, 70 at
+// 19; 96, 78.7, 80.8, 84 at 42; 212, 206, 200, 200 at 125.
+constexpr int ATTN_BEGIN = 2, ATTN_TC_BEGIN = 6, ATTN_TC_SHORT = 7;
 
 static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o)
 {
@@ -25,7 +29,8 @@ static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, At
 	if (rc) return rc;
 	const int rows = d.tokens * d.group;
 	o->dp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
-	o->tc = c->type != TG_CUDA_F32 && o->dp <= 128 && rows > ATTN_TC_ROWS;
+	const long long wide = (long long)c->seqs * c->nkv * ((c->max_len + 127) / 128 + 1); // the 128-row tiles, where one has all rows
+	o->tc = c->type != TG_CUDA_F32 && o->dp <= 128 && rows > (wide > (long long)ATTN_LONG * o->sms ? ATTN_TC_ROWS_LONG : ATTN_TC_ROWS);
 	o->mt = rows <= 16 || o->dp == 256 ? 1 : 2; // 256 dimensions of 32 rows do not fit in registers
 	o->fma = c->type == TG_CUDA_F32 && rows <= 8 ? rows <= 4 ? 4 : 8 : 0;
 	const int rt = o->tc ? 128 : o->fma ? o->fma : 16 * o->mt, tk = o->tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
@@ -33,7 +38,7 @@ static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, At
 	const long long units = (long long)c->seqs * c->nkv * o->row_tiles;
 	const long long tiles = (c->max_len + tk - 1) / tk + (d.tokens + tk - 1) / tk;
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
-	o->whole = tiles * tk <= ATTN_WHOLE, o->least = 128 / tk, o->begin = o->tc && units * tiles > (long long)ATTN_LONG * o->sms ? ATTN_TC_BEGIN : ATTN_BEGIN;
+	o->whole = tiles * tk <= ATTN_WHOLE, o->least = 128 / tk, o->begin = o->tc && units * tiles > (long long)ATTN_TC_SHORT * o->sms ? ATTN_TC_BEGIN : ATTN_BEGIN;
 	o->slot = (size_t)(rt * o->dp + 2 * rt) * 4;
 	const long long shares = (units * (tiles + o->begin) + o->least + o->begin - 1) / (o->least + o->begin), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : o->fma || (o->mt == 1 && c->type != TG_CUDA_F32) ? 3 : 2); // the tiles' CTAS
 	o->grid = (int)(o->whole ? units : shares < wave ? shares : wave);

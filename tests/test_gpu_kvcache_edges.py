@@ -249,3 +249,21 @@ def test_weights_of_every_key_over_pages(cuda, page, order, dtype, dim, tokens, 
     heads; what lies past a sequence's end is NaN."""
     c = Case([1, 127, 129, 700, 0], 2, group, dim, page, order, dtype, tokens)
     check_weights(c, random_mask(5, tokens, 7), acc=torch.rand(5, 2, 700, generator=torch.Generator().manual_seed(1)))
+
+
+def with_room(c, positions):
+    """The same cache with a table for so many positions and max_len with it: calls are cut as for long sequences."""
+    more = torch.full((len(c.lens), -(-positions // c.page)), -7, dtype=torch.int32, device="cuda")
+    more[:, :c.table.shape[1]] = c.table
+    c.cache = kvcache.PagedKV(c.pk, c.pv, more, c.len, max_len=positions)
+    return c
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (BF16, 72), (F32, 64), (BF16, 256)])
+@pytest.mark.parametrize("tokens,group", [(1, 2), (8, 2), (17, 1), (16, 2), (40, 1)])
+@pytest.mark.parametrize("positions", [4096, 60000])
+def test_attention_cut_for_long_sequences(cuda, dtype, dim, tokens, group, positions):
+    """What a CTA has to do at most decides which kernel takes a call: the results are the definition's with each."""
+    c = with_room(Case([500, 0, 129, 1, 128, 700, 64], 2, group, dim, 16, "head", dtype, tokens), positions)
+    mask = random_mask(7, tokens, 3)
+    check(attend(c, mask), plain(c, mask), dtype)
