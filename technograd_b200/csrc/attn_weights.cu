@@ -215,9 +215,10 @@ static int weights_run_tc(WeightArgs &p, int sms, int dev, cudaStream_t st, cons
 	if (rc) return rc;
 	const long long units = (long long)p.seqs * p.c.nkv, tiles = (p.c.max_len + W::TK - 1) / W::TK + 1;
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences", who, p.seqs);
-	// a unit's start is worth about 6 tiles, except where every CTA has one of its own anyway (32-token windows over 16
-	// sequences of up to 16001 positions: 120 us at 2, 84 at 4, 82 at 8)
-	p.row_tiles = 1, p.whole = 0, p.least = 1, p.begin = units * tiles > 24ll * sms ? 6 : 2, p.split = nullptr;
+	// a unit's start is worth about 4 tiles (32-token windows, us at 2, 4, 6, 8 and 12: 16 sequences of up to 16001 positions 128,
+	// 90.7, 90.8, 93, 97; 16 of up to 6001 60, 49, 50, 54, 56; 32 of up to 1280 37.6, 34, 35.5, 38, 39; 8 of up to 1280 20, 20.5, 21,
+	// 21.2, 23)
+	p.row_tiles = 1, p.whole = 0, p.least = 1, p.begin = 4, p.split = nullptr;
 	const long long shares = (units * (tiles + p.begin) + p.begin) / (1 + p.begin);
 	CUtensorMap map = {};
 	if (!pg_map(&map, p.c, p.c.k, std::is_same<T, __half>::value, 32, &p.box)) p.box.rows = 0;
@@ -226,16 +227,20 @@ static int weights_run_tc(WeightArgs &p, int sms, int dev, cudaStream_t st, cons
 	return TG_CUDA_OK;
 }
 
-// From so many query rows per key head on (and up to TW_ROWS), 16-bit caches take attn_weights_tc.cuh (64 rows: 81 us
-// against 136).
-constexpr int WEIGHTS_TC_ROWS = 32;
+// Of up to TW_ROWS query rows per key head, 16-bit caches take attn_weights_tc.cuh where a CTA has more than so many of its tiles,
+// whatever the rows: below, latency decides, and this file's kernel has more CTAs and warps. Measured, us, tiles of 128 keys
+// against this file's (8 key heads, bf16, 2 / 32 / 64 / 120 rows), at 128 dimensions 17.2, 17.5, 23.3, 35.6 and 17.1, 19.1, 23.6, 33.0 at
+// 10 tiles a CTA; 22.4, 23.0, 31.4, 49.9 and 25.2, 28.8, 35.5, 49.9 at 16; 28.3, 29.3, 38.7, 58.1 and 31.9, 37.5, 48.1, 68.3 at 28;
+// 82.7, 69.5, 88.8, 142 and 104, 119, 148, 212 at 110. At 64 dimensions 27.3, 27.4, 37.5, 58.1 and 25.2, 29.4, 35.5, 49.6 at 28; 35.5,
+// 35.5, 47.9, 76.2 and 37.6, 43.7, 54, 74.5 at 42; 63.1, 64, 88.8, 142 and 88.5, 100, 120, 159 at 110.
+constexpr int WEIGHTS_TC_TILES_128 = 14, WEIGHTS_TC_TILES_64 = 40;
 
 template <class T>
 static int weights_type(WeightArgs &p, int sms, int dev, cudaStream_t st, const char *who)
 {
 	if constexpr (sizeof(T) == 2) {
-		const int rows = p.d.tokens * p.d.group;
-		if (p.c.dim <= 128 && rows > WEIGHTS_TC_ROWS && rows <= TW_ROWS)
+		const long long tiles = (long long)p.seqs * p.c.nkv * ((p.c.max_len + 127) / 128 + 1);
+		if (p.c.dim <= 128 && p.d.tokens * p.d.group <= TW_ROWS && tiles > (long long)(p.c.dim > 64 ? WEIGHTS_TC_TILES_128 : WEIGHTS_TC_TILES_64) * sms)
 			return p.c.dim > 64 ? weights_run_tc<T, 128>(p, sms, dev, st, who) : weights_run_tc<T, 64>(p, sms, dev, st, who);
 	}
 	if (p.c.dim > 128) return weights_run<T, 256>(p, sms, dev, st, who);

@@ -267,3 +267,12 @@ def test_attention_cut_for_long_sequences(cuda, dtype, dim, tokens, group, posit
     c = with_room(Case([500, 0, 129, 1, 128, 700, 64], 2, group, dim, 16, "head", dtype, tokens), positions)
     mask = random_mask(7, tokens, 3)
     check(attend(c, mask), plain(c, mask), dtype)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (BF16, 72), (F32, 64)])
+@pytest.mark.parametrize("tokens,group", [(1, 1), (1, 2), (8, 2), (17, 1), (16, 2), (40, 1), (64, 4), (64, 5)])
+@pytest.mark.parametrize("positions", [4096, 20000, 70000])
+def test_weights_cut_for_long_sequences(cuda, dtype, dim, tokens, group, positions):
+    """... and the weights', with what was there before and zeros past each sequence's end."""
+    c = with_room(Case([500, 0, 129, 1, 128, 700, 64], 2, group, dim, 16, "head", dtype, tokens), positions)
+    check_weights(c, random_mask(7, tokens, 3), acc=torch.rand(7, 2, positions, generator=torch.Generator().manual_seed(1)))
