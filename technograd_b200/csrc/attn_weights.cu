@@ -12,9 +12,9 @@ namespace tgc {
 // registers and, at the tile's end, over lanes. Every key is one warp's, so nothing is joined and results
 // do not depend on timing. Up to QR rows stay in shared memory for a unit; more are taken in turns at
 // every tile.
-// What bounds it: HBM while the rows are few, then instruction issue (about 540 a warp for 16 keys and 64 rows);
-// 16-bit caches of more rows take attn_weights_tc.cuh. Measured: one token of 16 query heads over 8 sequences of up to
-// 1280 positions 14 us a call.
+// What bounds it: latency where the shares are short, then instruction issue (about 540 a warp for 16 keys and 64 rows);
+// 16-bit caches with long shares take attn_weights_tc.cuh (rule and figures below). Measured: one token of 16 query heads over 8
+// sequences of up to 1280 positions 14.4 us a call.
 template <class T, int DP> struct WeightTile {
 	// eight warps where the keys' registers allow two such CTAs per SM: the products' latencies need them
 	static constexpr int NW = sizeof(T) == 2 && DP <= 128 ? 8 : 4, THREADS = 32 * NW;

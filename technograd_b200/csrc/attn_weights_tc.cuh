@@ -1,4 +1,4 @@
-// attn_weights_tc.cuh -- the attention weight of many query rows on tcgen05 (16-bit caches).
+// attn_weights_tc.cuh -- the attention weight of many keys a CTA on tcgen05 (16-bit caches).
 //
 // S^T = K Q^T: 128 keys are the product's M, the query rows (up to 256) its N, so that a key's scores lie in
 // one TMEM lane and its weight is one thread's sum over columns, with nothing to exchange. Units, shares and
@@ -8,9 +8,11 @@
 //   4    MMA issue, into one of two TMEM score buffers
 //   5-8  fetching: the tile's keys through the page table into the operand layout (four stages), by TMA boxes
 //        where the pages suit them (k_tree_attn_tc), and at a unit's beginning its q
-// What bounds it: HBM up to about 128 rows (a tile's 32 KB take 1425 cycles of the measured rate, its exponentials
-// 8 cycles a row), then the exponentials. Measured: windows of 32 tokens (64 rows) over 16 sequences of up to 16001
-// positions 81 us, 4.1 TB/s (pages of 24; 78 us by boxes of 16 or 64). Every wait is bounded (tc.cuh).
+// What bounds it: HBM while the rows are few (a tile's 32 KB take 1425 cycles of the measured rate), then the sums, some 19
+// cycles a row and tile: 32 rows take as long as 1 (16 sequences of up to 16001 positions, us: 76 and 76; 64 rows 91, 120 rows 143, 256
+// rows 252). Measured: windows of 32 tokens (64 rows) over those 92 us, 3.6 TB/s, pages of 24 like pages of 64. The exponent is taken
+// from the difference (weight_of): s log2 e - lse log2 e, one product less, took 82 to 88 us here, but with scores of 3200 it is off by
+// 2e-4 of a weight. Every wait is bounded (tc.cuh).
 #pragma once
 
 #include "tree_attn_tc.cuh"

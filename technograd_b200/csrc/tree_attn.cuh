@@ -55,8 +55,8 @@ __device__ __forceinline__ float weight_of(float s, float scale, float lse) { re
 // wave take equal shares of all units' tiles, in order; the ring runs on across unit boundaries. A
 // unit that ends in its CTA's share is written out; of one that spans several, each CTA leaves
 // (O, mr, l), and k_attn_join adds them in CTA order: results do not depend on timing.
-// Measured: a decode wave of 256 sequences of up to 1280 positions (16 query heads over 8, 128 dimensions, bf16) 176 us
-// in a stream of calls, 5.6 TB/s.
+// Measured: a decode wave of 256 sequences of up to 1280 positions (16 query heads over 8, 128 dimensions, bf16) 183 us
+// in a stream of calls, 5.4 TB/s (167 in the first few hundred, before the card is at its power limit).
 template <class T> struct AttnScale; // SHIFT: exponent given to probabilities near 1
 template <> struct AttnScale<float> { static constexpr float SHIFT = 0, RAISE = 8; };
 template <> struct AttnScale<__nv_bfloat16> { static constexpr float SHIFT = 0, RAISE = 8; };
@@ -67,8 +67,8 @@ template <class T, int DP, int MT> struct AttnTile {
 	static constexpr int KW = sizeof(T) == 4 ? 8 : 16, NT = KW / 8, TK = 4 * KW, RT = 16 * MT;
 	static constexpr int P = DP * (int)sizeof(T), CH = P / 16;
 	static constexpr int STAGE = 2 * KW * P; // also 16 x DP floats, what the end of a unit needs
-	// 16 rows of 16-bit elements: three CTAs per SM with a stage ahead each, 167 us for a 256-sequence decode wave
-	// against 184 of two CTAs with two ahead; the others' registers allow two
+	// 16 rows of 16-bit elements: three CTAs per SM with a stage ahead each, 183 us for a 256-sequence decode wave
+	// against 195 of two CTAs with two ahead; the others' registers allow two
 	static constexpr int CTAS = DP == 256 ? 1 : MT == 1 && sizeof(T) == 2 ? 3 : 2;
 	static constexpr int NST = CTAS == 3 || DP == 256 || (DP == 128 && MT == 2 && sizeof(T) == 4) ? 2 : 3;
 	static constexpr int Q = 0, RING = RT * P, MASK = RING + 4 * NST * STAGE, ML = MASK + RT * 8, SCAN = ML + 4 * RT * 8;

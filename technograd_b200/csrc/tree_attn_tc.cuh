@@ -2,8 +2,8 @@
 // (drafted tokens x heads of a key head's group) and 16-bit caches.
 //
 // The 128 rows of a unit's tile (k_tree_attn's unit, shares and partial results, tree_attn.cuh) are the M of both
-// products, 128 keys a tile: S = Q K^T into one of two TMEM score buffers; P over S in V's type, the operand of
-// O += P V that comes from TMEM; O in TMEM. The two halves of a tile's keys have a reference, a sum and an O of
+// products, 128 keys a tile: S = Q K^T into one of two TMEM score buffers; P over S in V's type, a high and a low part
+// (split16), the operand of O += P V that comes from TMEM; O in TMEM. The two halves of a tile's keys have a reference, a sum and an O of
 // their own, so their softmax warps need nothing of each other before the unit's end. Warps:
 //   0-7   softmax, a query row per thread (TMEM lane = row), warps 4-7 for the tile's second 64 keys: the running
 //         reference mr, p = 2^(z - mr) to P; where a score exceeds mr by more than RAISE, O is rescaled in TMEM,
@@ -11,20 +11,21 @@
 //         joins and writes half of the row's dimensions.
 //   8-15  fetching, two warps each for K and V of even and of odd tiles, through the page table into the
 //         128-byte-swizzled operand layout (K rows = N, K-major; V rows = the product's k, so V is read MN-major).
-//         Pages of 8, 16, 32 or a multiple of 64 rows come by TMA, a box per page or 64 rows of one; any other
+//         Pages of 8, 16, 32 or a multiple of 64 rows come by TMA, a box per page or 64 rows of one (BOX); any other
 //         page size or stride, the drafted rows, and V's last tile (what is past its end must be zeros) by
-//         16-byte cp.async, about 1000 instructions a tile more: the server case below takes 198 us that way.
+//         16-byte cp.async, about 1000 instructions a tile more: the server case below takes 257 us that way.
 //         The copies themselves arrive on the stage's barrier when they have landed, so three stages are on
 //         their way at once; the issuing thread's proxy fence orders them before the product's reads. A
 //         tile's table entries are read before the tile ahead of it is fetched.
 //   16-18 issue of the MMAs, one thread each for S and the halves' P V, as soon as the operands are there: S of the
 //         next tiles overlaps the softmax of this one. (One thread for all was busy 3200 cycles a tile with its
 //         barriers, commits and issues, more than the tile's bytes take.)
-// What bounds it: with up to 128 rows the cache's bytes (a 64 KB tile pair takes 2850 cycles of the measured HBM
-// rate), then the chain of a tile (3060 to 3140 cycles). Of the 608 x 96 registers of the launch the fetching warps
+// What bounds it: the chain of a tile and the card's power. (A 64 KB tile pair takes 2850 cycles of the measured HBM rate;
+// with P in one part, whose outputs had 1.2 to 1.35 times the error, a tile took 3060 to 3140, and the two cases below 212
+// and 69 us: of the difference the second product is about 60%.) Of the 608 x 96 registers of the launch the fetching warps
 // give 32 each to the softmax warps, which hold 64 scores. Measured: 48 sequences of up to 6001 positions with 64
-// drafted tokens (16 query heads over 8, bf16) 187 us in short runs, up to 218 us in a long one, which draws 995 W
-// and runs at 1550 MHz; 131009 positions with 5 tokens of 8 heads per key head (f16) 67 to 70 us, 4.0 TB/s. Every wait
+// drafted tokens (16 query heads over 8, bf16) 213 us in short runs, 250 us in a long one, which draws 993 W
+// and runs at 1545 MHz; 131009 positions with 5 tokens of 8 heads per key head (f16) 84 us, 3.2 TB/s. Every wait
 // is bounded (tc.cuh): a timeout sets the status word and all roles leave.
 #pragma once
 
