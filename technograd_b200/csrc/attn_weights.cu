@@ -215,9 +215,8 @@ static int weights_run_tc(WeightArgs &p, int sms, int dev, cudaStream_t st, cons
 	if (rc) return rc;
 	const long long units = (long long)p.seqs * p.c.nkv, tiles = (p.c.max_len + W::TK - 1) / W::TK + 1;
 	if (units > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences", who, p.seqs);
-	// a unit's start is worth about 4 tiles (32-token windows, us at 2, 4, 6, 8 and 12: 16 sequences of up to 16001 positions 128,
-	// 90.7, 90.8, 93, 97; 16 of up to 6001 60, 49, 50, 54, 56; 32 of up to 1280 37.6, 34, 35.5, 38, 39; 8 of up to 1280 20, 20.5, 21,
-	// 21.2, 23)
+	// a unit's start is worth about 4 tiles (32-token windows, us at 2, 4, 6 and 8: 16 sequences of up to 16001 positions 131, 91, 89,
+	// 91; 16 of up to 6001 61, 48, 50, 52; 32 of up to 1280 37.6, 34, 35.6, 37.6; 8 of up to 1280 21, 20, 20.7, 21)
 	p.row_tiles = 1, p.whole = 0, p.least = 1, p.begin = 4, p.split = nullptr;
 	const long long shares = (units * (tiles + p.begin) + p.begin) / (1 + p.begin);
 	CUtensorMap map = {};
@@ -229,10 +228,10 @@ static int weights_run_tc(WeightArgs &p, int sms, int dev, cudaStream_t st, cons
 
 // Of up to TW_ROWS query rows per key head, 16-bit caches take attn_weights_tc.cuh where a CTA has more than so many of its tiles,
 // whatever the rows: below, latency decides, and this file's kernel has more CTAs and warps. Measured, us, tiles of 128 keys
-// against this file's (8 key heads, bf16, 2 / 32 / 64 / 120 rows), at 128 dimensions 17.2, 17.5, 23.3, 35.6 and 17.1, 19.1, 23.6, 33.0 at
-// 10 tiles a CTA; 22.4, 23.0, 31.4, 49.9 and 25.2, 28.8, 35.5, 49.9 at 16; 28.3, 29.3, 38.7, 58.1 and 31.9, 37.5, 48.1, 68.3 at 28;
-// 82.7, 69.5, 88.8, 142 and 104, 119, 148, 212 at 110. At 64 dimensions 27.3, 27.4, 37.5, 58.1 and 25.2, 29.4, 35.5, 49.6 at 28; 35.5,
-// 35.5, 47.9, 76.2 and 37.6, 43.7, 54, 74.5 at 42; 63.1, 64, 88.8, 142 and 88.5, 100, 120, 159 at 110.
+// against this file's (8 key heads, bf16, 2 / 32 / 64 / 256 rows), at 128 dimensions 17.9, 18.5, 23.3, 59 and 17, 19.1, 23.7, 68 at
+// 10 tiles a CTA; 21.4, 21.9, 29.3, 81 and 25.2, 29.4, 35.4, 114 at 16; 27.2, 27.2, 36.1, 103 and 32.3, 37.5, 48.5, 161 at 29;
+// 69, 70, 92, 271 and 106, 121, 150, 538 at 110. At 64 dimensions 20.8, 21, 27.2, 71 and 20.5, 23.1, 27.8, 58 at 16; 25.1, 25.2, 33.5, 92
+// and 25.2, 29.3, 35.6, 76 at 29; 33.4, 33.5, 43.7, 124 and 37.6, 45.7, 55.5, 118 at 42; 62, 63, 85, 231 and 90, 102, 121, 246 at 110.
 constexpr int WEIGHTS_TC_TILES_128 = 14, WEIGHTS_TC_TILES_64 = 40;
 
 template <class T>

@@ -5,14 +5,15 @@
 // tiles as in tree_attn.cuh. Warps:
 //   0-3  a key per thread: sum over the rows' columns of exp(scale s - lse); what the key had, and the result,
 //        are one coalesced access each
-//   4    MMA issue, into one of two TMEM score buffers
+//   4    MMA issue, into one of two TMEM score buffers (one for more than 128 rows of 128 dimensions)
 //   5-8  fetching: the tile's keys through the page table into the operand layout (four stages), by TMA boxes
 //        where the pages suit them (k_tree_attn_tc), and at a unit's beginning its q
-// What bounds it: HBM while the rows are few (a tile's 32 KB take 1425 cycles of the measured rate), then the sums, some 19
-// cycles a row and tile: 32 rows take as long as 1 (16 sequences of up to 16001 positions, us: 76 and 76; 64 rows 91, 120 rows 143, 256
-// rows 252). Measured: windows of 32 tokens (64 rows) over those 92 us, 3.6 TB/s, pages of 24 like pages of 64. The exponent is taken
-// from the difference (weight_of): s log2 e - lse log2 e, one product less, took 82 to 88 us here, but with scores of 3200 it is off by
-// 2e-4 of a weight. Every wait is bounded (tc.cuh).
+// What bounds it: HBM while the rows are few (a tile's 32 KB take 1425 cycles of the measured rate), then the sums, some 20
+// cycles a row and tile: 32 rows take as long as 1 (16 sequences of up to 16001 positions, us: 70 and 69; 64 rows 92, 120 rows 144, 256
+// rows 271). Measured: windows of 32 tokens (64 rows) over those 93 us, 3.6 TB/s, pages of 24 like pages of 64. The exponent is taken
+// from the difference (weight_of): s log2 e - lse log2 e, one product less, is off by 2e-4 of a weight with scores of 3200. Scores of
+// 128 dimensions in one sum, whose last bits the tensor core drops, had 1.6 times the error of the form here; they took as
+// long up to 128 rows and 252 us for 256. Every wait is bounded (tc.cuh).
 #pragma once
 
 #include "tree_attn_tc.cuh"
@@ -24,7 +25,7 @@ struct TwBars {
 	uint32_t tmem;
 	int abort;
 	long long scan[16];
-	float lse[2][256];              // by the unit's parity
+	float less[2][256];              // -lse, by the unit's parity
 	unsigned long long mask[2][256]; // the drafted tokens a row counts for
 };
 
@@ -57,6 +58,9 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p, 
 		fence_barrier_init();
 	}
 	const int rows = p.d.tokens * p.d.group, cols = (rows + 31) & ~31, chunks = p.c.dim / 8;
+	// a score of 128 dimensions is two sums of 64, `high` columns apart, added in f32 (see add4: a weight is an f32 output); where
+	// they fill TMEM there is one buffer
+	const int high = cols <= TW_ROWS / 2 ? TW_ROWS / 2 : TW_ROWS, bufs = DP > 64 && high == TW_ROWS ? 1 : 2;
 	AttnCursor c;
 	long long left_, pos, share;
 	if (!attn_share<TK, W::NW>(p, B->scan, 1, c, left_, pos, share)) return; // the whole CTA
@@ -143,15 +147,15 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p, 
 			const uint32_t id = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(128 >> 4) << 24) | ((uint32_t)(cols >> 3) << 17);
 			const uint32_t base = smem_u32(sm);
 			for (int j = 0; j < left; j++) {
-				if (j >= 2 && !ta_poll(B, &B->s_free[j & 1], ((j >> 1) - 1) & 1, p.c)) break;
+				if (j >= bufs && !ta_poll(B, &B->s_free[(j - bufs) & 1], ((j - bufs) >> 1) & 1, p.c)) break;
 				if (!ta_poll(B, &B->kfull[j % NST], j / NST & 1, p.c)) break;
 				fence_async_smem();
 				tc_fence_after();
 				const uint32_t k = base + W::K + j % NST * W::KB;
 #pragma unroll
 				for (int kk = 0; kk < DP / 16; kk++)
-					tc_mma_f16(tmem + (j & 1) * TW_ROWS, sw128_kmajor_desc(k + (kk >> 2) * 16384 + (kk & 3) * 32),
-						   sw128_kmajor_desc(base + (kk >> 2) * (TW_ROWS * 128) + (kk & 3) * 32), id, kk > 0);
+					tc_mma_f16(tmem + j % bufs * TW_ROWS + (kk >> 2) * high, sw128_kmajor_desc(k + (kk >> 2) * 16384 + (kk & 3) * 32),
+						   sw128_kmajor_desc(base + (kk >> 2) * (TW_ROWS * 128) + (kk & 3) * 32), id, (kk & 3) > 0);
 				tc_commit(&B->s_full[j & 1]);
 				tc_commit(&B->kfree[j % NST]);
 			}
@@ -173,7 +177,7 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p, 
 					const int t = r / p.d.group;
 					const bool on = r < rows && t < cnt && (sel >> t & 1);
 					const float lse = on ? p.lse[((long long)c.b * p.d.tokens + t) * p.d.nq + c.h * p.d.group + r - t * p.d.group] : -INFINITY;
-					B->lse[unit & 1][r] = lse;
+					B->less[unit & 1][r] = -lse;
 					B->mask[unit & 1][r] = lse == -INFINITY ? 0 : p.d.sees(c.b, t, cnt);
 				}
 				mbar_arrive_warp(&B->rows_full);
@@ -188,15 +192,28 @@ __global__ void __launch_bounds__(288, 1) k_attn_weights_tc(const WeightArgs p, 
 			float w[4] = {0, 0, 0, 0};
 			for (int x = 0; x < cols; x += 32) {
 				float v[32];
-				tmem_ld32(lanes + (j & 1) * TW_ROWS + x, v);
-				const float *lse = &B->lse[unit & 1][x];
+				tmem_ld32(lanes + j % bufs * TW_ROWS + x, v);
+				if constexpr (DP > 64) {
+					float u[32];
+					tmem_ld32(lanes + j % bufs * TW_ROWS + high + x, u);
+#pragma unroll
+					for (int e = 0; e < 32; e += 2) {
+						const float2 y = add2(make_float2(v[e], v[e + 1]), make_float2(u[e], u[e + 1]));
+						v[e] = y.x, v[e + 1] = y.y;
+					}
+				}
+				const float *less = &B->less[unit & 1][x];
 				if (drafted) {
 					const unsigned long long *mask = &B->mask[unit & 1][x];
 #pragma unroll
-					for (int e = 0; e < 32; e++) w[e & 3] += tid < 64 && mask[e] >> (tid & 63) & 1 ? weight_of(v[e], p.d.scale, lse[e]) : 0;
+					for (int e = 0; e < 32; e++) w[e & 3] += tid < 64 && mask[e] >> (tid & 63) & 1 ? weight_of(v[e], p.d.scale, -less[e]) : 0;
 				} else {
 #pragma unroll
-					for (int e = 0; e < 32; e++) w[e & 3] += lse[e] != -INFINITY ? weight_of(v[e], p.d.scale, lse[e]) : 0;
+					for (int e = 0; e < 32; e += 2) { // weight_of, two at a time
+						const float2 l = *(const float2 *)(less + e), d = fma2(make_float2(v[e], v[e + 1]), make_float2(p.d.scale, p.d.scale), l);
+						const float2 y = mul2(d, make_float2(1.4426950408889634f, 1.4426950408889634f));
+						w[e & 3] += l.x != INFINITY ? ex2(y.x) : 0, w[e + 1 & 3] += l.y != INFINITY ? ex2(y.y) : 0;
+					}
 				}
 			}
 			tc_fence_before();

@@ -276,3 +276,31 @@ def test_weights_cut_for_long_sequences(cuda, dtype, dim, tokens, group, positio
     """... and the weights', with what was there before and zeros past each sequence's end."""
     c = with_room(Case([500, 0, 129, 1, 128, 700, 64], 2, group, dim, 16, "head", dtype, tokens), positions)
     check_weights(c, random_mask(7, tokens, 3), acc=torch.rand(7, 2, positions, generator=torch.Generator().manual_seed(1)))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens,group", [(1, 2), (16, 2), (32, 4), (64, 4), (64, 5)])
+@pytest.mark.parametrize("positions", [300, 200000])
+def test_weights_of_long_score_sums(cuda, dtype, tokens, group, positions):
+    """A score of 128 dimensions is two sums of 64, added and rounded once. Here the first is 4096 and the second 1.75 units of its
+    last place, in four steps of 0.44: the score is off by half a unit (2^-12) at most, where one sum that loses each step would be
+    by 1.75. The rest of the tolerance as in test_weights_of_large_scores."""
+    c = Case([150, 3], 1, group, 128, 16, "head", dtype, tokens)
+    c.q[:] = 1
+    key = torch.zeros(128)
+    key[:64] = 64
+    key[64::16] = 0.4375 * 2.0 ** -11
+    for b, n in enumerate(c.lens):
+        for p in range(n):
+            c.pk[int(c.table[b, p // 16]), :, p % 16] = key.to(dtype).cuda()
+    c.kn[:] = key.to(dtype)
+    c = with_room(c, positions)
+    lse = 512 + 2 * torch.rand(2, tokens, group, generator=torch.Generator().manual_seed(2))
+    acc, fresh = (x.cpu().double() for x in kvcache.attention_weights(c.cache, c.q.cuda(), c.kn.cuda(), lse.cuda(), scale=0.125))
+    d = 0.125 * (4096 + 1.75 * 2.0 ** -11) - lse.double()
+    w = torch.exp(d)
+    tol = w * (0.125 * 2.0 ** -12 + 3 * 2.0 ** -24 * d.abs() + 2.0 ** -22 + 2.0 ** -24 * tokens * group)
+    for b, n in enumerate(c.lens):
+        near(acc[b, 0, :n], w[b].sum().expand(n), tol[b].sum().expand(n), "acc")
+        for u in range(tokens):
+            near(fresh[b, 0, u:u + 1], w[b, u:].sum()[None], tol[b, u:].sum()[None], "fresh")
