@@ -393,9 +393,17 @@ def ref_qwen3_line(P, per_seq_tokens: int, what: str) -> dict:
             "forward_s_per_core": fwd}
 
 
+def ref_vm_built() -> bool:
+    """Whether the reference's VM is there: oracle/_ref is built only where the reference's sources are."""
+    from oracle import refvm
+    return refvm.lib() is not None
+
+
 def cpu_baseline_decode():
     """One pass over the pieces of a 1024-token forward (config 5: int4 GPTQ): the reference
-    has no KV cache, so every generated token costs a forward of its whole prefix."""
+    has no KV cache, so every generated token costs a forward of its whole prefix. None without the reference."""
+    if not ref_vm_built():
+        return None
     P = ref_qwen3(PROMPT, 4, True, 5)
     try:
         for piece in ("attn", "gate", "down", "head"):
@@ -483,7 +491,9 @@ def bench_prefill(args, world, rank, local):
 
 def cpu_baseline_prefill():
     """One pass over the pieces of a 512-token forward (config 4: int8 RTN), the prefill of
-    one sequence per core."""
+    one sequence per core. None without the reference."""
+    if not ref_vm_built():
+        return None
     P = ref_qwen3(PF_T, 8, False, 4)
     try:
         for piece in ("attn", "gate", "down", "head"):
@@ -602,9 +612,11 @@ SSM_REF_T = 256
 
 def cpu_baseline_ssm(S=None, runs: int = 1):
     """The config-3 program on the reference's own VM (oracle/refvm.py SsmSample): one
-    sequence of SSM_REF_T steps per host core, all at once."""
+    sequence of SSM_REF_T steps per host core, all at once. None without the reference."""
     from oracle import refvm
     own = S is None
+    if own and not ref_vm_built():
+        return None
     S = S or refvm.SsmSample(SSM_REF_T)
     try:
         t = statistics.median([S.run() for _ in range(runs)])
@@ -920,6 +932,8 @@ def reference_arm(args) -> list:
                     "data": "synthetic", "config": cfg, "cpu_baseline": base,
                     "e2e": {"value": v, "unit": unit, "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0}})
 
+    if wl not in ("lr", "gemm") and not ref_vm_built():
+        return [{"impl": "reference", "unavailable": "oracle/_ref/libtgref.so was not built (needs the reference sources)"}]
     if wl == "lr":
         rows = lr_inputs(LR_ROWS)
         if cpu_baseline_lr(rows) is None:
