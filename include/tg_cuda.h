@@ -399,12 +399,13 @@ typedef struct {
  * the sum of exp(scale q.k). A token that sees nothing, or only scores of -infinity, has
  * out 0 and lse -infinity, and so have tokens past count. What a masked row holds
  * (infinities and NaN too) does not matter, and a drafted row that a token sees with a
- * probability of 0 in f32 adds nothing to it, whatever its v. An infinity or NaN in the v of
- * a cached row makes that element of the outputs that see it an infinity or NaN (where the
- * row's probability is 0, possibly). Scores, softmax and sums are f32, and with 16-bit
- * caches each probability's product with v keeps 2^-15 of it or better: an output's error is
- * that of an f32 softmax rounded once. work: scratch of at least tg_cuda_tree_attn_workspace bytes, 16-byte aligned, not shared with a call
- * that may run at the same time (NULL where that is 0). */
+ * probability of 0 in f32 adds nothing to it, whatever its v. An infinity or NaN in the v
+ * of a cached row makes that element of the outputs that see it an infinity or NaN (where
+ * the row's probability is 0, possibly). Scores, softmax and sums are f32, and with 16-bit
+ * caches each probability's product with v keeps 2^-15 of it or better: an output's error
+ * is that of an f32 softmax rounded once. work: scratch of at least
+ * tg_cuda_tree_attn_workspace bytes, 16-byte aligned, not shared with a call that may run
+ * at the same time (NULL where that is 0), and not given back before the call returns. */
 long long tg_cuda_tree_attn_workspace(const tg_cuda_kv *c, const tg_cuda_drafts *d);
 int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, void *out, long long out_seq, long long out_tok,
 		      long long out_head, float *lse, void *work, long long work_bytes, void *stream);
