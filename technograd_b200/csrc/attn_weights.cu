@@ -261,6 +261,7 @@ extern "C" int tg_cuda_attn_weights(const tg_cuda_kv *c, const tg_cuda_drafts *d
 	if (c->seqs && (!lse || !fresh || (!acc_out && c->max_len))) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);
 	if (((uintptr_t)select & 7) || (((uintptr_t)lse | (uintptr_t)acc | (uintptr_t)acc_out | (uintptr_t)fresh) & 3))
 		return set_err(TG_CUDA_EINVAL, "%s: a pointer is not on a boundary of its type", who);
+	if (acc && ((acc_seq < 0 && c->seqs > 1) || (acc_head < 0 && c->nkv > 1))) return set_err(TG_CUDA_EINVAL, "%s: negative strides", who);
 	if (acc && acc == acc_out && (acc_head != c->max_len || acc_seq != (long long)c->nkv * c->max_len))
 		return set_err(TG_CUDA_EINVAL, "%s: acc may be acc_out with acc_out's own strides only", who);
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0 || (rc = pg_sms(who, &dev, &sms))) return rc;

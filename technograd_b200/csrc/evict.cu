@@ -302,6 +302,7 @@ extern "C" int tg_cuda_kv_evict(const tg_cuda_kv *src, const tg_cuda_kv *dst, co
 		return set_err(TG_CUDA_EINVAL, "%s: budget %d, recent %d, sink %d", who, budget, recent, sink);
 	if (src->seqs && (!keep || !acc_out || !len_out || (!acc && src->max_len))) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);
 	if (((uintptr_t)acc | (uintptr_t)keep | (uintptr_t)acc_out | (uintptr_t)len_out) & 3) return set_err(TG_CUDA_EINVAL, "%s: a pointer is not on a 4-byte boundary", who);
+	if ((acc_seq < 0 && src->seqs > 1) || (acc_head < 0 && src->nkv > 1)) return set_err(TG_CUDA_EINVAL, "%s: negative strides", who);
 	if (len_out == src->len && src->seqs) return set_err(TG_CUDA_EINVAL, "%s: len_out may not be the cache's len", who);
 	if ((rc = pg_device(who, &sms, &p.src.status)) || src->seqs == 0) return rc;
 	p.dst.status = p.src.status;

@@ -160,3 +160,10 @@ def test_pointers_off_their_type_are_refused():
         w[at] += 1
         assert L.tg_cuda_kv_commit(p(c), p(d), w[0], w[1], w[2], w[3], 200, 100, 100, None) == E
         assert L.tg_cuda_kv_evict(p(kv()), p(c), w[0], 120, 60, 32, 4, 1, w[1], w[2], w[3], None) == E
+
+
+@pytest.mark.parametrize("seq,head", [(-120, 60), (120, -60)])
+def test_negative_strides_of_weights_are_refused(seq, head):
+    L, p, E = kvcache._lib.lib(), C.byref, kvcache._lib.EINVAL
+    assert L.tg_cuda_attn_weights(p(kv()), p(drafts()), 0x70000, None, 0xB0000, seq, head, 0x80000, 0x90000, None) == E
+    assert L.tg_cuda_kv_evict(p(kv()), p(kv()), 0xB0000, seq, head, 32, 4, 1, 0x80000, 0x90000, 0xA0000, None) == E
