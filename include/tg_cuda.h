@@ -431,6 +431,37 @@ int tg_cuda_attn_weights(const tg_cuda_kv *c, const tg_cuda_drafts *d, const flo
 int tg_cuda_kv_commit(const tg_cuda_kv *c, const tg_cuda_drafts *d, const int *path, int *len_out, const float *fresh,
 		      float *acc, long long acc_seq, long long acc_head, int acc_cols, void *stream);
 
+/* Rotary positions: of a head's first `dim` elements, element a and its partner b become
+ *   gain (x_a cos f - x_b sin f) and gain (x_a sin f + x_b cos f),  f = pos freq[i],
+ * (a, b) = (i, i + dim / 2) or, interleaved, (2 i, 2 i + 1), for i < dim / 2; the others pass. The angle
+ * is exact to 2^-53 of itself however far the position, and a result is rounded once. */
+typedef struct {
+	int dim;                 /* elements that turn: even, 0 to head_dim */
+	int interleaved;         /* 0 or 1: which elements are partners */
+	int inverse;             /* 1: by -f, which is the gradient of the rotation by f */
+	float gain;              /* 1; some extensions of the context have another */
+	const double *freq;      /* [dim / 2] radians per position, device memory */
+	const int *pos;          /* [seqs][tokens] positions, rows pos_seq apart (0: one row for all); NULL: see the calls */
+	long long pos_seq;
+} tg_cuda_rotary;
+
+/* out = x rotated; x and out [seqs][tokens][heads][head_dim] in elements of `type` with strides in elements, rows
+ * as in a cache (16-byte boundaries, at most 256 elements). out may be x with the same strides. pos NULL: token t is at
+ * position t. */
+int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tokens, int heads, int head_dim, const void *x, long long x_seq,
+		 long long x_tok, long long x_head, void *out, long long out_seq, long long out_tok, long long out_head, void *stream);
+
+/* New tokens into the cache, rotated on the way: for i < count[b], cache row len[b] + i receives d->k's row i, rotated (r NULL:
+ * as it is), and d->v's as it is; len_out[b] = len[b] + count[b] (len_out may not be len). d->q, where not NULL, goes to q_out,
+ * rotated; k_out, where not NULL, receives the rotated keys too (drafted rows for tg_cuda_tree_attn): rows of q_out and
+ * k_out past count are 0, and they may be d->q and d->k with the same strides. q_norm, k_norm (f32 [head_dim], NULL: none): before the
+ * rotation a row x becomes x / sqrt(mean(x^2) + eps) * norm. pos NULL: token i is at position len + i. tokens may be any
+ * number, d->mask and d->scale are not read, and max_len bounds len before the call. A row past the table is not written and is
+ * reported like a bad page. No two rows written may share a page row. */
+int tg_cuda_kv_append(const tg_cuda_kv *c, const tg_cuda_drafts *d, const tg_cuda_rotary *r, const float *q_norm, const float *k_norm,
+		      float eps, void *q_out, long long q_out_seq, long long q_out_tok, long long q_out_head, void *k_out,
+		      long long k_out_seq, long long k_out_tok, long long k_out_head, int *len_out, void *stream);
+
 /* Eviction: for every sequence and kv head, at most `budget` positions of src go to dst in
  * ascending order. A sequence of at most budget positions keeps all; a longer one keeps its
  * first `sink` and last `recent` and, of those between, the budget - sink - recent with the

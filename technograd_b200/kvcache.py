@@ -24,6 +24,9 @@ from . import _lib
 _pack_drafts = struct.Struct("@2if4xP3q2P3q2P").pack
 assert struct.calcsize("@2if4xP3q2P3q2P") == C.sizeof(_lib.Drafts)
 
+_pack_rotary = struct.Struct("@3if2Pq").pack
+assert struct.calcsize("@3if2Pq") == C.sizeof(_lib.Rotary)
+
 _TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
@@ -67,6 +70,13 @@ def _stream(cache: "PagedKV") -> int:
     return torch._C._cuda_getCurrentRawStream(cache.index)  # torch.cuda.current_stream's handle without its object
 
 
+def _stream_of(index: int) -> int:
+    """The same for tensors of a call that has no cache."""
+    if index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on cuda:{index}, which is not the current device")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 class _ForwardOnly(torch.autograd.Function):
     """out and lse as results of inputs that want a gradient: there is none, and asking for it is an error."""
 
@@ -77,6 +87,19 @@ class _ForwardOnly(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         raise RuntimeError("kvcache.tree_attention has no backward pass")
+
+
+class _NoGradient(torch.autograd.Function):
+    """The first n of the tensors as results of the others, as above, for the call of this name."""
+
+    @staticmethod
+    def forward(ctx, name, n, *tensors):
+        ctx.name = name
+        return tuple(x.detach() for x in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"kvcache.{ctx.name} has no backward pass")
 
 
 class PagedKV:
@@ -207,6 +230,136 @@ def commit(cache: PagedKV, k, v, count, path=None, new=None, acc=None):
                                             None if acc is None else new.data_ptr(), None if acc is None else acc.data_ptr(), sa[0], sa[1],
                                             0 if acc is None else acc.shape[2], _stream(cache)))
     return lens
+
+
+def rotary_frequencies(part: int, theta: float = 1e4, factor: float = 1.0, original: int | None = None, fast: float = 32.0,
+                       slow: float = 1.0) -> torch.Tensor:
+    """Radians per position of each pair of a rotation of `part` elements, f64 on the CPU: theta^(-2 i / part).
+
+    factor: how much longer the context is than the one a model was trained on. Without `original` every frequency is
+    divided by it. With `original`, that context's length, pairs that turn `fast` times or more in it keep theirs, pairs that turn
+    `slow` times or less are divided, and in between the two are mixed in proportion to the logarithm of the turns."""
+    _need(part >= 0 and part % 2 == 0, f"part: expected an even number of elements, got {part}")
+    _need(theta > 0 and factor > 0, "theta and factor: expected positive numbers")
+    f = float(theta) ** (-2 * torch.arange(part // 2, dtype=torch.float64) / max(part, 1))
+    if original is None or factor == 1:
+        return f / factor
+    _need(original > 0 and fast > slow > 0, "original, fast, slow: expected positive numbers, fast above slow")
+    keep = (torch.log(original * f / (2 * math.pi * slow)) / math.log(fast / slow)).clamp(0, 1)
+    return f * (keep + (1 - keep) / factor)
+
+
+class Rotary:
+    """A rotation of heads of head_dim elements by position (tg_cuda_rotary): its frequencies, on the device, and its form.
+
+    freq: f64 [part / 2] radians per position, a CUDA tensor; None: rotary_frequencies(part, theta) on the current device. part: leading
+    elements of a head that turn (default: two for each frequency, or the whole head). interleaved: neighbours 2 i and
+    2 i + 1 are partners, else i and i + part / 2. gain: a factor of the turned elements."""
+
+    def __init__(self, head_dim: int, freq: torch.Tensor | None = None, theta: float = 1e4, part: int | None = None, gain: float = 1.0,
+                 interleaved: bool = False):
+        if freq is None:
+            freq = rotary_frequencies(head_dim if part is None else part, theta).cuda()
+        _need(freq.dim() == 1 and freq.dtype is torch.float64 and freq.is_cuda and freq.is_contiguous(), "freq: expected a contiguous float64 CUDA tensor [part / 2]")
+        self.part = 2 * freq.shape[0]
+        _need(part is None or part == self.part, f"part: {part} elements, but {freq.shape[0]} frequencies")
+        _need(0 < head_dim <= 256 and self.part <= head_dim, f"{self.part} elements of a head of {head_dim} turn")
+        self.freq, self.head_dim, self.gain, self.interleaved, self.index = freq, head_dim, float(gain), bool(interleaved), freq.get_device()
+        self._at = freq.data_ptr()
+
+    def _pack(self, pos, seqs: int, tokens: int, index: int, dim: int, inverse: bool = False) -> bytes:
+        """The C description for these positions, int32 [seqs, tokens] or [tokens] (None: the call's own), checked."""
+        if index != self.index or dim != self.head_dim:
+            raise ValueError(f"rotary: made for heads of {self.head_dim} on cuda:{self.index}, not of {dim} on cuda:{index}")
+        at, row = 0, 0
+        if pos is not None:
+            n = pos.shape
+            if pos.dtype is not torch.int32 or pos.get_device() != index or n not in ((seqs, tokens), (tokens,)) or (tokens > 1 and pos.stride(-1) != 1):
+                raise ValueError(f"pos: expected an int32 tensor [{seqs}, {tokens}] or [{tokens}] on cuda:{index} with contiguous rows, got {pos.dtype} "
+                                 f"{tuple(n)} strides {pos.stride()} on {pos.device}")
+            at, row = pos.data_ptr(), pos.stride(0) if len(n) == 2 else 0
+        return _pack_rotary(self.part, self.interleaved, inverse, self.gain, self._at, at, row)
+
+
+def _turn(x, rotary, pos, inverse, out):
+    n, s, index = x.shape, x.stride(), x.get_device()
+    if x.dtype not in _TYPES or len(n) != 4 or (n[3] > 1 and s[3] != 1) or index < 0:
+        raise ValueError(f"x: expected an f32, f16 or bf16 CUDA tensor [seqs, tokens, heads, head_dim] with contiguous rows, got {x.dtype} {tuple(n)} "
+                         f"strides {s} on {x.device}")
+    r = rotary._pack(pos, n[0], n[1], index, n[3], inverse)
+    if out is None:
+        out = torch.empty_like(x)
+    elif out.dtype is not x.dtype or out.get_device() != index or out.shape != n or (n[3] > 1 and out.stride(3) != 1):
+        raise ValueError(f"out: expected x's type, shape and device and contiguous rows, got {out.dtype} {tuple(out.shape)} strides {out.stride()} on {out.device}")
+    elif out.data_ptr() == x.data_ptr() and not _alike(out, x):
+        raise ValueError("out: x's memory with other strides")
+    o = out.stride()
+    _lib.check(_lib.lib().tg_cuda_rope(r, _TYPES[x.dtype], n[0], n[1], n[2], n[3], x.data_ptr(), s[0], s[1], s[2], out.data_ptr(), o[0], o[1], o[2],
+                                       _stream_of(index)))
+    return out
+
+
+class _Rope(torch.autograd.Function):
+    """A rotation's gradient is the rotation by the negative angle, with the same gain."""
+
+    @staticmethod
+    def forward(ctx, x, rotary, pos, inverse):
+        ctx.rotary, ctx.inverse = rotary, inverse
+        ctx.save_for_backward(*(() if pos is None else (pos,)))
+        return _turn(x, rotary, pos, inverse, None)
+
+    @staticmethod
+    def backward(ctx, grad):
+        pos = ctx.saved_tensors[0] if ctx.saved_tensors else None
+        if grad.shape[3] > 1 and grad.stride(3) != 1 or grad.data_ptr() % 16 or any(s * grad.element_size() % 16 for s in grad.stride()[:3]):
+            grad = grad.contiguous()  # (an expanded or transposed gradient)
+        return rope(grad, ctx.rotary, pos, not ctx.inverse), None, None, None
+
+
+def rope(x, rotary: Rotary, pos=None, inverse: bool = False, out=None):
+    """x [seqs, tokens, heads, head_dim] rotated to its tokens' positions (tg_cuda_rope); pos int32 [seqs, tokens] or [tokens] (None: 0, 1, ...).
+
+    inverse: by the negative angle. out: where to (x itself: in place). Differentiable with respect to x, without out."""
+    if torch.is_grad_enabled() and x.requires_grad:
+        _need(out is None, "out: not with a gradient")
+        return _Rope.apply(x, rotary, pos, inverse)
+    return _turn(x, rotary, pos, inverse, out)
+
+
+def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None, count=None, q_norm=None, k_norm=None, eps: float = 1e-6,
+           keys: bool = False):
+    """New tokens into the cache's pages, normed and rotated on the way (tg_cuda_kv_append).
+
+    k, v [seqs, tokens, nkv, head_dim] and q [seqs, tokens, nq, head_dim]: a projection's output, any number of tokens; count int32
+    [seqs]: tokens there are (None: all). Cache row lens + i receives token i's k, rotated to its position (pos, None: lens + i), and v. q_norm, k_norm
+    f32 [head_dim]: weights of an RMS norm of each head before the rotation. keys: return the rotated keys too, which tree_attention and
+    shared_attention take as the tokens' own with the lengths from before. Returns (the new lengths, q rotated or
+    None, k rotated or None), rows past count 0; the pages are written in place. Forward only, like tree_attention."""
+    d = _drafts(cache, q, k, v, None, count, 1.0)
+    n, dim, index = k.shape, cache.head_dim, cache.index
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None:
+            _check(name, w, torch.float32, (dim,), index)
+    _need(q is not None or q_norm is None, "q_norm: without q")
+    _need(rotary is not None or pos is None, "pos: without a rotation")
+    r = None if rotary is None else rotary._pack(pos, n[0], n[1], index, dim)
+    lens = torch.empty_like(cache.lens)
+    qo, sq, ko, sk = None, (0, 0, 0), None, (0, 0, 0)
+    if q is not None:
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        sq = qo.stride()
+    if keys:
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        sk = ko.stride()
+    _lib.check(_lib.lib().tg_cuda_kv_append(cache._at, d, r, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+                                            None if qo is None else qo.data_ptr(), sq[0], sq[1], sq[2], None if ko is None else ko.data_ptr(), sk[0], sk[1], sk[2],
+                                            lens.data_ptr(), _stream(cache)))
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
+        made = [x for x in (qo, ko) if x is not None]
+        if made:
+            made = list(_NoGradient.apply("append", len(made), *made, *(x for x in (q, k, v) if x is not None)))
+            qo, ko = made.pop(0) if qo is not None else None, made.pop(0) if ko is not None else None
+    return lens, qo, ko
 
 
 def evict(cache: PagedKV, dst: PagedKV, acc, budget: int, recent: int = 0, sink: int = 0):
