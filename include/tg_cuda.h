@@ -410,6 +410,26 @@ long long tg_cuda_tree_attn_workspace(const tg_cuda_kv *c, const tg_cuda_drafts 
 int tg_cuda_tree_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, void *out, long long out_seq, long long out_tok,
 		      long long out_head, float *lse, void *work, long long work_bytes, void *stream);
 
+/* Groups of sequences whose caches begin with the same rows of the pools (a system prompt, a document, samples of one
+ * prompt): the first shared[g] positions of the members[g] sequences from first[g] on lie in the same rows, which
+ * their tables all name. Groups do not overlap and stand in ascending order; group[b] is sequence b's, -1 for none. All
+ * four are read by the kernels: what does not fit together (a sequence shorter than its group's prefix, one outside its group) is
+ * reported like a bad page. max_own, a bound of the positions a sequence has behind what it shares, only sizes the launches. */
+typedef struct {
+	int groups;              /* at most seqs */
+	int max_shared;          /* upper bound of shared, at most max_len */
+	int max_own;
+	const int *first, *members, *shared; /* [groups] */
+	const int *group;        /* [seqs] */
+} tg_cuda_prefix;
+
+/* The results of tg_cuda_tree_attn, for all that its description says, with the prefixes' rows read once for the rows of a whole
+ * group instead of once for each sequence. (What does not share goes its usual way; with groups 0 the call is
+ * tg_cuda_tree_attn.) work: as there, tg_cuda_shared_attn_workspace bytes. */
+long long tg_cuda_shared_attn_workspace(const tg_cuda_kv *c, const tg_cuda_drafts *d, const tg_cuda_prefix *x);
+int tg_cuda_shared_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, const tg_cuda_prefix *x, void *out, long long out_seq,
+			long long out_tok, long long out_head, float *lse, void *work, long long work_bytes, void *stream);
+
 /* The attention weight that positions receive: for cached position x,
  *   acc_out[b][h][x] = acc[b][h][x] + sum of exp(scale q.k_x - lse) over the tokens t < count
  *   whose bit in select[b] is set and the query heads of h,

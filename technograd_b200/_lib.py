@@ -32,7 +32,7 @@ SYMBOLS = ["tg_cuda_error", "tg_cuda_init", "tg_cuda_ngpus", "tg_cuda_selftest_w
            "tg_cuda_lm_get_stats", "tg_cuda_ssm_load", "tg_cuda_ssm_forward", "tg_cuda_ssm_forward_device",
            "tg_cuda_ssm_free", "tg_cuda_ssm_profile", "tg_cuda_ssm_get_stats",
            "tg_cuda_tree_attn_workspace", "tg_cuda_tree_attn", "tg_cuda_attn_weights", "tg_cuda_kv_commit",
-           "tg_cuda_kv_evict", "tg_cuda_rope", "tg_cuda_kv_append"]
+           "tg_cuda_kv_evict", "tg_cuda_rope", "tg_cuda_kv_append", "tg_cuda_shared_attn_workspace", "tg_cuda_shared_attn"]
 
 
 class TgCudaError(RuntimeError):
@@ -122,6 +122,11 @@ class Drafts(C.Structure):
                 ("mask", C.c_void_p), ("count", C.c_void_p)]
 
 
+class Prefix(C.Structure):
+    _fields_ = [("groups", C.c_int), ("max_shared", C.c_int), ("max_own", C.c_int), ("first", C.c_void_p), ("members", C.c_void_p),
+                ("shared", C.c_void_p), ("group", C.c_void_p)]
+
+
 class Rotary(C.Structure):
     _fields_ = [("dim", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int), ("gain", C.c_float), ("freq", C.c_void_p),
                 ("pos", C.c_void_p), ("pos_seq", C.c_longlong)]
@@ -181,6 +186,8 @@ def lib() -> C.CDLL:
             "tg_cuda_attn_weights": ([vp, vp, vp, vp, vp, ll, ll, vp, vp, vp], i),
             "tg_cuda_kv_commit": ([vp, vp, vp, vp, vp, vp, ll, ll, i, vp], i),
             "tg_cuda_kv_evict": ([vp, vp, vp, ll, ll, i, i, i, vp, vp, vp, vp], i),
+            "tg_cuda_shared_attn_workspace": ([vp, vp, vp], ll),
+            "tg_cuda_shared_attn": ([vp, vp, vp, vp, ll, ll, ll, vp, vp, ll, vp], i),
             "tg_cuda_rope": ([vp, i, i, i, i, i, vp, ll, ll, ll, vp, ll, ll, ll, vp], i),
             "tg_cuda_kv_append": ([vp, vp, vp, vp, vp, C.c_float, vp, ll, ll, ll, vp, ll, ll, ll, vp, vp], i),
         }

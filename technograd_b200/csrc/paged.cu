@@ -50,10 +50,11 @@ int pg_device(const char *who, int *sms, int **status)
 	int met[PG_WORDS], any = 0;
 	for (int i = 0; i < PG_WORDS; i++) any |= met[i] = __atomic_exchange_n(g.host + i, 0, __ATOMIC_ACQ_REL);
 	if (any)
-		return set_err(TG_CUDA_EDEVICE, "%s: an earlier call on this device met%s%s%s%s%s", who,
+		return set_err(TG_CUDA_EDEVICE, "%s: an earlier call on this device met%s%s%s%s%s%s", who,
 			       met[PG_LEN] ? " a len outside [0, max_len];" : "", met[PG_PAGE] ? " a page number outside the pool;" : "",
 			       met[PG_PATH] ? " a path entry outside the drafted tokens;" : "",
-			       met[PG_ROOM] ? " a row past the table or the weights;" : "", met[PG_WAIT] ? " a wait that timed out;" : "");
+			       met[PG_ROOM] ? " a row past the table or the weights;" : "", met[PG_WAIT] ? " a wait that timed out;" : "",
+			       met[PG_GROUP] ? " a group of sequences or a shared length that does not suit;" : "");
 	*status = g.dev;
 	return TG_CUDA_OK;
 }

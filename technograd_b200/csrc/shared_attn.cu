@@ -1,0 +1,117 @@
+// shared_attn.cu -- tg_cuda_shared_attn: checks, how a call is cut, and its launches.
+#include <algorithm>
+
+#include "shared_attn.cuh"
+
+namespace tgc {
+
+extern template int shared_type<float>(const JoinArgs &, const SharedPlan &, const CUtensorMap *, cudaStream_t);
+extern template int shared_type<__half>(const JoinArgs &, const SharedPlan &, const CUtensorMap *, cudaStream_t);
+extern template int shared_type<__nv_bfloat16>(const JoinArgs &, const SharedPlan &, const CUtensorMap *, cudaStream_t);
+
+static int shared_check(const char *who, const tg_cuda_kv *c, const tg_cuda_prefix *x)
+{
+	if (!x) return set_err(TG_CUDA_EINVAL, "%s: NULL prefixes", who);
+	if (x->groups < 0 || x->groups > c->seqs || x->max_shared < 0 || x->max_shared > c->max_len || x->max_own < 0)
+		return set_err(TG_CUDA_EINVAL, "%s: %d groups of %d sequences, at most %d positions shared and %d not, of %d", who, x->groups, c->seqs, x->max_shared, x->max_own, c->max_len);
+	if (x->groups && (!x->first || !x->members || !x->shared || !x->group)) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer in the prefixes", who);
+	if (((uintptr_t)x->first | (uintptr_t)x->members | (uintptr_t)x->shared | (uintptr_t)x->group) & 3)
+		return set_err(TG_CUDA_EINVAL, "%s: a pointer of the prefixes is not on a 4-byte boundary", who);
+	return TG_CUDA_OK;
+}
+
+// Nothing is shared: tree attention itself.
+static bool shared_none(const tg_cuda_kv *c, const tg_cuda_prefix *x) { return !c->seqs || !x->groups || !x->max_shared; }
+
+static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, const tg_cuda_prefix *x, SharedPlan *o)
+{
+	tg_cuda_kv tail = *c;
+	tail.max_len = std::min(c->max_len, x->max_own);
+	int rc = attn_plan(who, &tail, d, &o->own);
+	if (rc) return rc;
+	AttnPlan &p = o->pre;
+	p = {};
+	p.dev = o->own.dev, p.sms = o->own.sms, o->dp = p.dp = o->own.dp;
+	const long long rows = (long long)c->seqs * d.tokens * d.group;
+	p.tc = c->type != TG_CUDA_F32 && p.dp <= 128;
+	p.mt = rows <= 16 || p.dp == 256 ? 1 : 2;
+	const int rt = p.tc ? 128 : 16 * p.mt, tk = p.tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
+	const long long pitch = rows / rt + x->groups + 1, units = c->nkv * pitch, tiles = ((long long)x->max_shared + tk - 1) / tk;
+	if (units > 0x7fffffff || rows * c->nkv > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
+	p.least = 128 / tk, p.begin = p.tc && units * tiles > 7ll * p.sms ? 6 : 2;
+	p.slot = (size_t)(rt * p.dp + 2 * rt) * 4;
+	const long long shares = (units * (tiles + p.begin) + p.least + p.begin - 1) / (p.least + p.begin), wave = (long long)p.sms * (p.tc || p.dp == 256 ? 1 : p.mt == 1 && c->type != TG_CUDA_F32 ? 3 : 2);
+	p.grid = (int)std::min(shares, wave), p.units = (int)units, p.row_tiles = 1;
+	o->pitch = (int)pitch, o->rows = rows * c->nkv;
+	size_t at = 0;
+	auto take = [&](size_t n) { const size_t was = at; at = (at + n + 255) / 256 * 256; return was; };
+	for (int i = 0; i < 2; i++) {
+		const AttnPlan &q = i ? o->own : o->pre;
+		o->tab[i] = take((size_t)q.units * sizeof(int2)), o->whole_o[i] = take((size_t)o->rows * o->dp * 4), o->whole_ml[i] = take((size_t)o->rows * 8);
+		o->part[i] = take(q.whole ? 0 : (size_t)q.grid * 2 * q.slot);
+	}
+	o->bytes = at;
+	return TG_CUDA_OK;
+}
+
+} // namespace tgc
+
+using namespace tgc;
+
+extern "C" long long tg_cuda_shared_attn_workspace(const tg_cuda_kv *c, const tg_cuda_drafts *d, const tg_cuda_prefix *x)
+{
+	const char *who = "tg_cuda_shared_attn_workspace";
+	clear_err();
+	PgCache pc;
+	PgDrafts pd;
+	SharedPlan pl;
+	int rc;
+	if ((rc = pg_cache(who, c, &pc)) || (rc = pg_drafts(who, c, d, PG_USE_Q | PG_USE_K | PG_USE_V, 64, &pd)) || (rc = shared_check(who, c, x))) return rc;
+	if (shared_none(c, x)) return tg_cuda_tree_attn_workspace(c, d);
+	if ((rc = shared_plan(who, c, pd, x, &pl))) return rc;
+	return (long long)pl.bytes;
+}
+
+extern "C" int tg_cuda_shared_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, const tg_cuda_prefix *x, void *out, long long out_seq,
+				   long long out_tok, long long out_head, float *lse, void *work, long long work_bytes, void *stream)
+{
+	const char *who = "tg_cuda_shared_attn";
+	clear_err();
+	JoinArgs j = {};
+	SharedArgs &p = j.own;
+	SharedPlan pl;
+	int rc, sms;
+	if ((rc = pg_cache(who, c, &p.c)) || (rc = pg_drafts(who, c, d, PG_USE_Q | PG_USE_K | PG_USE_V, 64, &p.d)) || (rc = shared_check(who, c, x))) return rc;
+	if (shared_none(c, x)) return tg_cuda_tree_attn(c, d, out, out_seq, out_tok, out_head, lse, work, work_bytes, stream);
+	const int e = pg_size(c->type);
+	if (!out || !lse) return set_err(TG_CUDA_EINVAL, "%s: NULL output", who);
+	if (c->seqs <= 1) out_seq = 0; // strides along one element are not used
+	if (d->tokens <= 1) out_tok = 0;
+	if (d->nq <= 1) out_head = 0;
+	if ((uintptr_t)lse & 3) return set_err(TG_CUDA_EINVAL, "%s: lse is not on a 4-byte boundary", who);
+	if (((uintptr_t)out & 15) || ((out_seq | out_tok | out_head) * e & 15))
+		return set_err(TG_CUDA_EINVAL, "%s: out rows must start on 16-byte boundaries", who);
+	if ((rc = pg_apart(who, "out", c->head_dim, {out_seq, out_tok, out_head}, {c->seqs, d->tokens, d->nq}))) return rc;
+	if ((rc = pg_device(who, &sms, &p.c.status)) || (rc = shared_plan(who, c, p.d, x, &pl))) return rc;
+	if (!work || work_bytes < (long long)pl.bytes || ((uintptr_t)work & 15))
+		return set_err(TG_CUDA_EINVAL, "%s: needs %zu bytes of 16-byte aligned scratch", who, pl.bytes);
+	p.out = (char *)out, p.out_seq = out_seq * e, p.out_tok = out_tok * e, p.out_head = out_head * e, p.lse = lse, p.seqs = c->seqs;
+	p.first = x->first, p.members = x->members, p.shared = x->shared, p.group = x->group, p.groups = x->groups, p.max_shared = x->max_shared;
+	p.pitch = pl.pitch, p.align = 1;
+	CUtensorMap maps[2] = {};
+	PgBox box = {};
+	const bool f16 = c->type == TG_CUDA_F16;
+	if ((pl.pre.tc || pl.own.tc) && pg_map(&maps[0], p.c, p.c.k, f16, 64, &box) && pg_map(&maps[1], p.c, p.c.v, f16, 64, &box)) p.box = box, p.align = box.rows;
+	j.pre = p;
+	char *w = (char *)work;
+	for (int i = 0; i < 2; i++) {
+		const AttnPlan &q = i ? pl.own : pl.pre;
+		SharedArgs &a = i ? j.own : j.pre;
+		a.row_tiles = q.row_tiles, a.whole = q.whole, a.least = q.least, a.begin = q.begin, a.ctas = q.grid;
+		a.tab = (int2 *)(w + pl.tab[i]), a.whole_o = (float *)(w + pl.whole_o[i]), a.whole_ml = (float2 *)(w + pl.whole_ml[i]), a.part = (float *)(w + pl.part[i]);
+	}
+	auto rt = [](const AttnPlan &q) { return q.tc ? 128 : q.fma ? q.fma : 16 * q.mt; };
+	j.pre_rt = rt(pl.pre), j.own_rt = rt(pl.own), j.pre_ctas = pl.pre.grid, j.own_ctas = pl.own.grid, j.rows = pl.rows;
+	cudaStream_t st = (cudaStream_t)stream;
+	return c->type == TG_CUDA_F32 ? shared_type<float>(j, pl, maps, st) : f16 ? shared_type<__half>(j, pl, maps, st) : shared_type<__nv_bfloat16>(j, pl, maps, st);
+}

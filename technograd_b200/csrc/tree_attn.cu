@@ -23,7 +23,7 @@ constexpr int ATTN_TC_ROWS = 32, ATTN_TC_ROWS_LONG = 16, ATTN_LONG = 24;
 // 19; 96, 78.7, 80.8, 84 at 42; 212, 206, 200, 200 at 125.
 constexpr int ATTN_BEGIN = 2, ATTN_TC_BEGIN = 6, ATTN_TC_SHORT = 7;
 
-static int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o)
+int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o)
 {
 	int rc = pg_sms(who, &o->dev, &o->sms);
 	if (rc) return rc;

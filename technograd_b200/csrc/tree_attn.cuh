@@ -2,6 +2,8 @@
 // the join of partial results. One source per element type instantiates it (tree_attn_*.cu).
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "mma_sync.cuh"
 #include "paged.cuh"
@@ -33,6 +35,46 @@ struct WeightArgs : AttnArgs { // its lse is the input; out and part are not use
 	long long acc_seq, acc_head;
 	float *acc_out, *fresh;
 };
+
+// Attention below shared prefixes (shared_attn.cuh) runs the kernels twice: over the groups' prefixes, whose units have the rows of
+// all members, and over what each sequence has of its own. Neither writes results: what a CTA has of a unit as a whole goes to
+// rows of its own, parts as above, and a join of both follows.
+enum { ATTN_ALL, ATTN_PREFIX, ATTN_OWN };
+
+struct SharedArgs : AttnArgs {
+	const int *first, *members, *shared, *group;
+	int groups, max_shared;
+	int align;       // a prefix ends at a multiple of this, a power of two; what is left of it is the sequences' own
+	float *whole_o;  // [rows][DP]: the rows of units that one CTA had, O before the division
+	float2 *whole_ml; // their reference and sum
+	int2 *tab;       // [units]: the first and last CTA of a unit, x = -1: one CTA had it all
+	int pitch;       // prefixes: entries of tab per head
+
+	// positions that sequence b of n positions shares with its group, g: the group
+	__device__ __forceinline__ int from(int b, int n, int &g) const
+	{
+		g = group[b];
+		if ((unsigned)g >= (unsigned)groups) {
+			if (g != -1) c.report(PG_GROUP);
+			g = -1;
+			return 0;
+		}
+		const int s = shared[g], f = first[g];
+		if (s < 0 || s > max_shared || s > n || b < f || b - f >= members[g]) c.report(PG_GROUP);
+		return max(0, min(s, min(n, max_shared))) & -align;
+	}
+	// the sequences of group g and their shared positions
+	__device__ __forceinline__ void prefix(int g, int &seq, int &m, int &n) const
+	{
+		const int f = first[g], k = members[g];
+		if (f < 0 || k < 0 || f > seqs || k > seqs - f) c.report(PG_GROUP);
+		seq = max(0, min(f, seqs)), m = max(0, min(k, seqs - seq));
+		n = m == 0 ? 0 : max(0, min(shared[g], min(max_shared, c.length(seq)))) & -align;
+	}
+	// place of a prefix's first unit in a head's part of tab: groups follow one another, so that no two meet
+	__device__ __forceinline__ long long base(int g, int seq, int rt) const { return (long long)seq * d.tokens * d.group / rt + g; }
+};
+template <int MODE> using AttnArgsOf = std::conditional_t<MODE == ATTN_ALL, AttnArgs, SharedArgs>;
 
 // exp(scale s - lse). The difference is taken before anything is multiplied by log2(e): of a key with much weight it is
 // near 0, while scale s and lse may be tens, and their products' roundings would be errors of 1e-6 in the weight.
@@ -72,33 +114,51 @@ template <class T, int DP, int MT> struct AttnTile {
 	static constexpr int CTAS = DP == 256 ? 1 : MT == 1 && sizeof(T) == 2 ? 3 : 2;
 	static constexpr int NST = CTAS == 3 || DP == 256 || (DP == 128 && MT == 2 && sizeof(T) == 4) ? 2 : 3;
 	static constexpr int Q = 0, RING = RT * P, MASK = RING + 4 * NST * STAGE, ML = MASK + RT * 8, SCAN = ML + 4 * RT * 8;
-	static constexpr int SMEM = SCAN + 64;
+	static constexpr int SMEM = SCAN + 128;
 	static constexpr int SLOT = RT * DP + 2 * RT; // floats of a partial result
 };
 
 // A place in the list of tiles.
 struct AttnCursor {
 	int b, h, r, tile, ctx, n, all; // ctx: tiles of cached positions, all: with the drafted ones
+	int p0;                         // own positions: the first of them
+	int seq, rows, tiles;           // prefixes (b: the group): the first member, the unit's rows and row tiles
 };
 
-template <int TK>
-__device__ __forceinline__ void cursor_seq(const AttnArgs &p, AttnCursor &c, int extra)
+template <int TK, int MODE = ATTN_ALL, int RT = 1>
+__device__ __forceinline__ void cursor_seq(const AttnArgsOf<MODE> &p, AttnCursor &c, int extra)
 {
-	c.n = p.c.length(c.b);
-	c.ctx = (int)(((long long)c.n + TK - 1) / TK);
-	c.all = c.ctx + extra;
+	if constexpr (MODE == ATTN_PREFIX) {
+		int m;
+		p.prefix(c.b, c.seq, m, c.n);
+		c.rows = m * p.d.tokens * p.d.group, c.tiles = (c.rows + RT - 1) / RT;
+		c.ctx = c.all = (int)(((long long)c.n + TK - 1) / TK);
+	} else {
+		c.n = p.c.length(c.b);
+		if constexpr (MODE == ATTN_OWN) {
+			int g;
+			c.p0 = p.from(c.b, c.n, g);
+			c.ctx = (int)(((long long)c.n - c.p0 + TK - 1) / TK);
+		} else c.ctx = (int)(((long long)c.n + TK - 1) / TK);
+		c.all = c.ctx + extra;
+	}
 }
 
-template <int TK>
-__device__ __forceinline__ void cursor_next(const AttnArgs &p, AttnCursor &c, int extra)
+template <int TK, int MODE = ATTN_ALL, int RT = 1>
+__device__ __forceinline__ void cursor_next(const AttnArgsOf<MODE> &p, AttnCursor &c, int extra)
 {
 	if (++c.tile < c.all) return;
 	c.tile = 0;
-	if (++c.r < p.row_tiles) return;
+	if (++c.r < (MODE == ATTN_PREFIX ? c.tiles : p.row_tiles)) return;
 	c.r = 0;
 	if (++c.h < p.c.nkv) return;
 	c.h = 0;
-	if (++c.b < p.seqs) cursor_seq<TK>(p, c, extra);
+	if constexpr (MODE == ATTN_PREFIX) {
+		while (++c.b < p.groups) {
+			cursor_seq<TK, MODE, RT>(p, c, extra);
+			if (c.all) break;
+		}
+	} else if (++c.b < p.seqs) cursor_seq<TK, MODE, RT>(p, c, extra);
 }
 
 // Sum of a value over the CTA's NW warps, and the sum over the threads before this one.
@@ -128,57 +188,84 @@ __device__ __forceinline__ long long block_scan(long long v, long long *s, long 
 // a / b of numbers that nearly always fit 32 bits (a 64-bit division is a long chain of instructions)
 __device__ __forceinline__ long long quotient(long long a, unsigned b) { return a >> 32 ? a / b : (long long)((unsigned)a / b); }
 
-// What a CTA works on: `left` tiles from place c of the list. s: NW + 4 words of shared memory.
+// What a CTA works on: `left` tiles from place c of the list. s: NW + 4 words of shared memory, for prefixes 2 NW + 6.
 // False: nothing. A unit counts its tiles and p.begin more, spent before its first tile; the CTAs' shares of
 // the total are equal, share and pos being one's size and beginning.
-template <int TK, int NW>
-__device__ __forceinline__ bool attn_share(const AttnArgs &p, long long *s, int extra, AttnCursor &c, long long &left, long long &pos, long long &share)
+template <int TK, int NW, int MODE = ATTN_ALL, int RT = 1>
+__device__ __forceinline__ bool attn_share(const AttnArgsOf<MODE> &p, long long *s, int extra, AttnCursor &c, long long &left, long long &pos, long long &share)
 {
 	if (p.whole) {
 		c.r = blockIdx.x % p.row_tiles;
 		c.h = blockIdx.x / p.row_tiles % p.c.nkv;
 		c.b = blockIdx.x / p.row_tiles / p.c.nkv;
 		c.tile = 0;
-		cursor_seq<TK>(p, c, extra);
+		cursor_seq<TK, MODE, RT>(p, c, extra);
 		left = c.all, pos = 0, share = 1;
 		return true;
 	}
-	const int per = p.c.nkv * p.row_tiles;
-	auto weight = [&](int b) -> long long { return b < p.seqs ? (((long long)p.c.length(b) + TK - 1) / TK + extra + p.begin) * per : 0; };
-	const bool once = p.seqs <= 32 * NW; // a thread per sequence: one pass over the lengths
+	const int per = p.c.nkv * p.row_tiles, lists = MODE == ATTN_PREFIX ? ((const SharedArgs &)p).groups : p.seqs;
+	auto units = [&](int b) -> long long { // prefixes
+		AttnCursor x;
+		x.b = b;
+		if (b >= lists) return 0;
+		cursor_seq<TK, MODE, RT>(p, x, extra);
+		return x.all ? (long long)x.tiles * p.c.nkv : 0;
+	};
+	auto weight = [&](int b) -> long long {
+		if constexpr (MODE == ATTN_ALL) return b < p.seqs ? (((long long)p.c.length(b) + TK - 1) / TK + extra + p.begin) * per : 0;
+		else {
+			AttnCursor x;
+			x.b = b;
+			if (b >= lists) return 0;
+			cursor_seq<TK, MODE, RT>(p, x, extra);
+			return MODE == ATTN_OWN ? ((long long)x.all + p.begin) * per : x.all ? ((long long)x.all + p.begin) * p.c.nkv * x.tiles : 0;
+		}
+	};
+	const bool once = lists <= 32 * NW; // a thread per sequence: one pass over the lengths
 	long long mine = 0, before, all;
-	for (int b = threadIdx.x; b < p.seqs; b += 32 * NW) mine += weight(b);
+	for (int b = threadIdx.x; b < lists; b += 32 * NW) mine += weight(b);
 	all = block_scan<NW>(mine, s, before);
 	share = quotient(all + gridDim.x - 1, gridDim.x);
 	if (share < p.least + p.begin) share = p.least + p.begin;
 	pos = share * blockIdx.x;
-	if (threadIdx.x == 0 && p.split && !p.by_unit) p.split[blockIdx.x].x = -1;
+	if (MODE == ATTN_ALL && threadIdx.x == 0 && p.split && !p.by_unit) p.split[blockIdx.x].x = -1;
 	if (pos >= all) return false;
 	const long long to = all - pos < share ? all : pos + share; // the place after the share
 	long long base = 0;
+	long long *su = s + NW + 4; // prefixes: the units before the two places
+	long long ubase = 0, ubefore = 0;
 	for (int b0 = 0;; b0 += 32 * NW) { // ends: pos < to <= all
 		const int b = b0 + threadIdx.x;
 		const long long w = once ? mine : weight(b), sum = once ? all : block_scan<NW>(w, s, before);
-		if (pos >= base + before && pos < base + before + w) s[NW] = b, s[NW + 1] = base + before;
-		if (to - 1 >= base + before && to - 1 < base + before + w) s[NW + 2] = b, s[NW + 3] = base + before;
-		base += sum;
+		long long usum = 0;
+		if constexpr (MODE == ATTN_PREFIX) usum = block_scan<NW>(units(b), su, ubefore);
+		if (pos >= base + before && pos < base + before + w) {
+			s[NW] = b, s[NW + 1] = base + before;
+			if constexpr (MODE == ATTN_PREFIX) su[NW] = ubase + ubefore;
+		}
+		if (to - 1 >= base + before && to - 1 < base + before + w) {
+			s[NW + 2] = b, s[NW + 3] = base + before;
+			if constexpr (MODE == ATTN_PREFIX) su[NW + 1] = ubase + ubefore;
+		}
+		base += sum, ubase += usum;
 		if (to <= base) break;
 	}
 	__syncthreads();
 	// tiles before the place `off` into sequence b's units, whose units begin at place `first`
 	int u, t, in;
-	auto tiles = [&](long long b, long long first, long long off) {
+	auto tiles = [&](long long b, long long first, long long off, long long before) {
 		c.b = (int)b;
-		cursor_seq<TK>(p, c, extra);
+		cursor_seq<TK, MODE, RT>(p, c, extra);
 		u = (int)quotient(off, c.all + p.begin);
 		in = (int)(off - (long long)u * (c.all + p.begin));
 		t = in < p.begin ? 0 : in - p.begin;
-		return first - b * per * p.begin + (long long)u * c.all + t;
+		return first - (MODE == ATTN_PREFIX ? before : b * per) * p.begin + (long long)u * c.all + t;
 	};
-	left = tiles(s[NW + 2], s[NW + 3], to - 1 - s[NW + 3]);
+	left = tiles(s[NW + 2], s[NW + 3], to - 1 - s[NW + 3], MODE == ATTN_PREFIX ? su[NW + 1] : 0);
 	if (in >= p.begin) left++; // the last place is a tile's
-	left -= tiles(s[NW], s[NW + 1], pos - s[NW + 1]);
-	c.tile = t, c.h = u / p.row_tiles, c.r = u % p.row_tiles;
+	left -= tiles(s[NW], s[NW + 1], pos - s[NW + 1], MODE == ATTN_PREFIX ? su[NW] : 0);
+	const int rt = MODE == ATTN_PREFIX ? c.tiles : p.row_tiles;
+	c.tile = t, c.h = u / rt, c.r = u % rt;
 	return left > 0;
 }
 
@@ -189,6 +276,44 @@ __device__ __forceinline__ void attn_note(const AttnArgs &p, const AttnCursor &c
 	const int head = c.b * p.c.nkv + c.h;
 	p.split[p.by_unit ? (long long)head * p.row_tiles + c.r : blockIdx.x] =
 		whole ? make_int4(-1, 0, 0, 0) : make_int4(blockIdx.x, (int)((pos + share + (c.all - 2 - c.tile)) / share), head, c.r);
+}
+
+// The same in a table of all units. (An entry out of its bounds: lists of groups that overlap, which are reported.)
+template <int MODE, int RT>
+__device__ __forceinline__ void shared_note(const SharedArgs &p, const AttnCursor &c, bool whole, long long pos, long long share)
+{
+	const long long at = MODE == ATTN_PREFIX ? p.base(c.b, c.seq, RT) + c.r : ((long long)c.b * p.c.nkv + c.h) * p.row_tiles + c.r;
+	if (MODE == ATTN_PREFIX && at >= p.pitch) return;
+	p.tab[MODE == ATTN_PREFIX ? (long long)c.h * p.pitch + at : at] =
+		whole ? make_int2(-1, -1) : make_int2(blockIdx.x, (int)((pos + share + (c.all - 2 - c.tile)) / share));
+}
+
+// Row r of a unit: its sequence, token and query head.
+struct SharedRow {
+	int b, t, j;
+};
+template <int MODE> __device__ __forceinline__ SharedRow shared_row(const AttnArgs &p, const AttnCursor &c, int r)
+{
+	const int x = r / p.d.group, j = c.h * p.d.group + (r - x * p.d.group);
+	if constexpr (MODE != ATTN_PREFIX) return { c.b, x, j };
+	const int m = x / p.d.tokens;
+	return { c.seq + m, x - m * p.d.tokens, j };
+}
+__device__ __forceinline__ const char *q_row(const AttnArgs &p, SharedRow x) { return p.d.q + x.b * p.d.q_seq + x.t * p.d.q_tok + x.j * p.d.q_head; }
+__device__ __forceinline__ long long whole_row(const AttnArgs &p, SharedRow x) { return ((long long)x.b * p.d.tokens + x.t) * p.d.nq + x.j; }
+
+// The two passes and their join follow one another without a gap: the pass over own positions begins as soon as the prefixes' CTAs
+// leave room. Those have waited for what came before the call, and a grid counts as launched when all its CTAs have, so that
+// nothing before the call runs any more; and the own positions' CTAs end after the prefixes', so that the join
+// finds both.
+template <int MODE> __device__ __forceinline__ void shared_begin()
+{
+	if (MODE == ATTN_PREFIX) pdl_wait();
+	pdl_launch();
+}
+template <int MODE> __device__ __forceinline__ void shared_end()
+{
+	if (MODE == ATTN_OWN) pdl_wait();
 }
 
 // o (already over l, or a partial's) of 4 columns
@@ -243,14 +368,14 @@ __device__ __forceinline__ void store_row4(const AttnArgs &p, const AttnRow &x, 
 
 // A warp's fetching of its rows of the tiles to come, K and V: lane i < KW holds the place of the tile's row i, looked up
 // while the tile before is fetched.
-template <class T, int DP, class A> struct AttnFetch {
-	const AttnArgs &p;
+template <class T, int DP, class A, int MODE = ATTN_ALL> struct AttnFetch {
+	const AttnArgsOf<MODE> &p;
 	AttnCursor f;
 	long long left, fetched = 0;
 	uint32_t at = PG_NONE, ring;
 	int extra, chunks;
 
-	__device__ __forceinline__ AttnFetch(const AttnArgs &args, const AttnCursor &c, long long n, uint32_t stages, int drafted_tiles, int row_chunks)
+	__device__ __forceinline__ AttnFetch(const AttnArgsOf<MODE> &args, const AttnCursor &c, long long n, uint32_t stages, int drafted_tiles, int row_chunks)
 		: p(args), f(c), left(n), ring(stages), extra(drafted_tiles), chunks(row_chunks)
 	{
 		find();
@@ -261,10 +386,10 @@ template <class T, int DP, class A> struct AttnFetch {
 		at = PG_NONE;
 		if (lane >= A::KW || fetched >= left) return;
 		if (f.tile < f.ctx) {
-			const int x = f.tile * A::TK + warp * A::KW + lane;
+			const int x = (MODE == ATTN_OWN ? f.p0 : 0) + f.tile * A::TK + warp * A::KW + lane;
 			if (x < f.n) {
 				const int page = x / p.c.page;
-				at = p.c.at(p.c.table[(long long)f.b * p.c.cols + page], x - page * p.c.page);
+				at = p.c.at(p.c.table[(long long)(MODE == ATTN_PREFIX ? f.seq : f.b) * p.c.cols + page], x - page * p.c.page);
 			}
 		} else {
 			const int u = (f.tile - f.ctx) * A::TK + warp * A::KW + lane;
@@ -281,7 +406,7 @@ template <class T, int DP, class A> struct AttnFetch {
 			const long long head = ctx ? f.h * p.c.head_b : f.b * p.d.kv_seq + f.h * p.d.kv_head;
 			const char *kp = (ctx ? p.c.k : p.d.k) + head, *vp = (ctx ? p.c.v : p.d.v) + head;
 			const uint32_t sk = ring + stage * A::STAGE, sv = sk + A::KW * A::P, mine = at;
-			cursor_next<A::TK>(p, f, extra);
+			cursor_next<A::TK, MODE, A::RT>(p, f, extra);
 			fetched++;
 			find();
 #pragma unroll
@@ -298,8 +423,8 @@ template <class T, int DP, class A> struct AttnFetch {
 	}
 };
 
-template <class T, int DP, int MT>
-__global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(const AttnArgs p)
+template <class T, int DP, int MT, int MODE = ATTN_ALL>
+__global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(const AttnArgsOf<MODE> p)
 {
 	using A = AttnTile<T, DP, MT>;
 	constexpr int KW = A::KW, NT = A::NT, TK = A::TK, RT = A::RT, P = A::P, CH = A::CH, NST = A::NST;
@@ -310,17 +435,23 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 	long long *s_scan = (long long *)(smem + A::SCAN);
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
 	const uint32_t s0 = smem_u32(smem), ring = s0 + A::RING + warp * NST * A::STAGE;
-	const int extra = (p.d.tokens + TK - 1) / TK, rows = p.d.tokens * p.d.group, chunks = p.c.dim * (int)sizeof(T) / 16;
-	const bool twin = MT == 1 && sizeof(T) == 2 && rows <= 8; // rows 8 to 15 are rows 0 to 7 again (pv_tile)
+	const int extra = MODE == ATTN_PREFIX ? 0 : (p.d.tokens + TK - 1) / TK, chunks = p.c.dim * (int)sizeof(T) / 16;
+	int rows = p.d.tokens * p.d.group;
+	const bool twin = MT == 1 && sizeof(T) == 2 && MODE != ATTN_PREFIX && rows <= 8; // rows 8 to 15 are rows 0 to 7 again (pv_tile)
 	const float zs = p.d.scale * 1.4426950408889634f;
-	pdl_launch();
-	pdl_wait();
+	if constexpr (MODE == ATTN_ALL) {
+		pdl_launch();
+		pdl_wait();
+	} else shared_begin<MODE>();
 
 	AttnCursor c; // the tile being worked on; f, below: the next to be fetched
 	long long left, pos, share;
-	if (!attn_share<TK, 4>(p, s_scan, extra, c, left, pos, share)) return;
+	if (!attn_share<TK, 4, MODE, RT>(p, s_scan, extra, c, left, pos, share)) {
+		shared_end<MODE>();
+		return;
+	}
 
-	AttnFetch<T, DP, A> f(p, c, left, ring, extra, chunks);
+	AttnFetch<T, DP, A, MODE> f(p, c, left, ring, extra, chunks);
 	auto fetch = [&](int stage) { f.fetch(stage); };
 
 	float o[MT][DP / 8][4], mr[MT][2], l[MT][2];
@@ -334,15 +465,18 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 		if (first) { // a unit begins here, or goes on from the CTA before
 			first = false;
 			from_start = c.tile == 0;
-			cnt = p.d.drafted(c.b);
+			if constexpr (MODE == ATTN_PREFIX) rows = c.rows;
+			else cnt = p.d.drafted(c.b);
 			for (int x = tid; x < RT * CH; x += 128) {
 				const int row = x / CH, ch = x % CH, r = c.r * RT + (twin ? row & 7 : row), t = r / p.d.group;
 				uint4 v = make_uint4(0, 0, 0, 0);
-				if (r < rows && ch < chunks)
-					v = *(const uint4 *)(p.d.q + (long long)c.b * p.d.q_seq + (long long)t * p.d.q_tok + (long long)(c.h * p.d.group + r % p.d.group) * p.d.q_head + ch * 16);
+				if (r < rows && ch < chunks) {
+					if constexpr (MODE == ATTN_PREFIX) v = *(const uint4 *)(q_row(p, shared_row<MODE>(p, c, r)) + ch * 16);
+					else v = *(const uint4 *)(p.d.q + (long long)c.b * p.d.q_seq + (long long)t * p.d.q_tok + (long long)(c.h * p.d.group + r % p.d.group) * p.d.q_head + ch * 16);
+				}
 				*(uint4 *)(smem + row * P + ((ch ^ (row & 7)) << 4)) = v;
 			}
-			if (tid < RT) {
+			if (MODE != ATTN_PREFIX && tid < RT) {
 				const int t = (c.r * RT + (twin ? tid & 7 : tid)) / p.d.group;
 				s_mask[tid] = t < cnt ? p.d.sees(c.b, t, cnt) : 0;
 			}
@@ -373,7 +507,7 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 #pragma unroll
 				for (int e = 0; e < 4; e++) s[m][x][e] *= zs;
 		if (drafted || c.tile == c.ctx - 1) { // the mask's bits, or the end of the cache
-			const long long at = (long long)(drafted ? c.tile - c.ctx : c.tile) * TK + warp * KW;
+			const long long at = (long long)(drafted ? c.tile - c.ctx : c.tile) * TK + warp * KW + (MODE == ATTN_OWN && !drafted ? c.p0 : 0);
 #pragma unroll
 			for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -507,7 +641,14 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 						const float4 y = *(const float4 *)(smem + (ring - s0) + ((w - warp) * NST + stage) * A::STAGE + (row * DP + (col ^ ((row & 7) * 8))) * 4);
 						v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
 					}
-					if (complete) {
+					if (MODE != ATTN_ALL && complete) {
+						if (r0 + r < rows) {
+							const SharedArgs &sp = (const SharedArgs &)p;
+							const long long to = whole_row(p, shared_row<MODE>(p, c, r0 + r));
+							*(float4 *)(sp.whole_o + to * DP + col) = v;
+							if (col == 0) sp.whole_ml[to] = make_float2(top, sum);
+						}
+					} else if (complete) {
 						if (r0 + r < rows) {
 							const AttnRow to = attn_row(p, b, h, r0 + r, cnt, sum);
 							store_row4<T>(p, to, col, v);
@@ -520,14 +661,18 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 				}
 				__syncthreads();
 			}
-			if (from_start && tid == 0) attn_note(p, c, end, pos, share);
+			if (from_start && tid == 0) {
+				if constexpr (MODE == ATTN_ALL) attn_note(p, c, end, pos, share);
+				else shared_note<MODE, RT>(p, c, end, pos, share);
+			}
 			first = true;
 		}
 		__syncwarp(); // every lane is done with this stage
 		stage = (stage + 1) % NST;
-		cursor_next<TK>(p, c, extra);
+		cursor_next<TK, MODE, RT>(p, c, extra);
 	}
 	cp_wait<0>();
+	shared_end<MODE>();
 }
 
 // A partial result's place of 4 columns of a row (then come the rows' mr and l): as the kernel that
@@ -597,6 +742,9 @@ struct AttnPlan {
 	size_t slot; // bytes of a partial result
 	size_t bytes() const { return whole ? 0 : (size_t)grid * (2 * slot + sizeof(int4)); }
 };
+
+// tree_attn.cu: the cut of a call whose sequences have at most c->max_len positions.
+int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o);
 
 // Launches a planned call; T is the element type.
 template <class T> int attn_type(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st);

@@ -24,9 +24,10 @@ template <int DP, int R> struct FmaTile {
 	static constexpr int SLOT = RT * DP + 2 * RT;
 };
 
-template <int DP, int R>
-__global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(const AttnArgs p)
+template <int DP, int R, int MODE = ATTN_ALL>
+__global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(const AttnArgsOf<MODE> p)
 {
+	static_assert(MODE != ATTN_PREFIX, "rows of one sequence only");
 	using A = FmaTile<DP, R>;
 	constexpr int KW = A::KW, TK = A::TK, P = A::P, CH = A::CH, NST = A::NST, NP = DP / 64; // NP: pairs of a lane's dimensions
 	constexpr float RAISE = AttnScale<float>::RAISE;
@@ -37,12 +38,17 @@ __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(con
 	const uint32_t ring = smem_u32(smem) + A::RING + warp * NST * A::STAGE;
 	const int extra = (p.d.tokens + TK - 1) / TK, rows = p.d.tokens * p.d.group, chunks = p.c.dim / 4;
 	const float zs = p.d.scale * 1.4426950408889634f;
-	pdl_launch();
-	pdl_wait();
+	if constexpr (MODE == ATTN_ALL) {
+		pdl_launch();
+		pdl_wait();
+	} else shared_begin<MODE>();
 	AttnCursor c;
 	long long left, pos, share;
-	if (!attn_share<TK, 4>(p, (long long *)(smem + A::SCAN), extra, c, left, pos, share)) return;
-	AttnFetch<float, DP, A> f(p, c, left, ring, extra, chunks);
+	if (!attn_share<TK, 4, MODE>(p, (long long *)(smem + A::SCAN), extra, c, left, pos, share)) {
+		shared_end<MODE>();
+		return;
+	}
+	AttnFetch<float, DP, A, MODE> f(p, c, left, ring, extra, chunks);
 	float2 o[R][NP];
 	float mr[R], l[R];
 	int cnt = 0, stage = 0;
@@ -94,7 +100,7 @@ __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(con
 				d[r] = fma2(make_float2(k.z, k.w), make_float2(q.z, q.w), d[r]);
 			}
 		}
-		const long long key = (long long)(drafted ? c.tile - c.ctx : c.tile) * TK + warp * KW + g;
+		const long long key = (long long)(drafted ? c.tile - c.ctx : c.tile) * TK + warp * KW + g + (MODE == ATTN_OWN && !drafted ? c.p0 : 0);
 		float s[R];
 		bool up = false;
 #pragma unroll
@@ -183,6 +189,13 @@ __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(con
 				if (!complete) {
 					*(float4 *)(slot + r * DP + col) = v;
 					if (col == 0) slot[R * DP + r] = top, slot[R * DP + R + r] = sum;
+				} else if (MODE != ATTN_ALL) {
+					if (row < rows) {
+						const SharedArgs &sp = (const SharedArgs &)p;
+						const long long to = whole_row(p, shared_row<MODE>(p, c, row));
+						*(float4 *)(sp.whole_o + to * DP + col) = v;
+						if (col == 0) sp.whole_ml[to] = make_float2(top, sum);
+					}
 				} else if (row < rows) {
 					const AttnRow to = attn_row(p, c.b, c.h, row, cnt, sum);
 					store_row4<float>(p, to, col, v);
@@ -190,14 +203,18 @@ __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(con
 				}
 			}
 			__syncthreads();
-			if (from_start && tid == 0) attn_note(p, c, end, pos, share);
+			if (from_start && tid == 0) {
+				if constexpr (MODE == ATTN_ALL) attn_note(p, c, end, pos, share);
+				else shared_note<MODE, R>(p, c, end, pos, share);
+			}
 			first = true;
 		}
 		__syncwarp(); // every lane is done with this stage
 		stage = (stage + 1) % NST;
-		cursor_next<TK>(p, c, extra);
+		cursor_next<TK, MODE>(p, c, extra);
 	}
 	cp_wait<0>();
+	shared_end<MODE>();
 }
 
 } // namespace tgc

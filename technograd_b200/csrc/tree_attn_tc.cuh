@@ -43,7 +43,7 @@ struct TaBars {
 	uint32_t tmem;
 	int abort;
 	int odd[4][2]; // drafted tile: a V row held something not finite (tile & 3; half of its rows)
-	long long scan[24];
+	long long scan[44];
 	float2 ml[2][128];
 };
 
@@ -178,8 +178,8 @@ __device__ __forceinline__ bool ta_weighs(const AttnArgs &p, int b, int h, int t
 	return !(s * p.d.scale * 1.4426950408889634f - ref < -126); // (a score that is NaN counts)
 }
 
-template <class T, int DP, bool BOX>
-__global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
+template <class T, int DP, bool BOX, int MODE = ATTN_ALL>
+__global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgsOf<MODE> p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
 {
 	using A = TaTile<DP>;
 	constexpr int TK = A::TK, RT = A::RT, CH = A::CH;
@@ -205,12 +205,18 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 		B->abort = 0;
 		fence_barrier_init();
 	}
-	pdl_launch();
-	pdl_wait();
-	const int rows = p.d.tokens * p.d.group, chunks = p.c.dim / 8;
+	if constexpr (MODE == ATTN_ALL) {
+		pdl_launch();
+		pdl_wait();
+	} else shared_begin<MODE>();
+	constexpr int EXTRA = MODE == ATTN_PREFIX ? 0 : 1; // tiles of drafted rows
+	const int all_rows = p.d.tokens * p.d.group, chunks = p.c.dim / 8;
 	AttnCursor c;
 	long long left_, pos, share;
-	if (!attn_share<TK, A::NW>(p, B->scan, 1, c, left_, pos, share)) return; // the whole CTA
+	if (!attn_share<TK, A::NW, MODE, RT>(p, B->scan, EXTRA, c, left_, pos, share)) { // the whole CTA
+		shared_end<MODE>();
+		return;
+	}
 	const int left = (int)left_;
 	if (warp == 16) tmem_alloc(&B->tmem, 512); // S buffers at columns 0 and 128, the halves' O at 256 and 256 + DP
 	tc_fence_before();
@@ -233,24 +239,25 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 		// by TMA, lane i has box i / (DP / 64) of its half's 64 rows, and 64 of its dimensions
 		constexpr int ND = DP / 64;
 		const int boxes = BOX ? 64 / p.box.rows : 0;
-		auto by_box = [&]() { return BOX && c.tile < c.ctx - isv; };
+		// (a prefix ends where a box does, and what is past it arrives as zeros)
+		auto by_box = [&]() { return BOX && (MODE == ATTN_PREFIX || c.tile < c.ctx - isv); };
 		auto look = [&]() {
 			const bool drafted = c.tile >= c.ctx, box = by_box();
 #pragma unroll
 			for (int i = 0; i < 2; i++) {
-				const int x = (drafted ? 0 : c.tile * TK) + half * 64 + (box ? lane / ND * p.box.rows : i * 32 + lane);
+				const int x = (drafted ? 0 : c.tile * TK + (MODE == ATTN_OWN ? c.p0 : 0)) + half * 64 + (box ? lane / ND * p.box.rows : i * 32 + lane);
 				in_page[i] = -1;
 				if (drafted) {
 					if (x < p.d.drafted(c.b)) in_page[i] = x;
 				} else if (x < c.n && !(box && (i || lane >= boxes * ND))) {
 					const int page = x / p.c.page;
 					in_page[i] = x - page * p.c.page;
-					entry[i] = p.c.table[(long long)c.b * p.c.cols + page];
+					entry[i] = p.c.table[(long long)(MODE == ATTN_PREFIX ? c.seq : c.b) * p.c.cols + page];
 				}
 			}
 		};
 		if (par < left) {
-			if (par) cursor_next<TK>(p, c, 1);
+			if (par) cursor_next<TK, MODE, RT>(p, c, EXTRA);
 			look();
 		}
 		int last = -1; // tile asked for
@@ -260,15 +267,16 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 			const int sh = drafted ? 4 : p.c.shift;
 			const char *base = (drafted ? (isv ? p.d.v : p.d.k) + (long long)c.b * p.d.kv_seq + c.h * p.d.kv_head : (isv ? p.c.v : p.c.k) + c.h * p.c.head_b) + ch * 16;
 			const int st = j % A::NST;
-			const char *qb = p.d.q + (long long)c.b * p.d.q_seq + (long long)c.h * p.d.group * p.d.q_head + ch * 16;
+			const int seq = MODE == ATTN_PREFIX ? c.seq : c.b, rows = MODE == ATTN_PREFIX ? c.rows : all_rows; // of this tile's unit
+			const char *qb = p.d.q + (long long)seq * p.d.q_seq + (long long)c.h * p.d.group * p.d.q_head + ch * 16;
 			const int r0 = c.r * RT + half * 64 + lane;
 #pragma unroll
 			for (int i = 0; i < 2; i++)
 				at[i] = in_page[i] < 0 ? PG_NONE : box ? (uint32_t)((unsigned)entry[i] < (unsigned)p.c.pages ? in_page[i] : (p.c.report(PG_PAGE), -1)) : drafted ? (uint32_t)(in_page[i] * p.d.kv_tok >> 4) : p.c.at(entry[i], in_page[i]);
 			const int page = entry[0];
 			if (j + 2 < left) {
-				cursor_next<TK>(p, c, 1);
-				cursor_next<TK>(p, c, 1);
+				cursor_next<TK, MODE, RT>(p, c, EXTRA);
+				cursor_next<TK, MODE, RT>(p, c, EXTRA);
 				look();
 			}
 			const int tile = (isv ? A::V : A::K) + st * A::OP;
@@ -296,8 +304,22 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 				if (j > 0 && !ta_wait(B, &B->kfree[(j - 1) % A::NST], (j - 1) / A::NST & 1, p.c)) break;
 #pragma unroll 1
 				for (int i = 0; i < 2; i++) {
-					const int r = r0 + i * 32, t = r / p.d.group;
-					const uint32_t mine = r < rows ? (uint32_t)(((long long)t * p.d.q_tok + (long long)(r - t * p.d.group) * p.d.q_head) >> 4) : PG_NONE;
+					const int r = r0 + i * 32;
+					int t = r / p.d.group;
+					const int g = r - t * p.d.group;
+					if constexpr (MODE == ATTN_PREFIX) { // the members' rows lie further apart than 32 bits of places hold
+						const int m = t / p.d.tokens;
+						t -= m * p.d.tokens;
+						const unsigned long long place = r < rows ? (unsigned long long)((long long)m * p.d.q_seq + (long long)t * p.d.q_tok + (long long)g * p.d.q_head) : ~0ull;
+#pragma unroll 4
+						for (int y = 0; y < CH; y++) {
+							const unsigned long long o = __shfl_sync(~0u, place, y * RI + lane / CH);
+							const bool have = o != ~0ull && piece;
+							cp16(d0 + A::Q + (i * 32 + y * RI) * 128 + (x0 ^ ((y * RI & 7) << 4)), qb + (have ? o : 0), have);
+						}
+						continue;
+					}
+					const uint32_t mine = r < rows ? (uint32_t)(((long long)t * p.d.q_tok + (long long)g * p.d.q_head) >> 4) : PG_NONE;
 #pragma unroll 4
 					for (int y = 0; y < CH; y++) {
 						const uint32_t o = __shfl_sync(~0u, mine, y * RI + lane / CH);
@@ -363,7 +385,7 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 				const int f = warp - 17; // the half of the tile's keys
 				const uint32_t idO = id | ((uint32_t)(DP >> 3) << 17) | (1u << 16); // V MN-major
 				int unit = 0;
-				for (int j = 0; j < left; j++, cursor_next<TK>(p, c, 1)) {
+				for (int j = 0; j < left; j++, cursor_next<TK, MODE, RT>(p, c, EXTRA)) {
 					const bool first = j == 0 || c.tile == 0;
 					if (first && unit++ && !ta_poll(B, &B->o_free, unit & 1, p.c)) break; // the unit before has been read
 					if (!ta_poll(B, &B->vfull[j % A::NST], j / A::NST & 1, p.c) || !ta_poll(B, &B->p_full[f][j & 1], (j >> 1) & 1, p.c)) break;
@@ -396,9 +418,11 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 			const bool fresh = j == 0 || c.tile == 0, drafted = c.tile >= c.ctx;
 			if (fresh) { // a unit begins, or goes on from the CTA before
 				from_start = c.tile == 0;
-				cnt = p.d.drafted(c.b);
-				const int t = (c.r * RT + row) / p.d.group;
-				see = t < cnt ? p.d.sees(c.b, t, cnt) : 0;
+				if constexpr (MODE != ATTN_PREFIX) {
+					cnt = p.d.drafted(c.b);
+					const int t = (c.r * RT + row) / p.d.group;
+					see = t < cnt ? p.d.sees(c.b, t, cnt) : 0;
+				}
 				mr = -INFINITY, l = 0;
 			}
 			if (!ta_wait(B, &B->s_full[j & 1], (j >> 1) & 1, p.c)) break;
@@ -408,7 +432,7 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 			tmem_ld32(lanes + (j & 1) * TK + hf * 64 + 32, *(float (*)[32])(z + 32));
 			float mul = zs; // what turns z into the exponent
 			if (drafted || c.tile == c.ctx - 1) { // the mask's bits, or the end of the cache
-				const int n = drafted ? 0 : (int)(c.n - (long long)c.tile * TK) - hf * 64;
+				const int n = drafted ? 0 : (int)(c.n - (long long)c.tile * TK) - hf * 64 - (MODE == ATTN_OWN ? c.p0 : 0);
 				const unsigned long long ok = drafted ? (hf ? 0ull : see) : n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
 				const uint32_t lo = (uint32_t)ok, hi = (uint32_t)(ok >> 32);
 #pragma unroll
@@ -472,10 +496,13 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 				const float2 a = B->ml[0][row], d = B->ml[1][row];
 				const float both = fmaxf(a.x, d.x), fa = a.x == -INFINITY ? 0 : ex2(a.x - both), fd = d.x == -INFINITY ? 0 : ex2(d.x - both);
 				const float sl = (a.x == -INFINITY ? a.y : a.y * fa) + (d.x == -INFINITY ? d.y : d.y * fd);
-				const int r = c.r * RT + row, b = c.b, h = c.h;
+				const int r = c.r * RT + row, b = c.b, h = c.h, rows = MODE == ATTN_PREFIX ? c.rows : all_rows;
 				const bool complete = end && from_start, odd = drafted && (*(volatile int *)&B->odd[j & 3][0] | *(volatile int *)&B->odd[j & 3][1]);
 				float *slot = complete ? nullptr : p.part + (2ll * blockIdx.x + (from_start ? 1 : 0)) * A::SLOT;
-				const AttnRow to = attn_row(p, b, h, r < rows ? r : 0, cnt, sl);
+				AttnRow to = {};
+				long long place = 0;
+				if constexpr (MODE == ATTN_ALL) to = attn_row(p, b, h, r < rows ? r : 0, cnt, sl);
+				else place = whole_row(p, shared_row<MODE>(p, c, r < rows ? r : 0));
 #pragma unroll 1
 				for (int w = hf * (DP / 64); w < (hf + 1) * (DP / 64); w++) {
 					float v[32], u[32];
@@ -497,19 +524,31 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 					if (!complete) {
 #pragma unroll
 						for (int e = 0; e < 32; e += 4) *(float4 *)(slot + slot_at<DP, RT>(row, w * 32 + e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+					} else if (MODE != ATTN_ALL) {
+						if (r < rows) {
+#pragma unroll
+							for (int e = 0; e < 32; e += 4)
+								*(float4 *)(((const SharedArgs &)p).whole_o + place * DP + w * 32 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+						}
 					} else if (r < rows) {
 #pragma unroll
 						for (int e = 0; e < 32; e += 8) store_row8<T>(p, to, w * 32 + e, v + e);
 					}
 				}
-				if (complete && hf == 0 && r < rows) store_lse(to, both, sl);
+				if (complete && hf == 0 && r < rows) {
+					if constexpr (MODE == ATTN_ALL) store_lse(to, both, sl);
+					else ((const SharedArgs &)p).whole_ml[place] = make_float2(both, sl);
+				}
 				if (!complete && hf == 0) slot[RT * DP + row] = both, slot[RT * DP + RT + row] = sl;
-				if (from_start && tid == 0) attn_note(p, c, end, pos, share);
+				if (from_start && tid == 0) {
+					if constexpr (MODE == ATTN_ALL) attn_note(p, c, end, pos, share);
+					else shared_note<MODE, RT>(p, c, end, pos, share);
+				}
 				tc_fence_before();
 				mbar_arrive_warp(&B->o_free);
 				unit++;
 			}
-			cursor_next<TK>(p, c, 1);
+			cursor_next<TK, MODE, RT>(p, c, EXTRA);
 		}
 	}
 	tc_fence_before();
@@ -518,6 +557,7 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgs p, const
 		tc_fence_after();
 		tmem_dealloc(tmem, 512);
 	}
+	shared_end<MODE>();
 }
 
 } // namespace tgc

@@ -189,6 +189,62 @@ def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float 
     return out, lse
 
 
+class SharedPrefix:
+    """Which sequences of a cache begin with the same pages (tg_cuda_prefix): made once, when the batch's composition changes.
+
+    groups: (first sequence, sequences, shared positions) of each, ascending; sequences in none share nothing. The tables of a group's sequences
+    name the same pages for the shared positions. max_own: about how many positions a sequence has at most behind what it
+    shares (default: what max_len leaves); it only sizes the launches, and the lengths may grow past it."""
+
+    def __init__(self, cache: PagedKV, groups, max_own: int | None = None):
+        groups = [tuple(int(x) for x in g) for g in groups]
+        end, which = 0, [-1] * cache.seqs
+        for i, (first, members, shared) in enumerate(groups):
+            _need(first >= end and members > 0 and first + members <= cache.seqs, f"groups: sequences {first} to {first + members - 1} of {cache.seqs}, after {end - 1}")
+            _need(0 <= shared <= cache.page * cache.table.shape[1], f"groups: {shared} shared positions, of {cache.page * cache.table.shape[1]} that a table holds")
+            end = first + members
+            which[first:end] = [i] * members
+        self.groups, self.seqs, self.index = groups, cache.seqs, cache.index
+        lengths = [g[2] for g in groups]
+        self.max_shared = max(lengths, default=0)
+        if max_own is None:
+            max_own = cache.max_len - (min(lengths) if groups and -1 not in which else 0)
+        _need(max_own >= 0, f"max_own: {max_own}")
+        _int32(max_own=max_own)
+        made = torch.tensor([g[0] for g in groups] + [g[1] for g in groups] + lengths + which, dtype=torch.int32).to(cache.device)
+        n, at = len(groups), made.data_ptr()
+        self._held = made
+        self._struct = _lib.Prefix(n, self.max_shared, max_own, at, at + 4 * n, at + 8 * n, at + 12 * n)
+        self._at = C.addressof(self._struct)
+
+
+def shared_attention(cache: PagedKV, prefix: SharedPrefix, q, k, v, mask=None, count=None, scale: float | None = None):
+    """tree_attention for a batch whose sequences share prefixes, each read once for its whole group (tg_cuda_shared_attn).
+
+    Arguments and results as for tree_attention."""
+    if prefix.index != cache.index or prefix.seqs != cache.seqs or prefix.max_shared > cache.max_len:
+        raise ValueError(f"prefix: made for {prefix.seqs} sequences with up to {prefix.max_shared} positions shared on cuda:{prefix.index}, not for {cache.seqs} of "
+                         f"up to {cache.max_len} on cuda:{cache.index}")
+    d = _drafts(cache, q, k, v, mask, count, scale)
+    stream, shape = _stream(cache), q.shape
+    key = shape[1], shape[2], prefix
+    plan = cache._plans.get(key)
+    if plan is None:
+        size = _lib.lib().tg_cuda_shared_attn_workspace(cache._at, d, prefix._at)
+        if size < 0:
+            _lib.check(size)
+        plan = cache._plans[key] = size, cache._one.expand(shape[:3])
+    size, like = plan
+    out, lse = torch.empty_like(q), torch.empty_like(like)
+    work = q.new_empty(size, dtype=torch.uint8) if size else None  # held until the kernels are launched, as above
+    so = out.stride()
+    _lib.check(_lib.lib().tg_cuda_shared_attn(cache._at, d, prefix._at, out.data_ptr(), so[0], so[1], so[2], lse.data_ptr(),
+                                              work.data_ptr() if size else None, size, stream))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _NoGradient.apply("shared_attention", 2, out, lse, q, k, v)
+    return out, lse
+
+
 def attention_weights(cache: PagedKV, q, k, lse, mask=None, count=None, select=None, acc=None, scale: float | None = None):
     """The attention weight of the selected tokens on each position (tg_cuda_attn_weights).
 
@@ -332,8 +388,8 @@ def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None,
 
     k, v [seqs, tokens, nkv, head_dim] and q [seqs, tokens, nq, head_dim]: a projection's output, any number of tokens; count int32
     [seqs]: tokens there are (None: all). Cache row lens + i receives token i's k, rotated to its position (pos, None: lens + i), and v. q_norm, k_norm
-    f32 [head_dim]: weights of an RMS norm of each head before the rotation. keys: return the rotated keys too, which tree_attention and
-    shared_attention take as the tokens' own with the lengths from before. Returns (the new lengths, q rotated or
+    f32 [head_dim]: weights of an RMS norm of each head before the rotation. keys: return the rotated keys too, with k's strides, which tree_attention and
+    shared_attention take with v as the tokens' own, the lengths being those from before. Returns (the new lengths, q rotated or
     None, k rotated or None), rows past count 0; the pages are written in place. Forward only, like tree_attention."""
     d = _drafts(cache, q, k, v, None, count, 1.0)
     n, dim, index = k.shape, cache.head_dim, cache.index
@@ -349,7 +405,8 @@ def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None,
         qo = torch.empty_like(q, memory_format=torch.contiguous_format)
         sq = qo.stride()
     if keys:
-        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        sk = k.stride()  # v's, so that the two are drafted rows together
+        ko = torch.empty_strided(n, sk, dtype=k.dtype, device=k.device) if all(x <= 1 or s for x, s in zip(n, sk)) else torch.empty_like(k, memory_format=torch.contiguous_format)
         sk = ko.stride()
     _lib.check(_lib.lib().tg_cuda_kv_append(cache._at, d, r, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
                                             None if qo is None else qo.data_ptr(), sq[0], sq[1], sq[2], None if ko is None else ko.data_ptr(), sk[0], sk[1], sk[2],
