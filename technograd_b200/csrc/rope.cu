@@ -12,20 +12,20 @@ struct TurnRows {
 	char *dst, *pool;                  // either may be NULL
 	long long s_seq, s_tok, s_head, d_seq, d_tok, d_head; // bytes
 	const float *norm;                 // [dim] or NULL
-	int heads, turn;
+	int heads, turn, chunks;           // chunks: warps that have a token's rows of this kind
 };
 
 struct TurnArgs {
 	PgCache c;                         // table and len NULL: no cache
 	TurnRows rows[3];
-	int nrows, heads;                  // of them, and all their heads
+	int nrows, heads, chunks;          // of them, and all their heads and chunks
 	const double *freq;
 	const int *pos;
 	long long pos_seq;
 	const int *count;
 	int *len_out;
 	long long all;                     // seqs * tokens
-	int tokens, dim, part, inverse, per; // per: tokens of a block
+	int tokens, dim, part, inverse;
 	float gain, eps;
 };
 
@@ -47,30 +47,163 @@ __device__ __forceinline__ float2 turn_of(double freq, int pos)
 
 enum { TURN_HALF, TURN_PAIRS, TURN_ANY }; // halves that begin at 16-byte pieces; neighbours; halves that begin anywhere
 
+// A row's norm, its inverse: the sum over the `lanes` threads that have the row's elements x.
+template <int N> __device__ __forceinline__ float turn_norm(const float (&x)[N], int lanes, float dim, float eps)
+{
+	float ss = 0;
+#pragma unroll
+	for (int e = 0; e < N; e++) ss = fmaf(x[e], x[e], ss);
+	for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+	return __frsqrt_rn(ss / dim + eps);
+}
+
+// a / b of numbers that nearly always fit 32 bits (a 64-bit division is a long chain of instructions)
+__device__ __forceinline__ long long over(long long a, int b) { return a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
+
+// Position of a token. (An addition past 32 bits comes round, as an angle may.)
+__device__ __forceinline__ int turn_pos(const TurnArgs &p, long long b, int i, int len)
+{
+	return p.pos ? p.pos[b * p.pos_seq + i] : (int)((unsigned)len + (unsigned)i);
+}
+
+// A warp has UN rounds of one token's rows of one kind (q, k or v): 1 << lg threads a row, each with two 16-byte pieces, those
+// that turn with each other. So a thread has the same E pairs in all its rows and keeps their cos and sin in registers; the warp's
+// threads of one place compute PART of them each and pass them round. No shared memory, no barrier, and all rounds'
+// loads on their way at once. A row's threads lie in one warp, so that a row may be written where it is read.
+// What bounds it: HBM where there are many tokens, latency where there are few.
+template <class T, int FORM, bool NORM, int PART, int UN>
+__global__ void __launch_bounds__(256) k_turn(const TurnArgs p, int lg)
+{
+	constexpr int E = 16 / (int)sizeof(T);
+	const int lane = threadIdx.x & 31, lanes = 1 << lg, mine = lane & (lanes - 1), at = lane >> lg, half = p.part >> 1, n = (half + E - 1) / E, nch = p.dim / E;
+	const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), w0 = over(item, p.chunks);
+	if (w0 >= p.all) return;
+	int chunk = (int)(item - w0 * p.chunks), g = 0;
+	while (chunk >= p.rows[g].chunks) chunk -= p.rows[g++].chunks;
+	const TurnRows &w = p.rows[g];
+	const long long b = over(w0, p.tokens);
+	const int i = (int)(w0 - b * p.tokens), h0 = chunk * (UN << (5 - lg)) + at;
+	int live = 1, len = 0, cnt = p.tokens;
+	if (p.count) {
+		cnt = p.count[b];
+		live = i < cnt;
+		cnt = max(0, min(cnt, p.tokens));
+	}
+	const bool turn = w.turn && mine < n;
+	const int c0 = FORM == TURN_PAIRS ? 2 * mine : mine < n ? mine : 2 * mine, c1 = FORM == TURN_HALF && mine < n ? mine + n : c0 + 1;
+	const char *src = w.src + b * w.s_seq + i * w.s_tok;
+	uint4 raw[UN][2];
+#pragma unroll
+	for (int u = 0; u < UN; u++) {
+		const int h = h0 + (u << (5 - lg));
+		const bool in = live && h < w.heads;
+		raw[u][0] = in && c0 < nch ? __ldcs((const uint4 *)(src + h * w.s_head + c0 * 16)) : make_uint4(0, 0, 0, 0);
+		raw[u][1] = in && c1 < nch ? __ldcs((const uint4 *)(src + h * w.s_head + c1 * 16)) : make_uint4(0, 0, 0, 0);
+	}
+	long long row = -1;
+	if (p.c.len) {
+		len = p.c.length((int)b);
+		if (item == w0 * p.chunks && i == 0 && lane == 0) p.len_out[b] = len + cnt;
+		if (w.pool && live) {
+			const long long to = (long long)len + i;
+			if (to >= (long long)p.c.page * p.c.cols || to > 0x7fffffff) p.c.report(PG_ROOM);
+			else row = p.c.row(p.c.table + b * p.c.cols, (int)to);
+		}
+	}
+	float2 cs[E];
+	if (w.turn && live) { // the whole warp
+		const int pos = turn_pos(p, b, i, len);
+		float2 own[PART];
+#pragma unroll
+		for (int x = 0; x < PART; x++) {
+			const int e = at * PART + x, a = mine * E + e;
+			own[x] = make_float2(1, 0);
+			if (e < E && a < half) {
+				own[x] = turn_of(p.freq[a], pos);
+				own[x].x *= p.gain, own[x].y *= p.inverse ? -p.gain : p.gain;
+			}
+		}
+#pragma unroll
+		for (int e = 0; e < E; e++)
+			cs[e] = make_float2(__shfl_sync(~0u, own[e % PART].x, (e / PART << lg) + mine), __shfl_sync(~0u, own[e % PART].y, (e / PART << lg) + mine));
+	}
+	float wn[2 * E];
+	if (NORM && w.norm) {
+#pragma unroll
+		for (int e = 0; e < 2 * E; e++) {
+			const int c = e < E ? c0 : c1;
+			wn[e] = c < nch ? w.norm[c * E + e % E] : 0;
+		}
+	}
+#pragma unroll
+	for (int u = 0; u < UN; u++) {
+		const int h = h0 + (u << (5 - lg));
+		const bool in = h < w.heads;
+		if (live && (w.turn || (NORM && w.norm))) { // (else the bits pass as they are)
+			float x[2 * E];
+#pragma unroll
+			for (int e = 0; e < 2 * E; e++) x[e] = PgElem<T>::get(((const T *)raw[u])[e]);
+			if constexpr (NORM) {
+				if (w.norm) {
+					const float inv = turn_norm(x, lanes, (float)p.dim, p.eps);
+#pragma unroll
+					for (int e = 0; e < 2 * E; e++) x[e] = x[e] * inv * wn[e];
+				}
+			}
+			if (turn) {
+#pragma unroll
+				for (int e = 0; e < E; e++) {
+					if (FORM == TURN_PAIRS && mine * E + e >= half) break; // what passes, infinities too
+					const int a = FORM == TURN_HALF ? e : 2 * e, o = FORM == TURN_HALF ? e + E : 2 * e + 1;
+					const float y = x[a], z = x[o];
+					x[a] = fmaf(y, cs[e].x, -(z * cs[e].y)), x[o] = fmaf(y, cs[e].y, z * cs[e].x);
+				}
+			}
+#pragma unroll
+			for (int e = 0; e < 2 * E; e++) ((T *)raw[u])[e] = PgElem<T>::put(x[e]);
+		}
+		if (w.dst && in) {
+			char *to = w.dst + b * w.d_seq + i * w.d_tok + h * w.d_head;
+			if (c0 < nch) *(uint4 *)(to + c0 * 16) = raw[u][0];
+			if (c1 < nch) *(uint4 *)(to + c1 * 16) = raw[u][1];
+		}
+		if (row >= 0 && in) {
+			char *to = w.pool + row + h * p.c.head_b;
+			if (c0 < nch) *(uint4 *)(to + c0 * 16) = raw[u][0];
+			if (c1 < nch) *(uint4 *)(to + c1 * 16) = raw[u][1];
+		}
+	}
+}
+
 struct TurnToken {
 	long long b, row; // its sequence, and its cache row in bytes (-1: none)
 	int i, live;
 };
 
-// A thread has two 16-byte pieces of a row (TURN_HALF: the two that turn with each other), a row's threads lie in one
-// warp, so that a row may be written where it is read. cos and sin of a token are computed once for all its heads.
-template <class T, int FORM, bool NORM>
-__global__ void __launch_bounds__(256) k_turn(const TurnArgs p, int lanes, int lg)
+// Halves that begin within a 16-byte piece: elements find their partners one by one in the row, which the first read has
+// brought near. A block has `per` tokens and their cos and sin in shared memory.
+template <class T, bool NORM>
+__global__ void __launch_bounds__(256) k_turn_any(const TurnArgs p, int lg, int per_)
 {
 	constexpr int E = 16 / (int)sizeof(T);
-	extern __shared__ __align__(16) float2 cs[]; // [per][n * E]
+	extern __shared__ __align__(16) float2 cs[]; // [per][half]
 	__shared__ TurnToken tok[8];
-	const int tid = threadIdx.x, half = p.part >> 1, n = (half + E - 1) / E, nch = p.dim / E, width = FORM == TURN_ANY ? half : n * E;
-	const long long t0 = (long long)blockIdx.x * p.per;
-	const int per = (int)min((long long)p.per, p.all - t0);
+	const int tid = threadIdx.x, lanes = 1 << lg, half = p.part >> 1, nch = p.dim / E;
+	const long long t0 = (long long)blockIdx.x * per_;
+	const int per = (int)min((long long)per_, p.all - t0);
 	if (tid < per) {
 		TurnToken k;
 		k.b = (t0 + tid) / p.tokens, k.i = (int)(t0 + tid - k.b * p.tokens), k.live = 1, k.row = -1;
-		if (p.count) k.live = k.i < p.count[k.b];
+		int cnt = p.tokens;
+		if (p.count) {
+			cnt = p.count[k.b];
+			k.live = k.i < cnt;
+			cnt = max(0, min(cnt, p.tokens));
+		}
 		if (p.c.len) {
-			const int len = p.c.length((int)k.b), all = p.count ? max(0, min(p.count[k.b], p.tokens)) : p.tokens;
+			const int len = p.c.length((int)k.b);
 			const long long at = (long long)len + k.i;
-			if (k.i == 0) p.len_out[k.b] = len + all;
+			if (k.i == 0) p.len_out[k.b] = len + cnt;
 			if (k.live) {
 				if (at >= (long long)p.c.page * p.c.cols || at > 0x7fffffff) p.c.report(PG_ROOM);
 				else k.row = p.c.row(p.c.table + k.b * p.c.cols, (int)at);
@@ -78,74 +211,44 @@ __global__ void __launch_bounds__(256) k_turn(const TurnArgs p, int lanes, int l
 		}
 		tok[tid] = k;
 	}
-	for (int x = tid; x < per * width; x += 256) {
-		const int t = per == 1 ? 0 : x / width, a = x - t * width;
-		const long long b = (t0 + t) / p.tokens;
-		const int i = (int)(t0 + t - b * p.tokens);
-		float2 v = make_float2(1, 0);
-		if (a < half) {
-			const int at = p.pos ? p.pos[b * p.pos_seq + i] : p.c.len ? (int)((unsigned)p.c.length((int)b) + (unsigned)i) : i;
-			v = turn_of(p.freq[a], at);
-			v.x *= p.gain, v.y *= p.inverse ? -p.gain : p.gain;
-		}
-		// the pairs of a thread in 16-byte pieces, the pieces of neighbouring threads next to each other
-		cs[t * width + (FORM == TURN_ANY ? a : (((a % E) >> 1) * n + a / E) * 2 + (a & 1))] = v;
+	for (int x = tid; x < per * half; x += 256) {
+		const long long w = t0 + x / half, b = w / p.tokens;
+		float2 v = turn_of(p.freq[x % half], turn_pos(p, b, (int)(w - b * p.tokens), p.c.len ? p.c.length((int)b) : 0));
+		v.x *= p.gain, v.y *= p.inverse ? -p.gain : p.gain;
+		cs[x] = v;
 	}
 	__syncthreads();
-	const int mine = tid & (lanes - 1), total = per * p.heads;
+	const int mine = tid & (lanes - 1), c0 = 2 * mine, total = per * p.heads;
 	for (int r0 = 0; r0 < total; r0 += 256 >> lg) {
 		const int r = r0 + (tid >> lg), t = min(r, total - 1) / p.heads;
 		int h = min(r, total - 1) - t * p.heads, g = 0;
-		while (g + 1 < p.nrows && h >= p.rows[g].heads) h -= p.rows[g++].heads;
+		while (h >= p.rows[g].heads) h -= p.rows[g++].heads;
 		const TurnRows &w = p.rows[g];
 		const TurnToken k = tok[t];
-		const bool turn = w.turn && FORM != TURN_ANY && mine < n;
-		const int c0 = FORM != TURN_HALF ? 2 * mine : mine < n ? mine : 2 * mine, c1 = FORM == TURN_HALF && mine < n ? mine + n : c0 + 1;
-		const bool in = r < total, h0 = in && c0 < nch, h1 = in && c1 < nch;
+		const bool in = r < total, in0 = in && c0 < nch, in1 = in && c0 + 1 < nch;
 		const char *src = w.src + k.b * w.s_seq + k.i * w.s_tok + h * w.s_head;
 		uint4 raw[2] = {};
-		if (k.live && h0) raw[0] = *(const uint4 *)(src + c0 * 16);
-		if (k.live && h1) raw[1] = *(const uint4 *)(src + c1 * 16);
-		float x[2 * E];
+		if (k.live && in0) raw[0] = *(const uint4 *)(src + c0 * 16);
+		if (k.live && in1) raw[1] = *(const uint4 *)(src + c0 * 16 + 16);
+		float x[2 * E], inv = 1;
 #pragma unroll
 		for (int e = 0; e < 2 * E; e++) x[e] = PgElem<T>::get(((const T *)raw)[e]);
-		float inv = 1;
 		if constexpr (NORM) {
-			float ss = 0;
-#pragma unroll
-			for (int e = 0; e < 2 * E; e++) ss = fmaf(x[e], x[e], ss);
-			for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+			inv = turn_norm(x, lanes, (float)p.dim, p.eps);
 			if (w.norm) {
-				inv = __frsqrt_rn(ss / (float)p.dim + p.eps);
 #pragma unroll
-				for (int e = 0; e < 2 * E; e++) {
-					const int c = e < E ? c0 : c1;
-					x[e] = x[e] * inv * (c < nch ? w.norm[c * E + e % E] : 0);
-				}
+				for (int e = 0; e < 2 * E; e++) x[e] = x[e] * inv * (c0 + e / E < nch ? w.norm[c0 * E + e] : 0);
 			}
 		}
-		if constexpr (FORM == TURN_ANY) {
-			if (w.turn && k.live) {
+		if (w.turn && k.live && in) {
 #pragma unroll
-				for (int e = 0; e < 2 * E; e++) {
-					const int el = (e < E ? c0 : c1) * E + e % E, a = el < half ? el : el - half, other = el < half ? el + half : a;
-					if (in && el < p.part) {
-						float y = PgElem<T>::get(((const T *)src)[other]);
-						if (NORM && w.norm) y = y * inv * w.norm[other];
-						const float2 v = cs[t * width + a];
-						x[e] = fmaf(x[e], v.x, el < half ? -(y * v.y) : y * v.y);
-					}
-				}
-			}
-		} else if (turn) {
-			const float4 *table = (const float4 *)(cs + t * width) + mine;
-#pragma unroll
-			for (int i = 0; i < E / 2; i++) {
-				const float4 v = table[i * n];
-				const int a0 = FORM == TURN_HALF ? 2 * i : 4 * i, b0 = FORM == TURN_HALF ? a0 + E : a0 + 1, a1 = FORM == TURN_HALF ? a0 + 1 : a0 + 2, b1 = FORM == TURN_HALF ? b0 + 1 : a0 + 3;
-				const float p0 = x[a0], q0 = x[b0], p1 = x[a1], q1 = x[b1];
-				x[a0] = fmaf(p0, v.x, -(q0 * v.y)), x[b0] = fmaf(p0, v.y, q0 * v.x);
-				x[a1] = fmaf(p1, v.z, -(q1 * v.w)), x[b1] = fmaf(p1, v.w, q1 * v.z);
+			for (int e = 0; e < 2 * E; e++) {
+				const int el = c0 * E + e, a = el < half ? el : el - half, other = el < half ? el + half : a;
+				if (el >= p.part) continue;
+				float y = PgElem<T>::get(((const T *)src)[other]);
+				if (NORM && w.norm) y = y * inv * w.norm[other];
+				const float2 v = cs[t * half + a];
+				x[e] = fmaf(x[e], v.x, el < half ? -(y * v.y) : y * v.y);
 			}
 		}
 		if (w.turn || (NORM && w.norm)) { // (else the bits pass as they are)
@@ -154,14 +257,14 @@ __global__ void __launch_bounds__(256) k_turn(const TurnArgs p, int lanes, int l
 		}
 		__syncwarp(); // the row has been read
 		if (w.dst) {
-			char *to = w.dst + k.b * w.d_seq + k.i * w.d_tok + h * w.d_head;
-			if (h0) *(uint4 *)(to + c0 * 16) = k.live ? raw[0] : make_uint4(0, 0, 0, 0);
-			if (h1) *(uint4 *)(to + c1 * 16) = k.live ? raw[1] : make_uint4(0, 0, 0, 0);
+			char *to = w.dst + k.b * w.d_seq + k.i * w.d_tok + h * w.d_head + c0 * 16;
+			if (in0) *(uint4 *)to = k.live ? raw[0] : make_uint4(0, 0, 0, 0);
+			if (in1) *(uint4 *)(to + 16) = k.live ? raw[1] : make_uint4(0, 0, 0, 0);
 		}
 		if (w.pool && k.row >= 0) {
-			char *to = w.pool + k.row + h * p.c.head_b;
-			if (h0) *(uint4 *)(to + c0 * 16) = raw[0];
-			if (h1) *(uint4 *)(to + c1 * 16) = raw[1];
+			char *to = w.pool + k.row + h * p.c.head_b + c0 * 16;
+			if (in0) *(uint4 *)to = raw[0];
+			if (in1) *(uint4 *)(to + 16) = raw[1];
 		}
 	}
 }
@@ -177,30 +280,55 @@ static int turn_check(const char *who, const tg_cuda_rotary *r, int head_dim, in
 	return TG_CUDA_OK;
 }
 
-template <class T, int FORM>
-static int turn_launch(TurnArgs &p, bool norm, cudaStream_t st)
+constexpr int TURN_UN = 2; // rounds of a warp
+
+static int turn_grid(long long blocks)
+{
+	return blocks > 0x7fffffff ? set_err(TG_CUDA_EINVAL, "rotary positions: a grid of %lld blocks", blocks) : TG_CUDA_OK;
+}
+
+template <class T, int FORM, int PART>
+static int turn_launch(TurnArgs &p, bool norm, int lg, cudaStream_t st)
+{
+	p.chunks = 0;
+	for (int g = 0; g < p.nrows; g++) p.chunks += p.rows[g].chunks = (p.rows[g].heads + (TURN_UN << (5 - lg)) - 1) / (TURN_UN << (5 - lg));
+	const __int128 items = (__int128)p.all * p.chunks;
+	const long long blocks = items > 0x3ffffffffll ? 0x80000000ll : (long long)(items + 7) / 8;
+	if (turn_grid(blocks)) return TG_CUDA_EINVAL;
+	if (norm) k_turn<T, FORM, true, PART, TURN_UN><<<(unsigned)blocks, 256, 0, st>>>(p, lg);
+	else k_turn<T, FORM, false, PART, TURN_UN><<<(unsigned)blocks, 256, 0, st>>>(p, lg);
+	TGC_LAUNCH_CHECK();
+	return TG_CUDA_OK;
+}
+
+template <class T, int FORM> static int turn_part(TurnArgs &p, bool norm, int lg, cudaStream_t st)
+{
+	constexpr int E = 16 / (int)sizeof(T);
+	const int part = (E << lg) / 32; // pairs that a thread computes for those of its place in other rows
+	if constexpr (E == 8) {
+		if (part == 8) return turn_launch<T, FORM, 8>(p, norm, lg, st);
+	}
+	return part == 4 ? turn_launch<T, FORM, 4>(p, norm, lg, st) : part == 2 ? turn_launch<T, FORM, 2>(p, norm, lg, st) : turn_launch<T, FORM, 1>(p, norm, lg, st);
+}
+
+template <class T> static int turn_form(TurnArgs &p, int pairs, bool norm, cudaStream_t st)
 {
 	constexpr int E = 16 / (int)sizeof(T);
 	const int items = (p.dim / E + 1) / 2;
 	int lg = 0;
 	while (1 << lg < items) lg++;
+	if (pairs) return turn_part<T, TURN_PAIRS>(p, norm, lg, st);
+	if (p.part * (int)sizeof(T) % 32 == 0) return turn_part<T, TURN_HALF>(p, norm, lg, st);
 	p.heads = 0;
 	for (int g = 0; g < p.nrows; g++) p.heads += p.rows[g].heads;
-	p.per = std::max(1, std::min(8, 256 / std::max(1, std::min(256, p.heads << lg))));
-	const long long blocks = (p.all + p.per - 1) / p.per;
-	if (blocks > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "rotary positions: %lld tokens", p.all);
-	const int width = FORM == TURN_ANY ? p.part / 2 : (p.part / 2 + E - 1) / E * E;
-	const size_t smem = (size_t)p.per * width * sizeof(float2);
-	if (norm) k_turn<T, FORM, true><<<(unsigned)blocks, 256, smem, st>>>(p, 1 << lg, lg);
-	else k_turn<T, FORM, false><<<(unsigned)blocks, 256, smem, st>>>(p, 1 << lg, lg);
+	const int per = std::max(1, std::min(8, 256 / std::min(256, p.heads << lg)));
+	const long long blocks = (p.all + per - 1) / per;
+	if (turn_grid(blocks)) return TG_CUDA_EINVAL;
+	const size_t smem = (size_t)per * (p.part / 2) * sizeof(float2);
+	if (norm) k_turn_any<T, true><<<(unsigned)blocks, 256, smem, st>>>(p, lg, per);
+	else k_turn_any<T, false><<<(unsigned)blocks, 256, smem, st>>>(p, lg, per);
 	TGC_LAUNCH_CHECK();
 	return TG_CUDA_OK;
-}
-
-template <class T> static int turn_form(TurnArgs &p, int pairs, bool norm, cudaStream_t st)
-{
-	if (pairs) return turn_launch<T, TURN_PAIRS>(p, norm, st);
-	return p.part * (int)sizeof(T) % 32 ? turn_launch<T, TURN_ANY>(p, norm, st) : turn_launch<T, TURN_HALF>(p, norm, st);
 }
 
 static int turn_type(TurnArgs &p, int type, int pairs, bool norm, void *stream)
@@ -243,7 +371,7 @@ extern "C" int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tok
 	if (((uintptr_t)x & 15) || ((s[0] | s[1] | s[2]) * e & 15)) return set_err(TG_CUDA_EINVAL, "%s: x rows must start on 16-byte boundaries", who);
 	if (!none && (rc = turn_out(who, "out", out, o, seqs, tokens, heads, head_dim, e))) return rc;
 	if ((rc = pg_sms(who, &dev, &sms)) || none) return rc;
-	p.rows[0] = { (const char *)x, (char *)out, nullptr, s[0] * e, s[1] * e, s[2] * e, o[0] * e, o[1] * e, o[2] * e, nullptr, heads, 1 };
+	p.rows[0] = { (const char *)x, (char *)out, nullptr, s[0] * e, s[1] * e, s[2] * e, o[0] * e, o[1] * e, o[2] * e, nullptr, heads, r->dim > 0, 0 };
 	p.nrows = 1, p.all = (long long)seqs * tokens, p.tokens = tokens, p.dim = head_dim;
 	return turn_type(p, type, r->interleaved, false, stream);
 }
@@ -272,9 +400,9 @@ extern "C" int tg_cuda_kv_append(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	if (k_out && (rc = turn_out(who, "k_out", k_out, ko, c->seqs, d->tokens, c->nkv, c->head_dim, e))) return rc;
 	if ((rc = pg_apart(who, "the cache", c->head_dim, {c->page_stride, c->head_stride, c->pos_stride}, {c->pages, c->nkv, c->page}))) return rc;
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0) return rc;
-	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim };
-	p.rows[p.nrows++] = { pd.k, (char *)k_out, p.c.k, pd.kv_seq, pd.kv_tok, pd.kv_head, ko[0] * e, ko[1] * e, ko[2] * e, k_norm, c->nkv, r && r->dim };
-	p.rows[p.nrows++] = { pd.v, nullptr, p.c.v, pd.kv_seq, pd.kv_tok, pd.kv_head, 0, 0, 0, nullptr, c->nkv, 0 };
+	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim, 0 };
+	p.rows[p.nrows++] = { pd.k, (char *)k_out, p.c.k, pd.kv_seq, pd.kv_tok, pd.kv_head, ko[0] * e, ko[1] * e, ko[2] * e, k_norm, c->nkv, r && r->dim, 0 };
+	p.rows[p.nrows++] = { pd.v, nullptr, p.c.v, pd.kv_seq, pd.kv_tok, pd.kv_head, 0, 0, 0, nullptr, c->nkv, 0, 0 };
 	p.count = d->count, p.len_out = len_out, p.all = (long long)c->seqs * d->tokens, p.tokens = d->tokens, p.dim = c->head_dim, p.eps = eps;
 	return turn_type(p, c->type, r && r->interleaved, q_norm || k_norm, stream);
 }

@@ -86,6 +86,20 @@ def test_frequencies_of_any_size(cuda):
     close(got[..., keep], want[..., keep], tol[..., keep] + 2.0 ** -30, F32)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim,part", [(64, 6), (64, 32), (80, 20), (128, 34)])
+@pytest.mark.parametrize("pairs", [False, True])
+def test_what_passes_stays_as_it_is(cuda, dtype, dim, part, pairs):
+    """Infinities and NaN behind the rotated part reach nothing, and are what they were."""
+    x = torch.randn(2, 3, 5, dim, generator=torch.Generator().manual_seed(12)).to(dtype)
+    r, pos = kvcache.Rotary(dim, theta=1e4, part=part, interleaved=pairs), positions(2, 3, 13)
+    x[..., part:] = torch.tensor([math.inf, -math.inf, math.nan, -0.0]).to(dtype)[torch.arange(dim - part) % 4]
+    got = kvcache.rope(x.cuda(), r, pos.cuda()).cpu()
+    want, tol = turned(x[..., :part].double(), pos, r.freq, pairs=pairs)
+    close(got[..., :part], want, tol, dtype)
+    assert torch.equal(torch.nan_to_num(got[..., part:].float(), 7, 8, 9), torch.nan_to_num(x[..., part:].float(), 7, 8, 9))
+
+
 @pytest.mark.parametrize("dtype,dim,part,pairs", [(BF16, 128, 128, False), (F16, 80, 20, False), (F32, 64, 64, True), (F16, 64, 48, True)])
 def test_in_place_and_strided(cuda, dtype, dim, part, pairs):
     g = torch.Generator().manual_seed(5)
