@@ -2,6 +2,7 @@
 // paged cache with the norm and the rotation on the way.
 #include <algorithm>
 
+#include "mma_sync.cuh"
 #include "paged.cuh"
 
 namespace tgc {
@@ -12,7 +13,8 @@ struct TurnRows {
 	char *dst, *pool;                  // either may be NULL
 	long long s_seq, s_tok, s_head, d_seq, d_tok, d_head; // bytes
 	const float *norm;                 // [dim] or NULL
-	int heads, turn, chunks;           // chunks: warps that have a token's rows of this kind
+	int heads, turn;
+	int chunks, aligned;               // warps that have a token's rows of this kind; norm lies on a 16-byte boundary
 };
 
 struct TurnArgs {
@@ -26,39 +28,73 @@ struct TurnArgs {
 	int *len_out;
 	long long all;                     // seqs * tokens
 	int tokens, dim, part, inverse;
-	float gain, eps;
+	float gain, eps, over_dim;         // 1 / dim
 };
 
 // cos and sin of pos * freq. The angle is taken in turns, as 64 bits behind the point: whole turns fall off the product by
 // themselves, so a far position's angle is as exact as a near one's (2^-55 turns of the frequency times the position).
-// What is left of the nearest quarter turn has 24 significant bits of its own in f32.
+// The first 32 bits of it, 2^-32 turns, are a quarter turn and a rest of at most an eighth, x = 2 pi rest, whose sine and cosine
+// are their Taylor series up to x^9 and x^10: what is left out is below (pi/4)^11 / 11! = 1.8e-9 and (pi/4)^12 / 12! = 1.2e-10.
 __device__ __forceinline__ float2 turn_of(double freq, int pos)
 {
-	double x = freq * 0.15915494309189535; // 1 / 2 pi
-	x -= rint(x);
-	const unsigned long long f = (unsigned long long)__double2ll_rn(x * 0x1p63) << 1;
-	const unsigned long long t = f * (unsigned long long)(long long)pos;
-	const unsigned q = (unsigned)((t + (1ull << 61)) >> 62);
-	float s, c;
-	sincospif((float)(long long)(t - ((unsigned long long)q << 62)) * 0x1p-63f, &s, &c);
+	double f = freq * 0.15915494309189535; // 1 / 2 pi
+	f -= rint(f);
+	const unsigned long long u = (unsigned long long)__double2ll_rn(f * 0x1p63) << 1;
+	const unsigned t = (unsigned)(u * (unsigned long long)(long long)pos >> 32), q = (t + (1u << 29)) >> 30;
+	const float x = (float)(int)(t - (q << 30)) * 1.4629180792671596e-9f, z = x * x; // 2 pi / 2^32
+	const float s = x * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1 / 362880.f, -1 / 5040.f), 1 / 120.f), -1 / 6.f), 1.f);
+	const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1 / 3628800.f, 1 / 40320.f), -1 / 720.f), 1 / 24.f), -0.5f), 1.f);
 	const float a = q & 1 ? s : c, b = q & 1 ? c : s;
-	return make_float2(q == 1 || q == 2 ? -a : a, q & 2 ? -b : b);
+	return make_float2((q + 1) & 2 ? -a : a, q & 2 ? -b : b);
+}
+
+// 16 bytes of elements as pairs of f32, and back, rounded to nearest
+__device__ __forceinline__ void turn_get(float2 (&x)[2], const uint4 &w, float)
+{
+	x[0] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y)), x[1] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
+}
+__device__ __forceinline__ void turn_get(float2 (&x)[4], const uint4 &w, __nv_bfloat16)
+{
+	const uint32_t v[4] = { w.x, w.y, w.z, w.w };
+#pragma unroll
+	for (int i = 0; i < 4; i++) x[i] = make_float2(__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void turn_get(float2 (&x)[4], const uint4 &w, __half)
+{
+	const uint32_t v[4] = { w.x, w.y, w.z, w.w };
+#pragma unroll
+	for (int i = 0; i < 4; i++) x[i] = __half22float2(*(const __half2 *)&v[i]);
+}
+__device__ __forceinline__ uint4 turn_put(const float2 (&x)[2], float)
+{
+	return make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y));
+}
+template <class T> __device__ __forceinline__ uint4 turn_put(const float2 (&x)[4], T)
+{
+	return make_uint4(pack16(x[0].x, x[0].y, T()), pack16(x[1].x, x[1].y, T()), pack16(x[2].x, x[2].y, T()), pack16(x[3].x, x[3].y, T()));
 }
 
 enum { TURN_HALF, TURN_PAIRS, TURN_ANY }; // halves that begin at 16-byte pieces; neighbours; halves that begin anywhere
 
-// A row's norm, its inverse: the sum over the `lanes` threads that have the row's elements x.
-template <int N> __device__ __forceinline__ float turn_norm(const float (&x)[N], int lanes, float dim, float eps)
+// A row's norm, its inverse: the sum over the `lanes` threads that have the row's elements x and y.
+template <int N> __device__ __forceinline__ float turn_norm(const float2 (&x)[N], const float2 (&y)[N], int lanes, float over_dim, float eps)
 {
-	float ss = 0;
+	float2 s = make_float2(0, 0);
 #pragma unroll
-	for (int e = 0; e < N; e++) ss = fmaf(x[e], x[e], ss);
+	for (int e = 0; e < N; e++) s = fma2(x[e], x[e], fma2(y[e], y[e], s));
+	float ss = s.x + s.y;
 	for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
-	return __frsqrt_rn(ss / dim + eps);
+	return rsqrtf(fmaf(ss, over_dim, eps));
 }
 
 // a / b of numbers that nearly always fit 32 bits (a 64-bit division is a long chain of instructions)
 __device__ __forceinline__ long long over(long long a, int b) { return a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
+
+// Four weights of a norm, which may begin at any word
+__device__ __forceinline__ float4 turn_weights(const TurnRows &w, int at)
+{
+	return w.aligned ? *(const float4 *)(w.norm + at) : make_float4(w.norm[at], w.norm[at + 1], w.norm[at + 2], w.norm[at + 3]);
+}
 
 // Position of a token. (An addition past 32 bits comes round, as an angle may.)
 __device__ __forceinline__ int turn_pos(const TurnArgs &p, long long b, int i, int len)
@@ -72,11 +108,11 @@ __device__ __forceinline__ int turn_pos(const TurnArgs &p, long long b, int i, i
 // loads on their way at once. A row's threads lie in one warp, so that a row may be written where it is read.
 // What bounds it: HBM where there are many tokens, latency where there are few.
 template <class T, int FORM, bool NORM, int PART, int UN>
-__global__ void __launch_bounds__(256) k_turn(const TurnArgs p, int lg)
+__global__ void __launch_bounds__(128, NORM ? 4 : 5) k_turn(const TurnArgs p, int lg)
 {
 	constexpr int E = 16 / (int)sizeof(T);
 	const int lane = threadIdx.x & 31, lanes = 1 << lg, mine = lane & (lanes - 1), at = lane >> lg, half = p.part >> 1, n = (half + E - 1) / E, nch = p.dim / E;
-	const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), w0 = over(item, p.chunks);
+	const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), w0 = over(item, p.chunks);
 	if (w0 >= p.all) return;
 	int chunk = (int)(item - w0 * p.chunks), g = 0;
 	while (chunk >= p.rows[g].chunks) chunk -= p.rows[g++].chunks;
@@ -127,48 +163,57 @@ __global__ void __launch_bounds__(256) k_turn(const TurnArgs p, int lg)
 		for (int e = 0; e < E; e++)
 			cs[e] = make_float2(__shfl_sync(~0u, own[e % PART].x, (e / PART << lg) + mine), __shfl_sync(~0u, own[e % PART].y, (e / PART << lg) + mine));
 	}
-	float wn[2 * E];
+	float2 wx[E / 2], wy[E / 2];
 	if (NORM && w.norm) {
 #pragma unroll
-		for (int e = 0; e < 2 * E; e++) {
-			const int c = e < E ? c0 : c1;
-			wn[e] = c < nch ? w.norm[c * E + e % E] : 0;
+		for (int e = 0; e < E; e += 4) {
+			const float4 v = c0 < nch ? turn_weights(w, c0 * E + e) : make_float4(0, 0, 0, 0), y = c1 < nch ? turn_weights(w, c1 * E + e) : make_float4(0, 0, 0, 0);
+			wx[e / 2] = make_float2(v.x, v.y), wx[e / 2 + 1] = make_float2(v.z, v.w);
+			wy[e / 2] = make_float2(y.x, y.y), wy[e / 2 + 1] = make_float2(y.z, y.w);
 		}
 	}
+	const char *dst = w.dst + b * w.d_seq + i * w.d_tok, *pool = w.pool + row;
 #pragma unroll
 	for (int u = 0; u < UN; u++) {
 		const int h = h0 + (u << (5 - lg));
+		if (h - at >= w.heads) break; // the whole warp
 		const bool in = h < w.heads;
 		if (live && (w.turn || (NORM && w.norm))) { // (else the bits pass as they are)
-			float x[2 * E];
-#pragma unroll
-			for (int e = 0; e < 2 * E; e++) x[e] = PgElem<T>::get(((const T *)raw[u])[e]);
+			float2 x[E / 2], y[E / 2];
+			turn_get(x, raw[u][0], T()), turn_get(y, raw[u][1], T());
 			if constexpr (NORM) {
 				if (w.norm) {
-					const float inv = turn_norm(x, lanes, (float)p.dim, p.eps);
+					const float inv = turn_norm(x, y, lanes, p.over_dim, p.eps);
 #pragma unroll
-					for (int e = 0; e < 2 * E; e++) x[e] = x[e] * inv * wn[e];
+					for (int e = 0; e < E / 2; e++)
+						x[e] = mul2(mul2(x[e], make_float2(inv, inv)), wx[e]), y[e] = mul2(mul2(y[e], make_float2(inv, inv)), wy[e]);
 				}
 			}
 			if (turn) {
+				if constexpr (FORM == TURN_HALF) {
 #pragma unroll
-				for (int e = 0; e < E; e++) {
-					if (FORM == TURN_PAIRS && mine * E + e >= half) break; // what passes, infinities too
-					const int a = FORM == TURN_HALF ? e : 2 * e, o = FORM == TURN_HALF ? e + E : 2 * e + 1;
-					const float y = x[a], z = x[o];
-					x[a] = fmaf(y, cs[e].x, -(z * cs[e].y)), x[o] = fmaf(y, cs[e].y, z * cs[e].x);
+					for (int e = 0; e < E / 2; e++) { // two pairs at a time
+						const float2 c = make_float2(cs[2 * e].x, cs[2 * e + 1].x), s = make_float2(cs[2 * e].y, cs[2 * e + 1].y), v = x[e];
+						x[e] = fma2(y[e], make_float2(-s.x, -s.y), mul2(v, c)), y[e] = fma2(v, s, mul2(y[e], c));
+					}
+				} else {
+#pragma unroll
+					for (int e = 0; e < E; e++) {
+						if (mine * E + e >= half) break; // what passes, infinities too
+						float2 &v = e < E / 2 ? x[e] : y[e - E / 2];
+						v = make_float2(fmaf(v.x, cs[e].x, -(v.y * cs[e].y)), fmaf(v.x, cs[e].y, v.y * cs[e].x));
+					}
 				}
 			}
-#pragma unroll
-			for (int e = 0; e < 2 * E; e++) ((T *)raw[u])[e] = PgElem<T>::put(x[e]);
+			raw[u][0] = turn_put(x, T()), raw[u][1] = turn_put(y, T());
 		}
 		if (w.dst && in) {
-			char *to = w.dst + b * w.d_seq + i * w.d_tok + h * w.d_head;
+			char *to = (char *)dst + h * w.d_head;
 			if (c0 < nch) *(uint4 *)(to + c0 * 16) = raw[u][0];
 			if (c1 < nch) *(uint4 *)(to + c1 * 16) = raw[u][1];
 		}
 		if (row >= 0 && in) {
-			char *to = w.pool + row + h * p.c.head_b;
+			char *to = (char *)pool + h * p.c.head_b;
 			if (c0 < nch) *(uint4 *)(to + c0 * 16) = raw[u][0];
 			if (c1 < nch) *(uint4 *)(to + c1 * 16) = raw[u][1];
 		}
@@ -230,31 +275,22 @@ __global__ void __launch_bounds__(256) k_turn_any(const TurnArgs p, int lg, int 
 		uint4 raw[2] = {};
 		if (k.live && in0) raw[0] = *(const uint4 *)(src + c0 * 16);
 		if (k.live && in1) raw[1] = *(const uint4 *)(src + c0 * 16 + 16);
-		float x[2 * E], inv = 1;
+		float2 x[2][E / 2];
+		float inv = 1;
+		turn_get(x[0], raw[0], T()), turn_get(x[1], raw[1], T());
+		if constexpr (NORM) inv = turn_norm(x[0], x[1], lanes, p.over_dim, p.eps);
 #pragma unroll
-		for (int e = 0; e < 2 * E; e++) x[e] = PgElem<T>::get(((const T *)raw)[e]);
-		if constexpr (NORM) {
-			inv = turn_norm(x, lanes, (float)p.dim, p.eps);
-			if (w.norm) {
-#pragma unroll
-				for (int e = 0; e < 2 * E; e++) x[e] = x[e] * inv * (c0 + e / E < nch ? w.norm[c0 * E + e] : 0);
-			}
+		for (int e = 0; e < 2 * E; e++) {
+			const int el = c0 * E + e, a = el < half ? el : el - half, other = el < half ? el + half : a;
+			float &z = e % 2 ? x[e / E][e % E / 2].y : x[e / E][e % E / 2].x;
+			if (NORM && w.norm) z = z * inv * (el < p.dim ? w.norm[el] : 0);
+			if (!w.turn || !k.live || !in || el >= p.part) continue;
+			float y = PgElem<T>::get(((const T *)src)[other]);
+			if (NORM && w.norm) y = y * inv * w.norm[other];
+			const float2 v = cs[t * half + a];
+			z = fmaf(z, v.x, el < half ? -(y * v.y) : y * v.y);
 		}
-		if (w.turn && k.live && in) {
-#pragma unroll
-			for (int e = 0; e < 2 * E; e++) {
-				const int el = c0 * E + e, a = el < half ? el : el - half, other = el < half ? el + half : a;
-				if (el >= p.part) continue;
-				float y = PgElem<T>::get(((const T *)src)[other]);
-				if (NORM && w.norm) y = y * inv * w.norm[other];
-				const float2 v = cs[t * half + a];
-				x[e] = fmaf(x[e], v.x, el < half ? -(y * v.y) : y * v.y);
-			}
-		}
-		if (w.turn || (NORM && w.norm)) { // (else the bits pass as they are)
-#pragma unroll
-			for (int e = 0; e < 2 * E; e++) ((T *)raw)[e] = PgElem<T>::put(x[e]);
-		}
+		if (w.turn || (NORM && w.norm)) raw[0] = turn_put(x[0], T()), raw[1] = turn_put(x[1], T()); // (else the bits pass as they are)
 		__syncwarp(); // the row has been read
 		if (w.dst) {
 			char *to = w.dst + k.b * w.d_seq + k.i * w.d_tok + h * w.d_head + c0 * 16;
@@ -280,25 +316,32 @@ static int turn_check(const char *who, const tg_cuda_rotary *r, int head_dim, in
 	return TG_CUDA_OK;
 }
 
-constexpr int TURN_UN = 2; // rounds of a warp
+constexpr int TURN_MANY = 2048; // tokens
 
 static int turn_grid(long long blocks)
 {
 	return blocks > 0x7fffffff ? set_err(TG_CUDA_EINVAL, "rotary positions: a grid of %lld blocks", blocks) : TG_CUDA_OK;
 }
 
-template <class T, int FORM, int PART>
+template <class T, int FORM, int PART, int UN>
 static int turn_launch(TurnArgs &p, bool norm, int lg, cudaStream_t st)
 {
 	p.chunks = 0;
-	for (int g = 0; g < p.nrows; g++) p.chunks += p.rows[g].chunks = (p.rows[g].heads + (TURN_UN << (5 - lg)) - 1) / (TURN_UN << (5 - lg));
+	for (int g = 0; g < p.nrows; g++) p.chunks += p.rows[g].chunks = (p.rows[g].heads + (UN << (5 - lg)) - 1) / (UN << (5 - lg));
 	const __int128 items = (__int128)p.all * p.chunks;
-	const long long blocks = items > 0x3ffffffffll ? 0x80000000ll : (long long)(items + 7) / 8;
+	const long long blocks = items > 0x1ffffffffll ? 0x80000000ll : (long long)(items + 3) / 4;
 	if (turn_grid(blocks)) return TG_CUDA_EINVAL;
-	if (norm) k_turn<T, FORM, true, PART, TURN_UN><<<(unsigned)blocks, 256, 0, st>>>(p, lg);
-	else k_turn<T, FORM, false, PART, TURN_UN><<<(unsigned)blocks, 256, 0, st>>>(p, lg);
+	if (norm) k_turn<T, FORM, true, PART, UN><<<(unsigned)blocks, 128, 0, st>>>(p, lg);
+	else k_turn<T, FORM, false, PART, UN><<<(unsigned)blocks, 128, 0, st>>>(p, lg);
 	TGC_LAUNCH_CHECK();
 	return TG_CUDA_OK;
+}
+
+// Few tokens: two rounds a warp, for more warps
+template <class T, int FORM, int PART>
+static int turn_rounds(TurnArgs &p, bool norm, int lg, cudaStream_t st)
+{
+	return p.all < TURN_MANY ? turn_launch<T, FORM, PART, 2>(p, norm, lg, st) : turn_launch<T, FORM, PART, 4>(p, norm, lg, st);
 }
 
 template <class T, int FORM> static int turn_part(TurnArgs &p, bool norm, int lg, cudaStream_t st)
@@ -306,9 +349,9 @@ template <class T, int FORM> static int turn_part(TurnArgs &p, bool norm, int lg
 	constexpr int E = 16 / (int)sizeof(T);
 	const int part = (E << lg) / 32; // pairs that a thread computes for those of its place in other rows
 	if constexpr (E == 8) {
-		if (part == 8) return turn_launch<T, FORM, 8>(p, norm, lg, st);
+		if (part == 8) return turn_rounds<T, FORM, 8>(p, norm, lg, st);
 	}
-	return part == 4 ? turn_launch<T, FORM, 4>(p, norm, lg, st) : part == 2 ? turn_launch<T, FORM, 2>(p, norm, lg, st) : turn_launch<T, FORM, 1>(p, norm, lg, st);
+	return part == 4 ? turn_rounds<T, FORM, 4>(p, norm, lg, st) : part == 2 ? turn_rounds<T, FORM, 2>(p, norm, lg, st) : turn_rounds<T, FORM, 1>(p, norm, lg, st);
 }
 
 template <class T> static int turn_form(TurnArgs &p, int pairs, bool norm, cudaStream_t st)
@@ -371,7 +414,7 @@ extern "C" int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tok
 	if (((uintptr_t)x & 15) || ((s[0] | s[1] | s[2]) * e & 15)) return set_err(TG_CUDA_EINVAL, "%s: x rows must start on 16-byte boundaries", who);
 	if (!none && (rc = turn_out(who, "out", out, o, seqs, tokens, heads, head_dim, e))) return rc;
 	if ((rc = pg_sms(who, &dev, &sms)) || none) return rc;
-	p.rows[0] = { (const char *)x, (char *)out, nullptr, s[0] * e, s[1] * e, s[2] * e, o[0] * e, o[1] * e, o[2] * e, nullptr, heads, r->dim > 0, 0 };
+	p.rows[0] = { (const char *)x, (char *)out, nullptr, s[0] * e, s[1] * e, s[2] * e, o[0] * e, o[1] * e, o[2] * e, nullptr, heads, r->dim > 0, 0, 0 };
 	p.nrows = 1, p.all = (long long)seqs * tokens, p.tokens = tokens, p.dim = head_dim;
 	return turn_type(p, type, r->interleaved, false, stream);
 }
@@ -400,9 +443,9 @@ extern "C" int tg_cuda_kv_append(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	if (k_out && (rc = turn_out(who, "k_out", k_out, ko, c->seqs, d->tokens, c->nkv, c->head_dim, e))) return rc;
 	if ((rc = pg_apart(who, "the cache", c->head_dim, {c->page_stride, c->head_stride, c->pos_stride}, {c->pages, c->nkv, c->page}))) return rc;
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0) return rc;
-	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim, 0 };
-	p.rows[p.nrows++] = { pd.k, (char *)k_out, p.c.k, pd.kv_seq, pd.kv_tok, pd.kv_head, ko[0] * e, ko[1] * e, ko[2] * e, k_norm, c->nkv, r && r->dim, 0 };
-	p.rows[p.nrows++] = { pd.v, nullptr, p.c.v, pd.kv_seq, pd.kv_tok, pd.kv_head, 0, 0, 0, nullptr, c->nkv, 0, 0 };
-	p.count = d->count, p.len_out = len_out, p.all = (long long)c->seqs * d->tokens, p.tokens = d->tokens, p.dim = c->head_dim, p.eps = eps;
+	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim, 0, !((uintptr_t)q_norm & 15) };
+	p.rows[p.nrows++] = { pd.k, (char *)k_out, p.c.k, pd.kv_seq, pd.kv_tok, pd.kv_head, ko[0] * e, ko[1] * e, ko[2] * e, k_norm, c->nkv, r && r->dim, 0, !((uintptr_t)k_norm & 15) };
+	p.rows[p.nrows++] = { pd.v, nullptr, p.c.v, pd.kv_seq, pd.kv_tok, pd.kv_head, 0, 0, 0, nullptr, c->nkv, 0, 0, 0 };
+	p.count = d->count, p.len_out = len_out, p.all = (long long)c->seqs * d->tokens, p.tokens = d->tokens, p.dim = c->head_dim, p.over_dim = 1.f / c->head_dim, p.eps = eps;
 	return turn_type(p, c->type, r && r->interleaved, q_norm || k_norm, stream);
 }

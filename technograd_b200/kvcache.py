@@ -393,24 +393,28 @@ def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None,
     None, k rotated or None), rows past count 0; the pages are written in place. Forward only, like tree_attention."""
     d = _drafts(cache, q, k, v, None, count, 1.0)
     n, dim, index = k.shape, cache.head_dim, cache.index
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None:
-            _check(name, w, torch.float32, (dim,), index)
-    _need(q is not None or q_norm is None, "q_norm: without q")
-    _need(rotary is not None or pos is None, "pos: without a rotation")
-    r = None if rotary is None else rotary._pack(pos, n[0], n[1], index, dim)
+    qn = kn = qo = ko = qp = kp = r = None
+    sq = sk = (0, 0, 0)
+    if q_norm is not None:
+        _check("q_norm", q_norm, torch.float32, (dim,), index)
+        _need(q is not None, "q_norm: without q")
+        qn = q_norm.data_ptr()
+    if k_norm is not None:
+        _check("k_norm", k_norm, torch.float32, (dim,), index)
+        kn = k_norm.data_ptr()
+    if rotary is not None:
+        r = rotary._pack(pos, n[0], n[1], index, dim)
+    elif pos is not None:
+        raise ValueError("pos: without a rotation")
     lens = torch.empty_like(cache.lens)
-    qo, sq, ko, sk = None, (0, 0, 0), None, (0, 0, 0)
     if q is not None:
-        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
-        sq = qo.stride()
+        qo = torch.empty_like(q)
+        sq, qp = qo.stride(), qo.data_ptr()
     if keys:
         sk = k.stride()  # v's, so that the two are drafted rows together
-        ko = torch.empty_strided(n, sk, dtype=k.dtype, device=k.device) if all(x <= 1 or s for x, s in zip(n, sk)) else torch.empty_like(k, memory_format=torch.contiguous_format)
-        sk = ko.stride()
-    _lib.check(_lib.lib().tg_cuda_kv_append(cache._at, d, r, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-                                            None if qo is None else qo.data_ptr(), sq[0], sq[1], sq[2], None if ko is None else ko.data_ptr(), sk[0], sk[1], sk[2],
-                                            lens.data_ptr(), _stream(cache)))
+        ko = k.new_empty_strided(n, sk) if 0 not in sk else torch.empty_like(k)
+        sk, kp = ko.stride(), ko.data_ptr()
+    _lib.check(_lib.lib().tg_cuda_kv_append(cache._at, d, r, qn, kn, eps, qp, sq[0], sq[1], sq[2], kp, sk[0], sk[1], sk[2], lens.data_ptr(), _stream(cache)))
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
         made = [x for x in (qo, ko) if x is not None]
         if made:
