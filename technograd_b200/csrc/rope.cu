@@ -14,13 +14,14 @@ struct TurnRows {
 	long long s_seq, s_tok, s_head, d_seq, d_tok, d_head; // bytes
 	const float *norm;                 // [dim] or NULL
 	int heads, turn;
-	int chunks, aligned;               // warps that have a token's rows of this kind; norm lies on a 16-byte boundary
+	int aligned, chunks;               // norm lies on a 16-byte boundary; warps that have a token's rows of this kind
 };
 
 struct TurnArgs {
 	PgCache c;                         // table and len NULL: no cache
 	TurnRows rows[3];
-	int nrows, heads, chunks;          // of them, and all their heads and chunks
+	int nrows, heads;                  // of them, and all their heads
+	int chunks;                        // warps that have a token's rows
 	const double *freq;
 	const int *pos;
 	long long pos_seq;
@@ -83,7 +84,9 @@ template <int N> __device__ __forceinline__ float turn_norm(const float2 (&x)[N]
 #pragma unroll
 	for (int e = 0; e < N; e++) s = fma2(x[e], x[e], fma2(y[e], y[e], s));
 	float ss = s.x + s.y;
-	for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+#pragma unroll
+	for (int o = 16; o; o >>= 1)
+		if (o < lanes) ss += __shfl_xor_sync(~0u, ss, o);
 	return rsqrtf(fmaf(ss, over_dim, eps));
 }
 
@@ -105,117 +108,136 @@ __device__ __forceinline__ int turn_pos(const TurnArgs &p, long long b, int i, i
 // A warp has UN rounds of one token's rows of one kind (q, k or v): 1 << lg threads a row, each with two 16-byte pieces, those
 // that turn with each other. So a thread has the same E pairs in all its rows and keeps their cos and sin in registers; the warp's
 // threads of one place compute PART of them each and pass them round. No shared memory, no barrier, and all rounds'
-// loads on their way at once. A row's threads lie in one warp, so that a row may be written where it is read.
-// What bounds it: HBM where there are many tokens, latency where there are few.
-template <class T, int FORM, bool NORM, int PART, int UN>
-__global__ void __launch_bounds__(128, NORM ? 4 : 5) k_turn(const TurnArgs p, int lg)
+// loads on their way at once. A row's pieces are read and written by the same thread, reads first, so that a row may
+// be written where it is read. FULL: every thread of a row has two pieces.
+// What bounds it: HBM where there are many tokens, latency where there are few; with norms the instructions, about 680 a warp of four
+// rounds. Measured (bf16, 128 dimensions): 8 x 6001 tokens of 16 heads 64 us, 6.1 TB/s (117 with cos and sin in shared memory and a
+// barrier); 16 prompts of up to 2047 tokens, 16 query heads and 8 key heads normed and rotated into the cache, 109 us, 4.2 TB/s (118 with
+// all of a token's rows in one warp, which then looks up each kind's strides as it goes).
+template <class T, int FORM, bool NORM, int PART, int UN, bool FULL>
+__global__ void __launch_bounds__(128, 5) k_turn(const TurnArgs p, int lg)
 {
 	constexpr int E = 16 / (int)sizeof(T);
 	const int lane = threadIdx.x & 31, lanes = 1 << lg, mine = lane & (lanes - 1), at = lane >> lg, half = p.part >> 1, n = (half + E - 1) / E, nch = p.dim / E;
-	const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), w0 = over(item, p.chunks);
-	if (w0 >= p.all) return;
-	int chunk = (int)(item - w0 * p.chunks), g = 0;
+	const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), w = over(item, p.chunks);
+	if (w >= p.all) return;
+	int chunk = (int)(item - w * p.chunks), g = 0;
+	const bool begin = chunk == 0;
 	while (chunk >= p.rows[g].chunks) chunk -= p.rows[g++].chunks;
-	const TurnRows &w = p.rows[g];
-	const long long b = over(w0, p.tokens);
-	const int i = (int)(w0 - b * p.tokens), h0 = chunk * (UN << (5 - lg)) + at;
-	int live = 1, len = 0, cnt = p.tokens;
-	if (p.count) {
-		cnt = p.count[b];
-		live = i < cnt;
-		cnt = max(0, min(cnt, p.tokens));
-	}
-	const bool turn = w.turn && mine < n;
-	const int c0 = FORM == TURN_PAIRS ? 2 * mine : mine < n ? mine : 2 * mine, c1 = FORM == TURN_HALF && mine < n ? mine + n : c0 + 1;
-	const char *src = w.src + b * w.s_seq + i * w.s_tok;
+	const long long b = over(w, p.tokens);
+	const int i = (int)(w - b * p.tokens), h0 = chunk * (UN << (5 - lg)) + at, heads = p.rows[g].heads, turns = p.rows[g].turn;
+	const float *norm = NORM ? p.rows[g].norm : nullptr;
+	const int c0 = FORM == TURN_PAIRS ? 2 * mine : mine < n ? mine : 2 * mine, c1 = FORM == TURN_HALF && mine < n ? mine + n : c0 + 1, apart = (c1 - c0) * 16;
+	const bool have0 = FULL || c0 < nch, have1 = FULL || c1 < nch;
+	int cnt = p.tokens, len = 0;
+	if (p.count) cnt = max(0, min(p.count[b], p.tokens));
+	const bool live = i < cnt;
 	uint4 raw[UN][2];
+	{
+		const long long s_head = p.rows[g].s_head;
+		const char *src = p.rows[g].src + b * p.rows[g].s_seq + i * p.rows[g].s_tok + h0 * s_head + c0 * 16;
 #pragma unroll
-	for (int u = 0; u < UN; u++) {
-		const int h = h0 + (u << (5 - lg));
-		const bool in = live && h < w.heads;
-		raw[u][0] = in && c0 < nch ? __ldcs((const uint4 *)(src + h * w.s_head + c0 * 16)) : make_uint4(0, 0, 0, 0);
-		raw[u][1] = in && c1 < nch ? __ldcs((const uint4 *)(src + h * w.s_head + c1 * 16)) : make_uint4(0, 0, 0, 0);
+		for (int u = 0; u < UN; u++) {
+			const bool in = live && h0 + (u << (5 - lg)) < heads;
+			if (!FULL || !live) raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+			if (in && have0) raw[u][0] = __ldcs((const uint4 *)src);
+			if (in && have1) raw[u][1] = __ldcs((const uint4 *)(src + apart));
+			src += s_head << (5 - lg);
+		}
 	}
-	long long row = -1;
+	char *pool = nullptr;
 	if (p.c.len) {
 		len = p.c.length((int)b);
-		if (item == w0 * p.chunks && i == 0 && lane == 0) p.len_out[b] = len + cnt;
-		if (w.pool && live) {
+		if (begin && i == 0 && lane == 0) p.len_out[b] = len + cnt;
+		if (p.rows[g].pool && live) {
 			const long long to = (long long)len + i;
 			if (to >= (long long)p.c.page * p.c.cols || to > 0x7fffffff) p.c.report(PG_ROOM);
-			else row = p.c.row(p.c.table + b * p.c.cols, (int)to);
-		}
-	}
-	float2 cs[E];
-	if (w.turn && live) { // the whole warp
-		const int pos = turn_pos(p, b, i, len);
-		float2 own[PART];
-#pragma unroll
-		for (int x = 0; x < PART; x++) {
-			const int e = at * PART + x, a = mine * E + e;
-			own[x] = make_float2(1, 0);
-			if (e < E && a < half) {
-				own[x] = turn_of(p.freq[a], pos);
-				own[x].x *= p.gain, own[x].y *= p.inverse ? -p.gain : p.gain;
+			else {
+				const long long row = p.c.row(p.c.table + b * p.c.cols, (int)to);
+				if (row >= 0) pool = p.rows[g].pool + row + h0 * p.c.head_b + c0 * 16;
 			}
 		}
-#pragma unroll
-		for (int e = 0; e < E; e++)
-			cs[e] = make_float2(__shfl_sync(~0u, own[e % PART].x, (e / PART << lg) + mine), __shfl_sync(~0u, own[e % PART].y, (e / PART << lg) + mine));
 	}
-	float2 wx[E / 2], wy[E / 2];
-	if (NORM && w.norm) {
+	if (live && (turns || norm)) { // (else the bits pass as they are)
+		float2 c[E / 2], s[E / 2], ns[E / 2], wx[E / 2], wy[E / 2]; // two pairs' cos, sin and -sin; the pieces' weights
+		if (turns) {
+			const int pos = turn_pos(p, b, i, len);
+			float2 own[PART];
 #pragma unroll
-		for (int e = 0; e < E; e += 4) {
-			const float4 v = c0 < nch ? turn_weights(w, c0 * E + e) : make_float4(0, 0, 0, 0), y = c1 < nch ? turn_weights(w, c1 * E + e) : make_float4(0, 0, 0, 0);
-			wx[e / 2] = make_float2(v.x, v.y), wx[e / 2 + 1] = make_float2(v.z, v.w);
-			wy[e / 2] = make_float2(y.x, y.y), wy[e / 2 + 1] = make_float2(y.z, y.w);
+			for (int x = 0; x < PART; x++) {
+				const int e = at * PART + x, a = mine * E + e;
+				own[x] = make_float2(1, 0);
+				if (e < E && a < half) {
+					own[x] = turn_of(p.freq[a], pos);
+					own[x].x *= p.gain, own[x].y *= p.inverse ? -p.gain : p.gain;
+				}
+			}
+#pragma unroll
+			for (int e = 0; e < E; e += 2) {
+				const int from = (e / PART << lg) + mine, next = ((e + 1) / PART << lg) + mine;
+				c[e / 2] = make_float2(__shfl_sync(~0u, own[e % PART].x, from), __shfl_sync(~0u, own[(e + 1) % PART].x, next));
+				s[e / 2] = make_float2(__shfl_sync(~0u, own[e % PART].y, from), __shfl_sync(~0u, own[(e + 1) % PART].y, next));
+				ns[e / 2] = make_float2(-s[e / 2].x, -s[e / 2].y);
+			}
 		}
-	}
-	const char *dst = w.dst + b * w.d_seq + i * w.d_tok, *pool = w.pool + row;
+		if (norm) {
 #pragma unroll
-	for (int u = 0; u < UN; u++) {
-		const int h = h0 + (u << (5 - lg));
-		if (h - at >= w.heads) break; // the whole warp
-		const bool in = h < w.heads;
-		if (live && (w.turn || (NORM && w.norm))) { // (else the bits pass as they are)
+			for (int e = 0; e < E / 2; e += 2) {
+				const float4 v = have0 ? turn_weights(p.rows[g], c0 * E + 2 * e) : make_float4(0, 0, 0, 0), z = have1 ? turn_weights(p.rows[g], c1 * E + 2 * e) : make_float4(0, 0, 0, 0);
+				wx[e] = make_float2(v.x, v.y), wx[e + 1] = make_float2(v.z, v.w);
+				wy[e] = make_float2(z.x, z.y), wy[e + 1] = make_float2(z.z, z.w);
+			}
+		}
+		const bool turn = turns && (FULL && FORM == TURN_HALF && 2 * n == nch || mine < n);
+#pragma unroll
+		for (int u = 0; u < UN; u++) {
+			if (u && h0 - at + (u << (5 - lg)) >= heads) break; // the whole warp
 			float2 x[E / 2], y[E / 2];
 			turn_get(x, raw[u][0], T()), turn_get(y, raw[u][1], T());
-			if constexpr (NORM) {
-				if (w.norm) {
-					const float inv = turn_norm(x, y, lanes, p.over_dim, p.eps);
+			if (NORM && norm) {
+				const float inv = turn_norm(x, y, lanes, p.over_dim, p.eps);
+				const float2 two = make_float2(inv, inv);
 #pragma unroll
-					for (int e = 0; e < E / 2; e++)
-						x[e] = mul2(mul2(x[e], make_float2(inv, inv)), wx[e]), y[e] = mul2(mul2(y[e], make_float2(inv, inv)), wy[e]);
-				}
+				for (int e = 0; e < E / 2; e++) x[e] = mul2(mul2(x[e], two), wx[e]), y[e] = mul2(mul2(y[e], two), wy[e]);
 			}
 			if (turn) {
 				if constexpr (FORM == TURN_HALF) {
 #pragma unroll
-					for (int e = 0; e < E / 2; e++) { // two pairs at a time
-						const float2 c = make_float2(cs[2 * e].x, cs[2 * e + 1].x), s = make_float2(cs[2 * e].y, cs[2 * e + 1].y), v = x[e];
-						x[e] = fma2(y[e], make_float2(-s.x, -s.y), mul2(v, c)), y[e] = fma2(v, s, mul2(y[e], c));
+					for (int e = 0; e < E / 2; e++) {
+						const float2 v = x[e];
+						x[e] = fma2(y[e], ns[e], mul2(v, c[e])), y[e] = fma2(v, s[e], mul2(y[e], c[e]));
 					}
 				} else {
 #pragma unroll
 					for (int e = 0; e < E; e++) {
 						if (mine * E + e >= half) break; // what passes, infinities too
 						float2 &v = e < E / 2 ? x[e] : y[e - E / 2];
-						v = make_float2(fmaf(v.x, cs[e].x, -(v.y * cs[e].y)), fmaf(v.x, cs[e].y, v.y * cs[e].x));
+						const float cc = e % 2 ? c[e / 2].y : c[e / 2].x, ss = e % 2 ? s[e / 2].y : s[e / 2].x;
+						v = make_float2(fmaf(v.x, cc, -(v.y * ss)), fmaf(v.x, ss, v.y * cc));
 					}
 				}
 			}
 			raw[u][0] = turn_put(x, T()), raw[u][1] = turn_put(y, T());
 		}
-		if (w.dst && in) {
-			char *to = (char *)dst + h * w.d_head;
-			if (c0 < nch) *(uint4 *)(to + c0 * 16) = raw[u][0];
-			if (c1 < nch) *(uint4 *)(to + c1 * 16) = raw[u][1];
+	}
+	if (p.rows[g].dst) {
+		const long long d_head = p.rows[g].d_head;
+		char *dst = p.rows[g].dst + b * p.rows[g].d_seq + i * p.rows[g].d_tok + h0 * d_head + c0 * 16;
+#pragma unroll
+		for (int u = 0; u < UN; u++) {
+			const bool in = h0 + (u << (5 - lg)) < heads;
+			if (in && have0) *(uint4 *)dst = raw[u][0];
+			if (in && have1) *(uint4 *)(dst + apart) = raw[u][1];
+			dst += d_head << (5 - lg);
 		}
-		if (row >= 0 && in) {
-			char *to = (char *)pool + h * p.c.head_b;
-			if (c0 < nch) *(uint4 *)(to + c0 * 16) = raw[u][0];
-			if (c1 < nch) *(uint4 *)(to + c1 * 16) = raw[u][1];
+	}
+	if (pool) {
+#pragma unroll
+		for (int u = 0; u < UN; u++) {
+			const bool in = h0 + (u << (5 - lg)) < heads;
+			if (in && have0) *(uint4 *)pool = raw[u][0];
+			if (in && have1) *(uint4 *)(pool + apart) = raw[u][1];
+			pool += p.c.head_b << (5 - lg);
 		}
 	}
 }
@@ -323,7 +345,7 @@ static int turn_grid(long long blocks)
 	return blocks > 0x7fffffff ? set_err(TG_CUDA_EINVAL, "rotary positions: a grid of %lld blocks", blocks) : TG_CUDA_OK;
 }
 
-template <class T, int FORM, int PART, int UN>
+template <class T, int FORM, int PART, int UN, bool FULL>
 static int turn_launch(TurnArgs &p, bool norm, int lg, cudaStream_t st)
 {
 	p.chunks = 0;
@@ -331,8 +353,8 @@ static int turn_launch(TurnArgs &p, bool norm, int lg, cudaStream_t st)
 	const __int128 items = (__int128)p.all * p.chunks;
 	const long long blocks = items > 0x1ffffffffll ? 0x80000000ll : (long long)(items + 3) / 4;
 	if (turn_grid(blocks)) return TG_CUDA_EINVAL;
-	if (norm) k_turn<T, FORM, true, PART, UN><<<(unsigned)blocks, 128, 0, st>>>(p, lg);
-	else k_turn<T, FORM, false, PART, UN><<<(unsigned)blocks, 128, 0, st>>>(p, lg);
+	if (norm) k_turn<T, FORM, true, PART, UN, FULL><<<(unsigned)blocks, 128, 0, st>>>(p, lg);
+	else k_turn<T, FORM, false, PART, UN, FULL><<<(unsigned)blocks, 128, 0, st>>>(p, lg);
 	TGC_LAUNCH_CHECK();
 	return TG_CUDA_OK;
 }
@@ -341,7 +363,9 @@ static int turn_launch(TurnArgs &p, bool norm, int lg, cudaStream_t st)
 template <class T, int FORM, int PART>
 static int turn_rounds(TurnArgs &p, bool norm, int lg, cudaStream_t st)
 {
-	return p.all < TURN_MANY ? turn_launch<T, FORM, PART, 2>(p, norm, lg, st) : turn_launch<T, FORM, PART, 4>(p, norm, lg, st);
+	const bool full = p.dim * (int)sizeof(T) == 32 << lg;
+	if (p.all < TURN_MANY) return full ? turn_launch<T, FORM, PART, 2, true>(p, norm, lg, st) : turn_launch<T, FORM, PART, 2, false>(p, norm, lg, st);
+	return full ? turn_launch<T, FORM, PART, 4, true>(p, norm, lg, st) : turn_launch<T, FORM, PART, 4, false>(p, norm, lg, st);
 }
 
 template <class T, int FORM> static int turn_part(TurnArgs &p, bool norm, int lg, cudaStream_t st)
@@ -360,10 +384,10 @@ template <class T> static int turn_form(TurnArgs &p, int pairs, bool norm, cudaS
 	const int items = (p.dim / E + 1) / 2;
 	int lg = 0;
 	while (1 << lg < items) lg++;
-	if (pairs) return turn_part<T, TURN_PAIRS>(p, norm, lg, st);
-	if (p.part * (int)sizeof(T) % 32 == 0) return turn_part<T, TURN_HALF>(p, norm, lg, st);
 	p.heads = 0;
 	for (int g = 0; g < p.nrows; g++) p.heads += p.rows[g].heads;
+	if (pairs) return turn_part<T, TURN_PAIRS>(p, norm, lg, st);
+	if (p.part * (int)sizeof(T) % 32 == 0) return turn_part<T, TURN_HALF>(p, norm, lg, st);
 	const int per = std::max(1, std::min(8, 256 / std::min(256, p.heads << lg)));
 	const long long blocks = (p.all + per - 1) / per;
 	if (turn_grid(blocks)) return TG_CUDA_EINVAL;
@@ -443,8 +467,8 @@ extern "C" int tg_cuda_kv_append(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	if (k_out && (rc = turn_out(who, "k_out", k_out, ko, c->seqs, d->tokens, c->nkv, c->head_dim, e))) return rc;
 	if ((rc = pg_apart(who, "the cache", c->head_dim, {c->page_stride, c->head_stride, c->pos_stride}, {c->pages, c->nkv, c->page}))) return rc;
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0) return rc;
-	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim, 0, !((uintptr_t)q_norm & 15) };
-	p.rows[p.nrows++] = { pd.k, (char *)k_out, p.c.k, pd.kv_seq, pd.kv_tok, pd.kv_head, ko[0] * e, ko[1] * e, ko[2] * e, k_norm, c->nkv, r && r->dim, 0, !((uintptr_t)k_norm & 15) };
+	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim, !((uintptr_t)q_norm & 15), 0 };
+	p.rows[p.nrows++] = { pd.k, (char *)k_out, p.c.k, pd.kv_seq, pd.kv_tok, pd.kv_head, ko[0] * e, ko[1] * e, ko[2] * e, k_norm, c->nkv, r && r->dim, !((uintptr_t)k_norm & 15), 0 };
 	p.rows[p.nrows++] = { pd.v, nullptr, p.c.v, pd.kv_seq, pd.kv_tok, pd.kv_head, 0, 0, 0, nullptr, c->nkv, 0, 0, 0 };
 	p.count = d->count, p.len_out = len_out, p.all = (long long)c->seqs * d->tokens, p.tokens = d->tokens, p.dim = c->head_dim, p.over_dim = 1.f / c->head_dim, p.eps = eps;
 	return turn_type(p, c->type, r && r->interleaved, q_norm || k_norm, stream);
