@@ -9,7 +9,7 @@
 
 #include "tree_attn.cuh"
 #include "tree_attn_fma.cuh"
-#include "tree_attn_tc.cuh"
+#include "prefix_tc.cuh"
 
 namespace tgc {
 
@@ -18,6 +18,7 @@ struct SharedPlan {
 	AttnPlan pre, own;
 	int pitch;                 // entries per head of the prefixes' table
 	int dp;
+	long long least_units;     // of the prefixes: as if all rows were one group's
 	long long rows;            // seqs * tokens * heads
 	size_t tab[2], whole_o[2], whole_ml[2], part[2], bytes; // offsets: prefixes, own positions
 };
@@ -28,55 +29,74 @@ struct JoinArgs {
 	long long rows;
 };
 
-// The parts of a row, a thread for 8 columns, in the order of their CTAs: prefix first.
-template <class T, int DP>
-__global__ void __launch_bounds__(256) k_shared_join(const JoinArgs p)
+// The parts of a row, prefix first, in the order of their CTAs; a thread has a row and 8 columns. The NG warps of a block
+// take the parts in turn, each with a running reference, and the first adds up what they have, in their order: few rows of a long
+// prefix have many parts, a chain of loads for one warp.
+template <class T, int DP, int NG>
+__global__ void __launch_bounds__(32 * (NG > 1 ? NG : 8)) k_shared_join(const JoinArgs p)
 {
+	__shared__ float s[NG > 1 ? NG : 1][10][32];
 	pdl_launch();
 	pdl_wait();
 	const SharedArgs &a = p.own;
-	const long long x = (long long)blockIdx.x * 256 + threadIdx.x, row = x / (DP / 8);
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	const long long x = NG > 1 ? (long long)blockIdx.x * 32 + lane : (long long)blockIdx.x * 256 + threadIdx.x, row = min(x / (DP / 8), p.rows - 1);
 	const int col = (int)(x % (DP / 8)) * 8;
-	if (row >= p.rows) return;
-	const long long bt = row / a.d.nq;
-	const int j = (int)(row - bt * a.d.nq), b = (int)(bt / a.d.tokens), t = (int)(bt - (long long)b * a.d.tokens), h = j / a.d.group, jj = j - h * a.d.group;
+	const bool there = x / (DP / 8) < p.rows;
+	const long long bt = quotient(row, (unsigned)a.d.nq);
+	const int j = (int)(row - bt * a.d.nq), b = (int)quotient(bt, (unsigned)a.d.tokens), t = (int)(bt - (long long)b * a.d.tokens), h = j / a.d.group, jj = j - h * a.d.group;
 	float top = -INFINITY, l = 0, v[8] = {};
-	auto add = [&](float m, float n, float4 y, float4 z) {
-		const float w[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+	auto add = [&](float m, float n, const float *w) {
 		const float to = fmaxf(top, m), f = top == -INFINITY ? 0 : ex2(top - to), g = m == -INFINITY ? 0 : ex2(m - to);
 		l = (top == -INFINITY ? l : l * f) + (m == -INFINITY ? n : n * g); // sums keep a NaN
 #pragma unroll
 		for (int i = 0; i < 8; i++) v[i] = (f == 0 ? 0 : v[i] * f) + (g == 0 ? 0 : w[i] * g);
 		top = to;
 	};
-	auto parts = [&](const SharedArgs &s, int2 e, int r, int rt, int ctas) {
-		if (e.x == -1) {
-			const float *o = s.whole_o + row * DP + col;
-			const float2 ml = s.whole_ml[row];
-			add(ml.x, ml.y, *(const float4 *)o, *(const float4 *)(o + 4));
-			return;
-		}
+	// parts k of n: begins at the warp's first, which it leaves for the next list
+	int first = NG > 1 ? warp : 0;
+	auto parts = [&](const SharedArgs &q, int2 e, int r, int rt, int ctas) {
+		const bool whole = e.x == -1;
 		// (after a wait that gave up, or with groups that overlap, the entry may be anything)
-		if (e.x < 0 || e.y < e.x || e.y >= ctas) return;
+		if (!whole && (e.x < 0 || e.y < e.x || e.y >= ctas)) return;
 		const long long slot = (long long)rt * (DP + 2);
 		const int at = rt == 128 ? slot_at<DP, 128>(r, col) : slot_at<DP, 1>(r, col), next = rt == 128 ? 512 : 4;
+		const int n = whole ? 1 : e.y - e.x + 1;
 #pragma unroll 4
-		for (int i = e.x; i <= e.y; i++) {
-			const float *q = s.part + (2ll * i + (i == e.x)) * slot;
-			add(q[rt * DP + r], q[rt * DP + rt + r], *(const float4 *)(q + at), *(const float4 *)(q + at + next));
+		for (int i = first; i < n; i += NG) {
+			const float *o = whole ? q.whole_o + row * DP + col : q.part + (2ll * (e.x + i) + (i == 0)) * slot;
+			const float4 y = *(const float4 *)(whole ? o : o + at), z = *(const float4 *)(whole ? o + 4 : o + at + next);
+			const float2 ml = whole ? q.whole_ml[row] : make_float2(o[rt * DP + r], o[rt * DP + rt + r]);
+			const float w[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+			add(ml.x, ml.y, w);
 		}
+		if (NG > 1) first = (first + NG - n % NG) % NG;
 	};
-	int g, seq, m, n;
-	const int from = a.from(b, a.c.length(b), g);
-	if (g >= 0 && from > 0) {
-		p.pre.prefix(g, seq, m, n);
-		if (n > 0 && b >= seq && b - seq < m) {
-			const long long r = ((long long)(b - seq) * a.d.tokens + t) * a.d.group + jj, u = p.pre.base(g, seq, p.pre_rt) + r / p.pre_rt;
-			if (u < p.pre.pitch) parts(p.pre, p.pre.tab[(long long)h * p.pre.pitch + u], (int)(r % p.pre_rt), p.pre_rt, p.pre_ctas);
+	const int r = t * a.d.group + jj;
+	const int2 e = a.tab[((long long)b * a.c.nkv + h) * a.row_tiles + r / p.own_rt];
+	int g;
+	if (a.from(b, a.c.length(b), g) > 0) {
+		const int seq = a.first[g];
+		const long long r = ((long long)(b - seq) * a.d.tokens + t) * a.d.group + jj, u = p.pre.base(g, seq, p.pre_rt) + r / p.pre_rt;
+		if (seq >= 0 && b >= seq && u < p.pre.pitch) parts(p.pre, p.pre.tab[(long long)h * p.pre.pitch + u], (int)(r % p.pre_rt), p.pre_rt, p.pre_ctas);
+	}
+	parts(a, e, r % p.own_rt, p.own_rt, p.own_ctas);
+	if constexpr (NG > 1) {
+		if (warp) {
+			s[warp][8][lane] = top, s[warp][9][lane] = l;
+#pragma unroll
+			for (int i = 0; i < 8; i++) s[warp][i][lane] = v[i];
+		}
+		__syncthreads();
+		if (warp) return;
+		for (int k = 1; k < NG; k++) {
+			float w[8];
+#pragma unroll
+			for (int i = 0; i < 8; i++) w[i] = s[k][i][lane];
+			add(s[k][8][lane], s[k][9][lane], w);
 		}
 	}
-	const int r = t * a.d.group + jj;
-	parts(a, a.tab[((long long)b * a.c.nkv + h) * a.row_tiles + r / p.own_rt], r % p.own_rt, p.own_rt, p.own_ctas);
+	if (!there) return;
 	const AttnRow to = attn_row(a, b, h, r, a.d.drafted(b), l);
 	store_row8<T>(a, to, col, v);
 	if (col == 0) store_lse(to, top, l);
@@ -123,13 +143,27 @@ static int shared_tc(const SharedArgs &p, const AttnPlan &pl, const CUtensorMap 
 	return TG_CUDA_OK;
 }
 
+template <class T, int DP>
+static int prefix_tc(const SharedArgs &p, const AttnPlan &pl, const CUtensorMap *maps, cudaStream_t st)
+{
+	using A = PtTile<DP>;
+	static std::atomic<unsigned long long> done{0};
+	auto *kernel = k_prefix_tc<T, DP>;
+	int rc = pg_smem(kernel, A::SMEM, pl.dev, done);
+	if (rc) return rc;
+	TGC_CUDA(launch_pdl(kernel, dim3(pl.grid), dim3(A::THREADS), A::SMEM, st, p, maps[0], maps[1]));
+	return TG_CUDA_OK;
+}
+
 // One pass. maps: of the pools, where p.box has rows.
 template <int MODE, class T>
 static int shared_pass(const SharedArgs &p, const AttnPlan &pl, const CUtensorMap *maps, cudaStream_t st)
 {
 	if constexpr (sizeof(T) == 2) {
 		if (pl.tc) {
-			if (p.box.rows) return pl.dp == 128 ? shared_tc<MODE, T, 128, true>(p, pl, maps, st) : shared_tc<MODE, T, 64, true>(p, pl, maps, st);
+			if constexpr (MODE == ATTN_PREFIX) {
+				if (p.box.rows) return pl.dp == 128 ? prefix_tc<T, 128>(p, pl, maps, st) : prefix_tc<T, 64>(p, pl, maps, st);
+			} else if (p.box.rows) return pl.dp == 128 ? shared_tc<MODE, T, 128, true>(p, pl, maps, st) : shared_tc<MODE, T, 64, true>(p, pl, maps, st);
 			return pl.dp == 128 ? shared_tc<MODE, T, 128, false>(p, pl, maps, st) : shared_tc<MODE, T, 64, false>(p, pl, maps, st);
 		}
 	}
@@ -146,9 +180,11 @@ static int shared_pass(const SharedArgs &p, const AttnPlan &pl, const CUtensorMa
 }
 
 template <class T, int DP>
-static int shared_join(const JoinArgs &j, cudaStream_t st)
+static int shared_join(const JoinArgs &j, const SharedPlan &pl, cudaStream_t st)
 {
-	TGC_CUDA(launch_pdl(k_shared_join<T, DP>, dim3((unsigned)((j.rows * (DP / 8) + 255) / 256)), dim3(256), 0, st, j));
+	const long long items = j.rows * (DP / 8);
+	if (pl.pre.grid >= 4ll * pl.least_units) TGC_CUDA(launch_pdl(k_shared_join<T, DP, 8>, dim3((unsigned)((items + 31) / 32)), dim3(256), 0, st, j));
+	else TGC_CUDA(launch_pdl(k_shared_join<T, DP, 1>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, j));
 	return TG_CUDA_OK;
 }
 
@@ -158,7 +194,7 @@ int shared_type(const JoinArgs &j, const SharedPlan &pl, const CUtensorMap *maps
 {
 	int rc;
 	if ((rc = shared_pass<ATTN_PREFIX, T>(j.pre, pl.pre, maps, st)) || (rc = shared_pass<ATTN_OWN, T>(j.own, pl.own, maps, st))) return rc;
-	return pl.dp == 256 ? shared_join<T, 256>(j, st) : pl.dp == 128 ? shared_join<T, 128>(j, st) : shared_join<T, 64>(j, st);
+	return pl.dp == 256 ? shared_join<T, 256>(j, pl, st) : pl.dp == 128 ? shared_join<T, 128>(j, pl, st) : shared_join<T, 64>(j, pl, st);
 }
 
 } // namespace tgc

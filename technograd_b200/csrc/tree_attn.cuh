@@ -316,6 +316,11 @@ template <int MODE> __device__ __forceinline__ void shared_end()
 	if (MODE == ATTN_OWN) pdl_wait();
 }
 
+// A partial result's place of 4 columns of a row (then come the rows' mr and l): as the kernel that
+// leaves it writes whole lines, a row's columns together from k_tree_attn, the rows of 4 columns together
+// from the row per thread of the tiles of 128 rows and more.
+template <int DP, int RT> __device__ __forceinline__ int slot_at(int row, int col) { return RT >= 128 ? (col / 4 * RT + row) * 4 : row * DP + col; }
+
 // o (already over l, or a partial's) of 4 columns
 __device__ __forceinline__ void store4(float *d, float4 v) { *(float4 *)d = v; }
 __device__ __forceinline__ void store4(__half *d, float4 v) { *(uint2 *)d = make_uint2(pack16(v.x, v.y, __half()), pack16(v.z, v.w, __half())); }
@@ -674,11 +679,6 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 	cp_wait<0>();
 	shared_end<MODE>();
 }
-
-// A partial result's place of 4 columns of a row (then come the rows' mr and l): as the kernel that
-// leaves it writes whole lines, a row's columns together from k_tree_attn, the rows of 4 columns together
-// from the row per thread of 128-row tiles.
-template <int DP, int RT> __device__ __forceinline__ int slot_at(int row, int col) { return RT == 128 ? (col / 4 * RT + row) * 4 : row * DP + col; }
 
 // The parts of the units that several CTAs shared. A thread has a row and 8 of its columns, and the threads of a
 // warp what lies together in a part; the NG warps of a block take the parts in turn (each with a running
