@@ -1,12 +1,13 @@
 // prefix_tc.cuh -- attention over shared prefixes on tcgen05: 16-bit caches of at most 128 dimensions whose pages suit TMA boxes.
 //
 // tree_attn_tc.cuh's tiles and chain (128 rows by 128 keys, S in two buffers, P in two parts over S, an O for either half of a
-// tile's keys) for rows that see every key: no masks, no drafted rows, and a prefix ends where a box does. With that a single warp
-// fetches, and twelve warps leave the softmax threads all the registers they ask for; within a unit a tile costs no
+// tile's keys) for rows that see every key: no masks, no drafted rows, and a prefix ends where a box does. Fifteen
+// warps leave the softmax threads the registers they ask for; within a unit a tile costs no
 // look at the list of units. Warps:
 //   0-7   softmax, a query row and half of a tile's keys per thread
-//   8     fetching: K and V in boxes, a unit's Q by 16-byte cp.async. What is past a prefix's end arrives as zeros.
-//   9-11  issue of the MMAs: S, and the halves' P V. The whole warp waits and counts and one thread issues: eight MMAs take 560
+//   8-11  fetching, two warps each for K (and a unit's Q, by 16-byte cp.async) and V, half a tile's rows each. A box takes the warp
+//         that asks for it about 100 cycles: with one warp for all of them pages of 16 rows took 3700 a tile.
+//   12-14 issue of the MMAs: S, and the halves' P V. The whole warp waits and counts and one thread issues: eight MMAs take 560
 //         cycles so, 1000 where a thread does all by itself.
 #pragma once
 
@@ -20,12 +21,12 @@ struct PtBars {
 	uint64_t x_full, o_free, done;                   // per unit: mr and l exchanged, O read
 	uint32_t tmem;
 	int abort;
-	long long scan[30];
+	long long scan[36];
 	float2 ml[2][128];
 };
 
 template <int DP> struct PtTile {
-	static constexpr int TK = 128, RT = 128, NW = 12, THREADS = 32 * NW, CH = DP / 8;
+	static constexpr int TK = 128, RT = 128, NW = 15, THREADS = 32 * NW, CH = DP / 8;
 	static constexpr int OP = 128 * DP * 2; // bytes of a Q, K or V tile
 	static constexpr int NST = 3, Q = 0, K = OP, V = (1 + NST) * OP, BARS = (1 + 2 * NST) * OP;
 	static constexpr int SMEM = BARS + (int)sizeof(PtBars);
@@ -50,7 +51,7 @@ struct PtStage {
 };
 
 template <class T, int DP>
-__global__ void __launch_bounds__(384, 1) k_prefix_tc(const SharedArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
+__global__ void __launch_bounds__(480, 1) k_prefix_tc(const SharedArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
 {
 	using A = PtTile<DP>;
 	constexpr int TK = A::TK, RT = A::RT, CH = A::CH, NST = A::NST, MODE = ATTN_PREFIX;
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(384, 1) k_prefix_tc(const SharedArgs p, const 
 	}
 	if (tid == 0) {
 		for (int i = 0; i < NST; i++) {
-			mbar_init(&B->kfull[i], 32), mbar_init(&B->vfull[i], 32);
+			mbar_init(&B->kfull[i], 64), mbar_init(&B->vfull[i], 64);
 			mbar_init(&B->kfree[i], 1), mbar_init(&B->vfree[i], 2);
 		}
 		for (int i = 0; i < 2; i++) {
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(384, 1) k_prefix_tc(const SharedArgs p, const 
 	long long left_, pos, share;
 	if (!attn_share<TK, A::NW, MODE, RT>(p, B->scan, 0, c, left_, pos, share)) return; // the whole CTA
 	int left = __shfl_sync(~0u, (int)left_, 0);
-	if (warp == 9) tmem_alloc(&B->tmem, 512); // S buffers at columns 0 and 128, the halves' O at 256 and 256 + DP
+	if (warp == 12) tmem_alloc(&B->tmem, 512); // S buffers at columns 0 and 128, the halves' O at 256 and 256 + DP
 	tc_fence_before();
 	__syncthreads();
 	tc_fence_after();
@@ -93,13 +94,14 @@ __global__ void __launch_bounds__(384, 1) k_prefix_tc(const SharedArgs p, const 
 		cursor_next<TK, MODE, RT>(p, c, 0);
 	};
 
-	if (warp == 8) {
+	if (warp >= 8 && warp < 12) {
 		// ---------------- fetching ----------------
 		constexpr int RI = 32 / CH, ND = DP / 64; // rows an instruction copies; boxes side by side
-		const int ch = lane % CH, rows_of = p.box.rows, boxes = 128 / rows_of * ND, box = lane / ND * rows_of; // this lane's box: its first row
-		const bool mine = lane < boxes, piece = ch < p.c.dim / 8;
-		const uint32_t sm0 = smem_u32(sm), to = sm0 + lane % ND * 16384 + box * 128;
-		const uint32_t d0 = sm0 + A::Q + (uint32_t)((ch >> 3) * 16384 + lane / CH * 128), x0 = (uint32_t)((ch & 7) ^ (lane / CH)) << 4;
+		const int isv = warp - 8 >> 1, half = warp & 1, ch = lane % CH, rows_of = p.box.rows, box = half * 64 + lane / ND * rows_of; // this lane's box: its first row
+		const bool mine = lane < 64 / rows_of * ND, piece = ch < p.c.dim / 8;
+		const uint32_t sm0 = smem_u32(sm), to = sm0 + (isv ? A::V : A::K) + lane % ND * 16384 + box * 128;
+		const uint32_t d0 = sm0 + A::Q + (uint32_t)((ch >> 3) * 16384 + (half * 64 + lane / CH) * 128), x0 = (uint32_t)((ch & 7) ^ (lane / CH)) << 4;
+		uint64_t *const full = isv ? B->vfull : B->kfull, *const free = isv ? B->vfree : B->kfree;
 		PtStage st;
 		int j = 0;
 		bool ok = true;
@@ -117,34 +119,27 @@ __global__ void __launch_bounds__(384, 1) k_prefix_tc(const SharedArgs p, const 
 			for (int k = 0; k < n; k++, j++) {
 				if (page != -1 && (unsigned)page >= (unsigned)p.c.pages) p.c.report(PG_PAGE), page = -1;
 				int row1 = 0;
-				const int r = page < 0 ? 0 : row, g = page, next = k + 1 < n ? page_of(c.tile + k + 1, row1) : -1; // looked up before this tile is waited for
-				for (int v = 0; v < 2; v++) {
-					uint64_t *full = (v ? B->vfull : B->kfull) + st.at;
-					if (j >= NST && !(ok = ta_wait(B, (v ? B->vfree : B->kfree) + st.at, st.parity ^ 1, p.c))) break;
-					if (lane == 0) ta_expect(full, A::OP);
-					__syncwarp();
-					if (mine)
-						ta_box(to + (v ? A::V : A::K) + st.at * A::OP, v ? &vmap : &kmap, full, lane % ND * 64, p.box.swap ? h : r, p.box.swap ? r : h, g);
-					if (!v && k == 0) { // the unit's Q, once the last S of the unit before is done
-						if (j > 0 && !(ok = ta_wait(B, &B->kfree[(j - 1) % NST], (j - 1) / NST & 1, p.c))) {
-							cp_arrive(full);
-							break;
-						}
-						const char *qb = p.d.q + (long long)c.seq * p.d.q_seq + (long long)h * p.d.group * p.d.q_head + ch * 16;
+				const int r = page < 0 ? 0 : row, next = k + 1 < n ? page_of(c.tile + k + 1, row1) : -1; // looked up before this tile is waited for
+				if (j >= NST && !(ok = ta_wait(B, &free[st.at], st.parity ^ 1, p.c))) break;
+				if (lane == 0) ta_expect(&full[st.at], A::OP / 2);
+				__syncwarp();
+				if (mine) ta_box(to + st.at * A::OP, isv ? &vmap : &kmap, &full[st.at], lane % ND * 64, p.box.swap ? h : r, p.box.swap ? r : h, page < 0 ? -1 : page);
+				if (!isv && k == 0) { // the unit's Q, once the last S of the unit before is done
+					ok = j == 0 || ta_wait(B, &B->kfree[(j - 1) % NST], (j - 1) / NST & 1, p.c);
+					const char *qb = p.d.q + (long long)c.seq * p.d.q_seq + (long long)h * p.d.group * p.d.q_head + ch * 16;
 #pragma unroll 1
-						for (int i = 0; i < 4; i++) {
-							const int x = c.r * RT + i * 32 + lane, t = x / p.d.group, m = t / p.d.tokens;
-							const unsigned long long place = x < c.rows ? (unsigned long long)((long long)m * p.d.q_seq + (long long)(t - m * p.d.tokens) * p.d.q_tok + (long long)(x - t * p.d.group) * p.d.q_head) : ~0ull;
+					for (int i = 0; ok && i < 2; i++) {
+						const int x = c.r * RT + half * 64 + i * 32 + lane, t = x / p.d.group, m = t / p.d.tokens;
+						const unsigned long long place = x < c.rows ? (unsigned long long)((long long)m * p.d.q_seq + (long long)(t - m * p.d.tokens) * p.d.q_tok + (long long)(x - t * p.d.group) * p.d.q_head) : ~0ull;
 #pragma unroll 4
-							for (int y = 0; y < CH; y++) {
-								const unsigned long long o = __shfl_sync(~0u, place, y * RI + lane / CH);
-								const bool have = o != ~0ull && piece;
-								cp16(d0 + (i * 32 + y * RI) * 128 + (x0 ^ ((y * RI & 7) << 4)), qb + (have ? o : 0), have);
-							}
+						for (int y = 0; y < CH; y++) {
+							const unsigned long long o = __shfl_sync(~0u, place, y * RI + lane / CH);
+							const bool have = o != ~0ull && piece;
+							cp16(d0 + (i * 32 + y * RI) * 128 + (x0 ^ ((y * RI & 7) << 4)), qb + (have ? o : 0), have);
 						}
 					}
-					cp_arrive(full);
 				}
+				cp_arrive(&full[st.at]);
 				if (!ok) break;
 				st.next();
 				page = next, row = row1;
@@ -153,17 +148,14 @@ __global__ void __launch_bounds__(384, 1) k_prefix_tc(const SharedArgs p, const 
 		}
 		cp_commit();
 		cp_wait<0>();
-		// boxes still on their way land before the CTA's shared memory is released (after an abort tile j's K may be one of them)
-		for (int i = max(0, j - NST); i < j + !ok; i++) {
-			mbar_wait(&B->kfull[i % NST], i / NST & 1, nullptr, 0);
-			if (i < j) mbar_wait(&B->vfull[i % NST], i / NST & 1, nullptr, 0);
-		}
-	} else if (warp >= 9) {
+		// boxes still on their way land before the CTA's shared memory is released (after an abort tile j's may be among them)
+		for (int i = max(0, j - NST); i < j + !ok; i++) mbar_wait(&full[i % NST], i / NST & 1, nullptr, 0);
+	} else if (warp >= 12) {
 		// ---------------- MMA issue ----------------
 		const uint32_t id = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(RT >> 4) << 24); // f32 += f16 or bf16 products
 		const uint32_t base = smem_u32(sm);
 		PtStage st;
-		if (warp == 9) {
+		if (warp == 12) {
 			const uint32_t idS = id | ((uint32_t)(TK >> 3) << 17);
 			const uint64_t qd = sw128_kmajor_desc(base + A::Q);
 			for (int j = 0; j < left; j++, st.next()) {
@@ -185,7 +177,7 @@ __global__ void __launch_bounds__(384, 1) k_prefix_tc(const SharedArgs p, const 
 				__syncwarp();
 			}
 		} else {
-			const int f = warp - 10; // the half of the tile's keys
+			const int f = warp - 13; // the half of the tile's keys
 			const uint32_t idO = id | ((uint32_t)(DP >> 3) << 17) | (1u << 16), o = tmem + 256 + f * DP; // V MN-major
 			int j = 0, unit = 0;
 			bool ok = true;
@@ -329,7 +321,7 @@ __global__ void __launch_bounds__(384, 1) k_prefix_tc(const SharedArgs p, const 
 	}
 	tc_fence_before();
 	__syncthreads();
-	if (warp == 9) {
+	if (warp == 12) {
 		tc_fence_after();
 		tmem_dealloc(tmem, 512);
 	}

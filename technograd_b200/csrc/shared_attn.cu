@@ -42,7 +42,7 @@ static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, 
 	p.slot = (size_t)(rt * p.dp + 2 * rt) * 4;
 	const long long shares = (units * (tiles + p.begin) + p.least + p.begin - 1) / (p.least + p.begin), wave = (long long)p.sms * (p.tc || p.dp == 256 ? 1 : p.mt == 1 && c->type != TG_CUDA_F32 ? 3 : 2);
 	p.grid = (int)std::min(shares, wave), p.units = (int)units, p.row_tiles = 1;
-	o->least_units = (rows + rt - 1) / rt * c->nkv, o->pitch = (int)pitch, o->rows = rows * c->nkv;
+	o->least_units = std::max((rows + rt - 1) / rt, (long long)x->groups) * c->nkv, o->pitch = (int)pitch, o->rows = rows * c->nkv;
 	size_t at = 0;
 	auto take = [&](size_t n) { const size_t was = at; at = (at + n + 255) / 256 * 256; return was; };
 	for (int i = 0; i < 2; i++) {

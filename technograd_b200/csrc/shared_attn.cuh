@@ -18,7 +18,7 @@ struct SharedPlan {
 	AttnPlan pre, own;
 	int pitch;                 // entries per head of the prefixes' table
 	int dp;
-	long long least_units;     // of the prefixes: as if all rows were one group's
+	long long least_units;     // of the prefixes: the groups, or their rows if they filled whole tiles
 	long long rows;            // seqs * tokens * heads
 	size_t tab[2], whole_o[2], whole_ml[2], part[2], bytes; // offsets: prefixes, own positions
 };
@@ -183,7 +183,7 @@ template <class T, int DP>
 static int shared_join(const JoinArgs &j, const SharedPlan &pl, cudaStream_t st)
 {
 	const long long items = j.rows * (DP / 8);
-	if (pl.pre.grid >= 4ll * pl.least_units) TGC_CUDA(launch_pdl(k_shared_join<T, DP, 8>, dim3((unsigned)((items + 31) / 32)), dim3(256), 0, st, j));
+	if (pl.pre.grid >= 4 * pl.least_units) TGC_CUDA(launch_pdl(k_shared_join<T, DP, 8>, dim3((unsigned)((items + 31) / 32)), dim3(256), 0, st, j));
 	else TGC_CUDA(launch_pdl(k_shared_join<T, DP, 1>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, j));
 	return TG_CUDA_OK;
 }
