@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(480, 1) k_prefix_tc(const SharedArgs p, const 
 	extern __shared__ __align__(1024) uint8_t ta_raw[];
 	uint8_t *sm = ta_raw;
 	PtBars *B = (PtBars *)(sm + A::BARS);
+	static_assert(sizeof(B->scan) / 8 >= 2 * A::NW + 6, "attn_share's words");
 	const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
 	if (smem_u32(sm) & 1023) { // the operand tiles need 1024-byte alignment
 		if (tid == 0) p.c.report(PG_WAIT);

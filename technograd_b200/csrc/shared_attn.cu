@@ -20,6 +20,16 @@ static int shared_check(const char *who, const tg_cuda_kv *c, const tg_cuda_pref
 	return TG_CUDA_OK;
 }
 
+// What the sequences have of their own is often short, and a 128-row tile's chain is long: up to 64 rows take two 32-row tiles instead where
+// there are few tiles in all. The whole call, us, 32-row against 128-row tiles (8 key heads of 128 dimensions, 42 rows, bf16, a prefix of 1024):
+// 30.5 and 32.9 at 0.9 tiles an SM, 43.5 and 45.6 at 2.2, 65.7 and 78.2 at 4.3, 83.8 and 87.4 at 11, 157 and 188 at 13.8 (units of two
+// tiles), but 67.6 and 60 at 14.3 (units of 33), 108 and 98 at 19, 190 and 182 at 21. 128 rows: 53.5 and 50 at 2.2.
+constexpr int SHARED_MMA_ROWS = 64, SHARED_MMA_TILES = 14;
+
+// Units of a CTA each where there are few of them; CTAs of many waves would each wait for their first loads, and those of one
+// wave, with equal shares of all units, fetch the next unit while they work on one.
+constexpr int SHARED_WAVES = 1;
+
 // Nothing is shared: tree attention itself.
 static bool shared_none(const tg_cuda_kv *c, const tg_cuda_prefix *x) { return !c->seqs || !x->groups || !x->max_shared; }
 
@@ -29,18 +39,23 @@ static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, 
 	tail.max_len = std::min(c->max_len, x->max_own);
 	int rc = attn_plan(who, &tail, d, &o->own);
 	if (rc) return rc;
+	if (o->own.tc && d.tokens * d.group <= SHARED_MMA_ROWS && (long long)o->own.units * ((tail.max_len + 127) / 128 + 1) <= (long long)SHARED_MMA_TILES * o->own.sms &&
+	    (rc = attn_plan(who, &tail, d, &o->own, false)))
+		return rc;
+	if (o->own.whole && o->own.units > SHARED_WAVES * o->own.wave) o->own.whole = 0, o->own.grid = o->own.wave;
 	AttnPlan &p = o->pre;
 	p = {};
 	p.dev = o->own.dev, p.sms = o->own.sms, o->dp = p.dp = o->own.dp;
 	const long long rows = (long long)c->seqs * d.tokens * d.group;
 	p.tc = c->type != TG_CUDA_F32 && p.dp <= 128;
 	p.mt = rows <= 16 || p.dp == 256 ? 1 : 2;
-	const int rt = p.tc ? 128 : 16 * p.mt, tk = p.tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
+	p.fma = c->type == TG_CUDA_F32 && rows <= 8 ? rows <= 4 ? 4 : 8 : 0;
+	const int rt = p.tc ? 128 : p.fma ? p.fma : 16 * p.mt, tk = p.tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
 	const long long pitch = rows / rt + x->groups + 1, units = c->nkv * pitch, tiles = ((long long)x->max_shared + tk - 1) / tk;
 	if (units > 0x7fffffff || rows * c->nkv > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
 	p.least = 128 / tk, p.begin = p.tc && units * tiles > 7ll * p.sms ? 6 : 2;
 	p.slot = (size_t)(rt * p.dp + 2 * rt) * 4;
-	const long long shares = (units * (tiles + p.begin) + p.least + p.begin - 1) / (p.least + p.begin), wave = (long long)p.sms * (p.tc || p.dp == 256 ? 1 : p.mt == 1 && c->type != TG_CUDA_F32 ? 3 : 2);
+	const long long shares = (units * (tiles + p.begin) + p.least + p.begin - 1) / (p.least + p.begin), wave = (long long)p.sms * (p.tc || p.dp == 256 ? 1 : p.fma || (p.mt == 1 && c->type != TG_CUDA_F32) ? 3 : 2);
 	p.grid = (int)std::min(shares, wave), p.units = (int)units, p.row_tiles = 1;
 	o->least_units = std::max((rows + rt - 1) / rt, (long long)x->groups) * c->nkv, o->pitch = (int)pitch, o->rows = rows * c->nkv;
 	size_t at = 0;

@@ -74,9 +74,10 @@ __global__ void __launch_bounds__(32 * (NG > 1 ? NG : 8)) k_shared_join(const Jo
 	};
 	const int r = t * a.d.group + jj;
 	const int2 e = a.tab[((long long)b * a.c.nkv + h) * a.row_tiles + r / p.own_rt];
-	int g;
-	if (a.from(b, a.c.length(b), g) > 0) {
-		const int seq = a.first[g];
+	int g, n;
+	if (a.from(b, n, g) > 0) {
+		const int seq = a.first[g], m = a.members[g];
+		if (seq < 0 || b < seq || b - seq >= m || m > a.seqs - seq) a.c.report(PG_GROUP);
 		const long long r = ((long long)(b - seq) * a.d.tokens + t) * a.d.group + jj, u = p.pre.base(g, seq, p.pre_rt) + r / p.pre_rt;
 		if (seq >= 0 && b >= seq && u < p.pre.pitch) parts(p.pre, p.pre.tab[(long long)h * p.pre.pitch + u], (int)(r % p.pre_rt), p.pre_rt, p.pre_ctas);
 	}
@@ -114,12 +115,12 @@ static int shared_mma(const SharedArgs &p, const AttnPlan &pl, cudaStream_t st)
 	return TG_CUDA_OK;
 }
 
-template <int DP, int R>
+template <int MODE, int DP, int R>
 static int shared_fma(const SharedArgs &p, const AttnPlan &pl, cudaStream_t st)
 {
 	using A = FmaTile<DP, R>;
 	static std::atomic<unsigned long long> done{0};
-	auto *kernel = k_tree_attn_fma<DP, R, ATTN_OWN>;
+	auto *kernel = k_tree_attn_fma<DP, R, MODE>;
 	int rc = pg_smem(kernel, A::SMEM, pl.dev, done);
 	if (rc) return rc;
 	TGC_CUDA(launch_pdl(kernel, dim3(pl.grid), dim3(128), A::SMEM, st, p));
@@ -167,9 +168,9 @@ static int shared_pass(const SharedArgs &p, const AttnPlan &pl, const CUtensorMa
 			return pl.dp == 128 ? shared_tc<MODE, T, 128, false>(p, pl, maps, st) : shared_tc<MODE, T, 64, false>(p, pl, maps, st);
 		}
 	}
-	if constexpr (MODE == ATTN_OWN && sizeof(T) == 4) {
-		if (pl.fma == 4) return pl.dp == 256 ? shared_fma<256, 4>(p, pl, st) : pl.dp == 128 ? shared_fma<128, 4>(p, pl, st) : shared_fma<64, 4>(p, pl, st);
-		if (pl.fma == 8) return pl.dp == 256 ? shared_fma<256, 8>(p, pl, st) : pl.dp == 128 ? shared_fma<128, 8>(p, pl, st) : shared_fma<64, 8>(p, pl, st);
+	if constexpr (sizeof(T) == 4) {
+		if (pl.fma == 4) return pl.dp == 256 ? shared_fma<MODE, 256, 4>(p, pl, st) : pl.dp == 128 ? shared_fma<MODE, 128, 4>(p, pl, st) : shared_fma<MODE, 64, 4>(p, pl, st);
+		if (pl.fma == 8) return pl.dp == 256 ? shared_fma<MODE, 256, 8>(p, pl, st) : pl.dp == 128 ? shared_fma<MODE, 128, 8>(p, pl, st) : shared_fma<MODE, 64, 8>(p, pl, st);
 	}
 	if (pl.dp == 256) return shared_mma<MODE, T, 256, 1>(p, pl, st);
 	if constexpr (MODE == ATTN_OWN || sizeof(T) == 4) {

@@ -23,14 +23,14 @@ constexpr int ATTN_TC_ROWS = 32, ATTN_TC_ROWS_LONG = 16, ATTN_LONG = 24;
 // 19; 96, 78.7, 80.8, 84 at 42; 212, 206, 200, 200 at 125.
 constexpr int ATTN_BEGIN = 2, ATTN_TC_BEGIN = 6, ATTN_TC_SHORT = 7;
 
-int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o)
+int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o, bool wide)
 {
 	int rc = pg_sms(who, &o->dev, &o->sms);
 	if (rc) return rc;
 	const int rows = d.tokens * d.group;
 	o->dp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
-	const long long wide = (long long)c->seqs * c->nkv * ((c->max_len + 127) / 128 + 1); // the 128-row tiles, where one has all rows
-	o->tc = c->type != TG_CUDA_F32 && o->dp <= 128 && rows > (wide > (long long)ATTN_LONG * o->sms ? ATTN_TC_ROWS_LONG : ATTN_TC_ROWS);
+	const long long tiles128 = (long long)c->seqs * c->nkv * ((c->max_len + 127) / 128 + 1); // the 128-row tiles, where one has all rows
+	o->tc = wide && c->type != TG_CUDA_F32 && o->dp <= 128 && rows > (tiles128 > (long long)ATTN_LONG * o->sms ? ATTN_TC_ROWS_LONG : ATTN_TC_ROWS);
 	o->mt = rows <= 16 || o->dp == 256 ? 1 : 2; // 256 dimensions of 32 rows do not fit in registers
 	o->fma = c->type == TG_CUDA_F32 && rows <= 8 ? rows <= 4 ? 4 : 8 : 0;
 	const int rt = o->tc ? 128 : o->fma ? o->fma : 16 * o->mt, tk = o->tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
@@ -42,7 +42,7 @@ int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan 
 	o->slot = (size_t)(rt * o->dp + 2 * rt) * 4;
 	const long long shares = (units * (tiles + o->begin) + o->least + o->begin - 1) / (o->least + o->begin), wave = (long long)o->sms * (o->tc || o->dp == 256 ? 1 : o->fma || (o->mt == 1 && c->type != TG_CUDA_F32) ? 3 : 2); // the tiles' CTAS
 	o->grid = (int)(o->whole ? units : shares < wave ? shares : wave);
-	o->units = (int)units, o->by_unit = !o->whole && units <= o->grid;
+	o->wave = (int)wave, o->units = (int)units, o->by_unit = !o->whole && units <= o->grid;
 	return TG_CUDA_OK;
 }
 

@@ -50,17 +50,18 @@ struct SharedArgs : AttnArgs {
 	int2 *tab;       // [units]: the first and last CTA of a unit, x = -1: one CTA had it all
 	int pitch;       // prefixes: entries of tab per head
 
-	// positions that sequence b of n positions shares with its group, g: the group
-	__device__ __forceinline__ int from(int b, int n, int &g) const
+	// Sequence b's positions n, and how many of them it shares with its group g (-1: none). The length and the group are read at
+	// once: each further load in a row would be another half of a microsecond before a unit begins.
+	__device__ __forceinline__ int from(int b, int &n, int &g) const
 	{
+		const int len = c.len[b];
 		g = group[b];
-		if ((unsigned)g >= (unsigned)groups) {
-			if (g != -1) c.report(PG_GROUP);
-			g = -1;
-			return 0;
-		}
-		const int s = shared[g], f = first[g];
-		if (s < 0 || s > max_shared || s > n || b < f || b - f >= members[g]) c.report(PG_GROUP);
+		const bool in = (unsigned)g < (unsigned)groups;
+		const int s = in ? shared[g] : 0;
+		if (len < 0 || len > c.max_len) c.report(PG_LEN);
+		n = max(0, min(len, c.max_len));
+		if (s < 0 || s > max_shared || s > n || (!in && g != -1)) c.report(PG_GROUP);
+		if (!in) g = -1;
 		return max(0, min(s, min(n, max_shared))) & -align;
 	}
 	// the sequences of group g and their shared positions
@@ -114,7 +115,7 @@ template <class T, int DP, int MT> struct AttnTile {
 	static constexpr int CTAS = DP == 256 ? 1 : MT == 1 && sizeof(T) == 2 ? 3 : 2;
 	static constexpr int NST = CTAS == 3 || DP == 256 || (DP == 128 && MT == 2 && sizeof(T) == 4) ? 2 : 3;
 	static constexpr int Q = 0, RING = RT * P, MASK = RING + 4 * NST * STAGE, ML = MASK + RT * 8, SCAN = ML + 4 * RT * 8;
-	static constexpr int SMEM = SCAN + 128;
+	static constexpr int SMEM = SCAN + 128; // attn_share: 2 * 4 + 6 words
 	static constexpr int SLOT = RT * DP + 2 * RT; // floats of a partial result
 };
 
@@ -134,12 +135,14 @@ __device__ __forceinline__ void cursor_seq(const AttnArgsOf<MODE> &p, AttnCursor
 		c.rows = m * p.d.tokens * p.d.group, c.tiles = (c.rows + RT - 1) / RT;
 		c.ctx = c.all = (int)(((long long)c.n + TK - 1) / TK);
 	} else {
-		c.n = p.c.length(c.b);
 		if constexpr (MODE == ATTN_OWN) {
 			int g;
 			c.p0 = p.from(c.b, c.n, g);
 			c.ctx = (int)(((long long)c.n - c.p0 + TK - 1) / TK);
-		} else c.ctx = (int)(((long long)c.n + TK - 1) / TK);
+		} else {
+			c.n = p.c.length(c.b);
+			c.ctx = (int)(((long long)c.n + TK - 1) / TK);
+		}
 		c.all = c.ctx + extra;
 	}
 }
@@ -738,13 +741,13 @@ __global__ void __launch_bounds__(32 * NG) k_attn_join(const AttnArgs p)
 
 // How a call is cut.
 struct AttnPlan {
-	int dp, mt, row_tiles, whole, least, begin, grid, by_unit, units, sms, dev, tc, fma; // fma: rows of tree_attn_fma.cuh, 0: another kernel; mt: 16-row products of a tile; tc: 128-row tiles on tcgen05
+	int dp, mt, row_tiles, whole, least, begin, grid, wave, by_unit, units, sms, dev, tc, fma; // wave: CTAs that run at once; fma: rows of tree_attn_fma.cuh, 0: another kernel; mt: 16-row products of a tile; tc: 128-row tiles on tcgen05
 	size_t slot; // bytes of a partial result
 	size_t bytes() const { return whole ? 0 : (size_t)grid * (2 * slot + sizeof(int4)); }
 };
 
-// tree_attn.cu: the cut of a call whose sequences have at most c->max_len positions.
-int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o);
+// tree_attn.cu: the cut of a call whose sequences have at most c->max_len positions; wide: 128-row tiles may be taken.
+int attn_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, AttnPlan *o, bool wide = true);
 
 // Launches a planned call; T is the element type.
 template <class T> int attn_type(const AttnArgs &p, const AttnPlan &pl, cudaStream_t st);

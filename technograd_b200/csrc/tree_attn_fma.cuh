@@ -20,14 +20,13 @@ template <int DP, int R> struct FmaTile {
 	static constexpr int STAGE = 2 * KW * P; // also R x DP floats, what the end of a unit needs
 	static constexpr int CTAS = DP == 256 ? 1 : 3, NST = 2;
 	static constexpr int Q = 0, RING = RT * P, MASK = RING + 4 * NST * STAGE, ML = MASK + RT * 8, SCAN = ML + 4 * RT * 8;
-	static constexpr int SMEM = SCAN + 64;
+	static constexpr int SMEM = SCAN + 128; // attn_share: 2 * 4 + 6 words
 	static constexpr int SLOT = RT * DP + 2 * RT;
 };
 
 template <int DP, int R, int MODE = ATTN_ALL>
 __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(const AttnArgsOf<MODE> p)
 {
-	static_assert(MODE != ATTN_PREFIX, "rows of one sequence only");
 	using A = FmaTile<DP, R>;
 	constexpr int KW = A::KW, TK = A::TK, P = A::P, CH = A::CH, NST = A::NST, NP = DP / 64; // NP: pairs of a lane's dimensions
 	constexpr float RAISE = AttnScale<float>::RAISE;
@@ -36,7 +35,8 @@ __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(con
 	float2 *s_ml = (float2 *)(smem + A::ML);
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
 	const uint32_t ring = smem_u32(smem) + A::RING + warp * NST * A::STAGE;
-	const int extra = (p.d.tokens + TK - 1) / TK, rows = p.d.tokens * p.d.group, chunks = p.c.dim / 4;
+	const int extra = MODE == ATTN_PREFIX ? 0 : (p.d.tokens + TK - 1) / TK, chunks = p.c.dim / 4;
+	int rows = p.d.tokens * p.d.group;
 	const float zs = p.d.scale * 1.4426950408889634f;
 	if constexpr (MODE == ATTN_ALL) {
 		pdl_launch();
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(con
 	} else shared_begin<MODE>();
 	AttnCursor c;
 	long long left, pos, share;
-	if (!attn_share<TK, 4, MODE>(p, (long long *)(smem + A::SCAN), extra, c, left, pos, share)) {
+	if (!attn_share<TK, 4, MODE, R>(p, (long long *)(smem + A::SCAN), extra, c, left, pos, share)) {
 		shared_end<MODE>();
 		return;
 	}
@@ -60,15 +60,17 @@ __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(con
 		if (first) { // a unit begins here, or goes on from the CTA before
 			first = false;
 			from_start = c.tile == 0;
-			cnt = p.d.drafted(c.b);
+			if constexpr (MODE == ATTN_PREFIX) rows = c.rows;
+			else cnt = p.d.drafted(c.b);
 			for (int x = tid; x < R * CH; x += 128) {
 				const int row = x / CH, ch = x % CH, r = c.r * R + row, t = r / p.d.group;
 				float4 v = make_float4(0, 0, 0, 0);
-				if (r < rows && ch < chunks)
+				if (MODE == ATTN_PREFIX && r < rows && ch < chunks) v = *(const float4 *)(q_row(p, shared_row<MODE>(p, c, r)) + ch * 16);
+				else if (r < rows && ch < chunks)
 					v = *(const float4 *)(p.d.q + (long long)c.b * p.d.q_seq + (long long)t * p.d.q_tok + (long long)(c.h * p.d.group + r - t * p.d.group) * p.d.q_head + ch * 16);
 				*(float4 *)(smem + row * P + ch * 16) = v;
 			}
-			if (tid < R) {
+			if (MODE != ATTN_PREFIX && tid < R) {
 				const int t = (c.r * R + tid) / p.d.group;
 				s_mask[tid] = t < cnt ? p.d.sees(c.b, t, cnt) : 0;
 			}
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(128, FmaTile<DP, R>::CTAS) k_tree_attn_fma(con
 		}
 		__syncwarp(); // every lane is done with this stage
 		stage = (stage + 1) % NST;
-		cursor_next<TK, MODE>(p, c, extra);
+		cursor_next<TK, MODE, R>(p, c, extra);
 	}
 	cp_wait<0>();
 	shared_end<MODE>();

@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgsOf<MODE> 
 	extern __shared__ __align__(1024) uint8_t ta_raw[];
 	uint8_t *sm = ta_raw;
 	TaBars *B = (TaBars *)(sm + A::BARS);
+	static_assert(sizeof(B->scan) / 8 >= 2 * A::NW + 6, "attn_share's words");
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 	if (smem_u32(sm) & 1023) { // the operand tiles need 1024-byte alignment
 		if (tid == 0) p.c.report(PG_WAIT);

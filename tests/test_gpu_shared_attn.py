@@ -91,6 +91,17 @@ def test_many_groups(cuda, dtype, dim):
     check(Shared(own, groups, 1, 2, dim, 16, "head", dtype, 2))
 
 
+@pytest.mark.parametrize("dim", [4, 64, 68, 128, 256])
+@pytest.mark.parametrize("members,tokens,group", [(1, 1, 1), (2, 1, 2), (2, 2, 2), (3, 1, 3), (4, 1, 2), (2, 4, 1), (8, 1, 1), (9, 1, 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_rows_in_all(cuda, dtype, dim, members, tokens, group):
+    """1 to 9 rows a key head of all sequences together: f32 takes the FMA units up to 8."""
+    if dtype is BF16 and dim % 8:
+        return
+    for pages in (1, 9, 130):
+        check(Shared([7, 0, 40, 1, 2, 3, 90, 5, 6][:members], [(0, members, pages, pages * 16)], 2, group, dim, 16, "pos", dtype, tokens))
+
+
 @pytest.mark.parametrize("max_own", [0, 1, 10 ** 6])
 @pytest.mark.parametrize("dtype,tokens", [(F32, 1), (BF16, 1), (BF16, 30)])
 def test_max_own_is_a_hint(cuda, max_own, dtype, tokens):
