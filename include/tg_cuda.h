@@ -419,13 +419,14 @@ typedef struct {
 	int groups;              /* at most seqs */
 	int max_shared;          /* upper bound of shared, at most max_len */
 	int max_own;
+	int always;              /* 0: where reading the prefixes for each sequence is faster (few sequences, short prefixes), that is done; 1: never */
 	const int *first, *members, *shared; /* [groups] */
 	const int *group;        /* [seqs] */
 } tg_cuda_prefix;
 
 /* The results of tg_cuda_tree_attn, for all that its description says, with the prefixes' rows read once for the rows of a whole
- * group instead of once for each sequence. (What does not share goes its usual way; with groups 0 the call is
- * tg_cuda_tree_attn.) work: as there, tg_cuda_shared_attn_workspace bytes. */
+ * group instead of once for each sequence. (What does not share goes its usual way. Where sharing costs more than it saves, by the host's
+ * numbers alone, and with groups 0, the call is tg_cuda_tree_attn.) work: as there, tg_cuda_shared_attn_workspace bytes. */
 long long tg_cuda_shared_attn_workspace(const tg_cuda_kv *c, const tg_cuda_drafts *d, const tg_cuda_prefix *x);
 int tg_cuda_shared_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, const tg_cuda_prefix *x, void *out, long long out_seq,
 			long long out_tok, long long out_head, float *lse, void *work, long long work_bytes, void *stream);

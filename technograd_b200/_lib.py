@@ -123,7 +123,7 @@ class Drafts(C.Structure):
 
 
 class Prefix(C.Structure):
-    _fields_ = [("groups", C.c_int), ("max_shared", C.c_int), ("max_own", C.c_int), ("first", C.c_void_p), ("members", C.c_void_p),
+    _fields_ = [("groups", C.c_int), ("max_shared", C.c_int), ("max_own", C.c_int), ("always", C.c_int), ("first", C.c_void_p), ("members", C.c_void_p),
                 ("shared", C.c_void_p), ("group", C.c_void_p)]
 
 

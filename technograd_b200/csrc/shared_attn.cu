@@ -12,8 +12,9 @@ extern template int shared_type<__nv_bfloat16>(const JoinArgs &, const SharedPla
 static int shared_check(const char *who, const tg_cuda_kv *c, const tg_cuda_prefix *x)
 {
 	if (!x) return set_err(TG_CUDA_EINVAL, "%s: NULL prefixes", who);
-	if (x->groups < 0 || x->groups > c->seqs || x->max_shared < 0 || x->max_shared > c->max_len || x->max_own < 0)
-		return set_err(TG_CUDA_EINVAL, "%s: %d groups of %d sequences, at most %d positions shared and %d not, of %d", who, x->groups, c->seqs, x->max_shared, x->max_own, c->max_len);
+	if (x->groups < 0 || x->groups > c->seqs || x->max_shared < 0 || x->max_shared > c->max_len || x->max_own < 0 || x->always & ~1)
+		return set_err(TG_CUDA_EINVAL, "%s: %d groups of %d sequences, at most %d positions shared and %d not, of %d (always %d)", who, x->groups, c->seqs, x->max_shared, x->max_own,
+			       c->max_len, x->always);
 	if (x->groups && (!x->first || !x->members || !x->shared || !x->group)) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer in the prefixes", who);
 	if (((uintptr_t)x->first | (uintptr_t)x->members | (uintptr_t)x->shared | (uintptr_t)x->group) & 3)
 		return set_err(TG_CUDA_EINVAL, "%s: a pointer of the prefixes is not on a 4-byte boundary", who);
@@ -30,8 +31,23 @@ constexpr int SHARED_MMA_ROWS = 64, SHARED_MMA_TILES = 14;
 // wave, with equal shares of all units, fetch the next unit while they work on one.
 constexpr int SHARED_WAVES = 1;
 
-// Nothing is shared: tree attention itself.
-static bool shared_none(const tg_cuda_kv *c, const tg_cuda_prefix *x) { return !c->seqs || !x->groups || !x->max_shared; }
+// Whether tree attention itself does it: nothing is shared, or reading a prefix for each sequence takes less time than two passes and
+// their join. What each takes, from the bytes of keys and values it reads (as if all sequences had the longest prefix): tree
+// attention 1 us for 8.5 MB (many of them from L2, since the sequences' tables name the same pages); here 5 us more to begin with, 1 for 4.5 MB, 20 ns
+// a unit of a sequence and key head, and for f32 33 ns for each million operations of split products. Measured, us, here and tree attention
+// (8 key heads of 128 dimensions, two query heads each, 65 positions of their own; bf16 unless f32): 4 sequences below 1024 positions 18.9 and
+// 15.6, below 4096 19.9 and 19.6; 8 below 1024 19.1 and 16.7, below 2048 18.9 and 20.2; 16 below 512 18.5 and 16.8, below 1024 18.7 and 22.0; 64 below 256 30.6 and
+// 28.0, below 1024 35.5 and 51.1; 64 in 32 groups below 2048 68 and 62, below 4096 95 and 107; f32: 4 below 4096 30 and 30, 16 below 1024 44 and 31,
+// below 2048 47 and 55, 64 below 512 56 and 73.
+static bool shared_tree(const tg_cuda_kv *c, const PgDrafts &d, const tg_cuda_prefix *x)
+{
+	if (!c->seqs || !x->groups || !x->max_shared) return true;
+	if (x->always) return false;
+	const double row = 2.0 * c->nkv * c->head_dim * pg_size(c->type), own = (double)c->seqs * std::min(x->max_own, c->max_len) * row;
+	const double all = own + (double)c->seqs * x->max_shared * row, once = own + (double)x->groups * x->max_shared * row;
+	const double products = c->type == TG_CUDA_F32 ? 4.0 * c->seqs * d.tokens * d.nq * c->head_dim * x->max_shared : 0;
+	return all / 8.5e6 < 5 + once / 4.5e6 + 0.02 * c->seqs * c->nkv + products * 33e-9; // us
+}
 
 static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, const tg_cuda_prefix *x, SharedPlan *o)
 {
@@ -46,10 +62,10 @@ static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, 
 	AttnPlan &p = o->pre;
 	p = {};
 	p.dev = o->own.dev, p.sms = o->own.sms, o->dp = p.dp = o->own.dp;
-	const long long rows = (long long)c->seqs * d.tokens * d.group;
+	const long long rows = (long long)c->seqs * d.tokens * d.group, each = (rows + x->groups - 1) / x->groups; // each: a group's, about
 	p.tc = c->type != TG_CUDA_F32 && p.dp <= 128;
-	p.mt = rows <= 16 || p.dp == 256 ? 1 : 2;
-	p.fma = c->type == TG_CUDA_F32 && rows <= 8 ? rows <= 4 ? 4 : 8 : 0;
+	p.mt = each <= 16 || p.dp == 256 ? 1 : 2;
+	p.fma = c->type == TG_CUDA_F32 && each <= 8 ? each <= 4 ? 4 : 8 : 0;
 	const int rt = p.tc ? 128 : p.fma ? p.fma : 16 * p.mt, tk = p.tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
 	const long long pitch = rows / rt + x->groups + 1, units = c->nkv * pitch, tiles = ((long long)x->max_shared + tk - 1) / tk;
 	if (units > 0x7fffffff || rows * c->nkv > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
@@ -82,7 +98,7 @@ extern "C" long long tg_cuda_shared_attn_workspace(const tg_cuda_kv *c, const tg
 	SharedPlan pl;
 	int rc;
 	if ((rc = pg_cache(who, c, &pc)) || (rc = pg_drafts(who, c, d, PG_USE_Q | PG_USE_K | PG_USE_V, 64, &pd)) || (rc = shared_check(who, c, x))) return rc;
-	if (shared_none(c, x)) return tg_cuda_tree_attn_workspace(c, d);
+	if (shared_tree(c, pd, x)) return tg_cuda_tree_attn_workspace(c, d);
 	if ((rc = shared_plan(who, c, pd, x, &pl))) return rc;
 	return (long long)pl.bytes;
 }
@@ -97,7 +113,7 @@ extern "C" int tg_cuda_shared_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d,
 	SharedPlan pl;
 	int rc, sms;
 	if ((rc = pg_cache(who, c, &p.c)) || (rc = pg_drafts(who, c, d, PG_USE_Q | PG_USE_K | PG_USE_V, 64, &p.d)) || (rc = shared_check(who, c, x))) return rc;
-	if (shared_none(c, x)) return tg_cuda_tree_attn(c, d, out, out_seq, out_tok, out_head, lse, work, work_bytes, stream);
+	if (shared_tree(c, p.d, x)) return tg_cuda_tree_attn(c, d, out, out_seq, out_tok, out_head, lse, work, work_bytes, stream);
 	const int e = pg_size(c->type);
 	if (!out || !lse) return set_err(TG_CUDA_EINVAL, "%s: NULL output", who);
 	if (c->seqs <= 1) out_seq = 0; // strides along one element are not used

@@ -194,9 +194,10 @@ class SharedPrefix:
 
     groups: (first sequence, sequences, shared positions) of each, ascending; sequences in none share nothing. The tables of a group's sequences
     name the same pages for the shared positions. max_own: about how many positions a sequence has at most behind what it
-    shares (default: what max_len leaves); it only sizes the launches, and the lengths may grow past it."""
+    shares (default: what max_len leaves); it only sizes the launches, and the lengths may grow past it. always: share even where
+    tree_attention's way, a prefix read for each sequence, is faster (few sequences, short prefixes)."""
 
-    def __init__(self, cache: PagedKV, groups, max_own: int | None = None):
+    def __init__(self, cache: PagedKV, groups, max_own: int | None = None, always: bool = False):
         groups = [tuple(int(x) for x in g) for g in groups]
         end, which = 0, [-1] * cache.seqs
         for i, (first, members, shared) in enumerate(groups):
@@ -214,7 +215,7 @@ class SharedPrefix:
         made = torch.tensor([g[0] for g in groups] + [g[1] for g in groups] + lengths + which, dtype=torch.int32).to(cache.device)
         n, at = len(groups), made.data_ptr()
         self._held = made
-        self._struct = _lib.Prefix(n, self.max_shared, max_own, at, at + 4 * n, at + 8 * n, at + 12 * n)
+        self._struct = _lib.Prefix(n, self.max_shared, max_own, bool(always), at, at + 4 * n, at + 8 * n, at + 12 * n)
         self._at = C.addressof(self._struct)
 
 

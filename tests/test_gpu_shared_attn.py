@@ -30,7 +30,7 @@ class Shared(Case):
                 self.k[b][:pages * page], self.v[b][:pages * page] = self.k[first][:pages * page], self.v[first][:pages * page]
         self.table = table.cuda()
         self.cache = kvcache.PagedKV(self.pk, self.pv, self.table, self.len, max_len=max(lens))
-        self.prefix = kvcache.SharedPrefix(self.cache, [(f, m, s) for f, m, _, s in groups], max_own=max(own) if max_own is None else max_own)
+        self.prefix = kvcache.SharedPrefix(self.cache, [(f, m, s) for f, m, _, s in groups], max_own=max(own) if max_own is None else max_own, always=True)
 
 
 def run(c, mask=None, count=None, **kw):
@@ -153,9 +153,22 @@ def test_same_as_without_sharing(cuda):
     c.prefix = kvcache.SharedPrefix(c.cache, [])
     none = run(c)
     assert torch.equal(none[0], want[0]) and torch.equal(none[1], want[1])
-    c.prefix = kvcache.SharedPrefix(c.cache, [(0, 9, 0)])
+    c.prefix = kvcache.SharedPrefix(c.cache, [(0, 9, 0)], always=True)
     none = run(c)
     assert torch.equal(none[0], want[0]) and torch.equal(none[1], want[1])
+    c.prefix = kvcache.SharedPrefix(c.cache, [(f, m, s) for f, m, _, s in GROUPS])  # so small that sharing costs more
+    none = run(c)
+    assert torch.equal(none[0], want[0]) and torch.equal(none[1], want[1])
+
+
+@pytest.mark.parametrize("dtype,seqs,pages", [(BF16, 40, 130), (F32, 24, 200), (F16, 8, 300)])
+def test_where_sharing_pays(cuda, dtype, seqs, pages):
+    """Without being told to, and with the same bits as when told."""
+    c = Shared([b % 50 for b in range(seqs)], [(0, seqs, pages, pages * 16)], 8, 2, 128, 16, "head", dtype, 1)
+    want = check(c)
+    c.prefix = kvcache.SharedPrefix(c.cache, [(0, seqs, pages * 16)], max_own=49)
+    got = run(c)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
 def test_strides_and_scale(cuda):
@@ -237,7 +250,7 @@ def test_device_data_that_does_not_suit_is_reported(cuda):
     for name, values in (("shared", [65, 48]), ("shared", [-5, 48]), ("shared", [2 ** 31 - 1, -2 ** 31]), ("first", [0, 1]), ("first", [-1, 2]), ("first", [10 ** 6, 2]),
                          ("members", [2, 3]), ("members", [2 ** 31 - 1, 2]), ("members", [-7, 2]), ("members", [1, 2]), ("group", [0, 0, 2, 1]), ("group", [-2, 0, 1, 1]),
                          ("group", [1, 0, 0, 1])):
-        x = kvcache.SharedPrefix(c.cache, [(0, 2, 64), (2, 2, 48)])
+        x = kvcache.SharedPrefix(c.cache, [(0, 2, 64), (2, 2, 48)], always=True)
         x._held[fields[name]:fields[name] + len(values)] = torch.tensor(values, dtype=torch.int32, device="cuda")
         kvcache.shared_attention(c.cache, x, q, k, v)
         assert "group of sequences" in reported(good), (name, values)
@@ -292,7 +305,7 @@ def test_a_decode_step_together(cuda):
     lens, _, _ = kvcache.append(one, k[:1, :half], v[:1, :half], rotary=rotary, k_norm=norms["k_norm"])
     assert lens.tolist() == [half]
     cache = kvcache.PagedKV(*pools, table.cuda(), lens.expand(B).contiguous(), max_len=half)
-    prefix = kvcache.SharedPrefix(cache, [(0, B, half)], max_own=T + 3 - half)
+    prefix = kvcache.SharedPrefix(cache, [(0, B, half)], max_own=T + 3 - half, always=True)
     lens, _, _ = kvcache.append(cache, k[:, half:T], v[:, half:T], rotary=rotary, k_norm=norms["k_norm"])
     outs = []
     for t in range(T, T + 3):

@@ -41,7 +41,7 @@ def test_bad_drafts(bad):
 
 
 @pytest.mark.parametrize("bad", [dict(groups=-1), dict(groups=3), dict(max_shared=-1), dict(max_shared=61), dict(max_own=-1), dict(first=0), dict(members=0), dict(shared=0),
-                                 dict(group=0), dict(first=0x8002), dict(members=0x8101), dict(shared=0x8203), dict(group=0x8302)])
+                                 dict(group=0), dict(first=0x8002), dict(members=0x8101), dict(shared=0x8203), dict(group=0x8302), dict(always=2), dict(always=-1)])
 def test_bad_prefixes(bad):
     refused(size(x=prefix(**bad)))
     refused(attend(x=prefix(**bad)))
@@ -49,9 +49,9 @@ def test_bad_prefixes(bad):
 
 @pytest.mark.parametrize("bad", [dict(out=(0, 768, 256, 64)), dict(out=(0x60008, 768, 256, 64)), dict(out=(0x60000, 768, 252, 64)), dict(out=(0x60000, 0, 256, 64)),
                                  dict(out=(0x60000, 512, 256, 64)), dict(out=(0x60000, 768, 256, -64)), dict(lse=None), dict(lse=0x70002)])
-@pytest.mark.parametrize("groups", [0, 1])
-def test_bad_outputs(bad, groups):
-    refused(attend(x=prefix(groups=groups), **bad))
+@pytest.mark.parametrize("kw", [dict(groups=0), dict(always=0), dict(always=1)])
+def test_bad_outputs(bad, kw):
+    refused(attend(x=prefix(**kw), **bad))
 
 
 def test_null():
