@@ -49,6 +49,29 @@ static bool shared_tree(const tg_cuda_kv *c, const PgDrafts &d, const tg_cuda_pr
 	return all / 8.5e6 < 5 + once / 4.5e6 + 0.02 * c->seqs * c->nkv + products * 33e-9; // us
 }
 
+// The two passes follow one another, each on all SMs, or run next to each other, the prefixes on some SMs and the own positions on the rest
+// (their CTAs do not fit on one SM, and the second pass's begin wherever the first's are not): then the shorter one's beginning, 8 us or more
+// of looking things up, fetching and a first chain of products, costs nothing. What each is reckoned to take, in us of an SM: 2 a
+// prefix's tile; of own positions 0.77 a tile of 16 rows by 64 keys, 1.2 of 32 rows, 1.5 of 128 rows by 128 keys, a unit's beginning counting as 3
+// tiles or 6, and lengths as half of their bound. The constants are those that chose best over 119 shapes whose times differ (8 to 256
+// sequences, 1 to 24 tokens, prefixes of 1024 to 16384, up to 1024 own positions): 1.8% slower than the better of both each time, where always next
+// to each other is 2.5% and always one after the other 13.7%. E.g. (us, next to each other and one after the other) 64 sequences of up
+// to 513 positions behind 2048 shared ones 35 and 45, with 16 SMs for the prefix (40 with 8, 46 with 64); 8 of 200 behind 131008 71 and 87, with 140;
+// 256 of up to 1024 in 6 groups of up to 8000 176 and 158; 256 of 64 in 8 groups behind 16384 100 and 76.
+static void shared_split(AttnPlan &pre, AttnPlan &own, int own_len)
+{
+	const double tiles = 0.5 * own_len / (own.tc ? 128 : 64); // (own_len is a bound)
+	const double wo = own.units * (own.tc ? (tiles + 6) * 1.5 : (tiles + 3) * (own.mt == 1 ? 0.77 : 1.2)), wp = pre.units * 2.0;
+	auto next_to = [&](int n) { return std::max(9 + wp / n, 8 + wo / (pre.sms - n)); };
+	int n = 1;
+	while (n + 1 < pre.sms && next_to(n + 1) <= next_to(n)) n++;
+	if (next_to(n) >= 0.9 * (17 + (wp + wo) / pre.sms) || n >= pre.grid) return;
+	const int rest = (pre.sms - n) * (own.wave / own.sms);
+	pre.grid = n;
+	if (own.units > rest) own.whole = 0, own.grid = rest;
+	else if (own.grid > rest) own.grid = rest;
+}
+
 static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, const tg_cuda_prefix *x, SharedPlan *o)
 {
 	tg_cuda_kv tail = *c;
@@ -73,6 +96,12 @@ static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, 
 	p.slot = (size_t)(rt * p.dp + 2 * rt) * 4;
 	const long long shares = (units * (tiles + p.begin) + p.least + p.begin - 1) / (p.least + p.begin), wave = (long long)p.sms * (p.tc || p.dp == 256 ? 1 : p.fma || (p.mt == 1 && c->type != TG_CUDA_F32) ? 3 : 2);
 	p.grid = (int)std::min(shares, wave), p.units = (int)units, p.row_tiles = 1;
+	if (p.tc) {
+		AttnPlan reckoned = p;
+		reckoned.units = (int)std::min<long long>(tiles * std::max((rows + rt - 1) / rt, (long long)x->groups) * c->nkv, 0x7fffffff); // tiles of all units
+		shared_split(reckoned, o->own, tail.max_len);
+		p.grid = reckoned.grid;
+	}
 	o->least_units = std::max((rows + rt - 1) / rt, (long long)x->groups) * c->nkv, o->pitch = (int)pitch, o->rows = rows * c->nkv;
 	size_t at = 0;
 	auto take = [&](size_t n) { const size_t was = at; at = (at + n + 255) / 256 * 256; return was; };
