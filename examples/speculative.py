@@ -1,6 +1,6 @@
 """Speculative decoding over a paged key/value cache of bounded size, with the operators of
 technograd_b200.kvcache: a toy decoder (random weights) drafts trees of tokens from the bigrams it has
-seen, checks each tree in one pass (tree_attention), keeps the longest path that its own greedy
+seen, checks each tree in one pass (rope to the drafted positions, tree_attention), keeps the longest path that its own greedy
 choices confirm (commit), sums up the attention each cached position receives (attention_weights),
 and drops the least attended ones when the cache is full (evict).
 
@@ -29,6 +29,7 @@ class Toy:
     def __init__(self, layers=2, hidden=64, nq=4, nkv=2, dim=32, vocab=64, seed=0):
         g = torch.Generator(device="cuda").manual_seed(seed)
         self.layers, self.nq, self.nkv, self.dim, self.vocab = layers, nq, nkv, dim, vocab
+        self.rotary = kvcache.Rotary(dim, theta=1e4)
 
         def w(*s):
             return torch.randn(s, generator=g, device="cuda") * s[0] ** -0.5
@@ -43,18 +44,12 @@ class Toy:
         def norm(x):
             return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)
 
-        half = self.dim // 2
-        angle = positions[..., None, None] * 1e4 ** (-torch.arange(half, device="cuda") / half)
-
-        def rotate(x):
-            a, b = x[..., :half], x[..., half:]
-            return torch.cat([a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()], -1)
-
+        at = positions.to(torch.int32).contiguous()
         x = self.embed[tokens]
         for i, p in enumerate(self.blocks):
             qkv = (norm(x) @ p["qkv"]).unflatten(-1, (-1, self.dim))
             q, k, v = qkv.split([self.nq, self.nkv, self.nkv], 2)
-            x = x + attend(i, rotate(q), rotate(k), v.contiguous()).flatten(2) @ p["out"]
+            x = x + attend(i, kvcache.rope(q, self.rotary, at), kvcache.rope(k, self.rotary, at), v.contiguous()).flatten(2) @ p["out"]
             h = norm(x)
             x = x + (torch.nn.functional.silu(h @ p["gate"]) * (h @ p["up"])) @ p["down"]
         return norm(x) @ self.head

@@ -20,7 +20,7 @@ struct TurnRows {
 struct TurnArgs {
 	PgCache c;                         // table and len NULL: no cache
 	TurnRows rows[3];
-	int nrows, heads;                  // of them, and all their heads
+	int nrows;
 	int chunks;                        // warps that have a token's rows
 	const double *freq;
 	const int *pos;
@@ -75,7 +75,8 @@ template <class T> __device__ __forceinline__ uint4 turn_put(const float2 (&x)[4
 	return make_uint4(pack16(x[0].x, x[0].y, T()), pack16(x[1].x, x[1].y, T()), pack16(x[2].x, x[2].y, T()), pack16(x[3].x, x[3].y, T()));
 }
 
-enum { TURN_HALF, TURN_PAIRS, TURN_ANY }; // halves that begin at 16-byte pieces; neighbours; halves that begin anywhere
+enum { TURN_HALF, TURN_PAIRS }; // halves that begin at 16-byte pieces; neighbours
+constexpr int TURN_ANY_ROWS = 4; // rows of a warp in k_turn_any
 
 // A row's norm, its inverse: the sum over the `lanes` threads that have the row's elements x and y.
 template <int N> __device__ __forceinline__ float turn_norm(const float2 (&x)[N], const float2 (&y)[N], int lanes, float over_dim, float eps)
@@ -242,87 +243,97 @@ __global__ void __launch_bounds__(128, 5) k_turn(const TurnArgs p, int lg)
 	}
 }
 
-struct TurnToken {
-	long long b, row; // its sequence, and its cache row in bytes (-1: none)
-	int i, live;
-};
-
-// Halves that begin within a 16-byte piece: elements find their partners one by one in the row, which the first read has
-// brought near. A block has `per` tokens and their cos and sin in shared memory.
-template <class T, bool NORM>
-__global__ void __launch_bounds__(256) k_turn_any(const TurnArgs p, int lg, int per_)
+// Halves that begin within a 16-byte piece: a warp a row, element by element. A thread has the pairs lane, lane + 32, ... of a row
+// (behind the rotated part, neighbours), and so the same in all rows of one kind that the warp has. NI: pairs of a thread.
+// What bounds it: the instructions of 2-byte loads and stores. Measured: 16 x 2000 tokens of 16 heads of 128 dimensions, 100 of them
+// rotated, bf16 88 us, f32 95 us (114 and 169 with whole pieces whose elements look their partners up one by one).
+template <class T, bool NORM, int NI>
+__global__ void __launch_bounds__(128) k_turn_any(const TurnArgs p)
 {
-	constexpr int E = 16 / (int)sizeof(T);
-	extern __shared__ __align__(16) float2 cs[]; // [per][half]
-	__shared__ TurnToken tok[8];
-	const int tid = threadIdx.x, lanes = 1 << lg, half = p.part >> 1, nch = p.dim / E;
-	const long long t0 = (long long)blockIdx.x * per_;
-	const int per = (int)min((long long)per_, p.all - t0);
-	if (tid < per) {
-		TurnToken k;
-		k.b = (t0 + tid) / p.tokens, k.i = (int)(t0 + tid - k.b * p.tokens), k.live = 1, k.row = -1;
-		int cnt = p.tokens;
-		if (p.count) {
-			cnt = p.count[k.b];
-			k.live = k.i < cnt;
-			cnt = max(0, min(cnt, p.tokens));
+	const int lane = threadIdx.x & 31, half = p.part >> 1, pairs = p.dim / 2;
+	const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), w = over(item, p.chunks);
+	if (w >= p.all) return;
+	int chunk = (int)(item - w * p.chunks), g = 0;
+	const bool begin = chunk == 0;
+	while (chunk >= p.rows[g].chunks) chunk -= p.rows[g++].chunks;
+	const TurnRows &k = p.rows[g];
+	const long long b = over(w, p.tokens);
+	const int i = (int)(w - b * p.tokens), first = chunk * TURN_ANY_ROWS, last = min(k.heads, first + TURN_ANY_ROWS);
+	int cnt = p.tokens, len = 0;
+	if (p.count) cnt = max(0, min(p.count[b], p.tokens));
+	const bool live = i < cnt;
+	long long row = -1;
+	if (p.c.len) {
+		len = p.c.length((int)b);
+		if (begin && i == 0 && lane == 0) p.len_out[b] = len + cnt;
+		if (k.pool && live) {
+			const long long to = (long long)len + i;
+			if (to >= (long long)p.c.page * p.c.cols || to > 0x7fffffff) p.c.report(PG_ROOM);
+			else row = p.c.row(p.c.table + b * p.c.cols, (int)to);
 		}
-		if (p.c.len) {
-			const int len = p.c.length((int)k.b);
-			const long long at = (long long)len + k.i;
-			if (k.i == 0) p.len_out[k.b] = len + cnt;
-			if (k.live) {
-				if (at >= (long long)p.c.page * p.c.cols || at > 0x7fffffff) p.c.report(PG_ROOM);
-				else k.row = p.c.row(p.c.table + k.b * p.c.cols, (int)at);
+	}
+	int one[NI], two[NI]; // the elements of a pair, -1: none
+	float2 cs[NI], norm[NI];
+#pragma unroll
+	for (int n = 0; n < NI; n++) {
+		const int a = n * 32 + lane;
+		one[n] = a >= pairs ? -1 : a < half ? a : 2 * a;
+		two[n] = a < half ? a + half : 2 * a + 1;
+		cs[n] = make_float2(1, 0), norm[n] = make_float2(1, 1);
+		if (k.turn && live && a < half) {
+			cs[n] = turn_of(p.freq[a], turn_pos(p, b, i, len));
+			cs[n].x *= p.gain, cs[n].y *= p.inverse ? -p.gain : p.gain;
+		}
+		if (NORM && k.norm && one[n] >= 0) norm[n] = make_float2(k.norm[one[n]], k.norm[two[n]]);
+	}
+	const char *src = k.src + b * k.s_seq + i * k.s_tok;
+	char *dst = k.dst + b * k.d_seq + i * k.d_tok, *pool = k.pool + row;
+	T rows_x[TURN_ANY_ROWS][NI], rows_y[TURN_ANY_ROWS][NI]; // all on their way at once
+#pragma unroll
+	for (int r = 0; r < TURN_ANY_ROWS; r++) {
+		const T *s = (const T *)(src + (first + r) * k.s_head);
+#pragma unroll
+		for (int n = 0; n < NI; n++) {
+			rows_x[r][n] = rows_y[r][n] = PgElem<T>::put(0);
+			if (live && first + r < last && one[n] >= 0) rows_x[r][n] = s[one[n]], rows_y[r][n] = s[two[n]];
+		}
+	}
+#pragma unroll
+	for (int r = 0; r < TURN_ANY_ROWS; r++) {
+		const int h = first + r;
+		if (h >= last) break;
+		T(&x)[NI] = rows_x[r], (&y)[NI] = rows_y[r];
+		if (live && (k.turn || (NORM && k.norm))) { // (else the bits pass as they are)
+			float u[NI], v[NI], inv = 1;
+#pragma unroll
+			for (int n = 0; n < NI; n++) u[n] = PgElem<T>::get(x[n]), v[n] = PgElem<T>::get(y[n]);
+			if (NORM && k.norm) {
+				float ss = 0;
+#pragma unroll
+				for (int n = 0; n < NI; n++) ss = fmaf(u[n], u[n], fmaf(v[n], v[n], ss));
+#pragma unroll
+				for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+				inv = rsqrtf(fmaf(ss, p.over_dim, p.eps));
+			}
+#pragma unroll
+			for (int n = 0; n < NI; n++) {
+				if (NORM && k.norm) u[n] = u[n] * inv * norm[n].x, v[n] = v[n] * inv * norm[n].y;
+				const float a = u[n], z = v[n];
+				if (n * 32 + lane < half) u[n] = fmaf(a, cs[n].x, -(z * cs[n].y)), v[n] = fmaf(a, cs[n].y, z * cs[n].x); // (what passes does, infinities too)
+				x[n] = PgElem<T>::put(u[n]), y[n] = PgElem<T>::put(v[n]);
 			}
 		}
-		tok[tid] = k;
-	}
-	for (int x = tid; x < per * half; x += 256) {
-		const long long w = t0 + x / half, b = w / p.tokens;
-		float2 v = turn_of(p.freq[x % half], turn_pos(p, b, (int)(w - b * p.tokens), p.c.len ? p.c.length((int)b) : 0));
-		v.x *= p.gain, v.y *= p.inverse ? -p.gain : p.gain;
-		cs[x] = v;
-	}
-	__syncthreads();
-	const int mine = tid & (lanes - 1), c0 = 2 * mine, total = per * p.heads;
-	for (int r0 = 0; r0 < total; r0 += 256 >> lg) {
-		const int r = r0 + (tid >> lg), t = min(r, total - 1) / p.heads;
-		int h = min(r, total - 1) - t * p.heads, g = 0;
-		while (h >= p.rows[g].heads) h -= p.rows[g++].heads;
-		const TurnRows &w = p.rows[g];
-		const TurnToken k = tok[t];
-		const bool in = r < total, in0 = in && c0 < nch, in1 = in && c0 + 1 < nch;
-		const char *src = w.src + k.b * w.s_seq + k.i * w.s_tok + h * w.s_head;
-		uint4 raw[2] = {};
-		if (k.live && in0) raw[0] = *(const uint4 *)(src + c0 * 16);
-		if (k.live && in1) raw[1] = *(const uint4 *)(src + c0 * 16 + 16);
-		float2 x[2][E / 2];
-		float inv = 1;
-		turn_get(x[0], raw[0], T()), turn_get(x[1], raw[1], T());
-		if constexpr (NORM) inv = turn_norm(x[0], x[1], lanes, p.over_dim, p.eps);
+		if (k.dst) {
+			T *to = (T *)(dst + h * k.d_head);
 #pragma unroll
-		for (int e = 0; e < 2 * E; e++) {
-			const int el = c0 * E + e, a = el < half ? el : el - half, other = el < half ? el + half : a;
-			float &z = e % 2 ? x[e / E][e % E / 2].y : x[e / E][e % E / 2].x;
-			if (NORM && w.norm) z = z * inv * (el < p.dim ? w.norm[el] : 0);
-			if (!w.turn || !k.live || !in || el >= p.part) continue;
-			float y = PgElem<T>::get(((const T *)src)[other]);
-			if (NORM && w.norm) y = y * inv * w.norm[other];
-			const float2 v = cs[t * half + a];
-			z = fmaf(z, v.x, el < half ? -(y * v.y) : y * v.y);
+			for (int n = 0; n < NI; n++)
+				if (one[n] >= 0) to[one[n]] = x[n], to[two[n]] = y[n];
 		}
-		if (w.turn || (NORM && w.norm)) raw[0] = turn_put(x[0], T()), raw[1] = turn_put(x[1], T()); // (else the bits pass as they are)
-		__syncwarp(); // the row has been read
-		if (w.dst) {
-			char *to = w.dst + k.b * w.d_seq + k.i * w.d_tok + h * w.d_head + c0 * 16;
-			if (in0) *(uint4 *)to = k.live ? raw[0] : make_uint4(0, 0, 0, 0);
-			if (in1) *(uint4 *)(to + 16) = k.live ? raw[1] : make_uint4(0, 0, 0, 0);
-		}
-		if (w.pool && k.row >= 0) {
-			char *to = w.pool + k.row + h * p.c.head_b + c0 * 16;
-			if (in0) *(uint4 *)to = raw[0];
-			if (in1) *(uint4 *)(to + 16) = raw[1];
+		if (row >= 0) {
+			T *to = (T *)(pool + h * p.c.head_b);
+#pragma unroll
+			for (int n = 0; n < NI; n++)
+				if (one[n] >= 0) to[one[n]] = x[n], to[two[n]] = y[n];
 		}
 	}
 }
@@ -378,24 +389,28 @@ template <class T, int FORM> static int turn_part(TurnArgs &p, bool norm, int lg
 	return part == 4 ? turn_rounds<T, FORM, 4>(p, norm, lg, st) : part == 2 ? turn_rounds<T, FORM, 2>(p, norm, lg, st) : turn_rounds<T, FORM, 1>(p, norm, lg, st);
 }
 
+template <class T, int NI> static int turn_any(TurnArgs &p, bool norm, cudaStream_t st)
+{
+	const __int128 items = (__int128)p.all * p.chunks;
+	const long long blocks = items > 0x1ffffffffll ? 0x80000000ll : (long long)(items + 3) / 4;
+	if (turn_grid(blocks)) return TG_CUDA_EINVAL;
+	if (norm) k_turn_any<T, true, NI><<<(unsigned)blocks, 128, 0, st>>>(p);
+	else k_turn_any<T, false, NI><<<(unsigned)blocks, 128, 0, st>>>(p);
+	TGC_LAUNCH_CHECK();
+	return TG_CUDA_OK;
+}
+
 template <class T> static int turn_form(TurnArgs &p, int pairs, bool norm, cudaStream_t st)
 {
 	constexpr int E = 16 / (int)sizeof(T);
 	const int items = (p.dim / E + 1) / 2;
 	int lg = 0;
 	while (1 << lg < items) lg++;
-	p.heads = 0;
-	for (int g = 0; g < p.nrows; g++) p.heads += p.rows[g].heads;
 	if (pairs) return turn_part<T, TURN_PAIRS>(p, norm, lg, st);
 	if (p.part * (int)sizeof(T) % 32 == 0) return turn_part<T, TURN_HALF>(p, norm, lg, st);
-	const int per = std::max(1, std::min(8, 256 / std::min(256, p.heads << lg)));
-	const long long blocks = (p.all + per - 1) / per;
-	if (turn_grid(blocks)) return TG_CUDA_EINVAL;
-	const size_t smem = (size_t)per * (p.part / 2) * sizeof(float2);
-	if (norm) k_turn_any<T, true><<<(unsigned)blocks, 256, smem, st>>>(p, lg, per);
-	else k_turn_any<T, false><<<(unsigned)blocks, 256, smem, st>>>(p, lg, per);
-	TGC_LAUNCH_CHECK();
-	return TG_CUDA_OK;
+	p.chunks = 0;
+	for (int g = 0; g < p.nrows; g++) p.chunks += p.rows[g].chunks = (p.rows[g].heads + TURN_ANY_ROWS - 1) / TURN_ANY_ROWS;
+	return p.dim <= 64 ? turn_any<T, 1>(p, norm, st) : p.dim <= 128 ? turn_any<T, 2>(p, norm, st) : turn_any<T, 4>(p, norm, st);
 }
 
 static int turn_type(TurnArgs &p, int type, int pairs, bool norm, void *stream)
