@@ -175,6 +175,51 @@ def test_rope_on_a_side_stream_and_in_a_graph(cuda):
     assert torch.equal(got, kvcache.rope(x, r, pos)) and not torch.equal(got, want)
 
 
+def test_forward_and_gradient_in_a_graph(cuda):
+    r, x, w = kvcache.Rotary(64, theta=1e4), torch.randn(2, 9, 3, 64, device="cuda"), torch.randn(2, 9, 3, 64, device="cuda")
+    leaf = x.clone().requires_grad_()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(kvcache.rope(leaf, r), leaf, w)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = kvcache.rope(leaf, r)
+        d, = torch.autograd.grad(y, leaf, w)
+    with torch.no_grad():
+        leaf += 1
+    w *= 2
+    g.replay()
+    assert torch.equal(y, kvcache.rope(x + 1, r)) and torch.equal(d, kvcache.rope(w, r, inverse=True))
+
+
+@pytest.mark.parametrize("part,pairs", [(128, False), (128, True), (100, False)])
+def test_rope_past_32_bits(cuda, part, pairs):
+    """Sequences 4 GB apart, in and out."""
+    r = kvcache.Rotary(128, theta=1e6, part=part, interleaved=pairs)
+    far = torch.empty(2, (1 << 31) + 4096, dtype=BF16, device="cuda")
+    x = far[:, :3 * 2 * 128].view(2, 3, 2, 128)
+    x.copy_(torch.randn(2, 3, 2, 128, generator=torch.Generator().manual_seed(14)))
+    want = kvcache.rope(x.contiguous(), r)
+    assert torch.equal(kvcache.rope(x, r), want) and torch.equal(kvcache.rope(x, r, out=x), want)
+
+
+@pytest.mark.parametrize("tokens,heads,part", [(3000, 33, 64), (2500, 7, 64), (3000, 9, 20), (1, 1000, 64), (2100, 1, 64)])
+@pytest.mark.parametrize("pairs", [False, True])
+def test_many_tokens_and_heads(cuda, tokens, heads, part, pairs):
+    """Both ways of sharing a token's rows among warps, with rows that do not fill one."""
+    x = torch.randn(1, tokens, heads, 64, generator=torch.Generator().manual_seed(15))
+    r, pos = kvcache.Rotary(64, theta=1e4, part=part, interleaved=pairs), positions(1, tokens, 16)
+    want, tol = turned(x.double(), pos, r.freq, pairs=pairs)
+    for dt in (BF16, F32):
+        if dt is BF16:
+            w, t = turned(x.to(BF16).double(), pos, r.freq, pairs=pairs)
+        else:
+            w, t = want, tol
+        close(kvcache.rope(x.to(dt).cuda(), r, pos.cuda()), w, t, dt)
+
+
 def test_rope_refusals(cuda):
     r, x = kvcache.Rotary(64, theta=1e4), torch.zeros(2, 3, 4, 64, device="cuda")
     pos = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
