@@ -22,6 +22,7 @@ struct PtBars {
 	uint32_t tmem;
 	int abort;
 	long long scan[36];
+	AttnCursor begin; // of the CTA's share
 	float2 ml[2][128];
 };
 
@@ -83,15 +84,33 @@ __global__ void __launch_bounds__(480, 1) k_prefix_tc(const SharedArgs p, const 
 	long long left_, pos, share;
 	if (!attn_share<TK, A::NW, MODE, RT>(p, B->scan, 0, c, left_, pos, share)) return; // the whole CTA
 	int left = __shfl_sync(~0u, (int)left_, 0);
+	// A share that ends one unit and begins another takes the second first: units of one head lie next to each other in the list, so that
+	// CTAs at work on them then go through its keys together, from the first on, and most of them find a tile in L2.
+	int n1 = 0; // tiles of that second unit
+	if (left > c.all - c.tile) {
+		AttnCursor next = c;
+		next.tile = c.all - 1;
+		cursor_next<TK, MODE, RT>(p, next, 0);
+		const int rest = left - (c.all - c.tile);
+		if (rest <= next.all) {
+			if (tid == 0) B->begin = c;
+			n1 = rest, c = next;
+		}
+	}
 	if (warp == 12) tmem_alloc(&B->tmem, 512); // S buffers at columns 0 and 128, the halves' O at 256 and 256 + DP
 	tc_fence_before();
 	__syncthreads();
 	tc_fence_after();
 	const uint32_t tmem = __shfl_sync(~0u, B->tmem, 0);
 	// the tiles of a unit that are this CTA's; then the next unit
-	auto here = [&]() { return min(left, c.all - c.tile); };
+	auto here = [&]() { return n1 ? n1 : min(left, c.all - c.tile); };
 	auto leave = [&](int n) {
-		left -= n, c.tile += n - 1;
+		left -= n;
+		if (n1) {
+			n1 = 0, c = B->begin;
+			return;
+		}
+		c.tile += n - 1;
 		cursor_next<TK, MODE, RT>(p, c, 0);
 	};
 

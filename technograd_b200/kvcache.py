@@ -65,14 +65,14 @@ def _weights(name: str, x, cache: "PagedKV", least: int) -> tuple:
 
 def _stream(cache: "PagedKV") -> int:
     """The current stream of the cache's device, which has to be the current one."""
-    if cache.index != torch.cuda.current_device():
+    if cache.index != torch._C._cuda_getDevice():
         raise ValueError(f"the cache is on cuda:{cache.index}, which is not the current device")
     return torch._C._cuda_getCurrentRawStream(cache.index)  # torch.cuda.current_stream's handle without its object
 
 
 def _stream_of(index: int) -> int:
     """The same for tensors of a call that has no cache."""
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         raise ValueError(f"the tensors are on cuda:{index}, which is not the current device")
     return torch._C._cuda_getCurrentRawStream(index)
 
