@@ -34,6 +34,24 @@ template <int DP> struct PtTile {
 	static_assert(SMEM <= 232448, "shared memory of a CTA");
 };
 
+// ta_wait whose warp sleeps in the barrier between its looks: with fifteen warps looking all the time 40 trees of 21 tokens over 32768
+// positions, which run at the card's power limit, took 358 us, so 340.
+template <class BARS>
+__device__ __forceinline__ bool pt_wait(BARS *B, uint64_t *bar, uint32_t parity, const PgCache &c)
+{
+	if (__all_sync(~0u, mbar_try(bar, parity))) return true;
+	const long long t0 = clock64();
+	for (;;) {
+		if (__all_sync(~0u, mbar_try(bar, parity))) return true;
+		if (__any_sync(~0u, *(volatile int *)&B->abort)) return false;
+		if (__any_sync(~0u, clock64() - t0 > WAIT_CYCLES)) {
+			c.report(PG_WAIT);
+			*(volatile int *)&B->abort = 1;
+			return false;
+		}
+	}
+}
+
 // One thread of a warp that is together, always the same
 __device__ __forceinline__ bool elect_one()
 {
@@ -140,12 +158,12 @@ __global__ void __launch_bounds__(480, 1) k_prefix_tc(const SharedArgs p, const 
 				if (page != -1 && (unsigned)page >= (unsigned)p.c.pages) p.c.report(PG_PAGE), page = -1;
 				int row1 = 0;
 				const int r = page < 0 ? 0 : row, next = k + 1 < n ? page_of(c.tile + k + 1, row1) : -1; // looked up before this tile is waited for
-				if (j >= NST && !(ok = ta_wait(B, &free[st.at], st.parity ^ 1, p.c))) break;
+				if (j >= NST && !(ok = pt_wait(B, &free[st.at], st.parity ^ 1, p.c))) break;
 				if (lane == 0) ta_expect(&full[st.at], A::OP / 2);
 				__syncwarp();
 				if (mine) ta_box(to + st.at * A::OP, isv ? &vmap : &kmap, &full[st.at], lane % ND * 64, p.box.swap ? h : r, p.box.swap ? r : h, page < 0 ? -1 : page);
 				if (!isv && k == 0) { // the unit's Q, once the last S of the unit before is done
-					ok = j == 0 || ta_wait(B, &B->kfree[(j - 1) % NST], (j - 1) / NST & 1, p.c);
+					ok = j == 0 || pt_wait(B, &B->kfree[(j - 1) % NST], (j - 1) / NST & 1, p.c);
 					const char *qb = p.d.q + (long long)c.seq * p.d.q_seq + (long long)h * p.d.group * p.d.q_head + ch * 16;
 #pragma unroll 1
 					for (int i = 0; ok && i < 2; i++) {
@@ -180,8 +198,8 @@ __global__ void __launch_bounds__(480, 1) k_prefix_tc(const SharedArgs p, const 
 			const uint64_t qd = sw128_kmajor_desc(base + A::Q);
 			for (int j = 0; j < left; j++, st.next()) {
 				// over the P of two tiles before, once that has been used
-				if (j >= 2 && (!ta_wait(B, &B->p_empty[0][j & 1], ((j >> 1) - 1) & 1, p.c) || !ta_wait(B, &B->p_empty[1][j & 1], ((j >> 1) - 1) & 1, p.c))) break;
-				if (!ta_wait(B, &B->kfull[st.at], st.parity, p.c)) break;
+				if (j >= 2 && (!pt_wait(B, &B->p_empty[0][j & 1], ((j >> 1) - 1) & 1, p.c) || !pt_wait(B, &B->p_empty[1][j & 1], ((j >> 1) - 1) & 1, p.c))) break;
+				if (!pt_wait(B, &B->kfull[st.at], st.parity, p.c)) break;
 				tc_fence_after();
 				if (elect_one()) {
 					fence_async_smem();
@@ -203,9 +221,9 @@ __global__ void __launch_bounds__(480, 1) k_prefix_tc(const SharedArgs p, const 
 			bool ok = true;
 			while (left > 0 && ok) {
 				const int n = here();
-				if (unit++ && !ta_wait(B, &B->o_free, unit & 1, p.c)) break; // the unit before has been read
+				if (unit++ && !pt_wait(B, &B->o_free, unit & 1, p.c)) break; // the unit before has been read
 				for (int k = 0; k < n; k++, j++, st.next()) {
-					if (!(ok = ta_wait(B, &B->vfull[st.at], st.parity, p.c) && ta_wait(B, &B->p_full[f][j & 1], (j >> 1) & 1, p.c))) break;
+					if (!(ok = pt_wait(B, &B->vfull[st.at], st.parity, p.c) && pt_wait(B, &B->p_full[f][j & 1], (j >> 1) & 1, p.c))) break;
 					tc_fence_after();
 					if (elect_one()) {
 						fence_async_smem();
@@ -239,7 +257,7 @@ __global__ void __launch_bounds__(480, 1) k_prefix_tc(const SharedArgs p, const 
 			const int keys = c.n - c.tile * TK - hf * 64; // of this half, from the first tile on
 			float mr = -INFINITY, l = 0;
 			for (int k = 0; k < n; k++, j++) {
-				if (!(ok = ta_wait(B, &B->s_full[j & 1], (j >> 1) & 1, p.c))) break;
+				if (!(ok = pt_wait(B, &B->s_full[j & 1], (j >> 1) & 1, p.c))) break;
 				tc_fence_after();
 				const uint32_t s = lanes + (j & 1) * TK + hf * 64;
 				float z[64];
@@ -266,7 +284,7 @@ __global__ void __launch_bounds__(480, 1) k_prefix_tc(const SharedArgs p, const 
 				const bool raise = top > mr + (SHIFT + RAISE), scale = raise && ref0 != -INFINITY;
 				if (raise) mr = top - SHIFT;
 				if (__any_sync(~0u, scale)) { // once the product of the tile before is done (scale: there is one)
-					if (!(ok = ta_wait(B, &B->p_empty[hf][(j - 1) & 1], ((j - 1) >> 1) & 1, p.c))) break;
+					if (!(ok = pt_wait(B, &B->p_empty[hf][(j - 1) & 1], ((j - 1) >> 1) & 1, p.c))) break;
 					const float by = scale ? ex2(ref0 - mr) : 1;
 					l *= by;
 					tc_fence_after();
@@ -300,11 +318,11 @@ __global__ void __launch_bounds__(480, 1) k_prefix_tc(const SharedArgs p, const 
 			}
 			if (!ok) break;
 			// the unit's end, or the share's: the two halves join; j is the next tile
-			if (unit && !ta_wait(B, &B->o_free, (unit - 1) & 1, p.c)) break; // over the unit before's, once the other half has read them too
+			if (unit && !pt_wait(B, &B->o_free, (unit - 1) & 1, p.c)) break; // over the unit before's, once the other half has read them too
 			B->ml[hf][row] = make_float2(mr, l);
 			mbar_arrive_warp(&B->x_full);
-			if (!ta_wait(B, &B->x_full, unit & 1, p.c) || !ta_wait(B, &B->p_empty[0][(j - 1) & 1], ((j - 1) >> 1) & 1, p.c) ||
-			    !ta_wait(B, &B->p_empty[1][(j - 1) & 1], ((j - 1) >> 1) & 1, p.c))
+			if (!pt_wait(B, &B->x_full, unit & 1, p.c) || !pt_wait(B, &B->p_empty[0][(j - 1) & 1], ((j - 1) >> 1) & 1, p.c) ||
+			    !pt_wait(B, &B->p_empty[1][(j - 1) & 1], ((j - 1) >> 1) & 1, p.c))
 				break;
 			tc_fence_after();
 			const float2 a = B->ml[0][row], d = B->ml[1][row];
