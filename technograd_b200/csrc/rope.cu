@@ -7,7 +7,7 @@
 
 namespace tgc {
 
-// Rows that the kernel moves: heads of every token, from src to dst and, with `cache`, to the token's cache row.
+// Rows that the kernel moves: heads of every token, from src to dst and, keys and values, to the token's cache row in pool.
 struct TurnRows {
 	const char *src;
 	char *dst, *pool;                  // either may be NULL
@@ -34,7 +34,7 @@ struct TurnArgs {
 
 // cos and sin of pos * freq. The angle is taken in turns, as 64 bits behind the point: whole turns fall off the product by
 // themselves, so a far position's angle is as exact as a near one's (2^-55 turns of the frequency times the position).
-// The first 32 bits of it, 2^-32 turns, are a quarter turn and a rest of at most an eighth, x = 2 pi rest, whose sine and cosine
+// Its first 32 bits, to 2^-32 turns, are a quarter turn and a rest of at most an eighth, x = 2 pi rest, whose sine and cosine
 // are their Taylor series up to x^9 and x^10: what is left out is below (pi/4)^11 / 11! = 1.8e-9 and (pi/4)^12 / 12! = 1.2e-10.
 __device__ __forceinline__ float2 turn_of(double freq, int pos)
 {
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(128) k_turn_any(const TurnArgs p)
 	}
 }
 
-static int turn_check(const char *who, const tg_cuda_rotary *r, int head_dim, int e, int seqs, int tokens, TurnArgs *p)
+static int turn_check(const char *who, const tg_cuda_rotary *r, int head_dim, int seqs, TurnArgs *p)
 {
 	if (r->dim < 0 || r->dim > head_dim || r->dim & 1) return set_err(TG_CUDA_EINVAL, "%s: %d elements of a head of %d turn", who, r->dim, head_dim);
 	if (r->interleaved & ~1 || r->inverse & ~1) return set_err(TG_CUDA_EINVAL, "%s: interleaved %d, inverse %d", who, r->interleaved, r->inverse);
@@ -383,9 +383,6 @@ template <class T, int FORM> static int turn_part(TurnArgs &p, bool norm, int lg
 {
 	constexpr int E = 16 / (int)sizeof(T);
 	const int part = (E << lg) / 32; // pairs that a thread computes for those of its place in other rows
-	if constexpr (E == 8) {
-		if (part == 8) return turn_rounds<T, FORM, 8>(p, norm, lg, st);
-	}
 	return part == 4 ? turn_rounds<T, FORM, 4>(p, norm, lg, st) : part == 2 ? turn_rounds<T, FORM, 2>(p, norm, lg, st) : turn_rounds<T, FORM, 1>(p, norm, lg, st);
 }
 
@@ -445,7 +442,7 @@ extern "C" int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tok
 	if (head_dim <= 0 || head_dim > 256 || head_dim * e % 16) return set_err(TG_CUDA_EINVAL, "%s: head_dim %d: at most 256, in rows of a multiple of 16 bytes", who, head_dim);
 	TurnArgs p = {};
 	int rc, dev, sms;
-	if ((rc = turn_check(who, r, head_dim, e, seqs, tokens, &p))) return rc;
+	if ((rc = turn_check(who, r, head_dim, seqs, &p))) return rc;
 	const bool none = !seqs || !tokens || !heads;
 	if (!none && (!x || !out)) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);
 	long long s[3] = { seqs > 1 ? x_seq : 0, tokens > 1 ? x_tok : 0, heads > 1 ? x_head : 0 }, o[3] = { out_seq, out_tok, out_head };
@@ -472,7 +469,7 @@ extern "C" int tg_cuda_kv_append(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	const int e = pg_size(c->type);
 	if (c->nkv > 1 << 20) return set_err(TG_CUDA_EINVAL, "%s: nkv %d is over 2^20", who, c->nkv);
 	p.gain = 1;
-	if (r && (rc = turn_check(who, r, c->head_dim, e, c->seqs, d->tokens, &p))) return rc;
+	if (r && (rc = turn_check(who, r, c->head_dim, c->seqs, &p))) return rc;
 	if (c->seqs && (!len_out || !d->q != !q_out)) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);
 	if (len_out == c->len && c->seqs) return set_err(TG_CUDA_EINVAL, "%s: len_out may not be the cache's len", who);
 	if (((uintptr_t)len_out | (uintptr_t)q_norm | (uintptr_t)k_norm) & 3) return set_err(TG_CUDA_EINVAL, "%s: a pointer is not on a 4-byte boundary", who);

@@ -27,10 +27,6 @@ static int shared_check(const char *who, const tg_cuda_kv *c, const tg_cuda_pref
 // tiles), but 67.6 and 60 at 14.3 (units of 33), 108 and 98 at 19, 190 and 182 at 21. 128 rows: 53.5 and 50 at 2.2.
 constexpr int SHARED_MMA_ROWS = 64, SHARED_MMA_TILES = 14;
 
-// Units of a CTA each where there are few of them; CTAs of many waves would each wait for their first loads, and those of one
-// wave, with equal shares of all units, fetch the next unit while they work on one.
-constexpr int SHARED_WAVES = 1;
-
 // Whether tree attention itself does it: nothing is shared, or reading a prefix for each sequence takes less time than two passes and
 // their join. What each takes, from the bytes of keys and values it reads (as if all sequences had the longest prefix): tree
 // attention 1 us for 8.5 MB (many of them from L2, since the sequences' tables name the same pages); here 5 us more to begin with, 1 for 4.5 MB, 20 ns
@@ -81,7 +77,6 @@ static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, 
 	if (o->own.tc && d.tokens * d.group <= SHARED_MMA_ROWS && (long long)o->own.units * ((tail.max_len + 127) / 128 + 1) <= (long long)SHARED_MMA_TILES * o->own.sms &&
 	    (rc = attn_plan(who, &tail, d, &o->own, false)))
 		return rc;
-	if (o->own.whole && o->own.units > SHARED_WAVES * o->own.wave) o->own.whole = 0, o->own.grid = o->own.wave;
 	AttnPlan &p = o->pre;
 	p = {};
 	p.dev = o->own.dev, p.sms = o->own.sms, o->dp = p.dp = o->own.dp;

@@ -240,8 +240,7 @@ __global__ void __launch_bounds__(608, 1) k_tree_attn_tc(const AttnArgsOf<MODE> 
 		// by TMA, lane i has box i / (DP / 64) of its half's 64 rows, and 64 of its dimensions
 		constexpr int ND = DP / 64;
 		const int boxes = BOX ? 64 / p.box.rows : 0;
-		// (a prefix ends where a box does, and what is past it arrives as zeros)
-		auto by_box = [&]() { return BOX && (MODE == ATTN_PREFIX || c.tile < c.ctx - isv); };
+		auto by_box = [&]() { return BOX && c.tile < c.ctx - isv; };
 		auto look = [&]() {
 			const bool drafted = c.tile >= c.ctx, box = by_box();
 #pragma unroll
