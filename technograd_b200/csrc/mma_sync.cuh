@@ -119,9 +119,20 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool have)
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// S[16 rows x KW keys] += Q K^T over DP dimensions. KW is 16 for 16-bit elements and 8 for f32.
+// The low parts of four f32 elements (tf32_split)
+__device__ __forceinline__ uint4 tf32_low(uint4 x)
+{
+	uint32_t hi;
+	uint4 lo;
+	tf32_split(x.x, hi, lo.x), tf32_split(x.y, hi, lo.y), tf32_split(x.z, hi, lo.z), tf32_split(x.w, hi, lo.w);
+	return lo;
+}
+
+// S[16 rows x KW keys] += Q K^T over DP dimensions. KW is 16 for 16-bit elements and 8 for f32, whose Q has its low parts `low` bytes on:
+// taken once a unit instead of for every tile of keys, they save a third of the products' instructions (840 rows a key head over 8192 shared
+// positions 2293 us, 2802 before).
 template <class T, int DP, int MT, int NT>
-__device__ __forceinline__ void qk_tile(float (&s)[MT][NT][4], uint32_t sq, uint32_t sk, int lane)
+__device__ __forceinline__ void qk_tile(float (&s)[MT][NT][4], uint32_t sq, uint32_t sk, int lane, int low)
 {
 	constexpr int P = DP * (int)sizeof(T);
 	const int l7 = lane & 7, mi = lane >> 3;
@@ -153,9 +164,10 @@ __device__ __forceinline__ void qk_tile(float (&s)[MT][NT][4], uint32_t sq, uint
 #pragma unroll
 				for (int e = 0; e < 2; e++) {
 					uint32_t a[4], ah[4], al[4];
-					ldsm4(a, qrow + m * 16 * P + (((4 * k + 2 * e + (mi >> 1)) ^ l7) << 4));
+					const uint32_t at = qrow + m * 16 * P + (((4 * k + 2 * e + (mi >> 1)) ^ l7) << 4);
+					ldsm4(a, at), ldsm4(al, at + low);
 #pragma unroll
-					for (int i = 0; i < 4; i++) tf32_split(a[i], ah[i], al[i]);
+					for (int i = 0; i < 4; i++) asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(ah[i]) : "f"(__uint_as_float(a[i])));
 					mma8(t, al, bh[2 * e], bh[2 * e + 1]);
 					mma8(t, ah, bl[2 * e], bl[2 * e + 1]);
 					mma8(t, ah, bh[2 * e], bh[2 * e + 1]);

@@ -114,7 +114,7 @@ template <class T, int DP, int MT> struct AttnTile {
 	// against 195 of two CTAs with two ahead; the others' registers allow two
 	static constexpr int CTAS = DP == 256 ? 1 : MT == 1 && sizeof(T) == 2 ? 3 : 2;
 	static constexpr int NST = CTAS == 3 || DP == 256 || (DP == 128 && MT == 2 && sizeof(T) == 4) ? 2 : 3;
-	static constexpr int Q = 0, RING = RT * P, MASK = RING + 4 * NST * STAGE, ML = MASK + RT * 8, SCAN = ML + 4 * RT * 8;
+	static constexpr int Q = 0, QLO = RT * P, RING = sizeof(T) == 4 ? 2 * QLO : QLO, MASK = RING + 4 * NST * STAGE, ML = MASK + RT * 8, SCAN = ML + 4 * RT * 8; // QLO: Q's low parts, f32
 	static constexpr int SMEM = SCAN + 128; // attn_share: 2 * 4 + 6 words
 	static constexpr int SLOT = RT * DP + 2 * RT; // floats of a partial result
 };
@@ -483,6 +483,7 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 					else v = *(const uint4 *)(p.d.q + (long long)c.b * p.d.q_seq + (long long)t * p.d.q_tok + (long long)(c.h * p.d.group + r % p.d.group) * p.d.q_head + ch * 16);
 				}
 				*(uint4 *)(smem + row * P + ((ch ^ (row & 7)) << 4)) = v;
+				if constexpr (sizeof(T) == 4) *(uint4 *)(smem + A::QLO + row * P + ((ch ^ (row & 7)) << 4)) = tf32_low(v);
 			}
 			if (MODE != ATTN_PREFIX && tid < RT) {
 				const int t = (c.r * RT + (twin ? tid & 7 : tid)) / p.d.group;
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(128, AttnTile<T, DP, MT>::CTAS) k_tree_attn(co
 		for (int m = 0; m < MT; m++)
 #pragma unroll
 			for (int x = 0; x < NT; x++) s[m][x][0] = s[m][x][1] = s[m][x][2] = s[m][x][3] = 0;
-		qk_tile<T, DP, MT, NT>(s, s0, sk, lane);
+		qk_tile<T, DP, MT, NT>(s, s0, sk, lane, A::QLO);
 		unsplit_scores<T, DP, MT, NT>(s, s0, sk, lane);
 #pragma unroll
 		for (int m = 0; m < MT; m++)
