@@ -9,6 +9,9 @@
 //         that asks for it about 100 cycles: with one warp for all of them pages of 16 rows took 3700 a tile.
 //   12-14 issue of the MMAs: S, and the halves' P V. The whole warp waits and counts and one thread issues: eight MMAs take 560
 //         cycles so, 1000 where a thread does all by itself.
+// What bounds it: with many row tiles the softmax warps' chain, 2560 cycles a tile of which 1024 are exponentials, and the card's power: 1680
+// rows a key head over 32768 positions (8 key heads, bf16) 300 us, 590 TFLOP/s. With one, HBM and the asking for boxes: 64 rows over
+// 131008 positions (4 key heads, f16, pages of 16) about 60 us, 4.4 TB/s.
 #pragma once
 
 #include "tree_attn_tc.cuh"

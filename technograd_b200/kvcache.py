@@ -1,15 +1,18 @@
-"""A decoder's key/value cache in pages, over libtgcuda: attention of drafted tokens, the attention
+"""A decoder's key/value cache in pages, over libtgcuda: rotary positions, new tokens into the cache with the
+norm and rotation on the way, attention of drafted tokens (also below prefixes that sequences share), the attention
 weight each position receives, the commit of accepted tokens, and eviction by that weight.
 
 The pools are torch CUDA tensors [pages, nkv, page, head_dim] (any strides, rows contiguous) in f32,
 f16 or bf16; position p of sequence b is row p % page of page table[b, p // page]. Everything is
-asynchronous on the current stream; results are new tensors, except that `commit` writes the cache's
+asynchronous on the current stream; results are new tensors, except that `append` and `commit` write the cache's
 pages (and `acc`) and `evict` the destination's. No reference counterpart: the reference recomputes
 every position's keys and values (examples/qwen3/import.py:90-132).
 
 A speculative decode step: draft tokens and their mask, `tree_attention` in every layer, compare
 with the model's own choices, `commit` the accepted path. When the cache is full, `evict` by the
-weights that `attention_weights` has summed up (examples/speculative.py runs all of it)."""
+weights that `attention_weights` has summed up (examples/speculative.py runs all of it). A plain one: `append`
+the token's projection with keys=True, then `tree_attention` or `shared_attention` over the lengths from before
+with the rotated q and k; `append` alone takes a prompt into the cache."""
 from __future__ import annotations
 
 import ctypes as C
@@ -132,7 +135,7 @@ class PagedKV:
         self._one = torch.empty(1, dtype=torch.float32, device=k.device)
 
     def with_lens(self, lens: torch.Tensor, max_len: int | None = None) -> "PagedKV":
-        """The same pages with other lengths (what `commit` returned)."""
+        """The same pages with other lengths (what `commit` or `append` returned)."""
         return PagedKV(self.k, self.v, self.table, lens, max_len)
 
 
