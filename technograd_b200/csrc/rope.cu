@@ -416,12 +416,15 @@ static int turn_type(TurnArgs &p, int type, int pairs, bool norm, void *stream)
 	return type == TG_CUDA_F32 ? turn_form<float>(p, pairs, norm, st) : type == TG_CUDA_F16 ? turn_form<__half>(p, pairs, norm, st) : turn_form<__nv_bfloat16>(p, pairs, norm, st);
 }
 
-// An output's rows: on 16-byte boundaries, and none over another. Strides along one element are not used.
-static int turn_out(const char *who, const char *what, void *out, long long (&s)[3], int seqs, int tokens, int heads, int dim, int e)
+// An output's rows: on 16-byte boundaries, none over another, and those of its input (strides in[], bytes) only each in its own place.
+// Strides along one element are not used.
+static int turn_out(const char *who, const char *what, void *out, long long (&s)[3], const void *x, const long long (&in)[3], int seqs, int tokens, int heads, int dim, int e)
 {
 	const int n[3] = { seqs, tokens, heads };
-	for (int i = 0; i < 3; i++)
+	for (int i = 0; i < 3; i++) {
 		if (n[i] <= 1) s[i] = 0;
+		else if (out == x && s[i] * e != in[i]) return set_err(TG_CUDA_EINVAL, "%s: %s is its input with other strides", who, what);
+	}
 	if (((uintptr_t)out & 15) || ((s[0] | s[1] | s[2]) * e & 15)) return set_err(TG_CUDA_EINVAL, "%s: %s rows must start on 16-byte boundaries", who, what);
 	return pg_apart(who, what, dim, { s[0], s[1], s[2] }, { seqs, tokens, heads });
 }
@@ -448,7 +451,7 @@ extern "C" int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tok
 	long long s[3] = { seqs > 1 ? x_seq : 0, tokens > 1 ? x_tok : 0, heads > 1 ? x_head : 0 }, o[3] = { out_seq, out_tok, out_head };
 	if (s[0] < 0 || s[1] < 0 || s[2] < 0) return set_err(TG_CUDA_EINVAL, "%s: negative strides", who);
 	if (((uintptr_t)x & 15) || ((s[0] | s[1] | s[2]) * e & 15)) return set_err(TG_CUDA_EINVAL, "%s: x rows must start on 16-byte boundaries", who);
-	if (!none && (rc = turn_out(who, "out", out, o, seqs, tokens, heads, head_dim, e))) return rc;
+	if (!none && (rc = turn_out(who, "out", out, o, x, { s[0] * e, s[1] * e, s[2] * e }, seqs, tokens, heads, head_dim, e))) return rc;
 	if ((rc = pg_sms(who, &dev, &sms)) || none) return rc;
 	p.rows[0] = { (const char *)x, (char *)out, nullptr, s[0] * e, s[1] * e, s[2] * e, o[0] * e, o[1] * e, o[2] * e, nullptr, heads, r->dim > 0, 0, 0 };
 	p.nrows = 1, p.all = (long long)seqs * tokens, p.tokens = tokens, p.dim = head_dim;
@@ -475,8 +478,8 @@ extern "C" int tg_cuda_kv_append(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	if (((uintptr_t)len_out | (uintptr_t)q_norm | (uintptr_t)k_norm) & 3) return set_err(TG_CUDA_EINVAL, "%s: a pointer is not on a 4-byte boundary", who);
 	if (q_norm && !q) return set_err(TG_CUDA_EINVAL, "%s: q_norm without q", who);
 	long long qo[3] = { q_out_seq, q_out_tok, q_out_head }, ko[3] = { k_out_seq, k_out_tok, k_out_head };
-	if (q && (rc = turn_out(who, "q_out", q_out, qo, c->seqs, d->tokens, d->nq, c->head_dim, e))) return rc;
-	if (k_out && (rc = turn_out(who, "k_out", k_out, ko, c->seqs, d->tokens, c->nkv, c->head_dim, e))) return rc;
+	if (q && (rc = turn_out(who, "q_out", q_out, qo, pd.q, { pd.q_seq, pd.q_tok, pd.q_head }, c->seqs, d->tokens, d->nq, c->head_dim, e))) return rc;
+	if (k_out && (rc = turn_out(who, "k_out", k_out, ko, pd.k, { pd.kv_seq, pd.kv_tok, pd.kv_head }, c->seqs, d->tokens, c->nkv, c->head_dim, e))) return rc;
 	if ((rc = pg_apart(who, "the cache", c->head_dim, {c->page_stride, c->head_stride, c->pos_stride}, {c->pages, c->nkv, c->page}))) return rc;
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0) return rc;
 	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim, !((uintptr_t)q_norm & 15), 0 };

@@ -49,6 +49,14 @@ def test_bad_rows(bad):
     refused(rope(**bad))
 
 
+def test_in_place_means_the_same_strides():
+    """Rows read by one warp would be written by another."""
+    refused(rope(out=(0x30000, 384, 128, 64), seqs=2, tokens=3, heads=2))
+    refused(rope(out=(0x30000, 768, 64, 192)))
+    refused(append(q=(0x30000, 1536, 512, 64)))
+    refused(append(k=(0x40000, 384, 64, 192)))
+
+
 def test_null_rotation():
     refused(_lib.lib().tg_cuda_rope(None, _lib.BF16, 2, 3, 4, 64, 0x30000, 768, 256, 64, *OUT, None))
 
