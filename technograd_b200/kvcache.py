@@ -359,6 +359,14 @@ def _turn(x, rotary, pos, inverse, out):
     return out
 
 
+def _rows(x):
+    """x, or a copy of it whose rows are contiguous and begin on 16-byte boundaries, as the library wants them."""
+    e = x.element_size()
+    if (x.shape[3] > 1 and x.stride(3) != 1) or x.data_ptr() % 16 or any(n > 1 and s * e % 16 for n, s in zip(x.shape[:3], x.stride())):
+        return x.clone(memory_format=torch.contiguous_format)  # (contiguous() gives x itself where only its beginning is off)
+    return x
+
+
 class _Rope(torch.autograd.Function):
     """A rotation's gradient is the rotation by the negative angle, with the same gain."""
 
@@ -371,9 +379,7 @@ class _Rope(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         pos = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        if grad.shape[3] > 1 and grad.stride(3) != 1 or grad.data_ptr() % 16 or any(s * grad.element_size() % 16 for s in grad.stride()[:3]):
-            grad = grad.contiguous()  # (an expanded or transposed gradient)
-        return rope(grad, ctx.rotary, pos, not ctx.inverse), None, None, None
+        return rope(_rows(grad), ctx.rotary, pos, not ctx.inverse), None, None, None
 
 
 def rope(x, rotary: Rotary, pos=None, inverse: bool = False, out=None):
