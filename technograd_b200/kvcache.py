@@ -20,6 +20,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -78,6 +79,11 @@ def _stream_of(index: int) -> int:
     if index != torch._C._cuda_getDevice():
         raise ValueError(f"the tensors are on cuda:{index}, which is not the current device")
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _tangent(*tensors) -> bool:
+    """Whether one of the tensors carries a tangent of forward-mode differentiation."""
+    return forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors)
 
 
 class _ForwardOnly(torch.autograd.Function):
@@ -368,27 +374,41 @@ def _rows(x):
 
 
 class _Rope(torch.autograd.Function):
-    """A rotation's gradient is the rotation by the negative angle, with the same gain."""
+    """A rotation's gradient is the rotation by the negative angle, with the same gain, and its derivative along a tangent is the tangent's
+    rotation. any_layout: of a gradient or tangent, whose rows may lie anyhow."""
 
     @staticmethod
-    def forward(ctx, x, rotary, pos, inverse):
+    def forward(ctx, x, rotary, pos, inverse, any_layout):
         ctx.rotary, ctx.inverse = rotary, inverse
-        ctx.save_for_backward(*(() if pos is None else (pos,)))
-        return _turn(x, rotary, pos, inverse, None)
+        saved = () if pos is None else (pos,)
+        ctx.save_for_backward(*saved)
+        ctx.save_for_forward(*saved)
+        return _turn(_rows(x) if any_layout else x, rotary, pos, inverse, None)
 
     @staticmethod
     def backward(ctx, grad):
-        pos = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        return rope(_rows(grad), ctx.rotary, pos, not ctx.inverse), None, None, None
+        return _along(ctx, grad, not ctx.inverse), None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *others):
+        return _along(ctx, tangent, ctx.inverse)
+
+
+def _along(ctx, x, inverse):
+    """A gradient or tangent rotated to _Rope's positions."""
+    pos = ctx.saved_tensors[0] if ctx.saved_tensors else None
+    if (torch.is_grad_enabled() and x.requires_grad) or _tangent(x):
+        return _Rope.apply(x, ctx.rotary, pos, inverse, True)
+    return _turn(_rows(x), ctx.rotary, pos, inverse, None)
 
 
 def rope(x, rotary: Rotary, pos=None, inverse: bool = False, out=None):
     """x [seqs, tokens, heads, head_dim] rotated to its tokens' positions (tg_cuda_rope); pos int32 [seqs, tokens] or [tokens] (None: 0, 1, ...).
 
-    inverse: by the negative angle. out: where to (x itself: in place). Differentiable with respect to x, without out."""
-    if torch.is_grad_enabled() and x.requires_grad:
-        _need(out is None, "out: not with a gradient")
-        return _Rope.apply(x, rotary, pos, inverse)
+    inverse: by the negative angle. out: where to (x itself: in place). Differentiable with respect to x in either mode, without out."""
+    if (torch.is_grad_enabled() and x.requires_grad) or _tangent(x, out):
+        _need(out is None, "out: not with a gradient or a tangent")
+        return _Rope.apply(x, rotary, pos, inverse, False)
     return _turn(x, rotary, pos, inverse, out)
 
 

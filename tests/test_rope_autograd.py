@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
+from torch.autograd import forward_ad  # noqa: E402
+
 from technograd_b200 import kvcache  # noqa: E402
 
 
@@ -45,3 +47,56 @@ def test_a_gradient_that_begins_off_a_boundary(calls, before):
     r, x, w = Rotation(), rows(1).requires_grad_(), torch.randn(before + 2 * 5 * 3 * 4)
     (torch.cat([torch.zeros(before), kvcache.rope(x, r).flatten()]) * w).sum().backward()
     assert torch.equal(x.grad, turned(w[before:].view(x.shape), r.freq, None, True))
+
+
+@pytest.mark.parametrize("learns", [False, True])
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("pos", [None, torch.tensor([3, 1, 4, 1, 5], dtype=torch.int32)])
+def test_a_tangent_is_rotated(calls, learns, inverse, pos):
+    """The rotation is linear: the result's tangent is the tangent rotated, whether or not x requires a gradient too."""
+    r, x, t = Rotation(), rows(1).requires_grad_(learns), rows(2)
+    with forward_ad.dual_level():
+        y = forward_ad.unpack_dual(kvcache.rope(forward_ad.make_dual(x, t), r, pos, inverse))
+        assert torch.equal(y.primal, turned(x, r.freq, pos, inverse)) and torch.equal(y.tangent, turned(t, r.freq, pos, inverse))
+        plain = kvcache.rope(rows(1), r, pos, inverse)
+        assert forward_ad.unpack_dual(plain).tangent is None
+        with torch.no_grad():  # which forward mode does not ask
+            y = forward_ad.unpack_dual(kvcache.rope(forward_ad.make_dual(rows(1), t), r, pos, inverse))
+            assert torch.equal(y.tangent, turned(t, r.freq, pos, inverse))
+
+
+def test_a_tangent_of_any_layout(calls):
+    r, x = Rotation(), rows(1)
+    wide, off = torch.randn(2, 5, 4, 3).transpose(2, 3), torch.randn(1 + 2 * 5 * 3 * 4)[1:].view(2, 5, 3, 4)
+    for t in (wide, off, torch.ones(1).expand(2, 5, 3, 4)):
+        with forward_ad.dual_level():
+            assert torch.equal(forward_ad.unpack_dual(kvcache.rope(forward_ad.make_dual(x, t), r)).tangent, turned(t, r.freq, None, False))
+
+
+def test_a_tangent_of_a_gradient(calls):
+    """Forward over backward: the derivative of 2 R^T R x along t is 2 t."""
+    r, x, t = Rotation(), rows(1).requires_grad_(), rows(2)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, t)
+        g, = torch.autograd.grad(kvcache.rope(d, r).square().sum(), d, create_graph=True)
+        h = forward_ad.unpack_dual(g).tangent
+    # each rotation: cos, sin and the two products and their sum of elements of up to |t| sqrt(2), five roundings of 2^-24
+    assert (h - 2 * t).abs().max() < 2 * 2 * 5 * 2.0 ** -24 * 2 ** 0.5 * 2 * t.abs().max()
+
+
+def test_transforms_of_the_call_are_refused(calls):
+    """torch.func's wrapped tensors have no memory of their own: an error, and no result without its derivative."""
+    r, x, t = Rotation(), rows(1), rows(2)
+    for f in (lambda: torch.func.jvp(lambda z: kvcache.rope(z, r), (x,), (t,)), lambda: torch.func.grad(lambda z: kvcache.rope(z, r).sum())(x)):
+        with pytest.raises(RuntimeError):
+            f()
+
+
+def test_a_tangent_and_out(calls):
+    r, x = Rotation(), rows(1)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, rows(2))
+        for kw in (dict(x=d, out=rows(3)), dict(x=d, out=d), dict(x=x, out=d)):
+            with pytest.raises(ValueError, match="out"):
+                kvcache.rope(rotary=r, **kw)
+    assert not calls
