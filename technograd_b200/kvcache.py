@@ -86,6 +86,13 @@ def _tangent(*tensors) -> bool:
     return forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors)
 
 
+def _written(*tensors) -> None:
+    """Autograd learns that the library has written these in place: what was saved of them for a backward pass is not used then."""
+    for x in tensors:
+        if not x.is_inference():  # (those have no version)
+            torch.autograd.graph.increment_version(x)
+
+
 class _ForwardOnly(torch.autograd.Function):
     """out and lse as results of inputs that want a gradient: there is none, and asking for it is an error."""
 
@@ -409,7 +416,12 @@ def rope(x, rotary: Rotary, pos=None, inverse: bool = False, out=None):
     if (torch.is_grad_enabled() and x.requires_grad) or _tangent(x, out):
         _need(out is None, "out: not with a gradient or a tangent")
         return _Rope.apply(x, rotary, pos, inverse, False)
-    return _turn(x, rotary, pos, inverse, out)
+    if out is not None and torch.is_grad_enabled() and out.requires_grad:
+        raise ValueError("out: requires a gradient, but the call's writes are not part of its history")
+    y = _turn(x, rotary, pos, inverse, out)
+    if out is not None:
+        _written(out)
+    return y
 
 
 def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None, count=None, q_norm=None, k_norm=None, eps: float = 1e-6,

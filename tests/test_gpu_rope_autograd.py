@@ -31,3 +31,17 @@ def test_a_tangent_is_rotated(cuda, dtype, dim, part, pairs, inverse):
             with forward_ad.dual_level():
                 y = forward_ad.unpack_dual(kvcache.rope(forward_ad.make_dual(x.clone().requires_grad_(learns), tangent), r, pos, inverse))
                 assert torch.equal(y.primal, kvcache.rope(x, r, pos, inverse)) and torch.equal(y.tangent, kvcache.rope(t, r, pos, inverse))
+
+
+def test_what_is_saved_does_not_change_unnoticed(cuda):
+    r, w, x = kvcache.Rotary(64, theta=1e4), torch.randn(2, 5, 3, 64, device="cuda", requires_grad=True), torch.randn(2, 5, 3, 64, device="cuda")
+    y = (x * w).sum()
+    kvcache.rope(x[:, 1:3], r, out=x[:, 1:3])
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.backward()
+    with pytest.raises(ValueError, match="out"):
+        kvcache.rope(x, r, out=w)
+    with torch.inference_mode():
+        z = torch.randn(2, 5, 3, 64, device="cuda")
+        want = kvcache.rope(z, r)
+        assert torch.equal(kvcache.rope(z, r, out=z), want)

@@ -100,3 +100,41 @@ def test_a_tangent_and_out(calls):
             with pytest.raises(ValueError, match="out"):
                 kvcache.rope(rotary=r, **kw)
     assert not calls
+
+
+def test_what_is_saved_does_not_change_unnoticed(calls):
+    """torch's own error where a tensor saved for a backward pass, or a view of one, was rotated in place."""
+    r, w = Rotation(), torch.randn(2, 5, 3, 4, requires_grad=True)
+    for view in (lambda x: x, lambda x: x[:1], lambda x: x[:, :, 1:2]):
+        x = rows(1)
+        y = (x * w).sum()
+        kvcache.rope(view(x), r, out=view(x))
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.backward()
+    x, out = rows(1), rows(2)
+    y = (out * w).sum() + (x * w).sum()
+    kvcache.rope(x, r, out=out)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.backward()
+    (x * w).sum().backward()  # x itself was only read
+    assert torch.equal(w.grad, x)
+
+
+def test_out_that_requires_a_gradient_is_refused(calls):
+    r, x = Rotation(), rows(1)
+    leaf = rows(2).requires_grad_()
+    for out in (leaf, leaf * 1):
+        with pytest.raises(ValueError, match="out"):
+            kvcache.rope(x, r, out=out)
+    assert not calls
+    with torch.no_grad():  # as torch's own in-place operations
+        version = leaf._version
+        assert kvcache.rope(x, r, out=leaf) is leaf and torch.equal(leaf, turned(x, r.freq, None, False)) and leaf._version == version + 1
+
+
+def test_out_in_inference_mode(calls):
+    r = Rotation()
+    with torch.inference_mode():
+        x = rows(1)
+        want = turned(x, r.freq, None, False)
+        assert torch.equal(kvcache.rope(x, r, out=x), want)
