@@ -386,8 +386,9 @@ class _Rope(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, rotary, pos, inverse, any_layout):
-        ctx.rotary, ctx.inverse = rotary, inverse
-        saved = () if pos is None else (pos,)
+        ctx.rotary, ctx.inverse, ctx.given = rotary, inverse, pos is not None
+        # the frequencies too, so that their change before the backward pass is an error (those made in inference mode have no version)
+        saved = (() if pos is None else (pos,)) + (() if rotary.freq.is_inference() else (rotary.freq,))
         ctx.save_for_backward(*saved)
         ctx.save_for_forward(*saved)
         return _turn(_rows(x) if any_layout else x, rotary, pos, inverse, None)
@@ -403,7 +404,8 @@ class _Rope(torch.autograd.Function):
 
 def _along(ctx, x, inverse):
     """A gradient or tangent rotated to _Rope's positions."""
-    pos = ctx.saved_tensors[0] if ctx.saved_tensors else None
+    saved = ctx.saved_tensors
+    pos = saved[0] if ctx.given else None
     if (torch.is_grad_enabled() and x.requires_grad) or _tangent(x):
         return _Rope.apply(x, ctx.rotary, pos, inverse, True)
     return _turn(_rows(x), ctx.rotary, pos, inverse, None)

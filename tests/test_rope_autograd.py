@@ -138,3 +138,23 @@ def test_out_in_inference_mode(calls):
         x = rows(1)
         want = turned(x, r.freq, None, False)
         assert torch.equal(kvcache.rope(x, r, out=x), want)
+
+
+def test_positions_and_frequencies_stay_until_the_backward_pass(calls):
+    """Other ones would give another rotation's gradient."""
+    for given in (None, torch.arange(5, dtype=torch.int32)):
+        for change in [lambda r: r.freq.mul_(2)] + ([] if given is None else [lambda r: given.add_(1)]):
+            r, x = Rotation(), rows(1).requires_grad_()
+            y = kvcache.rope(x, r, given)
+            change(r)
+            with pytest.raises(RuntimeError, match="inplace operation"):
+                y.sum().backward()
+            assert x.grad is None
+
+
+def test_frequencies_made_in_inference_mode(calls):
+    with torch.inference_mode():
+        r = Rotation()
+    x = rows(1).requires_grad_()
+    kvcache.rope(x, r).sum().backward()
+    assert torch.equal(x.grad, turned(torch.ones_like(x), r.freq, None, True))
