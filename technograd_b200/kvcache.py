@@ -459,10 +459,11 @@ def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None,
         ko = k.new_empty_strided(n, sk) if 0 not in sk else torch.empty_like(k)
         sk, kp = ko.stride(), ko.data_ptr()
     _lib.check(_lib.lib().tg_cuda_kv_append(cache._at, d, r, qn, kn, eps, qp, sq[0], sq[1], sq[2], kp, sk[0], sk[1], sk[2], lens.data_ptr(), _stream(cache)))
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
+    given = [x for x in (q, k, v, q_norm, k_norm) if x is not None] if torch.is_grad_enabled() else ()
+    if any(x.requires_grad for x in given):
         made = [x for x in (qo, ko) if x is not None]
         if made:
-            made = list(_NoGradient.apply("append", len(made), *made, *(x for x in (q, k, v) if x is not None)))
+            made = list(_NoGradient.apply("append", len(made), *made, *given))
             qo, ko = made.pop(0) if qo is not None else None, made.pop(0) if ko is not None else None
     return lens, qo, ko
 
