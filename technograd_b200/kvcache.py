@@ -333,6 +333,7 @@ class Rotary:
                  interleaved: bool = False):
         if freq is None:
             freq = rotary_frequencies(head_dim if part is None else part, theta).cuda()
+        _need(not freq.requires_grad, "freq: no gradient reaches the frequencies; give them detached")
         _need(freq.dim() == 1 and freq.dtype is torch.float64 and freq.is_cuda and freq.is_contiguous(), "freq: expected a contiguous float64 CUDA tensor [part / 2]")
         self.part = 2 * freq.shape[0]
         _need(part is None or part == self.part, f"part: {part} elements, but {freq.shape[0]} frequencies")

@@ -18,3 +18,8 @@ def test_a_gradient_of_norms_through_append_is_an_error(library, which):  # noqa
             y.float().sum().backward(retain_graph=True)
     with torch.no_grad():
         assert not any(y.requires_grad for y in kvcache.append(cache(), k, v, q=q, keys=True, **norms))
+
+
+def test_frequencies_that_learn_are_refused():
+    with pytest.raises(ValueError, match="gradient"):
+        kvcache.Rotary(64, torch.ones(32, dtype=torch.float64, requires_grad=True))
