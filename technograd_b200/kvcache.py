@@ -86,6 +86,11 @@ def _tangent(*tensors) -> bool:
     return forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors)
 
 
+def _no_tangent(name: str, *tensors) -> None:
+    if _tangent(*tensors):
+        raise RuntimeError(f"kvcache.{name} has no forward-mode derivative")
+
+
 def _written(*tensors) -> None:
     """Autograd learns that the library has written these in place: what was saved of them for a backward pass is not used then."""
     for x in tensors:
@@ -184,7 +189,9 @@ def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float 
     tokens. mask int64 [seqs, tokens]: bit u of an entry = the token attends to drafted token u (None:
     a chain). count int32 [seqs]: tokens drafted (None: all). Returns (out as q, lse f32 [seqs, tokens,
     nq]); a token that sees nothing has out 0 and lse -inf. Forward only: where q, k or v require a
-    gradient, a backward pass through the results is an error (the other calls' results never require one)."""
+    gradient, a backward pass through the results is an error, and so is a tangent of theirs (attention_weights', commit's and evict's
+    results never require a gradient and have no tangents)."""
+    _no_tangent("tree_attention", q, k, v)
     d = _drafts(cache, q, k, v, mask, count, scale)
     stream, shape = _stream(cache), q.shape
     plan = cache._plans.get(shape[1:3])
@@ -242,6 +249,7 @@ def shared_attention(cache: PagedKV, prefix: SharedPrefix, q, k, v, mask=None, c
     if prefix.index != cache.index or prefix.seqs != cache.seqs or prefix.max_shared > cache.max_len:
         raise ValueError(f"prefix: made for {prefix.seqs} sequences with up to {prefix.max_shared} positions shared on cuda:{prefix.index}, not for {cache.seqs} of "
                          f"up to {cache.max_len} on cuda:{cache.index}")
+    _no_tangent("shared_attention", q, k, v)
     d = _drafts(cache, q, k, v, mask, count, scale)
     stream, shape = _stream(cache), q.shape
     key = shape[1], shape[2], prefix
@@ -436,6 +444,7 @@ def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None,
     f32 [head_dim]: weights of an RMS norm of each head before the rotation. keys: return the rotated keys too, with k's strides, which tree_attention and
     shared_attention take with v as the tokens' own, the lengths being those from before. Returns (the new lengths, q rotated or
     None, k rotated or None), rows past count 0; the pages are written in place. Forward only, like tree_attention."""
+    _no_tangent("append", q, k, v, q_norm, k_norm)
     d = _drafts(cache, q, k, v, None, count, 1.0)
     n, dim, index = k.shape, cache.head_dim, cache.index
     qn = kn = qo = ko = qp = kp = r = None

@@ -2,6 +2,8 @@
 import pytest
 
 torch = pytest.importorskip("torch")
+from torch.autograd import forward_ad  # noqa: E402
+
 from technograd_b200 import kvcache  # noqa: E402
 from test_kvcache_host import cache, drafted, library  # noqa: E402, F401
 
@@ -23,3 +25,24 @@ def test_a_gradient_of_norms_through_append_is_an_error(library, which):  # noqa
 def test_frequencies_that_learn_are_refused():
     with pytest.raises(ValueError, match="gradient"):
         kvcache.Rotary(64, torch.ones(32, dtype=torch.float64, requires_grad=True))
+
+
+def test_tangents_through_the_calls_are_an_error(library):  # noqa: F811
+    """The results would have none: derivatives of zero. Nothing has been launched by then."""
+    c = cache(device=torch.device("cpu"), table=torch.zeros(2, 4, dtype=torch.int32))
+    prefix = kvcache.SharedPrefix(c, [(0, 2, 16)])
+    norm = torch.ones(64)
+    with forward_ad.dual_level():
+        for which in range(3):
+            q, k, v = (forward_ad.make_dual(x, torch.ones_like(x)) if i == which else x for i, x in enumerate(drafted()))
+            for name, call in (("tree_attention", lambda: kvcache.tree_attention(c, q, k, v)), ("shared_attention", lambda: kvcache.shared_attention(c, prefix, q, k, v)),
+                               ("append", lambda: kvcache.append(c, k, v, q=q))):
+                with pytest.raises(RuntimeError, match=f"{name} has no forward-mode"):
+                    call()
+        q, k, v = drafted()
+        for kw in (dict(q_norm=forward_ad.make_dual(norm, norm)), dict(k_norm=forward_ad.make_dual(norm, norm))):
+            with pytest.raises(RuntimeError, match="append has no forward-mode"):
+                kvcache.append(c, k, v, q=q, **kw)
+        assert not library.calls
+        kvcache.tree_attention(c, q, k, v), kvcache.shared_attention(c, prefix, q, k, v), kvcache.append(c, k, v, q_norm=None, k_norm=norm)
+    assert len(library.calls) == 5
