@@ -91,11 +91,21 @@ def _no_tangent(name: str, *tensors) -> None:
         raise RuntimeError(f"kvcache.{name} has no forward-mode derivative")
 
 
+def _versions(*tensors) -> tuple:
+    """Those of the tensors that autograd counts the writes of: not those made in inference mode."""
+    return tuple(x for x in tensors if not x.is_inference())
+
+
 def _written(*tensors) -> None:
     """Autograd learns that the library has written these in place: what was saved of them for a backward pass is not used then."""
-    for x in tensors:
-        if not x.is_inference():  # (those have no version)
-            torch.autograd.graph.increment_version(x)
+    torch.autograd.graph.increment_version(_versions(*tensors))
+
+
+def _pages_written(cache) -> None:
+    """The same for a cache's pools, in one call."""
+    pools = getattr(cache, "_versioned", ())
+    if pools:
+        torch._C._increment_version(pools)
 
 
 class _ForwardOnly(torch.autograd.Function):
@@ -150,6 +160,7 @@ class PagedKV:
         self._struct = s
         self._at = C.addressof(s)
         self._plans = {}  # (tokens, nq) -> bytes of tree_attention's scratch, and a shape to make its lse like
+        self._versioned = _versions(k, v)
         self._one = torch.empty(1, dtype=torch.float32, device=k.device)
 
     def with_lens(self, lens: torch.Tensor, max_len: int | None = None) -> "PagedKV":
@@ -310,6 +321,9 @@ def commit(cache: PagedKV, k, v, count, path=None, new=None, acc=None):
     _lib.check(_lib.lib().tg_cuda_kv_commit(cache._at, d, None if path is None else path.data_ptr(), lens.data_ptr(),
                                             None if acc is None else new.data_ptr(), None if acc is None else acc.data_ptr(), sa[0], sa[1],
                                             0 if acc is None else acc.shape[2], _stream(cache)))
+    _pages_written(cache)
+    if acc is not None:
+        _written(acc)
     return lens
 
 
@@ -469,6 +483,7 @@ def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None,
         ko = k.new_empty_strided(n, sk) if 0 not in sk else torch.empty_like(k)
         sk, kp = ko.stride(), ko.data_ptr()
     _lib.check(_lib.lib().tg_cuda_kv_append(cache._at, d, r, qn, kn, eps, qp, sq[0], sq[1], sq[2], kp, sk[0], sk[1], sk[2], lens.data_ptr(), _stream(cache)))
+    _pages_written(cache)
     given = [x for x in (q, k, v, q_norm, k_norm) if x is not None] if torch.is_grad_enabled() else ()
     if any(x.requires_grad for x in given):
         made = [x for x in (qo, ko) if x is not None]
@@ -494,4 +509,5 @@ def evict(cache: PagedKV, dst: PagedKV, acc, budget: int, recent: int = 0, sink:
     lens = torch.empty_like(cache.lens)
     _lib.check(_lib.lib().tg_cuda_kv_evict(cache._at, dst._at, acc.data_ptr(), sa[0], sa[1], budget, recent, sink, keep.data_ptr(), out.data_ptr(),
                                            lens.data_ptr(), _stream(cache)))
+    _pages_written(dst)
     return keep, out, lens

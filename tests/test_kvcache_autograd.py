@@ -5,7 +5,7 @@ torch = pytest.importorskip("torch")
 from torch.autograd import forward_ad  # noqa: E402
 
 from technograd_b200 import kvcache  # noqa: E402
-from test_kvcache_host import cache, drafted, library  # noqa: E402, F401
+from test_kvcache_host import BF16, cache, drafted, library  # noqa: E402, F401
 
 
 @pytest.mark.parametrize("which", ["q_norm", "k_norm"])
@@ -46,3 +46,34 @@ def test_tangents_through_the_calls_are_an_error(library):  # noqa: F811
         assert not library.calls
         kvcache.tree_attention(c, q, k, v), kvcache.shared_attention(c, prefix, q, k, v), kvcache.append(c, k, v, q_norm=None, k_norm=norm)
     assert len(library.calls) == 5
+
+
+def test_pages_that_are_written_have_a_new_version(library):  # noqa: F811
+    """A pool saved for a backward pass is not what it was after an append, a commit or an eviction into it."""
+    table, lens = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+
+    def paged():
+        k, v = torch.zeros(8, 2, 16, 64, dtype=BF16), torch.zeros(8, 2, 16, 64, dtype=BF16)
+        c = kvcache.PagedKV.__new__(kvcache.PagedKV)
+        vars(c).update(vars(cache(k=k, v=v, table=table, lens=lens)))
+        c._versioned = kvcache._versions(k, v)
+        return c, k, v
+
+    q, k, v = drafted()
+    count, acc = torch.ones(2, dtype=torch.int32), torch.zeros(2, 2, 40)
+    for write in (lambda c: kvcache.append(c, k, v, q=q), lambda c: kvcache.commit(c, k, v, count), lambda c: kvcache.evict(cache(), c, acc, 8)):
+        for pool in range(2):
+            c, *pools = paged()
+            w = torch.ones(pools[pool].shape, dtype=BF16, requires_grad=True)
+            y = (pools[pool] * w).sum()
+            write(c)
+            with pytest.raises(RuntimeError, match="inplace operation"):
+                y.backward()
+    w = torch.ones(acc.shape, requires_grad=True)
+    y = (acc * w).sum()
+    kvcache.commit(paged()[0], k, v, count, new=torch.zeros(2, 2, 3), acc=acc)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        c, *_ = paged()
+        kvcache.append(c, k, v)
