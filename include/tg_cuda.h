@@ -467,15 +467,15 @@ typedef struct {
 } tg_cuda_rotary;
 
 /* out = x rotated; x and out [seqs][tokens][heads][head_dim] in elements of `type` with strides in elements, rows
- * as in a cache (16-byte boundaries, at most 256 elements). out may be x with the same strides. pos NULL: token t is at
- * position t. */
+ * as in a cache (16-byte boundaries, at most 256 elements). out may be x with the same strides; else the two
+ * share no memory (rows between each other's, as of one projection, do not). pos NULL: token t is at position t. */
 int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tokens, int heads, int head_dim, const void *x, long long x_seq,
 		 long long x_tok, long long x_head, void *out, long long out_seq, long long out_tok, long long out_head, void *stream);
 
 /* New tokens into the cache, rotated on the way: for i < count[b], cache row len[b] + i receives d->k's row i, rotated (r NULL:
  * as it is), and d->v's as it is; len_out[b] = len[b] + count[b] (len_out may not be len). d->q, where not NULL, goes to q_out,
  * rotated; k_out, where not NULL, receives the rotated keys too (drafted rows for tg_cuda_tree_attn): rows of q_out and
- * k_out past count are 0, and they may be d->q and d->k with the same strides. q_norm, k_norm (f32 [head_dim], NULL: none): before the
+ * k_out past count are 0, and they may be d->q and d->k with the same strides, but else share no memory with d->q, d->k, d->v or each other. q_norm, k_norm (f32 [head_dim], NULL: none): before the
  * rotation a row x becomes x / sqrt(mean(x^2) + eps) * norm. pos NULL: token i is at position len + i. tokens may be any
  * number, d->mask and d->scale are not read, and max_len bounds len before the call. A row past the table is not written and is
  * reported like a bad page. No two rows written may share a page row. */

@@ -144,6 +144,53 @@ int pg_apart(const char *who, const char *what, int row, std::array<long long, 3
 	return TG_CUDA_OK;
 }
 
+// The dimensions of more than one row, ascending; a stride of 0 adds no rows.
+struct PgDims {
+	__int128 row;
+	int count = 0;
+	long long stride[3];
+	long long n[3];
+
+	explicit PgDims(const PgRows &x) : row(x.row)
+	{
+		for (int i = 0; i < 3; i++) {
+			if (x.n[i] <= 1 || x.stride[i] == 0) continue;
+			int k = count++;
+			for (; k && stride[k - 1] > x.stride[i]; k--) stride[k] = stride[k - 1], n[k] = n[k - 1];
+			stride[k] = x.stride[i], n[k] = x.n[i];
+		}
+	}
+	__int128 span(int dims) const // of its first dimensions
+	{
+		__int128 s = row;
+		for (int i = 0; i < dims; i++) s += (__int128)stride[i] * (n[i] - 1);
+		return s;
+	}
+};
+
+// b's rows `off` bytes behind a's, of the first na and nb dimensions
+static bool dims_meet(const PgDims &a, int na, const PgDims &b, int nb, __int128 off)
+{
+	if (off >= a.span(na) || off + b.span(nb) <= 0) return false;
+	if (!na && !nb) return true;
+	const long long s = std::max(na ? a.stride[na - 1] : 0, nb ? b.stride[nb - 1] : 0);
+	const int ia = na && a.stride[na - 1] == s ? na - 1 : na, ib = nb && b.stride[nb - 1] == s ? nb - 1 : nb; // what lies within a step of s
+	if (a.span(ia) > s || b.span(ib) > s) return true;
+	const __int128 ca = ia < na ? a.n[ia] : 1, cb = ib < nb ? b.n[ib] : 1;
+	const __int128 j = -(off >= 0 ? off / s : -((-off + s - 1) / s)); // b's element x + j begins less than s behind a's element x, x + j - 1 before it
+	for (__int128 k = j - 1; k <= j; k++)
+		if (k > -ca && k < cb && dims_meet(a, ia, b, ib, off + k * s)) return true;
+	return false;
+}
+
+bool pg_meet(const PgRows &a, const PgRows &b)
+{
+	for (const PgRows *x : { &a, &b })
+		if (!x->at || x->row <= 0 || x->n[0] <= 0 || x->n[1] <= 0 || x->n[2] <= 0) return false;
+	const PgDims da(a), db(b);
+	return dims_meet(da, da.count, db, db.count, (__int128)(uintptr_t)b.at - (__int128)(uintptr_t)a.at);
+}
+
 bool pg_map(CUtensorMap *m, const PgCache &c, const void *pool, bool f16, int rows, PgBox *box)
 {
 	static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;

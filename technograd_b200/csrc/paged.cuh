@@ -109,6 +109,16 @@ int pg_drafts(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *desc, 
 // EINVAL where rows of `row` elements that a call writes overlap: they would be written in any order. They lie apart where each
 // dimension's stride spans all of the dimensions of smaller strides.
 int pg_apart(const char *who, const char *what, int row, std::array<long long, 3> stride, std::array<int, 3> n);
+// A call's rows, in bytes: n elements along each dimension, stride apart
+struct PgRows {
+	const void *at;
+	long long row;
+	std::array<long long, 3> stride;
+	std::array<int, 3> n;
+};
+// Whether rows of a and of b share memory. Exact where dimensions of the same stride lie one within the other on both sides (views of
+// one projection); other layouts whose ranges cross count as sharing.
+bool pg_meet(const PgRows &a, const PgRows &b);
 // The device's number and SM count, and the address of its status word; EDEVICE when a kernel
 // of an earlier call reported something.
 int pg_device(const char *who, int *sms, int **status);

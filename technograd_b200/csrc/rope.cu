@@ -429,6 +429,14 @@ static int turn_out(const char *who, const char *what, void *out, long long (&s)
 	return pg_apart(who, what, dim, { s[0], s[1], s[2] }, { seqs, tokens, heads });
 }
 
+// Rows that a call writes may not be rows that it reads, which other warps read at any time, nor other rows that it writes; those that
+// `same` names may be it, each in its own place (turn_out has looked at the strides).
+static int turn_apart(const char *who, const char *what, const PgRows &out, const PgRows &other, const char *name, bool same)
+{
+	if ((same && out.at == other.at) || !pg_meet(out, other)) return TG_CUDA_OK;
+	return set_err(TG_CUDA_EINVAL, "%s: %s and %s share memory", who, what, name);
+}
+
 } // namespace tgc
 
 using namespace tgc;
@@ -452,6 +460,9 @@ extern "C" int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tok
 	if (s[0] < 0 || s[1] < 0 || s[2] < 0) return set_err(TG_CUDA_EINVAL, "%s: negative strides", who);
 	if (((uintptr_t)x & 15) || ((s[0] | s[1] | s[2]) * e & 15)) return set_err(TG_CUDA_EINVAL, "%s: x rows must start on 16-byte boundaries", who);
 	if (!none && (rc = turn_out(who, "out", out, o, x, { s[0] * e, s[1] * e, s[2] * e }, seqs, tokens, heads, head_dim, e))) return rc;
+	if (!none && (rc = turn_apart(who, "out", { out, head_dim * e, { o[0] * e, o[1] * e, o[2] * e }, { seqs, tokens, heads } },
+				      { x, head_dim * e, { s[0] * e, s[1] * e, s[2] * e }, { seqs, tokens, heads } }, "x", true)))
+		return rc;
 	if ((rc = pg_sms(who, &dev, &sms)) || none) return rc;
 	p.rows[0] = { (const char *)x, (char *)out, nullptr, s[0] * e, s[1] * e, s[2] * e, o[0] * e, o[1] * e, o[2] * e, nullptr, heads, r->dim > 0, 0, 0 };
 	p.nrows = 1, p.all = (long long)seqs * tokens, p.tokens = tokens, p.dim = head_dim;
@@ -480,6 +491,13 @@ extern "C" int tg_cuda_kv_append(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	long long qo[3] = { q_out_seq, q_out_tok, q_out_head }, ko[3] = { k_out_seq, k_out_tok, k_out_head };
 	if (q && (rc = turn_out(who, "q_out", q_out, qo, pd.q, { pd.q_seq, pd.q_tok, pd.q_head }, c->seqs, d->tokens, d->nq, c->head_dim, e))) return rc;
 	if (k_out && (rc = turn_out(who, "k_out", k_out, ko, pd.k, { pd.kv_seq, pd.kv_tok, pd.kv_head }, c->seqs, d->tokens, c->nkv, c->head_dim, e))) return rc;
+	const long long row = c->head_dim * e;
+	const PgRows rq = { q ? pd.q : nullptr, row, { pd.q_seq, pd.q_tok, pd.q_head }, { c->seqs, d->tokens, d->nq } }, rk = { pd.k, row, { pd.kv_seq, pd.kv_tok, pd.kv_head }, { c->seqs, d->tokens, c->nkv } },
+		     rv = { pd.v, row, rk.stride, rk.n }, ro = { q ? q_out : nullptr, row, { qo[0] * e, qo[1] * e, qo[2] * e }, rq.n }, rl = { k_out, row, { ko[0] * e, ko[1] * e, ko[2] * e }, rk.n };
+	if ((rc = turn_apart(who, "q_out", ro, rq, "q", true)) || (rc = turn_apart(who, "q_out", ro, rk, "k", false)) || (rc = turn_apart(who, "q_out", ro, rv, "v", false)) ||
+	    (rc = turn_apart(who, "k_out", rl, rq, "q", false)) || (rc = turn_apart(who, "k_out", rl, rk, "k", true)) || (rc = turn_apart(who, "k_out", rl, rv, "v", false)) ||
+	    (rc = turn_apart(who, "q_out", ro, rl, "k_out", false)))
+		return rc;
 	if ((rc = pg_apart(who, "the cache", c->head_dim, {c->page_stride, c->head_stride, c->pos_stride}, {c->pages, c->nkv, c->page}))) return rc;
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0) return rc;
 	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim, !((uintptr_t)q_norm & 15), 0 };

@@ -437,7 +437,7 @@ def _along(ctx, x, inverse):
 def rope(x, rotary: Rotary, pos=None, inverse: bool = False, out=None):
     """x [seqs, tokens, heads, head_dim] rotated to its tokens' positions (tg_cuda_rope); pos int32 [seqs, tokens] or [tokens] (None: 0, 1, ...).
 
-    inverse: by the negative angle. out: where to (x itself: in place). Differentiable with respect to x in either mode, without out."""
+    inverse: by the negative angle. out: where to (x itself: in place; else memory that x does not share). Differentiable with respect to x in either mode, without out."""
     if (torch.is_grad_enabled() and x.requires_grad) or _tangent(x, out):
         _need(out is None, "out: not with a gradient or a tangent")
         return _Rope.apply(x, rotary, pos, inverse, False)
