@@ -444,7 +444,7 @@ int tg_cuda_attn_weights(const tg_cuda_kv *c, const tg_cuda_drafts *d, const flo
 
 /* Accepted tokens into the cache: for i < count[b], cache row len[b] + i receives drafted
  * row path[b][i] (path [seqs][tokens]; NULL = row i), keys and values, and len_out[b] =
- * len[b] + count[b] (len_out may not be len). fresh and acc, both or neither: acc[b][h][len + i]
+ * len[b] + count[b] (len_out shares no memory with len or count). fresh and acc, both or neither: acc[b][h][len + i]
  * = fresh[b][h][path[b][i]], acc [seqs][nkv][acc_cols] with the given strides. tokens may be
  * any number here, d->q is not read, and max_len bounds len before the call. A row past the
  * table, a path entry outside [0, tokens) or a column past acc_cols is not written and is
@@ -473,7 +473,7 @@ int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tokens, int he
 		 long long x_tok, long long x_head, void *out, long long out_seq, long long out_tok, long long out_head, void *stream);
 
 /* New tokens into the cache, rotated on the way: for i < count[b], cache row len[b] + i receives d->k's row i, rotated (r NULL:
- * as it is), and d->v's as it is; len_out[b] = len[b] + count[b] (len_out may not be len). d->q, where not NULL, goes to q_out,
+ * as it is), and d->v's as it is; len_out[b] = len[b] + count[b] (len_out shares no memory with len or count). d->q, where not NULL, goes to q_out,
  * rotated; k_out, where not NULL, receives the rotated keys too (drafted rows for tg_cuda_tree_attn): rows of q_out and
  * k_out past count are 0, and they may be d->q and d->k with the same strides, but else share no memory with d->q, d->k, d->v or each other. q_norm, k_norm (f32 [head_dim], NULL: none): before the
  * rotation a row x becomes x / sqrt(mean(x^2) + eps) * norm. pos NULL: token i is at position len + i. tokens may be any

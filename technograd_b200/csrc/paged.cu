@@ -191,6 +191,14 @@ bool pg_meet(const PgRows &a, const PgRows &b)
 	return dims_meet(da, da.count, db, db.count, (__int128)(uintptr_t)b.at - (__int128)(uintptr_t)a.at);
 }
 
+int pg_len_out(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, const int *len_out)
+{
+	auto ints = [&](const int *at) -> PgRows { return { at, 4ll * c->seqs, {}, { 1, 1, 1 } }; };
+	if (pg_meet(ints(len_out), ints(c->len))) return set_err(TG_CUDA_EINVAL, "%s: len_out may not share memory with the cache's len", who);
+	if (pg_meet(ints(len_out), ints(d->count))) return set_err(TG_CUDA_EINVAL, "%s: len_out may not share memory with count", who);
+	return TG_CUDA_OK;
+}
+
 bool pg_map(CUtensorMap *m, const PgCache &c, const void *pool, bool f16, int rows, PgBox *box)
 {
 	static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
@@ -294,7 +302,7 @@ extern "C" int tg_cuda_kv_commit(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	if ((rc = pg_cache(who, c, &p.c)) || (rc = pg_drafts(who, c, d, PG_USE_K | PG_USE_V, 0, &p.d))) return rc;
 	if (c->seqs && (!len_out || !fresh != !acc)) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);
 	if (((uintptr_t)path | (uintptr_t)len_out | (uintptr_t)fresh | (uintptr_t)acc) & 3) return set_err(TG_CUDA_EINVAL, "%s: a pointer is not on a 4-byte boundary", who);
-	if (len_out == c->len && c->seqs) return set_err(TG_CUDA_EINVAL, "%s: len_out may not be the cache's len", who);
+	if ((rc = pg_len_out(who, c, d, len_out))) return rc;
 	if (acc && acc_cols < 0) return set_err(TG_CUDA_EINVAL, "%s: acc_cols %d", who, acc_cols);
 	if (acc && (rc = pg_apart(who, "acc", acc_cols, {acc_seq, acc_head, 0}, {c->seqs, c->nkv, 1}))) return rc;
 	if ((rc = pg_apart(who, "the cache", c->head_dim, {c->page_stride, c->head_stride, c->pos_stride}, {c->pages, c->nkv, c->page}))) return rc;

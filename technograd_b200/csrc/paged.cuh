@@ -119,6 +119,8 @@ struct PgRows {
 // Whether rows of a and of b share memory. Exact where dimensions of the same stride lie one within the other on both sides (views of
 // one projection); other layouts whose ranges cross count as sharing.
 bool pg_meet(const PgRows &a, const PgRows &b);
+// EINVAL where len_out of an append or a commit shares memory with len or count, which other warps read while it is written
+int pg_len_out(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, const int *len_out);
 // The device's number and SM count, and the address of its status word; EDEVICE when a kernel
 // of an earlier call reported something.
 int pg_device(const char *who, int *sms, int **status);

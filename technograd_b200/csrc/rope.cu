@@ -485,7 +485,7 @@ extern "C" int tg_cuda_kv_append(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 	p.gain = 1;
 	if (r && (rc = turn_check(who, r, c->head_dim, c->seqs, &p))) return rc;
 	if (c->seqs && (!len_out || !d->q != !q_out)) return set_err(TG_CUDA_EINVAL, "%s: NULL pointer", who);
-	if (len_out == c->len && c->seqs) return set_err(TG_CUDA_EINVAL, "%s: len_out may not be the cache's len", who);
+	if ((rc = pg_len_out(who, c, d, len_out))) return rc;
 	if (((uintptr_t)len_out | (uintptr_t)q_norm | (uintptr_t)k_norm) & 3) return set_err(TG_CUDA_EINVAL, "%s: a pointer is not on a 4-byte boundary", who);
 	if (q_norm && !q) return set_err(TG_CUDA_EINVAL, "%s: q_norm without q", who);
 	long long qo[3] = { q_out_seq, q_out_tok, q_out_head }, ko[3] = { k_out_seq, k_out_tok, k_out_head };

@@ -1,4 +1,5 @@
 """Rotations and appends whose outputs lie over what the call reads: one warp would read what another has written (CPU)."""
+import ctypes as C
 import itertools
 import random
 
@@ -6,7 +7,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 from technograd_b200 import _lib  # noqa: E402
-from test_kvcache_abi import drafts, refused  # noqa: E402
+from test_kvcache_abi import cache, drafts, refused  # noqa: E402
 from test_rope_abi import append, rope, rotary  # noqa: E402
 
 X, ROW, DIM = 0x30000, 64 * 2, 64
@@ -95,3 +96,17 @@ def test_append_of_a_projection_in_place(no_gpu):
     assert accepted(append(d=d, q=(0x60000, *s), k=(0x60000 + 4 * ROW, *s)))
     for q, k in ((0, 6), (2, 4), (0, 3), (4, 0)):
         assert append(d=d, q=(X + q * ROW, *s), k=(X + k * ROW, *s)) == _lib.EINVAL
+
+
+@pytest.mark.parametrize("at", [0x2000, 0x2004, 0x1ffc, 0x7000, 0x7004])
+def test_new_lengths_over_what_is_read(at):
+    """Of 2 sequences' len at 0x2000 and count at 0x7000."""
+    d = drafts(count=0x7000)
+    refused(append(d=d, lens=at))
+    refused(_lib.lib().tg_cuda_kv_commit(C.byref(cache()), C.byref(d), None, at, None, None, 0, 0, 0, None))
+
+
+@pytest.mark.parametrize("at", [0x2008, 0x1ff8, 0x7008])
+def test_new_lengths_beside_what_is_read(no_gpu, at):
+    assert accepted(append(d=drafts(count=0x7000), lens=at))
+    assert accepted(_lib.lib().tg_cuda_kv_commit(C.byref(cache()), C.byref(drafts(count=0x7000)), None, at, None, None, 0, 0, 0, None))
