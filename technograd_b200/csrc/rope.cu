@@ -10,10 +10,10 @@ namespace tgc {
 // Rows that the kernel moves: heads of every token, from src to dst and, keys and values, to the token's cache row in pool.
 struct TurnRows {
 	const char *src;
-	char *dst, *pool;                  // either may be NULL
+	char *dst, *pool;                  // dst NULL: not wanted
 	long long s_seq, s_tok, s_head, d_seq, d_tok, d_head; // bytes
 	const float *norm;                 // [dim] or NULL
-	int heads, turn;
+	int heads, turn, cached;           // cached: into the pool
 	int aligned, chunks;               // norm lies on a 16-byte boundary; warps that have a token's rows of this kind
 };
 
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(128, 5) k_turn(const TurnArgs p, int lg)
 	if (p.c.len) {
 		len = p.c.length((int)b);
 		if (begin && i == 0 && lane == 0) p.len_out[b] = len + cnt;
-		if (p.rows[g].pool && live) {
+		if (p.rows[g].cached && live) {
 			const long long to = (long long)len + i;
 			if (to >= (long long)p.c.page * p.c.cols || to > 0x7fffffff) p.c.report(PG_ROOM);
 			else {
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(128) k_turn_any(const TurnArgs p)
 	if (p.c.len) {
 		len = p.c.length((int)b);
 		if (begin && i == 0 && lane == 0) p.len_out[b] = len + cnt;
-		if (k.pool && live) {
+		if (k.cached && live) {
 			const long long to = (long long)len + i;
 			if (to >= (long long)p.c.page * p.c.cols || to > 0x7fffffff) p.c.report(PG_ROOM);
 			else row = p.c.row(p.c.table + b * p.c.cols, (int)to);
@@ -464,7 +464,7 @@ extern "C" int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tok
 				      { x, head_dim * e, { s[0] * e, s[1] * e, s[2] * e }, { seqs, tokens, heads } }, "x", true)))
 		return rc;
 	if ((rc = pg_sms(who, &dev, &sms)) || none) return rc;
-	p.rows[0] = { (const char *)x, (char *)out, nullptr, s[0] * e, s[1] * e, s[2] * e, o[0] * e, o[1] * e, o[2] * e, nullptr, heads, r->dim > 0, 0, 0 };
+	p.rows[0] = { (const char *)x, (char *)out, nullptr, s[0] * e, s[1] * e, s[2] * e, o[0] * e, o[1] * e, o[2] * e, nullptr, heads, r->dim > 0, 0, 0, 0 };
 	p.nrows = 1, p.all = (long long)seqs * tokens, p.tokens = tokens, p.dim = head_dim;
 	return turn_type(p, type, r->interleaved, false, stream);
 }
@@ -500,9 +500,9 @@ extern "C" int tg_cuda_kv_append(const tg_cuda_kv *c, const tg_cuda_drafts *d, c
 		return rc;
 	if ((rc = pg_apart(who, "the cache", c->head_dim, {c->page_stride, c->head_stride, c->pos_stride}, {c->pages, c->nkv, c->page}))) return rc;
 	if ((rc = pg_device(who, &sms, &p.c.status)) || c->seqs == 0) return rc;
-	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim, !((uintptr_t)q_norm & 15), 0 };
-	p.rows[p.nrows++] = { pd.k, (char *)k_out, p.c.k, pd.kv_seq, pd.kv_tok, pd.kv_head, ko[0] * e, ko[1] * e, ko[2] * e, k_norm, c->nkv, r && r->dim, !((uintptr_t)k_norm & 15), 0 };
-	p.rows[p.nrows++] = { pd.v, nullptr, p.c.v, pd.kv_seq, pd.kv_tok, pd.kv_head, 0, 0, 0, nullptr, c->nkv, 0, 0, 0 };
+	if (q) p.rows[p.nrows++] = { pd.q, (char *)q_out, nullptr, pd.q_seq, pd.q_tok, pd.q_head, qo[0] * e, qo[1] * e, qo[2] * e, q_norm, d->nq, r && r->dim, 0, !((uintptr_t)q_norm & 15), 0 };
+	p.rows[p.nrows++] = { pd.k, (char *)k_out, p.c.k, pd.kv_seq, pd.kv_tok, pd.kv_head, ko[0] * e, ko[1] * e, ko[2] * e, k_norm, c->nkv, r && r->dim, 1, !((uintptr_t)k_norm & 15), 0 };
+	p.rows[p.nrows++] = { pd.v, nullptr, p.c.v, pd.kv_seq, pd.kv_tok, pd.kv_head, 0, 0, 0, nullptr, c->nkv, 0, 1, 0, 0 };
 	p.count = d->count, p.len_out = len_out, p.all = (long long)c->seqs * d->tokens, p.tokens = d->tokens, p.dim = c->head_dim, p.over_dim = 1.f / c->head_dim, p.eps = eps;
 	return turn_type(p, c->type, r && r->interleaved, q_norm || k_norm, stream);
 }
