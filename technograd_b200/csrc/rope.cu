@@ -33,15 +33,20 @@ struct TurnArgs {
 };
 
 // cos and sin of pos * freq. The angle is taken in turns, as 64 bits behind the point: whole turns fall off the product by
-// themselves, so a far position's angle is as exact as a near one's (2^-55 turns of the frequency times the position).
-// Its first 32 bits, to 2^-32 turns, are a quarter turn and a rest of at most an eighth, x = 2 pi rest, whose sine and cosine
-// are their Taylor series up to x^9 and x^10: what is left out is below (pi/4)^11 / 11! = 1.8e-9 and (pi/4)^12 / 12! = 1.2e-10.
+// themselves, so a far position's angle is as exact as a near one's. freq / 2 pi is taken in two parts, of twice 53 bits, and rounded to
+// 2^-65 turns, which a position of 32 bits makes 2^-33; the product's first 32 bits are rounded to 2^-33 too: 2^-29.3 radians
+// together (for frequencies below 2^40; one part and no rounding left 2^-22 at positions of 2^31).
+// These 32 bits are a quarter turn and a rest of at most an eighth, x = 2 pi rest, whose sine and cosine
+// are their Taylor series up to x^9 and x^10: what is left out is below (pi/4)^11 / 11! = 1.8e-9 and (pi/4)^12 / 12! = 1.2e-10, and
+// over all 2^30 rests they are off by 1.10e-7 and 1.02e-7 at most, below 2^-23.
 __device__ __forceinline__ float2 turn_of(double freq, int pos)
 {
-	double f = freq * 0.15915494309189535; // 1 / 2 pi
-	f -= rint(f);
-	const unsigned long long u = (unsigned long long)__double2ll_rn(f * 0x1p63) << 1;
-	const unsigned t = (unsigned)(u * (unsigned long long)(long long)pos >> 32), q = (t + (1u << 29)) >> 30;
+	const double turns = freq * 0.15915494309189535; // 1 / 2 pi; what it is short of that is the next line's factor
+	const double low = fma(freq, -9.839338337591243e-18, fma(freq, 0.15915494309189535, -turns));
+	const double f = (turns - rint(turns)) * 0x1p63;
+	const long long i = __double2ll_rn(f);
+	const unsigned long long u = ((unsigned long long)i << 1) + (unsigned long long)__double2ll_rn(fma(low, 0x1p64, 2 * (f - (double)i)));
+	const unsigned t = (unsigned)((u * (unsigned long long)(long long)pos + (1ull << 31)) >> 32), q = (t + (1u << 29)) >> 30;
 	const float x = (float)(int)(t - (q << 30)) * 1.4629180792671596e-9f, z = x * x; // 2 pi / 2^32
 	const float s = x * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1 / 362880.f, -1 / 5040.f), 1 / 120.f), -1 / 6.f), 1.f);
 	const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1 / 3628800.f, 1 / 40320.f), -1 / 720.f), 1 / 24.f), -0.5f), 1.f);

@@ -1,0 +1,65 @@
+"""Angles of rotations against integers (GPU): pos freq / 2 pi, freq being the given f64 and 1 / 2 pi having 300 bits.
+
+The header's bounds: the angle to 2^-29, cos and sin of it to 2^-23. Rows (1, 0) turn into (cos, sin), with no further rounding in f32."""
+import math
+
+import pytest
+import torch
+
+from technograd_b200 import kvcache
+
+pytestmark = pytest.mark.gpu
+BITS = 300
+
+
+def arctan(n):
+    """2^BITS arctan(1 / n)."""
+    total, term, k = 0, (1 << BITS) // n, 1
+    while term:
+        total += (term // k) * (1 if k % 4 == 1 else -1)
+        term, k = term // (n * n), k + 2
+    return total
+
+
+TWO_PI = 8 * (4 * arctan(5) - arctan(239))  # 2^BITS times it, but for a few units
+
+
+ONE_TURN = (1 << 2 * BITS) // TWO_PI  # 2^BITS / 2 pi
+
+
+def angles(pos, freq):
+    """pos freq but for whole turns, [positions][frequencies] f64."""
+    def one(p, f):
+        m, d = f.as_integer_ratio()
+        turns = m * p * ONE_TURN // d % (1 << BITS)
+        turns -= (turns >> BITS - 1) << BITS
+        return (turns * TWO_PI >> BITS) / (1 << BITS)
+    return torch.tensor([[one(p, f) for f in freq] for p in pos], dtype=torch.float64)
+
+
+def check(got, want, what):
+    """got [rows][2 half] of rows (1, 0), f32, want their angles."""
+    half = want.shape[1]
+    for x, y in ((got[:, :half].double().cpu(), want.cos()), (got[:, half:].double().cpu(), want.sin())):
+        assert (x - y).abs().max() <= 2.0 ** -23 + 2.0 ** -29, (what, float((x - y).abs().max()))
+
+
+def test_two_pi():
+    assert abs(TWO_PI / (1 << BITS) - 2 * math.pi) < 1e-15
+
+
+FREQUENCIES = [kvcache.rotary_frequencies(256, 1e4), kvcache.rotary_frequencies(256, 1e6, 4.0, 32768), kvcache.rotary_frequencies(256, 5e5, 8.0),
+               torch.tensor([(-1) ** i * 3.7 ** (i / 4 - 20) for i in range(128)], dtype=torch.float64)]  # 1e-12 to 1e6, of both signs
+
+
+@pytest.mark.parametrize("freq", FREQUENCIES)
+@pytest.mark.parametrize("inverse", [False, True])
+def test_angles(cuda, freq, inverse):
+    """Near positions, far ones, and those at the ends of 32 bits."""
+    g = torch.Generator().manual_seed(30)
+    pos = torch.cat([torch.randint(-top, top, (40,), generator=g) for top in (100, 1 << 14, 1 << 20, 1 << 24, 1 << 27, 1 << 31)] +
+                    [torch.tensor([0, 1, -1, 2 ** 31 - 1, -2 ** 31, 2 ** 24 + 1, 2 ** 30 + 1])]).to(torch.int32)
+    x = torch.zeros(1, len(pos), 1, 256, device="cuda")
+    x[..., :128] = 1
+    y = kvcache.rope(x, kvcache.Rotary(256, freq.cuda()), pos.cuda(), inverse)
+    check(y[0, :, 0], angles([-p if inverse else p for p in pos.tolist()], freq.tolist()), "y")
