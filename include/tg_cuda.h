@@ -455,7 +455,8 @@ int tg_cuda_kv_commit(const tg_cuda_kv *c, const tg_cuda_drafts *d, const int *p
 /* Rotary positions: of a head's first `dim` elements, element a and its partner b become
  *   gain (x_a cos f - x_b sin f) and gain (x_a sin f + x_b cos f),  f = pos freq[i],
  * (a, b) = (i, i + dim / 2) or, interleaved, (2 i, 2 i + 1), for i < dim / 2; the others pass. The angle
- * is exact to 2^-29 radians however far the position (of freq as it is given, below 2^40), cos and sin of it to 2^-23, and a result is rounded once. */
+ * is exact to 2^-29 radians however far the position (of freq as it is given, below 2^40), cos and sin of it to 2^-23, and a result is rounded once. What turns
+ * by a freq that is an infinity or a NaN becomes NaN. */
 typedef struct {
 	int dim;                 /* elements that turn: even, 0 to head_dim */
 	int interleaved;         /* 0 or 1: which elements are partners */

@@ -44,6 +44,7 @@ __device__ __forceinline__ float2 turn_of(double freq, int pos)
 	const double turns = freq * 0.15915494309189535; // 1 / 2 pi; what it is short of that is the next line's factor
 	const double low = fma(freq, -9.839338337591243e-18, fma(freq, 0.15915494309189535, -turns));
 	const double f = (turns - rint(turns)) * 0x1p63;
+	if (isnan(f)) return make_float2(NAN, NAN); // freq is an infinity or no number
 	const long long i = __double2ll_rn(f);
 	const unsigned long long u = ((unsigned long long)i << 1) + (unsigned long long)__double2ll_rn(fma(low, 0x1p64, 2 * (f - (double)i)));
 	const unsigned t = (unsigned)((u * (unsigned long long)(long long)pos + (1ull << 31)) >> 32), q = (t + (1u << 29)) >> 30;

@@ -63,3 +63,19 @@ def test_angles(cuda, freq, inverse):
     x[..., :128] = 1
     y = kvcache.rope(x, kvcache.Rotary(256, freq.cuda()), pos.cuda(), inverse)
     check(y[0, :, 0], angles([-p if inverse else p for p in pos.tolist()], freq.tolist()), "y")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("part,pairs", [(16, False), (16, True), (14, False)])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_frequencies_that_are_no_numbers(cuda, dtype, part, pairs, inverse):
+    """NaN, at position 0 too, as the formula has it (0 times infinity), in that pair alone."""
+    freq = [1.0, math.nan, 0.5, math.inf, -math.inf, 0.0, 1e-300, 1e300][:part // 2]
+    x = torch.randn(1, 3, 5, 16, generator=torch.Generator().manual_seed(31)).to(dtype).cuda()
+    y = kvcache.rope(x, kvcache.Rotary(16, torch.tensor(freq, dtype=torch.float64).cuda(), interleaved=pairs), torch.tensor([0, 1, 7], dtype=torch.int32, device="cuda"), inverse)
+    bad = torch.zeros(16, dtype=torch.bool)
+    for i, f in enumerate(freq):
+        if not math.isfinite(f):
+            for e in (2 * i, 2 * i + 1) if pairs else (i, i + part // 2):
+                bad[e] = True
+    assert torch.isnan(y[..., bad.cuda()]).all() and torch.isfinite(y[..., ~bad.cuda()]).all()
