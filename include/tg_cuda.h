@@ -474,7 +474,7 @@ int tg_cuda_rope(const tg_cuda_rotary *r, int type, int seqs, int tokens, int he
 		 long long x_tok, long long x_head, void *out, long long out_seq, long long out_tok, long long out_head, void *stream);
 
 /* New tokens into the cache, rotated on the way: for i < count[b], cache row len[b] + i receives d->k's row i, rotated (r NULL:
- * as it is), and d->v's as it is; len_out[b] = len[b] + count[b] (len_out shares no memory with len or count). d->q, where not NULL, goes to q_out,
+ * as it is), and d->v's as it is; len_out[b] = len[b] + count[b], at most 2^31 - 1 (len_out shares no memory with len or count). d->q, where not NULL, goes to q_out,
  * rotated; k_out, where not NULL, receives the rotated keys too (drafted rows for tg_cuda_tree_attn): rows of q_out and
  * k_out past count are 0, and they may be d->q and d->k with the same strides, but else share no memory with d->q, d->k, d->v or each other. q_norm, k_norm (f32 [head_dim], NULL: none): before the
  * rotation a row x becomes x / sqrt(mean(x^2) + eps) * norm. pos NULL: token i is at position len + i. tokens may be any

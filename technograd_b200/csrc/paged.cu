@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(256) k_commit(const CommitArgs p)
 	const int i = (int)(w - b * p.d.tokens);
 	if (b >= p.seqs) return;
 	const int n = p.c.length((int)b), cnt = p.d.drafted((int)b);
-	if (i == 0 && lane == 0) p.len_out[b] = n + cnt;
+	if (i == 0 && lane == 0) p.len_out[b] = p.c.grown(n, cnt);
 	if (i >= cnt) return;
 	const int from = p.path ? p.path[b * p.d.tokens + i] : i;
 	const long long at = (long long)n + i;

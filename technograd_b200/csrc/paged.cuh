@@ -35,6 +35,8 @@ struct PgCache {
 		if (n < 0 || n > max_len) report(PG_LEN);
 		return n < 0 ? 0 : n > max_len ? max_len : n;
 	}
+	// a length with `more` rows behind it, at most the largest int
+	static __device__ __forceinline__ int grown(int n, int more) { return (int)min((unsigned)n + (unsigned)more, 0x7fffffffu); }
 	// byte offset of a sequence's row (head 0) at position p, -1 where the page number is not one
 	__device__ __forceinline__ long long row(const int *tab, int p) const
 	{

@@ -39,7 +39,7 @@ struct TurnArgs {
 // These 32 bits are a quarter turn and a rest of at most an eighth, x = 2 pi rest, whose sine and cosine
 // are their Taylor series up to x^9 and x^10: what is left out is below (pi/4)^11 / 11! = 1.8e-9 and (pi/4)^12 / 12! = 1.2e-10, and
 // over all 2^30 rests they are off by 1.10e-7 and 1.02e-7 at most, below 2^-23.
-__device__ __forceinline__ float2 turn_of(double freq, int pos)
+__device__ __forceinline__ float2 turn_of(double freq, long long pos)
 {
 	const double turns = freq * 0.15915494309189535; // 1 / 2 pi; what it is short of that is the next line's factor
 	const double low = fma(freq, -9.839338337591243e-18, fma(freq, 0.15915494309189535, -turns));
@@ -47,7 +47,7 @@ __device__ __forceinline__ float2 turn_of(double freq, int pos)
 	if (isnan(f)) return make_float2(NAN, NAN); // freq is an infinity or no number
 	const long long i = __double2ll_rn(f);
 	const unsigned long long u = ((unsigned long long)i << 1) + (unsigned long long)__double2ll_rn(fma(low, 0x1p64, 2 * (f - (double)i)));
-	const unsigned t = (unsigned)((u * (unsigned long long)(long long)pos + (1ull << 31)) >> 32), q = (t + (1u << 29)) >> 30;
+	const unsigned t = (unsigned)((u * (unsigned long long)pos + (1ull << 31)) >> 32), q = (t + (1u << 29)) >> 30;
 	const float x = (float)(int)(t - (q << 30)) * 1.4629180792671596e-9f, z = x * x; // 2 pi / 2^32
 	const float s = x * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1 / 362880.f, -1 / 5040.f), 1 / 120.f), -1 / 6.f), 1.f);
 	const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1 / 3628800.f, 1 / 40320.f), -1 / 720.f), 1 / 24.f), -0.5f), 1.f);
@@ -106,10 +106,10 @@ __device__ __forceinline__ float4 turn_weights(const TurnRows &w, int at)
 	return w.aligned ? *(const float4 *)(w.norm + at) : make_float4(w.norm[at], w.norm[at + 1], w.norm[at + 2], w.norm[at + 3]);
 }
 
-// Position of a token. (An addition past 32 bits comes round, as an angle may.)
-__device__ __forceinline__ int turn_pos(const TurnArgs &p, long long b, int i, int len)
+// Position of a token: behind a long cache past 32 bits
+__device__ __forceinline__ long long turn_pos(const TurnArgs &p, long long b, int i, int len)
 {
-	return p.pos ? p.pos[b * p.pos_seq + i] : (int)((unsigned)len + (unsigned)i);
+	return p.pos ? p.pos[b * p.pos_seq + i] : (long long)len + i;
 }
 
 // A warp has UN rounds of one token's rows of one kind (q, k or v): 1 << lg threads a row, each with two 16-byte pieces, those
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(128, 5) k_turn(const TurnArgs p, int lg)
 	char *pool = nullptr;
 	if (p.c.len) {
 		len = p.c.length((int)b);
-		if (begin && i == 0 && lane == 0) p.len_out[b] = len + cnt;
+		if (begin && i == 0 && lane == 0) p.len_out[b] = p.c.grown(len, cnt);
 		if (p.rows[g].cached && live) {
 			const long long to = (long long)len + i;
 			if (to >= (long long)p.c.page * p.c.cols || to > 0x7fffffff) p.c.report(PG_ROOM);
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(128, 5) k_turn(const TurnArgs p, int lg)
 	if (live && (turns || norm)) { // (else the bits pass as they are)
 		float2 c[E / 2], s[E / 2], ns[E / 2], wx[E / 2], wy[E / 2]; // two pairs' cos, sin and -sin; the pieces' weights
 		if (turns) {
-			const int pos = turn_pos(p, b, i, len);
+			const long long pos = turn_pos(p, b, i, len);
 			float2 own[PART];
 #pragma unroll
 			for (int x = 0; x < PART; x++) {
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(128) k_turn_any(const TurnArgs p)
 	long long row = -1;
 	if (p.c.len) {
 		len = p.c.length((int)b);
-		if (begin && i == 0 && lane == 0) p.len_out[b] = len + cnt;
+		if (begin && i == 0 && lane == 0) p.len_out[b] = p.c.grown(len, cnt);
 		if (k.cached && live) {
 			const long long to = (long long)len + i;
 			if (to >= (long long)p.c.page * p.c.cols || to > 0x7fffffff) p.c.report(PG_ROOM);

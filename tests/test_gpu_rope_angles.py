@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from technograd_b200 import kvcache
+from test_gpu_kvcache import F32, Case, reported
 
 pytestmark = pytest.mark.gpu
 BITS = 300
@@ -22,8 +23,6 @@ def arctan(n):
 
 
 TWO_PI = 8 * (4 * arctan(5) - arctan(239))  # 2^BITS times it, but for a few units
-
-
 ONE_TURN = (1 << 2 * BITS) // TWO_PI  # 2^BITS / 2 pi
 
 
@@ -79,3 +78,22 @@ def test_frequencies_that_are_no_numbers(cuda, dtype, part, pairs, inverse):
             for e in (2 * i, 2 * i + 1) if pairs else (i, i + part // 2):
                 bad[e] = True
     assert torch.isnan(y[..., bad.cuda()]).all() and torch.isfinite(y[..., ~bad.cuda()]).all()
+
+
+@pytest.mark.parametrize("part", [16, 6])
+def test_positions_behind_a_cache_of_nearly_32_bits(cuda, part):
+    """len + i past 2^31: such a row is not written to the cache, and its angle is that of its own position."""
+    dim, T, top = 16, 70000, 0x7fff0000
+    k = torch.zeros(0, 1, 1 << 30, dim, device="cuda")
+    table = torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    r = kvcache.Rotary(dim, theta=1e4, part=part)
+    cache = kvcache.PagedKV(k, k, table, torch.tensor([top - 7], dtype=torch.int32, device="cuda"), max_len=top)
+    x = torch.zeros(1, T, 1, dim, device="cuda")
+    x[..., :part // 2] = 1
+    lens, q, kr = kvcache.append(cache, x, x, q=x, rotary=r, keys=True)
+    good = Case([5], 1, 1, 64, 16, "head", F32, 1)
+    assert "past the table" in reported(lambda: kvcache.tree_attention(good.cache, good.q.cuda(), good.kn.cuda(), good.vn.cuda()))
+    assert lens.tolist() == [2 ** 31 - 1]
+    at = [0, 1, 65535, 65536 + 6, 65536 + 7, 65536 + 8, T - 1]
+    want = angles([top - 7 + i for i in at], r.freq.tolist())
+    check(q[0, at, 0, :part], want, "q"), check(kr[0, at, 0, :part], want, "k")
