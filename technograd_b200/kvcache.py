@@ -229,7 +229,8 @@ class SharedPrefix:
     groups: (first sequence, sequences, shared positions) of each, ascending; sequences in none share nothing. The tables of a group's sequences
     name the same pages for the shared positions. max_own: about how many positions a sequence has at most behind what it
     shares (default: what max_len leaves); it only sizes the launches, and the lengths may grow past it. always: share even where
-    tree_attention's way, a prefix read for each sequence, is faster (few sequences, short prefixes)."""
+    tree_attention's way, a prefix read for each sequence, is faster (few sequences, short prefixes). Like any input, it has to live as long as a
+    CUDA graph that was captured with it."""
 
     def __init__(self, cache: PagedKV, groups, max_own: int | None = None, always: bool = False):
         groups = [tuple(int(x) for x in g) for g in groups]
@@ -248,7 +249,7 @@ class SharedPrefix:
         _int32(max_own=max_own)
         made = torch.tensor([g[0] for g in groups] + [g[1] for g in groups] + lengths + which, dtype=torch.int32).to(cache.device)
         n, at = len(groups), made.data_ptr()
-        self._held = made
+        self._held, self._stream = made, torch._C._cuda_getCurrentRawStream(cache.index) if made.is_cuda else 0
         self._struct = _lib.Prefix(n, self.max_shared, max_own, bool(always), at, at + 4 * n, at + 8 * n, at + 12 * n)
         self._at = C.addressof(self._struct)
 
@@ -273,6 +274,8 @@ def shared_attention(cache: PagedKV, prefix: SharedPrefix, q, k, v, mask=None, c
     size, like = plan
     out, lse = torch.empty_like(q), torch.empty_like(like)
     work = q.new_empty(size, dtype=torch.uint8) if size else None  # held until the kernels are launched, as above
+    if stream != prefix._stream:  # the prefix may be dropped while this stream's kernels have yet to read it
+        prefix._held.record_stream(torch.cuda.current_stream(cache.index))
     so = out.stride()
     _lib.check(_lib.lib().tg_cuda_shared_attn(cache._at, d, prefix._at, out.data_ptr(), so[0], so[1], so[2], lse.data_ptr(),
                                               work.data_ptr() if size else None, size, stream))
