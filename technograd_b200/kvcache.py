@@ -252,6 +252,7 @@ class SharedPrefix:
         self._held, self._stream = made, torch._C._cuda_getCurrentRawStream(cache.index) if made.is_cuda else 0
         self._struct = _lib.Prefix(n, self.max_shared, max_own, bool(always), at, at + 4 * n, at + 8 * n, at + 12 * n)
         self._at = C.addressof(self._struct)
+        self._sizes = n, self.max_shared, max_own, bool(always)  # all that the scratch's size depends on
 
 
 def shared_attention(cache: PagedKV, prefix: SharedPrefix, q, k, v, mask=None, count=None, scale: float | None = None):
@@ -264,12 +265,14 @@ def shared_attention(cache: PagedKV, prefix: SharedPrefix, q, k, v, mask=None, c
     _no_tangent("shared_attention", q, k, v)
     d = _drafts(cache, q, k, v, mask, count, scale)
     stream, shape = _stream(cache), q.shape
-    key = shape[1], shape[2], prefix
+    key = shape[1], shape[2], prefix._sizes
     plan = cache._plans.get(key)
     if plan is None:
         size = _lib.lib().tg_cuda_shared_attn_workspace(cache._at, d, prefix._at)
         if size < 0:
             _lib.check(size)
+        if len(cache._plans) >= 64:  # a long-lived cache sees many batches
+            cache._plans.clear()
         plan = cache._plans[key] = size, cache._one.expand(shape[:3])
     size, like = plan
     out, lse = torch.empty_like(q), torch.empty_like(like)
