@@ -355,7 +355,20 @@ static int turn_check(const char *who, const tg_cuda_rotary *r, int head_dim, in
 	return TG_CUDA_OK;
 }
 
-constexpr int TURN_MANY = 2048; // tokens
+// Whether a warp takes four rounds rather than two: where there are many rows, and a token's heads leave few of four rounds' places empty (with norms,
+// whose weights are then looked up half as often, some more). Measured, us, two rounds and four (bf16, 128 dimensions, four rounds being 16
+// rows): 16 heads of 4096 tokens 8.1 and 8.3, of 32768 43.8 and 42.0; 32 heads of 2048 8.1 and 8.4, of 32768 84.3 and 80.5; 8 heads of 32768 23.6 and
+// 27.6, 1 head 18.3 and 22.9. Appends of 16 prompts of 2047 tokens with norms: 32 query heads over 8 191 and 161, 16 over 8 129 and 119, 8 key heads
+// alone 64 and 68; without, 16 over 8 89 and 94, 32 over 4 120 and 117. f32, 16 over 8: 173 and 161 with norms, 160 and 161 without.
+constexpr long long TURN_MANY = 3 << 15; // rows
+
+static bool turn_four(const TurnArgs &p, bool norm, int lg)
+{
+	const long long fit = 4 << (5 - lg);
+	long long rows = 0, places = 0;
+	for (int g = 0; g < p.nrows; g++) rows += p.rows[g].heads, places += (p.rows[g].heads + fit - 1) / fit * fit;
+	return p.all >= (TURN_MANY + rows - 1) / rows && rows * 8 >= places * (norm ? 5 : 6);
+}
 
 static int turn_grid(long long blocks)
 {
@@ -376,12 +389,11 @@ static int turn_launch(TurnArgs &p, bool norm, int lg, cudaStream_t st)
 	return TG_CUDA_OK;
 }
 
-// Few tokens: two rounds a warp, for more warps
 template <class T, int FORM, int PART>
 static int turn_rounds(TurnArgs &p, bool norm, int lg, cudaStream_t st)
 {
 	const bool full = p.dim * (int)sizeof(T) == 32 << lg;
-	if (p.all < TURN_MANY) return full ? turn_launch<T, FORM, PART, 2, true>(p, norm, lg, st) : turn_launch<T, FORM, PART, 2, false>(p, norm, lg, st);
+	if (!turn_four(p, norm, lg)) return full ? turn_launch<T, FORM, PART, 2, true>(p, norm, lg, st) : turn_launch<T, FORM, PART, 2, false>(p, norm, lg, st);
 	return full ? turn_launch<T, FORM, PART, 4, true>(p, norm, lg, st) : turn_launch<T, FORM, PART, 4, false>(p, norm, lg, st);
 }
 
