@@ -68,6 +68,12 @@ static void shared_split(AttnPlan &pre, AttnPlan &own, int own_len)
 	else if (own.grid > rest) own.grid = rest;
 }
 
+// What beginning a prefix's unit counts, in tiles of 128 rows: little where a CTA has few tiles and more shares shorten the call, more where shares
+// would else be uneven. The whole call, us, with 2 and with 6 (8 key heads of 128 dimensions, two query heads each, bf16): 4 sequences below 4096 21.4 and
+// 24.0, 8 below 2048 18.8 and 23.6, 16 below 8192 26.2 and 28.0, all below 7 tiles an SM; above, 8 below 16384 31.4 and 30.9, 8 of 8 query heads each below
+// 65536 52.9 and 50.9, 40 of 21 tokens below 16384 193 and 191.
+constexpr int SHARED_BEGIN = 2, SHARED_BEGIN_LONG = 6, SHARED_LONG = 7;
+
 static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, const tg_cuda_prefix *x, SharedPlan *o)
 {
 	tg_cuda_kv tail = *c;
@@ -87,7 +93,7 @@ static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, 
 	const int rt = p.tc ? 128 : p.fma ? p.fma : 16 * p.mt, tk = p.tc ? 128 : c->type == TG_CUDA_F32 ? 32 : 64;
 	const long long pitch = rows / rt + x->groups + 1, units = c->nkv * pitch, tiles = ((long long)x->max_shared + tk - 1) / tk;
 	if (units > 0x7fffffff || rows * c->nkv > 0x7fffffff) return set_err(TG_CUDA_EINVAL, "%s: %d sequences of %d tokens and %d heads", who, c->seqs, d.tokens, d.nq);
-	p.least = 128 / tk, p.begin = p.tc && units * tiles > 7ll * p.sms ? 6 : 2;
+	p.least = 128 / tk, p.begin = p.tc && units * tiles > (long long)SHARED_LONG * p.sms ? SHARED_BEGIN_LONG : SHARED_BEGIN;
 	p.slot = (size_t)(rt * p.dp + 2 * rt) * 4;
 	const long long shares = (units * (tiles + p.begin) + p.least + p.begin - 1) / (p.least + p.begin), wave = (long long)p.sms * (p.tc || p.dp == 256 ? 1 : p.fma || (p.mt == 1 && c->type != TG_CUDA_F32) ? 3 : 2);
 	p.grid = (int)std::min(shares, wave), p.units = (int)units, p.row_tiles = 1;
