@@ -355,19 +355,23 @@ static int turn_check(const char *who, const tg_cuda_rotary *r, int head_dim, in
 	return TG_CUDA_OK;
 }
 
-// Whether a warp takes four rounds rather than two: where there are many rows, and a token's heads leave few of four rounds' places empty (with norms,
-// whose weights are then looked up half as often, some more). Measured, us, two rounds and four (bf16, 128 dimensions, four rounds being 16
+// Whether a warp takes four rounds rather than two: where there are many bytes, and that saves a third of the warps, or with norms, whose weights
+// are then looked up half as often, a quarter (else its places are mostly empty). Measured, us, two rounds and four (bf16, 128 dimensions, four rounds being 16
 // rows): 16 heads of 4096 tokens 8.1 and 8.3, of 32768 43.8 and 42.0; 32 heads of 2048 8.1 and 8.4, of 32768 84.3 and 80.5; 8 heads of 32768 23.6 and
 // 27.6, 1 head 18.3 and 22.9. Appends of 16 prompts of 2047 tokens with norms: 32 query heads over 8 191 and 161, 16 over 8 129 and 119, 8 key heads
-// alone 64 and 68; without, 16 over 8 89 and 94, 32 over 4 120 and 117. f32, 16 over 8: 173 and 161 with norms, 160 and 161 without.
-constexpr long long TURN_MANY = 3 << 15; // rows
+// alone 64 and 68; without, 16 over 8 89 and 94, 32 over 4 120 and 117. f32, 16 over 8: 173 and 161 with norms, 160 and 161
+// without; 2 prompts of 1024 13.1 and 12.3, 11.2 and 9.7 (bf16 10.0 and 10.9, 7.0 and 8.0).
+constexpr long long TURN_MANY = 24 << 20; // bytes
 
-static bool turn_four(const TurnArgs &p, bool norm, int lg)
+static bool turn_four(const TurnArgs &p, bool norm, int lg, int e)
 {
-	const long long fit = 4 << (5 - lg);
-	long long rows = 0, places = 0;
-	for (int g = 0; g < p.nrows; g++) rows += p.rows[g].heads, places += (p.rows[g].heads + fit - 1) / fit * fit;
-	return p.all >= (TURN_MANY + rows - 1) / rows && rows * 8 >= places * (norm ? 5 : 6);
+	const int r = 1 << (5 - lg); // rows of a round
+	long long rows = 0, two = 0, four = 0; // of a token: rows, and the warps that have them
+	for (int g = 0; g < p.nrows; g++) {
+		const int h = p.rows[g].heads;
+		rows += h, two += (h + 2 * r - 1) / (2 * r), four += (h + 4 * r - 1) / (4 * r);
+	}
+	return p.all >= TURN_MANY / (rows * p.dim * e) && (norm ? four * 4 <= two * 3 : four * 3 <= two * 2);
 }
 
 static int turn_grid(long long blocks)
@@ -393,7 +397,7 @@ template <class T, int FORM, int PART>
 static int turn_rounds(TurnArgs &p, bool norm, int lg, cudaStream_t st)
 {
 	const bool full = p.dim * (int)sizeof(T) == 32 << lg;
-	if (!turn_four(p, norm, lg)) return full ? turn_launch<T, FORM, PART, 2, true>(p, norm, lg, st) : turn_launch<T, FORM, PART, 2, false>(p, norm, lg, st);
+	if (!turn_four(p, norm, lg, (int)sizeof(T))) return full ? turn_launch<T, FORM, PART, 2, true>(p, norm, lg, st) : turn_launch<T, FORM, PART, 2, false>(p, norm, lg, st);
 	return full ? turn_launch<T, FORM, PART, 4, true>(p, norm, lg, st) : turn_launch<T, FORM, PART, 4, false>(p, norm, lg, st);
 }
 
