@@ -35,18 +35,21 @@ struct TurnArgs {
 // cos and sin of pos * freq. The angle is taken in turns, as 64 bits behind the point: whole turns fall off the product by
 // themselves, so a far position's angle is as exact as a near one's. freq / 2 pi is taken in two parts, of twice 53 bits, and rounded to
 // 2^-65 turns, which a position of 32 bits makes 2^-33; the product's first 32 bits are rounded to 2^-33 too: 2^-29.3 radians
-// together (for frequencies below 2^40; one part and no rounding left 2^-22 at positions of 2^31).
+// together (for frequencies below 2^40; one part and no rounding left 2^-22 at positions of 2^31). Bits behind the point come from sums with
+// a number whose last bit is theirs: conversions between f64 and integers, at a quarter of f64's rate, took 99 us where these take 87 (k_turn_any's
+// example, below; 83 with one part).
 // These 32 bits are a quarter turn and a rest of at most an eighth, x = 2 pi rest, whose sine and cosine
 // are their Taylor series up to x^9 and x^10: what is left out is below (pi/4)^11 / 11! = 1.8e-9 and (pi/4)^12 / 12! = 1.2e-10, and
 // over all 2^30 rests they are off by 1.10e-7 and 1.02e-7 at most, below 2^-23.
 __device__ __forceinline__ float2 turn_of(double freq, long long pos)
 {
+	constexpr double WHOLE = 0x1.8p52, UPPER = 0x1.8p20, LOWER = 0x1.8p-12; // last bits 1, 2^-32 and 2^-64
 	const double turns = freq * 0.15915494309189535; // 1 / 2 pi; what it is short of that is the next line's factor
 	const double low = fma(freq, -9.839338337591243e-18, fma(freq, 0.15915494309189535, -turns));
-	const double f = (turns - rint(turns)) * 0x1p63;
+	const double f = turns - ((turns + WHOLE) - WHOLE);
 	if (isnan(f)) return make_float2(NAN, NAN); // freq is an infinity or no number
-	const long long i = __double2ll_rn(f);
-	const unsigned long long u = ((unsigned long long)i << 1) + (unsigned long long)__double2ll_rn(fma(low, 0x1p64, 2 * (f - (double)i)));
+	const double u0 = f + UPPER, u1 = (f - (u0 - UPPER)) + low + LOWER;
+	const unsigned long long u = ((unsigned long long)__double_as_longlong(u0) << 32) + (unsigned long long)(__double_as_longlong(u1) - __double_as_longlong(LOWER));
 	const unsigned t = (unsigned)((u * (unsigned long long)pos + (1ull << 31)) >> 32), q = (t + (1u << 29)) >> 30;
 	const float x = (float)(int)(t - (q << 30)) * 1.4629180792671596e-9f, z = x * x; // 2 pi / 2^32
 	const float s = x * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1 / 362880.f, -1 / 5040.f), 1 / 120.f), -1 / 6.f), 1.f);
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(128, 5) k_turn(const TurnArgs p, int lg)
 // Halves that begin within a 16-byte piece: a warp a row, element by element. A thread has the pairs lane, lane + 32, ... of a row
 // (behind the rotated part, neighbours), and so the same in all rows of one kind that the warp has. NI: pairs of a thread.
 // What bounds it: the instructions of 2-byte loads and stores. Measured: 16 x 2000 tokens of 16 heads of 128 dimensions, 100 of them
-// rotated, bf16 88 us, f32 95 us (114 and 169 with whole pieces whose elements look their partners up one by one).
+// rotated, bf16 87 us, f32 89 us (114 and 169 with whole pieces whose elements look their partners up one by one).
 template <class T, bool NORM, int NI>
 __global__ void __launch_bounds__(128) k_turn_any(const TurnArgs p)
 {
