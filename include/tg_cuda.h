@@ -424,9 +424,11 @@ typedef struct {
 	const int *group;        /* [seqs] */
 } tg_cuda_prefix;
 
-/* The results of tg_cuda_tree_attn, for all that its description says, with the prefixes' rows read once for the rows of a whole
- * group instead of once for each sequence. (What does not share goes its usual way. Where sharing costs more than it saves, by the host's
- * numbers alone, and with groups 0, the call is tg_cuda_tree_attn.) work: as there, tg_cuda_shared_attn_workspace bytes. */
+/* The results of tg_cuda_tree_attn, for all that its description says, with the prefixes' rows read once for every 128 rows (tokens
+ * times query heads of a key head) of a whole group instead of for each sequence; with f32, and with 16 bits of more than 128 dimensions, for every 4 to
+ * 32 rows, as many as suit groups of average size. (What does not share goes its usual way. Where sharing is reckoned to cost more than
+ * it saves, from the host's numbers alone, and with groups 0, the call is tg_cuda_tree_attn.) work: as there, tg_cuda_shared_attn_workspace bytes: 8 (d + 2)
+ * for each of the seqs * tokens * nq rows, d being head_dim rounded up to 64, 128 or 256, and up to about 40 MB. */
 long long tg_cuda_shared_attn_workspace(const tg_cuda_kv *c, const tg_cuda_drafts *d, const tg_cuda_prefix *x);
 int tg_cuda_shared_attn(const tg_cuda_kv *c, const tg_cuda_drafts *d, const tg_cuda_prefix *x, void *out, long long out_seq,
 			long long out_tok, long long out_head, float *lse, void *work, long long work_bytes, void *stream);

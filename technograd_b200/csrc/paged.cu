@@ -187,8 +187,15 @@ bool pg_meet(const PgRows &a, const PgRows &b)
 {
 	for (const PgRows *x : { &a, &b })
 		if (!x->at || x->row <= 0 || x->n[0] <= 0 || x->n[1] <= 0 || x->n[2] <= 0) return false;
+	const __int128 off = (__int128)(uintptr_t)b.at - (__int128)(uintptr_t)a.at;
+	auto span = [](const PgRows &x) {
+		__int128 n = x.row;
+		for (int i = 0; i < 3; i++) n += (__int128)x.stride[i] * (x.n[i] - 1);
+		return n;
+	};
+	if (off >= span(a) || off + span(b) <= 0) return false; // nearly always
 	const PgDims da(a), db(b);
-	return dims_meet(da, da.count, db, db.count, (__int128)(uintptr_t)b.at - (__int128)(uintptr_t)a.at);
+	return dims_meet(da, da.count, db, db.count, off);
 }
 
 int pg_len_out(const char *who, const tg_cuda_kv *c, const tg_cuda_drafts *d, const int *len_out)

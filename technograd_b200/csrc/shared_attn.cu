@@ -34,7 +34,11 @@ constexpr int SHARED_MMA_ROWS = 64, SHARED_MMA_TILES = 14;
 // (8 key heads of 128 dimensions, two query heads each, 65 positions of their own; bf16 unless f32): 4 sequences below 1024 positions 18.9 and
 // 15.6, below 4096 19.9 and 19.6; 8 below 1024 19.1 and 16.7, below 2048 18.9 and 20.2; 16 below 512 18.5 and 16.8, below 1024 18.7 and 22.0; 64 below 256 30.6 and
 // 28.0, below 1024 35.5 and 51.1; 64 in 32 groups below 2048 68 and 62, below 4096 95 and 107; f32: 4 below 4096 30 and 30, 16 below 1024 44 and 31,
-// below 2048 47 and 55, 64 below 512 56 and 73.
+// below 2048 47 and 55, 64 below 512 56 and 73. Over 370 other shapes (2 to 256 sequences of 1 to 64 tokens, 1 to 8 key heads and query heads each, 64 to 256
+// dimensions, prefixes of 128 to 32768) it is 2.9% slower than the better of both each time, where always and never sharing are 18%. It is most wrong where
+// it knows too little: many rows a sequence, whose tiles are full without sharing (190 of 32 tokens and 8 query heads a key head behind 696, pages of 24, 484
+// here and 242 with tree attention, sharing chosen); 256 dimensions of 16 bits, whose prefixes are read for every 16 rows (13 of 4 tokens behind 10368 57 and
+// 38, sharing chosen); f32 of many rows, whose products tree attention has too (213 of 8 query heads a key head behind 6240 238 and 426, tree attention chosen).
 static bool shared_tree(const tg_cuda_kv *c, const PgDrafts &d, const tg_cuda_prefix *x)
 {
 	if (!c->seqs || !x->groups || !x->max_shared) return true;
@@ -86,7 +90,7 @@ static int shared_plan(const char *who, const tg_cuda_kv *c, const PgDrafts &d, 
 	AttnPlan &p = o->pre;
 	p = {};
 	p.dev = o->own.dev, p.sms = o->own.sms, o->dp = p.dp = o->own.dp;
-	const long long rows = (long long)c->seqs * d.tokens * d.group, each = (rows + x->groups - 1) / x->groups; // each: a group's, about
+	const long long rows = (long long)c->seqs * d.tokens * d.group, each = (rows + x->groups - 1) / x->groups; // each: an average group's (members are not the host's to know)
 	p.tc = c->type != TG_CUDA_F32 && p.dp <= 128;
 	p.mt = each <= 16 || p.dp == 256 ? 1 : 2;
 	p.fma = c->type == TG_CUDA_F32 && each <= 8 ? each <= 4 ? 4 : 8 : 0;

@@ -87,6 +87,7 @@ def _tangent(*tensors) -> bool:
 
 
 def _no_tangent(name: str, *tensors) -> None:
+    """Called within a level of forward mode only."""
     if _tangent(*tensors):
         raise RuntimeError(f"kvcache.{name} has no forward-mode derivative")
 
@@ -202,7 +203,8 @@ def tree_attention(cache: PagedKV, q, k, v, mask=None, count=None, scale: float 
     nq]); a token that sees nothing has out 0 and lse -inf. Forward only: where q, k or v require a
     gradient, a backward pass through the results is an error, and so is a tangent of theirs (attention_weights', commit's and evict's
     results never require a gradient and have no tangents)."""
-    _no_tangent("tree_attention", q, k, v)
+    if forward_ad._current_level >= 0:
+        _no_tangent("tree_attention", q, k, v)
     d = _drafts(cache, q, k, v, mask, count, scale)
     stream, shape = _stream(cache), q.shape
     plan = cache._plans.get(shape[1:3])
@@ -258,11 +260,12 @@ class SharedPrefix:
 def shared_attention(cache: PagedKV, prefix: SharedPrefix, q, k, v, mask=None, count=None, scale: float | None = None):
     """tree_attention for a batch whose sequences share prefixes, each read once for its whole group (tg_cuda_shared_attn).
 
-    Arguments and results as for tree_attention."""
+    Arguments and results as for tree_attention. Its scratch has two f32 rows for each row of q."""
     if prefix.index != cache.index or prefix.seqs != cache.seqs or prefix.max_shared > cache.max_len:
         raise ValueError(f"prefix: made for {prefix.seqs} sequences with up to {prefix.max_shared} positions shared on cuda:{prefix.index}, not for {cache.seqs} of "
                          f"up to {cache.max_len} on cuda:{cache.index}")
-    _no_tangent("shared_attention", q, k, v)
+    if forward_ad._current_level >= 0:
+        _no_tangent("shared_attention", q, k, v)
     d = _drafts(cache, q, k, v, mask, count, scale)
     stream, shape = _stream(cache), q.shape
     key = shape[1], shape[2], prefix._sizes
@@ -461,10 +464,11 @@ def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None,
 
     k, v [seqs, tokens, nkv, head_dim] and q [seqs, tokens, nq, head_dim]: a projection's output, any number of tokens; count int32
     [seqs]: tokens there are (None: all). Cache row lens + i receives token i's k, rotated to its position (pos, None: lens + i), and v. q_norm, k_norm
-    f32 [head_dim]: weights of an RMS norm of each head before the rotation. keys: return the rotated keys too, with k's strides, which tree_attention and
+    f32 [head_dim]: weights of an RMS norm of each head before the rotation. keys: return the rotated keys too, with k's strides (and so the memory that k's projection spans), which tree_attention and
     shared_attention take with v as the tokens' own, the lengths being those from before. Returns (the new lengths, q rotated or
     None, k rotated or None), rows past count 0; the pages are written in place. Forward only, like tree_attention."""
-    _no_tangent("append", q, k, v, q_norm, k_norm)
+    if forward_ad._current_level >= 0:
+        _no_tangent("append", q, k, v, q_norm, k_norm)
     d = _drafts(cache, q, k, v, None, count, 1.0)
     n, dim, index = k.shape, cache.head_dim, cache.index
     qn = kn = qo = ko = qp = kp = r = None
@@ -490,11 +494,11 @@ def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None,
         sk, kp = ko.stride(), ko.data_ptr()
     _lib.check(_lib.lib().tg_cuda_kv_append(cache._at, d, r, qn, kn, eps, qp, sq[0], sq[1], sq[2], kp, sk[0], sk[1], sk[2], lens.data_ptr(), _stream(cache)))
     _pages_written(cache)
-    given = [x for x in (q, k, v, q_norm, k_norm) if x is not None] if torch.is_grad_enabled() else ()
-    if any(x.requires_grad for x in given):
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad) or
+                                    (q_norm is not None and q_norm.requires_grad) or (k_norm is not None and k_norm.requires_grad)):
         made = [x for x in (qo, ko) if x is not None]
         if made:
-            made = list(_NoGradient.apply("append", len(made), *made, *given))
+            made = list(_NoGradient.apply("append", len(made), *made, *(x for x in (q, k, v, q_norm, k_norm) if x is not None)))
             qo, ko = made.pop(0) if qo is not None else None, made.pop(0) if ko is not None else None
     return lens, qo, ko
 
