@@ -120,9 +120,9 @@ __device__ __forceinline__ long long turn_pos(const TurnArgs &p, long long b, in
 // threads of one place compute PART of them each and pass them round. No shared memory, no barrier, and all rounds'
 // loads on their way at once. A row's pieces are read and written by the same thread, reads first, so that a row may
 // be written where it is read. FULL: every thread of a row has two pieces.
-// What bounds it: HBM where there are many tokens, latency where there are few; with norms the instructions, about 680 a warp of four
-// rounds. Measured (bf16, 128 dimensions): 8 x 6001 tokens of 16 heads 64 us, 6.1 TB/s (117 with cos and sin in shared memory and a
-// barrier); 16 prompts of up to 2047 tokens, 16 query heads and 8 key heads normed and rotated into the cache, 109 us, 4.2 TB/s (118 with
+// What bounds it: HBM where there are many tokens, latency where there are few; with norms the instructions, about 700 a warp of four
+// rounds. Measured (bf16, 128 dimensions): 8 x 6001 tokens of 16 heads 60 us, 6.5 TB/s (117 with cos and sin in shared memory and a
+// barrier); 16 prompts of up to 2047 tokens, 16 query heads and 8 key heads normed and rotated into the cache, 111 us, 4.2 TB/s (118 with
 // all of a token's rows in one warp, which then looks up each kind's strides as it goes).
 template <class T, int FORM, bool NORM, int PART, int UN, bool FULL>
 __global__ void __launch_bounds__(128, 5) k_turn(const TurnArgs p, int lg)
