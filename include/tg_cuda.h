@@ -358,7 +358,7 @@ int tg_cuda_ssm_get_stats(const tg_cuda_ssm *g, tg_cuda_ssm_stats *out);
  * bytes; head_dim is at most 256. Strides are not negative (one along a single element is
  * not looked at). Rows that a call writes (out, the pools of a commit and of an eviction's
  * destination, a commit's acc) do not overlap: a stride spans all of the dimensions of smaller
- * strides. A pool is less than 2^32 times as long as its pages' and rows' common
+ * strides; nor do they share memory with what the call reads, but where it says so. A pool is less than 2^32 times as long as its pages' and rows' common
  * alignment (64 GB at 16 bytes).
  *
  * len and table are read by the kernels. A len outside [0, max_len] is taken as the

@@ -446,7 +446,8 @@ def _along(ctx, x, inverse):
 def rope(x, rotary: Rotary, pos=None, inverse: bool = False, out=None):
     """x [seqs, tokens, heads, head_dim] rotated to its tokens' positions (tg_cuda_rope); pos int32 [seqs, tokens] or [tokens] (None: 0, 1, ...).
 
-    inverse: by the negative angle. out: where to (x itself: in place; else memory that x does not share). Differentiable with respect to x in either mode, without out."""
+    inverse: by the negative angle. out: where to (x itself: in place; else memory that x does not share). Differentiable with respect to
+    x in reverse and forward mode, without out."""
     if (torch.is_grad_enabled() and x.requires_grad) or _tangent(x, out):
         _need(out is None, "out: not with a gradient or a tangent")
         return _Rope.apply(x, rotary, pos, inverse, False)
@@ -464,8 +465,8 @@ def append(cache: PagedKV, k, v, q=None, rotary: Rotary | None = None, pos=None,
 
     k, v [seqs, tokens, nkv, head_dim] and q [seqs, tokens, nq, head_dim]: a projection's output, any number of tokens; count int32
     [seqs]: tokens there are (None: all). Cache row lens + i receives token i's k, rotated to its position (pos, None: lens + i), and v. q_norm, k_norm
-    f32 [head_dim]: weights of an RMS norm of each head before the rotation. keys: return the rotated keys too, with k's strides (and so the memory that k's projection spans), which tree_attention and
-    shared_attention take with v as the tokens' own, the lengths being those from before. Returns (the new lengths, q rotated or
+    f32 [head_dim]: weights of an RMS norm of each head before the rotation. keys: return the rotated keys too, with k's strides (and so the memory
+    that k's projection spans), which tree_attention and shared_attention take with v as the tokens' own, the lengths being those from before. Returns (the new lengths, q rotated or
     None, k rotated or None), rows past count 0; the pages are written in place. Forward only, like tree_attention."""
     if forward_ad._current_level >= 0:
         _no_tangent("append", q, k, v, q_norm, k_norm)
